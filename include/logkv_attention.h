@@ -131,6 +131,52 @@ LOGKV_API int logkv_attention(const logkv_layout_t* layout, const logkv_state_t*
                               const logkv_prefix_t* prefix, const logkv_attention_args_t* args,
                               void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Attention of a tree of drafted tokens over the cache (speculative decoding; no reference
+ * counterpart).  The drafted tokens are not committed: token t of a batch row attends over
+ * [prefix | recent window | itself and its ancestors in the tree],
+ *   out = softmax(scale * (q . k_s + qx * mass_s)) v_s,
+ * where the ancestors of t are parents[t], parents[parents[t]], ...  parents[t] = -1: t follows the
+ * last committed token; 0 <= parents[t] < t: t follows token parents[t]; -2: no token (rows of a
+ * batch whose trees are smaller are padded so).  Any other value is treated as -2 and sets bit 18
+ * of `status`.  A token that is absent, or whose chain of parents reaches an absent token, writes a
+ * zero output row and is seen by no token: its K and V may hold anything.  A token whose V holds a
+ * NaN or an infinity makes the outputs of the tokens that see it NaN, and only those.
+ *
+ * q is [B,H,tokens,D], k_new and v_new are [B,G,tokens,D] (post-RoPE, storage dtype) with the given
+ * element strides of their batch, head and token axes; the head dim is contiguous and every row
+ * 16-byte aligned.  out is [B,H,tokens,D], contiguous.  Any number of query heads per group;
+ * tokens <= LOGKV_TREE_MAX_TOKENS.  Head dims: 16, 32, 64, 128 (and 256 for bf16 caches).
+ */
+#define LOGKV_TREE_MAX_TOKENS 256
+typedef struct logkv_tree_args {
+  const void* q;
+  const void* k_new;
+  const void* v_new;
+  void* out;
+  const void* parents;      /* [B, tokens] int32, or int64 with parents_wide   */
+  int64_t q_strides[3];
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t parents_stride;   /* elements between batch rows; 0: one tree for all */
+  int32_t parents_wide;     /* 1: parents are int64                             */
+  int32_t heads;            /* H, a multiple of groups                          */
+  int32_t tokens;
+  int32_t recent_count;     /* window rows [0, recent_count) are attended       */
+  float scale;
+  float qx;                 /* as logkv_attention_args_t                        */
+  int32_t* status;          /* device int32 or NULL                             */
+} logkv_tree_args_t;
+
+/* Scratch bytes of logkv_tree_attention (no initialisation needed; 0: shape not supported).  The
+ * scratch must not be shared by calls that may overlap on the GPU. */
+LOGKV_API size_t logkv_tree_attention_workspace_bytes(const logkv_layout_t* layout, int32_t heads, int32_t tokens,
+                                                      int32_t prefix_capacity);
+
+LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_state_t* state,
+                                   const logkv_prefix_t* prefix, const logkv_tree_args_t* args, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -94,6 +94,18 @@ class AttentionArgs(ctypes.Structure):
                 ("q_stride", ctypes.c_int32)]
 
 
+class TreeArgs(ctypes.Structure):
+    """logkv_tree_args_t (include/logkv_attention.h)."""
+    _fields_ = [("q", ctypes.c_void_p), ("k_new", ctypes.c_void_p), ("v_new", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("parents", ctypes.c_void_p), ("q_strides", ctypes.c_int64 * 3),
+                ("k_strides", ctypes.c_int64 * 3), ("v_strides", ctypes.c_int64 * 3),
+                ("parents_stride", ctypes.c_int64), ("parents_wide", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("tokens", ctypes.c_int32), ("recent_count", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("qx", ctypes.c_float), ("status", ctypes.c_void_p)]
+
+
+TREE_MAX_TOKENS = 256   # LOGKV_TREE_MAX_TOKENS
+
 _lib = None
 
 
@@ -181,6 +193,12 @@ def lib() -> ctypes.CDLL:
         handle.logkv_attention.restype = ctypes.c_int
         handle.logkv_attention.argtypes = [P(Layout), P(State), P(Prefix), P(AttentionArgs), ctypes.c_void_p,
                                            ctypes.c_size_t, ctypes.c_void_p]
+        handle.logkv_tree_attention_workspace_bytes.restype = ctypes.c_size_t
+        handle.logkv_tree_attention_workspace_bytes.argtypes = [P(Layout), ctypes.c_int32, ctypes.c_int32,
+                                                                ctypes.c_int32]
+        handle.logkv_tree_attention.restype = ctypes.c_int
+        handle.logkv_tree_attention.argtypes = [P(Layout), P(State), P(Prefix), P(TreeArgs), ctypes.c_void_p,
+                                                ctypes.c_size_t, ctypes.c_void_p]
         _lib = handle
     return _lib
 

@@ -7,6 +7,8 @@ first order) with the same names, arguments and errors:
   pack_mid_kv(cache, plan, ...)   log_kv_pack.pack_mid_kv                         (log_kv_pack.py:114-131)
   log_kv_chunk_attention(...)     log_kv_cache.log_kv_chunk_attention             (log_kv_cache.py:6802-6864)
 
+and one of its own: log_kv_tree_attention(...), a tree of drafted tokens over the same state.
+
 Everything runs through the C ABI of ``liblogkv_b200.so`` (include/logkv_attention.h);
 there is no CPU path.  The packed frozen prefix (merged slots rotated at their mid
 anchors, then the exact pool) only changes when a flush rewrites the ladder, so it
@@ -285,4 +287,88 @@ def log_kv_chunk_attention(cache, q_b, k_b, v_b, scale, second_order_scale=1.0, 
                                               ctypes.byref(args), ws.data_ptr(), ws.numel(), _stream(cache)),
                    "logkv_attention")
         t0 += n
+    return out
+
+
+def _rows16(t):
+    """``t`` with its head dim contiguous and every row 16-byte aligned (a copy where it is not)."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * t.element_size() % 16 == 0 for s in t.stride()[:3]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _tree_parents(cache, parents, T: int):
+    """Parents as an integer tensor on the cache's device ([T] or [B, T]); host values are checked."""
+    dev = cache.level_k.device
+    p = parents if isinstance(parents, torch.Tensor) else torch.as_tensor(parents)
+    if p.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"parents must be integers (int32 or int64), got {p.dtype}")
+    if tuple(p.shape) not in ((T,), (cache.batch_size, T)):
+        raise ValueError(f"parents must be [{T}] or [{cache.batch_size}, {T}], got {tuple(p.shape)}")
+    if p.device.type == "cpu":
+        if bool(((p < -2) | (p >= torch.arange(T))).any()):
+            raise ValueError("a token's parent must be an earlier token, -1 (the committed tokens) or -2 (no token)")
+        p = p.to(dev)
+    elif p.device != dev:
+        raise ValueError(f"parents must be on {dev}, got {p.device}")
+    return p if p.stride(-1) == 1 else p.contiguous()
+
+
+def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
+    """Attention of a tree of drafted tokens over the cache, committing nothing (no reference counterpart).
+
+    q [B, H, T, D] and k, v [B, G, T, D] are the T <= 256 drafted tokens of every batch row, post-RoPE
+    (a token's position is the committed length plus its depth), any strides.  ``parents`` ([T], or
+    [B, T] for one tree per row; int32 or int64) gives the tree: -1 for a token that follows the
+    committed tokens, an earlier token's index, or -2 for no token (rows with smaller trees are
+    padded so).  Token t attends over the frozen prefix, the window, its ancestors and itself; absent
+    tokens, and tokens below one, are seen by nobody and give zero rows.  Parents on the host are
+    checked here; a bad value in a device tensor counts as -2 and sets bit 18 of the read status.
+    Returns [B, H, T, D]; ``out`` may be given.  The scratch is allocated per call, so calls on
+    different streams, or captured graphs, never share it.  Forward-only.
+
+    After verification the accepted path is committed with ``cache.add_recent``.
+    """
+    if q.dim() != 4:
+        raise ValueError(f"q must be [B, H, T, D], got {tuple(q.shape)}")
+    B, H, T, kd = q.shape
+    dev = cache.level_k.device
+    if B != cache.batch_size or kd != cache.k_dim or q.dtype != cache.level_k.dtype:
+        raise ValueError(f"q must be [B={cache.batch_size}, H, T, {cache.k_dim}] in the cache dtype")
+    _check_kv(cache, k, v)
+    if k.size(2) != T:
+        raise ValueError("q, k and v must cover the same drafted tokens")
+    if H < 1 or H % cache.n_groups:
+        raise ValueError(f"query heads {H} must be a multiple of KV groups {cache.n_groups}")
+    if any(t.device != dev for t in (q, k, v)):
+        raise ValueError(f"q, k and v must be on the cache's device {dev}")
+    if T > _lib.TREE_MAX_TOKENS:
+        raise ValueError(f"{T} drafted tokens: at most {_lib.TREE_MAX_TOKENS}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+        raise NotImplementedError("logkv_b200 attention is forward-only")
+    if out is None:
+        out = torch.empty(B, H, T, cache.v_dim, dtype=q.dtype, device=dev)
+    elif out.shape != (B, H, T, cache.v_dim) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous [{B}, {H}, {T}, {cache.v_dim}] tensor in the cache dtype on {dev}")
+    if T == 0:
+        return out
+    p = _tree_parents(cache, parents, T)
+    with torch.cuda.device(dev):
+        rs = refresh_prefix(cache)
+        layout, state = _structs(cache)
+        q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        n = _lib.lib().logkv_tree_attention_workspace_bytes(ctypes.byref(layout), H, T, rs.capacity)
+        if not n:
+            raise ValueError(f"tree attention shape outside the supported range (heads={H}, tokens={T}, "
+                             f"head dim {kd}, {q.dtype})")
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        i64x3 = ctypes.c_int64 * 3
+        args = _lib.TreeArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p.data_ptr(),
+                             i64x3(*q.stride()[:3]), i64x3(*k.stride()[:3]), i64x3(*v.stride()[:3]),
+                             p.stride(0) if p.dim() == 2 else 0, int(p.dtype == torch.int64), H, T,
+                             int(cache.recent_count), float(scale), query_extra(scale, q.dtype), rs.status.data_ptr())
+        pre = rs.prefix_struct()
+        _lib.check(_lib.lib().logkv_tree_attention(ctypes.byref(layout), ctypes.byref(state), ctypes.byref(pre),
+                                                   ctypes.byref(args), ws.data_ptr(), n, _stream(cache)),
+                   "logkv_tree_attention")
     return out

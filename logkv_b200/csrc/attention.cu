@@ -17,12 +17,7 @@
 #include <type_traits>
 #include <cstring>
 
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
-#include "common.cuh"
-#include "tcgen05.cuh"
-#include "../../include/logkv_attention.h"
+#include "attn_common.cuh"
 
 namespace logkv {
 
@@ -322,20 +317,6 @@ __global__ void __launch_bounds__(256) pack_mid_kernel(PlanGeo pg, logkv_state_t
 }
 
 // ---------------------------------------------------------------- K4: slot attention
-__device__ __forceinline__ void cp_async16(void* smem, const void* gmem) {
-  const unsigned sa = (unsigned)__cvta_generic_to_shared(smem);
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(sa), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
-  const unsigned sa = (unsigned)__cvta_generic_to_shared(smem);
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(sa), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
-}
-
 __device__ __forceinline__ void unpack16(const uint4& u, float* out, const float*) {
   const float* f = reinterpret_cast<const float*>(&u);
 #pragma unroll
@@ -691,29 +672,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32) slot_attn_kernel(AttnGeo a, l
 // (prefix, window, new tokens), so a tile's K and V rows are contiguous blocks; each lane
 // copies 16-byte chunks into an XOR-swizzled stage (conflict-free ldmatrix), and a
 // __syncwarp after cp.async.wait_group makes every lane's chunks visible to the warp.
-__device__ __forceinline__ void ldsm_x4(unsigned addr, unsigned& r0, unsigned& r1, unsigned& r2, unsigned& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_t(unsigned addr, unsigned& r0, unsigned& r1, unsigned& r2, unsigned& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-__device__ __forceinline__ void mma_bf16(float* c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
-                                         unsigned b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};\n"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ unsigned pack_bf16x2(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const unsigned*>(&v);
-}
-
 template <int D, int ST = kMmaStages>
 struct MmaShape {
   static constexpr int TS = 16;             // slots per tile (two n8 score tiles, one k16 PV step)
@@ -1278,7 +1236,6 @@ __global__ void __launch_bounds__(kPfWarps * 32) chunk_attn_mma_kernel(AttnGeo a
 // mbarriers; every wait is bounded, and on expiry a role stops, the CTA records kStatusTimeout,
 // frees its tensor memory and returns.
 constexpr int kTcRows = 128;
-constexpr int kTcTS = 64;
 constexpr int kTcLoaders = 96;             // three loader warps
 constexpr int32_t kStatusTimeout = 1 << 17;
 constexpr long long kTcWaitBudget = 4000000000LL;   // clock cycles (about 2 s)
@@ -1704,30 +1661,12 @@ __global__ void __launch_bounds__(TcRoles<NQ>::WARPS * 32, 1)
 }
 
 // ---------------------------------------------------------------- host side
-static bool dtype_ok(int d) { return d == LOGKV_DTYPE_F32 || d == LOGKV_DTYPE_BF16; }
-static size_t esize_of(int d) { return d == LOGKV_DTYPE_F32 ? 4 : 2; }
-
-static int check_layout(const logkv_layout_t* l) {
-  if (!l) return LOGKV_E_POINTER;
-  if (!dtype_ok(l->dtype)) return LOGKV_E_DTYPE;
-  if (l->batch < 1 || l->groups < 1 || l->dim < 1 || l->clusters < 1 || l->clusters > kMaxClusters ||
-      l->levels < 1 || l->levels > kMaxLevels || l->slots < 1 || l->exact < 0)
-    return LOGKV_E_SHAPE;
-  if ((l->dim * esize_of(l->dtype)) % 16 != 0) return LOGKV_E_SHAPE;
-  return LOGKV_OK;
-}
-
 static int check_rope(const logkv_rope_t* r, int D) {
   if (!r) return LOGKV_E_POINTER;
   if (!dtype_ok(r->dtype)) return LOGKV_E_DTYPE;
   if (r->rope_n < 0 || r->rope_n > D || (r->rope_n & 1)) return LOGKV_E_SHAPE;
   if (r->rope_n > 0 && (!r->cos || !r->sin || r->rows < 1)) return LOGKV_E_POINTER;
   return LOGKV_OK;
-}
-
-static int launch_status() {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? LOGKV_OK : (int)e;
 }
 
 template <typename T>
@@ -1860,35 +1799,6 @@ static int launch_chunk_d(const AttnGeo& ag, const logkv_prefix_t& pre, const lo
       static_cast<const B16*>(x.k_new), static_cast<const B16*>(x.v_new), static_cast<const B16*>(x.q),
       static_cast<B16*>(x.out));
   return launch_status();
-}
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no link against libcuda).
-static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  }
-  return fn;
-}
-
-// [rows, D] bf16 rows of D * 2 bytes; 64 x 64-element boxes in the 128-byte swizzle; rows past
-// the end read as zeros.  False if the encoder is missing or refuses (e.g. a misaligned base).
-static bool encode_rows_map(CUtensorMap* m, const void* base, size_t rows, int D) {
-  auto enc = tensor_map_encoder();
-  if (!enc || !base || rows == 0 || (reinterpret_cast<uintptr_t>(base) & 15)) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)kTcTS};
-  const cuuint32_t estr[2] = {1, 1};
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Combine of the chunk kernel's key-range splits: one warp per output row (b, h, token), the

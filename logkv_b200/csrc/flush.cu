@@ -49,23 +49,6 @@ static size_t prep_smem_bytes(const Geo& g, size_t esize) {
 
 static size_t cascade_smem(const Geo& g, size_t esize) { return walk_smem(g, esize, kTileRows); }
 
-// Every flush kernel is launched with a programmatic dependency on the previous kernel of the
-// stream (each kernel begins with pdl_entry()), so launch latency overlaps the previous tail.
-template <typename... KArgs, typename... Args>
-static void launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kern, args...);
-}
-
 template <typename K>
 static void smem_limit(K* kern, size_t smem) {
   if (smem > 48 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

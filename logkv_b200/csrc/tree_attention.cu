@@ -1,0 +1,753 @@
+// Attention of a tree of drafted tokens over the LogKV cache (C ABI in include/logkv_attention.h).
+//
+// The query rows of a (b, g) lane are its rf heads times T tokens, r = h * T + t.  They attend over
+// three segments of keys: the packed prefix (log-mass term), the window, the T drafted tokens under
+// the tree's ancestor mask.  The keys of a lane are split over CTAs; every CTA keeps the running
+// maximum and sum of its rows' softmax in float32 and leaves (m, l, O) per row, which
+// tree_combine_kernel joins in split order.
+#include <algorithm>
+
+#include "attn_common.cuh"
+
+namespace logkv {
+
+constexpr int32_t kStatusBadParent = 1 << 18;
+constexpr int kTreeMaxTokens = LOGKV_TREE_MAX_TOKENS;
+constexpr int kTreeWords = kTreeMaxTokens / 32;
+
+struct TreeGeo {
+  int B, G, H, rf, T, D;
+  int rcap, rcount;
+  int nsplit;   // splits of the grid; a lane uses tree_splits() of them
+  int nsmin;    // splits that fill the SMs
+  int upw;      // key tiles a split has at least (a tile per warp)
+  float scale_log2, mass_log2;   // score = dot * scale_log2 + mass * mass_log2, in the log2 domain
+  const void* q;
+  const void* kn;
+  const void* vn;
+  long long qs[3], ks[3], vs[3];
+  const void* parents;
+  long long pstride;
+  int wide;
+};
+
+// Splits of a lane with `units` key tiles (the same value in the attention kernel and the combine).
+__device__ __forceinline__ int tree_splits(const TreeGeo& a, int units) {
+  return max(1, min(a.nsplit, min(a.nsmin, units / a.upw)));
+}
+
+__device__ __forceinline__ int prefix_length(const logkv_prefix_t& pre, int ln) {
+  return min(max(pre.length[ln], 0), pre.capacity);
+}
+
+// Ancestor masks of batch row b: bit j of mask[t] = token t sees token j; 0 for an absent token.
+// Pointer doubling: after round i the mask covers the 2^i nearest tokens of the chain and `up` is
+// the next one (-1: the committed tokens, -2: an absent token).  Called by the whole block.
+__device__ void tree_masks(const TreeGeo& a, int b, uint32_t (*mask)[kTreeWords], int* up, int32_t* status) {
+  const int T = a.T, words = (T + 31) >> 5;
+  for (int t = threadIdx.x; t < T; t += blockDim.x) {
+    const size_t at = (size_t)b * a.pstride + t;
+    const long long p = a.wide ? static_cast<const long long*>(a.parents)[at]
+                               : (long long)static_cast<const int32_t*>(a.parents)[at];
+    const bool bad = p < -2 || p >= t;
+    if (bad) set_status(status, kStatusBadParent);
+    up[t] = bad ? -2 : (int)p;
+    for (int w = 0; w < words; ++w) mask[t][w] = (t >> 5) == w ? 1u << (t & 31) : 0u;
+  }
+  __syncthreads();
+  for (int len = 1; len < T; len *= 2) {
+    uint32_t add[2][kTreeWords];   // blockDim.x >= kTreeMaxTokens / 2
+    int next[2];
+    bool more = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = threadIdx.x + i * blockDim.x;
+      next[i] = -1;
+      if (t < T && up[t] >= 0) {
+        more = true;
+        next[i] = up[up[t]];
+#pragma unroll
+        for (int w = 0; w < kTreeWords; ++w) add[i][w] = w < words ? mask[up[t]][w] : 0u;
+      }
+    }
+    if (!__syncthreads_or(more)) break;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = threadIdx.x + i * blockDim.x;
+      if (t < T && up[t] >= 0) {
+#pragma unroll
+        for (int w = 0; w < kTreeWords; ++w)
+          if (w < words) mask[t][w] |= add[i][w];
+        up[t] = next[i];
+      }
+    }
+    __syncthreads();
+  }
+  for (int t = threadIdx.x; t < T; t += blockDim.x)
+    if (up[t] == -2)
+      for (int w = 0; w < words; ++w) mask[t][w] = 0u;
+  __syncthreads();
+}
+
+// Partial of one row and split: [m, l, -, -, O[D]], O relative to 2^m.
+__device__ __forceinline__ float* tree_part(float* part, const TreeGeo& a, int split, size_t row) {
+  return part + ((size_t)split * a.B * a.H * a.T + row) * (a.D + 4);
+}
+
+// ---------------------------------------------------------------- bf16: mma.sync, 16 query rows per CTA
+// The 16 rows are the M of mma.sync.m16n8k16.  Each of the 4 warps streams 16-slot tiles of its own
+// through a private ring of cp.async stages (XOR-swizzled for ldmatrix); tiles do not cross segments.
+constexpr int kTreeWarps = 4;
+constexpr int kTreeStages = 3;
+
+template <int D>
+struct TreeShape {
+  static constexpr int TS = 16, CPR = D / 8, KS = D / 16, DT = D / 8;
+  static constexpr int STAGE_BYTES = 2 * TS * D * 2 + TS * 4;   // K, V, mass
+  static constexpr size_t smem = (size_t)kTreeWarps * kTreeStages * STAGE_BYTES;
+  __device__ __forceinline__ static int swz(int r, int c) {
+    if (CPR >= 8) return c ^ (r & 7);
+    return c ^ ((r * CPR / 8) & (CPR - 1));
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kTreeWarps * 32, D <= 128 ? 2 : 1)
+    tree_mma_kernel(TreeGeo a, logkv_prefix_t pre, const __nv_bfloat16* rk, const __nv_bfloat16* rv,
+                    __nv_bfloat16* out, float* part, int32_t* status) {
+  using S = TreeShape<D>;
+  using B16 = __nv_bfloat16;
+  constexpr int TS = S::TS, CPR = S::CPR, KS = S::KS, DT = S::DT, ST = kTreeStages;
+  extern __shared__ uint4 smem4[];
+  __shared__ uint32_t masks[kTreeMaxTokens][kTreeWords];
+  __shared__ int up_[kTreeMaxTokens];
+  __shared__ float wm_[kTreeWarps][16], wl_[kTreeWarps][16];
+  pdl_entry();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int g8 = lane >> 2, t4 = lane & 3;
+  const int ln = blockIdx.x, split = blockIdx.y, row0 = blockIdx.z * 16, g = ln % a.G, b = ln / a.G;
+  const int NQ = min(16, a.rf * a.T - row0), T = a.T;
+  const int Lp = prefix_length(pre, ln), R = a.rcount;
+  const int up = (Lp + TS - 1) / TS, ur = (R + TS - 1) / TS, uc = (T + TS - 1) / TS, U = up + ur + uc;
+  const int ns = tree_splits(a, U);
+  if (split >= ns) return;
+  const int u0 = (int)((long long)U * split / ns), u1 = (int)((long long)U * (split + 1) / ns);
+  const int mine = (u1 - u0) > warp ? (u1 - u0 - warp + kTreeWarps - 1) / kTreeWarps : 0;
+  if (u1 > up + ur) tree_masks(a, b, masks, up_, status);   // uniform over the block
+  unsigned char* wbase = reinterpret_cast<unsigned char*>(smem4) + (size_t)warp * ST * S::STAGE_BYTES;
+  const unsigned wbase_s = (unsigned)__cvta_generic_to_shared(wbase);
+  const B16* kn = static_cast<const B16*>(a.kn) + b * a.ks[0] + g * a.ks[1];
+  const B16* vn = static_cast<const B16*>(a.vn) + b * a.vs[0] + g * a.vs[1];
+
+  int tok[2];   // tokens of the lane's rows g8 and g8 + 8
+  unsigned qa[KS][4];
+#pragma unroll
+  for (int hr = 0; hr < 2; ++hr) {
+    const int r = g8 + 8 * hr, row = row0 + min(r, NQ - 1);
+    tok[hr] = row % T;
+    const B16* qp = static_cast<const B16*>(a.q) + b * a.qs[0] + (g * a.rf + row / T) * a.qs[1] + tok[hr] * a.qs[2];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qa[ks][hr] = r < NQ ? *reinterpret_cast<const unsigned*>(qp + ks * 16 + 2 * t4) : 0u;
+      qa[ks][2 + hr] = r < NQ ? *reinterpret_cast<const unsigned*>(qp + ks * 16 + 2 * t4 + 8) : 0u;
+    }
+  }
+
+  // Tile u: its segment, first row and row count.
+  auto tile = [&](int u, int& first, int& rows) {
+    if (u < up) {
+      first = u * TS;
+      rows = min(TS, Lp - first);
+      return 0;
+    }
+    if (u < up + ur) {
+      first = (u - up) * TS;
+      rows = min(TS, R - first);
+      return 1;
+    }
+    first = (u - up - ur) * TS;
+    rows = min(TS, T - first);
+    return 2;
+  };
+  auto issue = [&](int k, int stage) {
+    if (k < mine) {
+      int first, rows;
+      const int cls = tile(u0 + warp + k * kTreeWarps, first, rows);
+      const size_t r0 = cls == 0 ? (size_t)ln * pre.capacity + first : (size_t)ln * a.rcap + first;
+      const B16* kb = cls == 0 ? static_cast<const B16*>(pre.k) + r0 * D : cls == 1 ? rk + r0 * D : kn + first * a.ks[2];
+      const B16* vb = cls == 0 ? static_cast<const B16*>(pre.v) + r0 * D : cls == 1 ? rv + r0 * D : vn + first * a.vs[2];
+      const long long kst = cls == 2 ? a.ks[2] : D, vst = cls == 2 ? a.vs[2] : D;
+      unsigned char* sk = wbase + (size_t)stage * S::STAGE_BYTES;
+      unsigned char* sv = sk + TS * D * 2;
+      float* sm = reinterpret_cast<float*>(sk + 2 * TS * D * 2);
+#pragma unroll
+      for (int i = 0; i < (TS * CPR + 31) / 32; ++i) {
+        const int flat = i * 32 + lane, r = flat / CPR, c = flat % CPR;
+        if (flat < TS * CPR) {
+          const int off = r * D * 2 + S::swz(r, c) * 16;
+          if (r < rows) {
+            cp_async16(sk + off, kb + r * kst + c * 8);
+            cp_async16(sv + off, vb + r * vst + c * 8);
+          } else {
+            *reinterpret_cast<uint4*>(sk + off) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(sv + off) = make_uint4(0, 0, 0, 0);
+          }
+        }
+      }
+      if (lane < TS) {
+        if (cls == 0 && lane < rows) cp_async4(sm + lane, pre.mass + r0 + lane);
+        else sm[lane] = 0.f;
+      }
+    }
+    cp_async_commit();
+  };
+
+  float o[DT][4];
+#pragma unroll
+  for (int j = 0; j < DT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+  for (int k = 0; k < ST - 1; ++k) issue(k, k);
+  for (int k = 0; k < mine; ++k) {
+    issue(k + ST - 1, (k + ST - 1) % ST);
+    cp_async_wait<ST - 1>();
+    __syncwarp();
+    const int stage = k % ST;
+    int first, rows;
+    const int cls = tile(u0 + warp + k * kTreeWarps, first, rows);
+    unsigned char* st = wbase + (size_t)stage * S::STAGE_BYTES;
+    const unsigned sk = wbase_s + stage * S::STAGE_BYTES, sv = sk + TS * D * 2;
+    const float* sm = reinterpret_cast<const float*>(st + 2 * TS * D * 2);
+    // Columns each row sees; drafted tokens whose V is not finite, taken out of the product below.
+    unsigned see0 = (1u << rows) - 1, see1 = see0, poison = 0;
+    if (cls == 2) {
+      see0 = masks[tok[0]][first >> 5] >> (first & 31) & see0;
+      see1 = masks[tok[1]][first >> 5] >> (first & 31) & see1;
+      unsigned char* v = st + TS * D * 2;
+      const int r = lane & 15;   // two lanes per row of V
+      bool bad = false;
+      for (int c = lane >> 4; c < CPR; c += 2) {
+        uint4 x = *reinterpret_cast<const uint4*>(v + r * D * 2 + c * 16);
+        unsigned* w = reinterpret_cast<unsigned*>(&x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool lo = (w[i] & 0x7f80u) == 0x7f80u, hi = (w[i] & 0x7f800000u) == 0x7f800000u;
+          bad |= lo | hi;
+          w[i] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
+        }
+        *reinterpret_cast<uint4*>(v + r * D * 2 + c * 16) = x;
+      }
+      poison = __ballot_sync(0xffffffffu, bad);
+      poison = (poison | poison >> 16) & 0xffffu;
+      __syncwarp();
+    }
+    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int mi = lane >> 3, rr = (mi >> 1) * 8 + (lane & 7), cc = 2 * ks + (mi & 1);
+      unsigned b0, b1, b2, b3;
+      ldsm_x4(sk + rr * D * 2 + S::swz(rr, cc) * 16, b0, b1, b2, b3);
+      mma_bf16(sc[0], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b0, b1);
+      mma_bf16(sc[1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b2, b3);
+    }
+    float mt0 = -INFINITY, mt1 = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int col = 8 * j + 2 * t4 + e;
+        const float mass = sm[col] * a.mass_log2;
+        sc[j][e] = see0 >> col & 1 ? fmaf(sc[j][e], a.scale_log2, mass) : -INFINITY;
+        sc[j][2 + e] = see1 >> col & 1 ? fmaf(sc[j][2 + e], a.scale_log2, mass) : -INFINITY;
+        mt0 = fmaxf(mt0, sc[j][e]);
+        mt1 = fmaxf(mt1, sc[j][2 + e]);
+      }
+    }
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      mt0 = fmaxf(mt0, __shfl_xor_sync(0xffffffffu, mt0, off));
+      mt1 = fmaxf(mt1, __shfl_xor_sync(0xffffffffu, mt1, off));
+    }
+    const float mn0 = fmaxf(m0, mt0), mn1 = fmaxf(m1, mt1);
+    const float al0 = mn0 == -INFINITY ? 1.f : exp2f(m0 - mn0);
+    const float al1 = mn1 == -INFINITY ? 1.f : exp2f(m1 - mn1);
+    m0 = mn0;
+    m1 = mn1;
+    float p[2][4], s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        p[j][e] = sc[j][e] == -INFINITY ? 0.f : exp2f(sc[j][e] - mn0);
+        p[j][2 + e] = sc[j][2 + e] == -INFINITY ? 0.f : exp2f(sc[j][2 + e] - mn1);
+        s0 += p[j][e];
+        s1 += p[j][2 + e];
+      }
+    }
+    if (poison & see0) s0 = NAN;
+    if (poison & see1) s1 = NAN;
+    l0 = l0 * al0 + s0;
+    l1 = l1 * al1 + s1;
+    if (__any_sync(0xffffffffu, al0 != 1.f || al1 != 1.f)) {
+#pragma unroll
+      for (int jd = 0; jd < DT; ++jd) {
+        o[jd][0] *= al0;
+        o[jd][1] *= al0;
+        o[jd][2] *= al1;
+        o[jd][3] *= al1;
+      }
+    }
+    // P as bf16 (the matrix instruction's operand type: off by at most 2^-8 relative, as much as
+    // the output's own rounding); its row sums l stay float32 sums of the unrounded values.
+    const unsigned pa0 = pack_bf16x2(p[0][0], p[0][1]), pa1 = pack_bf16x2(p[0][2], p[0][3]);
+    const unsigned pa2 = pack_bf16x2(p[1][0], p[1][1]), pa3 = pack_bf16x2(p[1][2], p[1][3]);
+#pragma unroll
+    for (int jd = 0; jd < DT; jd += 2) {
+      const int mi = lane >> 3, rr = (mi & 1) * 8 + (lane & 7), cc = jd + (mi >> 1);
+      unsigned b0, b1, b2, b3;
+      ldsm_x4_t(sv + rr * D * 2 + S::swz(rr, cc) * 16, b0, b1, b2, b3);
+      mma_bf16(o[jd], pa0, pa1, pa2, pa3, b0, b1);
+      mma_bf16(o[jd + 1], pa0, pa1, pa2, pa3, b2, b3);
+    }
+    __syncwarp();
+  }
+  cp_async_wait<0>();
+  __syncwarp();
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+  }
+  // The warps' results of the 16 rows in shared memory (each in its own ring), joined in warp order.
+  float* wacc = reinterpret_cast<float*>(wbase);
+  if (t4 == 0) {
+    wm_[warp][g8] = m0;
+    wl_[warp][g8] = l0;
+    wm_[warp][g8 + 8] = m1;
+    wl_[warp][g8 + 8] = l1;
+  }
+#pragma unroll
+  for (int jd = 0; jd < DT; ++jd) {
+    const int c0 = jd * 8 + 2 * t4;
+    *reinterpret_cast<float2*>(wacc + g8 * D + c0) = make_float2(o[jd][0], o[jd][1]);
+    *reinterpret_cast<float2*>(wacc + (g8 + 8) * D + c0) = make_float2(o[jd][2], o[jd][3]);
+  }
+  __syncthreads();
+  for (int x = tid; x < NQ * D; x += blockDim.x) {
+    const int r = x / D, d = x % D;
+    float mx = -INFINITY;
+    for (int w = 0; w < kTreeWarps; ++w) mx = fmaxf(mx, wm_[w][r]);
+    float l = 0.f, ov = 0.f;
+    for (int w = 0; w < kTreeWarps; ++w) {
+      const float f = wm_[w][r] == -INFINITY ? 0.f : exp2f(wm_[w][r] - mx);
+      l += wl_[w][r] * f;
+      ov += reinterpret_cast<const float*>(reinterpret_cast<unsigned char*>(smem4) +
+                                           (size_t)w * ST * S::STAGE_BYTES)[r * D + d] * f;
+    }
+    const size_t row = (size_t)ln * a.rf * T + row0 + r;
+    float* pp = tree_part(part, a, split, row);
+    if (d == 0) {
+      pp[0] = mx;
+      pp[1] = l;
+    }
+    pp[4 + d] = ov;
+  }
+}
+
+// ---------------------------------------------------------------- float32: CUDA cores, 32 query rows per CTA
+// Q, K and V tiles in shared memory (rows padded by one 16-byte chunk), every thread a 4 x 4 block of
+// the 32 x 64 scores and a 4 x (D / 16) block of O.
+constexpr int kF32Rows = 32, kF32TS = 64, kF32Threads = 128;
+
+template <int D>
+struct TreeF32Shape {
+  static constexpr int LD = D + 4, LDP = kF32TS + 4;
+  static constexpr size_t smem = sizeof(float) * (kF32Rows * LD + 2 * kF32TS * LD + kF32Rows * LDP + kF32TS + 2 * kF32Rows);
+};
+
+template <int D>
+__global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(TreeGeo a, logkv_prefix_t pre, const float* rk,
+                                                              const float* rv, float* part, int32_t* status) {
+  using S = TreeF32Shape<D>;
+  constexpr int LD = S::LD, LDP = S::LDP, TS = kF32TS, NR = kF32Rows, C4 = D / 4, DC = D / 16;
+  extern __shared__ uint4 smem4[];
+  __shared__ uint32_t masks[kTreeMaxTokens][kTreeWords];
+  __shared__ int up_[kTreeMaxTokens];
+  __shared__ int sh_poison[2];
+  float* sq = reinterpret_cast<float*>(smem4);
+  float* sk = sq + NR * LD;
+  float* sv = sk + TS * LD;
+  float* sp = sv + TS * LD;
+  float* sm = sp + NR * LDP;
+  float* rm = sm + TS;   // [NR] running maximum and sum
+  float* rl = rm + NR;
+  pdl_entry();
+  const int tid = threadIdx.x;
+  const int ln = blockIdx.x, split = blockIdx.y, row0 = blockIdx.z * NR, g = ln % a.G, b = ln / a.G;
+  const int T = a.T, NQ = min(NR, a.rf * T - row0);
+  const int Lp = prefix_length(pre, ln), R = a.rcount;
+  const int up = (Lp + TS - 1) / TS, ur = (R + TS - 1) / TS, uc = (T + TS - 1) / TS, U = up + ur + uc;
+  const int ns = tree_splits(a, U);
+  if (split >= ns) return;
+  const int u0 = (int)((long long)U * split / ns), u1 = (int)((long long)U * (split + 1) / ns);
+  if (u1 > up + ur) tree_masks(a, b, masks, up_, status);
+  for (int x = tid; x < NR * C4; x += kF32Threads) {
+    const int r = x / C4, c = x % C4, row = row0 + r;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < NQ)
+      v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + b * a.qs[0] +
+                                           (g * a.rf + row / T) * a.qs[1] + (row % T) * a.qs[2] + 4 * c);
+    *reinterpret_cast<float4*>(sq + r * LD + 4 * c) = v;
+  }
+  if (tid < NR) {
+    rm[tid] = -INFINITY;
+    rl[tid] = 0.f;
+  }
+  const int ty = tid >> 4, tx = tid & 15;   // rows 4 ty .. 4 ty + 3; keys tx + 16 j; columns 4 (tx + 16 j)
+  float o[4][DC < 4 ? 4 : DC];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < (DC < 4 ? 4 : DC); ++j) o[i][j] = 0.f;
+  const float* kn = static_cast<const float*>(a.kn) + b * a.ks[0] + g * a.ks[1];
+  const float* vn = static_cast<const float*>(a.vn) + b * a.vs[0] + g * a.vs[1];
+  for (int u = u0; u < u1; ++u) {
+    const int cls = u < up ? 0 : u < up + ur ? 1 : 2;
+    const int first = (cls == 0 ? u : cls == 1 ? u - up : u - up - ur) * TS;
+    const int rows = min(TS, (cls == 0 ? Lp : cls == 1 ? R : T) - first);
+    const size_t r0 = cls == 0 ? (size_t)ln * pre.capacity + first : (size_t)ln * a.rcap + first;
+    const float* kb = cls == 0 ? static_cast<const float*>(pre.k) + r0 * D : cls == 1 ? rk + r0 * D : kn + first * a.ks[2];
+    const float* vb = cls == 0 ? static_cast<const float*>(pre.v) + r0 * D : cls == 1 ? rv + r0 * D : vn + first * a.vs[2];
+    const long long kst = cls == 2 ? a.ks[2] : D, vst = cls == 2 ? a.vs[2] : D;
+    __syncthreads();   // the previous tile's K, V and P have been read
+    if (tid < 2) sh_poison[tid] = 0;
+    for (int x = tid; x < TS * C4; x += kF32Threads) {
+      const int r = x / C4, c = x % C4;
+      if (r < rows) {
+        cp_async16(sk + r * LD + 4 * c, kb + r * kst + 4 * c);
+        cp_async16(sv + r * LD + 4 * c, vb + r * vst + 4 * c);
+      } else {
+        *reinterpret_cast<float4*>(sk + r * LD + 4 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(sv + r * LD + 4 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    if (tid < TS) sm[tid] = cls == 0 && tid < rows ? pre.mass[r0 + tid] * a.mass_log2 : 0.f;
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
+    if (cls == 2) {   // drafted tokens whose V is not finite leave the product; their rows' sums become NaN
+      for (int x = tid; x < rows * D; x += kF32Threads) {
+        float* v = sv + x / D * LD + x % D;
+        if (!isfinite(*v)) {
+          *v = 0.f;
+          atomicOr(&sh_poison[x / D >> 5], 1 << (x / D & 31));
+        }
+      }
+      __syncthreads();
+    }
+    float s[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < C4; ++c) {
+      float4 x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(sq + (4 * ty + i) * LD + 4 * c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * LD + 4 * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
+          s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
+          s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
+          s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * ty + i, t = (row0 + min(r, NQ - 1)) % T;
+      float mt = -INFINITY;
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int col = tx + 16 * j;
+        bool see = col < rows;
+        if (cls == 2 && see) {
+          see = masks[t][(first + col) >> 5] >> ((first + col) & 31) & 1;
+          bad |= see && (sh_poison[col >> 5] >> (col & 31) & 1);
+        }
+        s[i][j] = see ? fmaf(s[i][j], a.scale_log2, sm[col]) : -INFINITY;
+        mt = fmaxf(mt, s[i][j]);
+      }
+#pragma unroll
+      for (int off = 1; off < 16; off <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, off));
+      const float mo = rm[r], mn = fmaxf(mo, mt);
+      const float al = mn == -INFINITY ? 1.f : exp2f(mo - mn);
+      float sum = bad ? NAN : 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p = s[i][j] == -INFINITY ? 0.f : exp2f(s[i][j] - mn);
+        sp[r * LDP + tx + 16 * j] = p;
+        sum += p;
+      }
+#pragma unroll
+      for (int off = 1; off < 16; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      __syncwarp();   // every lane of the row has read its running maximum
+      if (tx == 0) {
+        rm[r] = mn;
+        rl[r] = rl[r] * al + sum;
+      }
+      // The row's 16 threads also own its columns of O.
+#pragma unroll
+      for (int j = 0; j < (DC < 4 ? 4 : DC); ++j) o[i][j] *= al;
+    }
+    __syncwarp();   // P of rows 4 ty .. 4 ty + 3 is written and read by the same half warp
+#pragma unroll 4
+    for (int n = 0; n < TS; ++n) {
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = sp[(4 * ty + i) * LDP + n];
+#pragma unroll
+      for (int j = 0; j < (DC + 3) / 4; ++j) {
+        const int c = 4 * (tx + 16 * j);
+        if (c < D) {
+          const float4 v = *reinterpret_cast<const float4*>(sv + n * LD + c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            o[i][4 * j] = fmaf(p[i], v.x, o[i][4 * j]);
+            o[i][4 * j + 1] = fmaf(p[i], v.y, o[i][4 * j + 1]);
+            o[i][4 * j + 2] = fmaf(p[i], v.z, o[i][4 * j + 2]);
+            o[i][4 * j + 3] = fmaf(p[i], v.w, o[i][4 * j + 3]);
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 4 * ty + i;
+    if (r >= NQ) continue;
+    float* pp = tree_part(part, a, split, (size_t)ln * a.rf * T + row0 + r);
+    if (tx == 0) {
+      pp[0] = rm[r];
+      pp[1] = rl[r];
+    }
+#pragma unroll
+    for (int j = 0; j < (DC + 3) / 4; ++j) {
+      const int c = 4 * (tx + 16 * j);
+      if (c < D) *reinterpret_cast<float4*>(pp + 4 + c) = make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- combine
+// One warp per output row: the splits' partials weighted by 2^(m_s - max m), in split order.  TS: the
+// key tile of the kernel that wrote them.  Rows of absent tokens are zero.
+template <typename T, int D, int TS>
+__global__ void __launch_bounds__(256) tree_combine_kernel(TreeGeo a, logkv_prefix_t pre, const float* part, T* out) {
+  pdl_entry();
+  const int lane = threadIdx.x & 31;
+  const size_t row = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (row >= (size_t)a.B * a.H * a.T) return;
+  const int ln = (int)(row / ((size_t)a.rf * a.T)), b = ln / a.G;
+  const int units = (prefix_length(pre, ln) + TS - 1) / TS + (a.rcount + TS - 1) / TS + (a.T + TS - 1) / TS;
+  const int ns = tree_splits(a, units);
+  // Absent, or under an absent token: walk up the tree.
+  long long t = (long long)(row % a.T);
+  for (int i = 0; i < a.T && t >= 0; ++i) {
+    const size_t at = (size_t)b * a.pstride + t;
+    const long long p = a.wide ? static_cast<const long long*>(a.parents)[at]
+                               : (long long)static_cast<const int32_t*>(a.parents)[at];
+    t = p < -2 || p >= t ? -2 : p;
+  }
+  const size_t stride = (size_t)a.B * a.H * a.T * (D + 4);
+  const float* p0 = part + row * (D + 4);
+  float mx = -INFINITY;
+  for (int s = 0; s < ns; ++s) mx = fmaxf(mx, p0[s * stride]);
+  float l = 0.f;
+  constexpr int PER = (D + 127) / 128;
+  float4 o[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < ns; ++s) {
+    const float* pp = p0 + s * stride;
+    const float m = pp[0], w = m == -INFINITY ? 0.f : exp2f(m - mx);
+    l += pp[1] * w;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int c = 4 * (lane + 32 * k);
+      if (c < D) {
+        const float4 v = *reinterpret_cast<const float4*>(pp + 4 + c);
+        o[k].x += v.x * w;
+        o[k].y += v.y * w;
+        o[k].z += v.z * w;
+        o[k].w += v.w * w;
+      }
+    }
+  }
+  const bool gone = t == -2;
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int c = 4 * (lane + 32 * k);
+    if (c < D) {
+      T* dst = out + row * D + c;
+      Elem<T>::store(dst, gone ? 0.f : o[k].x * inv);
+      Elem<T>::store(dst + 1, gone ? 0.f : o[k].y * inv);
+      Elem<T>::store(dst + 2, gone ? 0.f : o[k].z * inv);
+      Elem<T>::store(dst + 3, gone ? 0.f : o[k].w * inv);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host side
+struct TreePlan {
+  int tile_rows, ts, nsplit, nsmin, upw;   // query rows per CTA, key tile, splits
+};
+
+// Splits: two CTAs per SM over all lanes and row tiles, at least a key tile per warp each.
+static TreePlan tree_plan(const logkv_layout_t& l, int heads, int tokens, int prefix_capacity) {
+  TreePlan p;
+  const bool f32 = l.dtype == LOGKV_DTYPE_F32;
+  p.tile_rows = f32 ? kF32Rows : 16;
+  p.ts = f32 ? kF32TS : 16;
+  p.upw = f32 ? 1 : kTreeWarps;
+  const long long rows = (long long)(heads / l.groups) * tokens, tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  const long long ctas = (long long)l.batch * l.groups * tiles;
+  const int units = (prefix_capacity + l.recent_capacity + tokens) / p.ts + 3;
+  p.nsmin = (int)std::max(1LL, 296 / ctas);
+  p.nsplit = std::max(1, std::min(p.nsmin, units / p.upw));
+  return p;
+}
+
+static bool tree_dim_ok(const logkv_layout_t& l) {
+  return l.dim == 16 || l.dim == 32 || l.dim == 64 || l.dim == 128 || (l.dim == 256 && l.dtype == LOGKV_DTYPE_BF16);
+}
+
+static int check_tree(const logkv_layout_t* l, int heads, int tokens) {
+  const int rc = check_layout(l);
+  if (rc) return rc;
+  if (heads < l->groups || heads % l->groups || tokens < 1 || tokens > kTreeMaxTokens || !tree_dim_ok(*l))
+    return LOGKV_E_SHAPE;
+  // Grid limits: row tiles along z.
+  if ((long long)(heads / l->groups) * tokens > 16LL * 65535) return LOGKV_E_SHAPE;
+  return LOGKV_OK;
+}
+
+template <typename T, int D, int TS>
+static void launch_tree_combine(const TreeGeo& a, const logkv_prefix_t& pre, const float* part, void* out,
+                                cudaStream_t st) {
+  const size_t rows = (size_t)a.B * a.H * a.T;
+  launch_pdl(tree_combine_kernel<T, D, TS>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, a, pre, part,
+             static_cast<T*>(out));
+}
+
+template <int D>
+static int launch_tree_bf16(const TreeGeo& a, const TreePlan& p, const logkv_prefix_t& pre, const logkv_state_t& s,
+                            const logkv_tree_args_t& x, float* part, cudaStream_t st) {
+  using S = TreeShape<D>;
+  using B16 = __nv_bfloat16;
+  auto kern = tree_mma_kernel<D>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
+  if (e != cudaSuccess) return (int)e;
+  const unsigned tiles = (unsigned)((a.rf * a.T + p.tile_rows - 1) / p.tile_rows);
+  launch_pdl(kern, dim3(a.B * a.G, p.nsplit, tiles), kTreeWarps * 32, S::smem, st, a, pre,
+             static_cast<const B16*>(s.recent_k), static_cast<const B16*>(s.recent_v), static_cast<B16*>(x.out), part,
+             x.status);
+  launch_tree_combine<B16, D, 16>(a, pre, part, x.out, st);
+  return launch_status();
+}
+
+template <int D>
+static int launch_tree_f32(const TreeGeo& a, const TreePlan& p, const logkv_prefix_t& pre, const logkv_state_t& s,
+                           const logkv_tree_args_t& x, float* part, cudaStream_t st) {
+  using S = TreeF32Shape<D>;
+  auto kern = tree_f32_kernel<D>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
+  if (e != cudaSuccess) return (int)e;
+  const unsigned tiles = (unsigned)((a.rf * a.T + p.tile_rows - 1) / p.tile_rows);
+  launch_pdl(kern, dim3(a.B * a.G, p.nsplit, tiles), kF32Threads, S::smem, st, a, pre,
+             static_cast<const float*>(s.recent_k), static_cast<const float*>(s.recent_v), part, x.status);
+  launch_tree_combine<float, D, kF32TS>(a, pre, part, x.out, st);
+  return launch_status();
+}
+
+}  // namespace logkv
+
+using namespace logkv;
+
+extern "C" {
+
+LOGKV_API size_t logkv_tree_attention_workspace_bytes(const logkv_layout_t* layout, int32_t heads, int32_t tokens,
+                                                      int32_t prefix_capacity) {
+  if (check_tree(layout, heads, tokens) || prefix_capacity < 0) return 0;
+  const TreePlan p = tree_plan(*layout, heads, tokens, prefix_capacity);
+  return (size_t)p.nsplit * layout->batch * heads * tokens * (layout->dim + 4) * sizeof(float);
+}
+
+LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_state_t* state,
+                                   const logkv_prefix_t* prefix, const logkv_tree_args_t* x, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  if (!layout || !state || !prefix || !x) return LOGKV_E_POINTER;
+  const int rc = check_tree(layout, x->heads, x->tokens);
+  if (rc) return rc;
+  if (x->recent_count < 0 || x->recent_count > layout->recent_capacity || prefix->capacity < 0) return LOGKV_E_SHAPE;
+  auto a16 = [](const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  if (!a16(x->q) || !a16(x->k_new) || !a16(x->v_new) || !a16(x->out) || !a16(workspace) || !a16(state->recent_k) ||
+      !a16(state->recent_v) || !a16(prefix->k) || !a16(prefix->v) || !prefix->mass || !prefix->length || !x->parents)
+    return LOGKV_E_POINTER;
+  const long long e = (long long)esize_of(layout->dtype);
+  TreeGeo a{};
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = x->q_strides[i];
+    a.ks[i] = x->k_strides[i];
+    a.vs[i] = x->v_strides[i];
+    if (a.qs[i] * e % 16 || a.ks[i] * e % 16 || a.vs[i] * e % 16) return LOGKV_E_POINTER;
+  }
+  if (workspace_bytes < logkv_tree_attention_workspace_bytes(layout, x->heads, x->tokens, prefix->capacity))
+    return LOGKV_E_WORKSPACE;
+  const TreePlan p = tree_plan(*layout, x->heads, x->tokens, prefix->capacity);
+  a.B = layout->batch;
+  a.G = layout->groups;
+  a.H = x->heads;
+  a.rf = a.H / a.G;
+  a.T = x->tokens;
+  a.D = layout->dim;
+  a.rcap = layout->recent_capacity;
+  a.rcount = x->recent_count;
+  a.nsplit = p.nsplit;
+  a.nsmin = p.nsmin;
+  a.upw = p.upw;
+  a.scale_log2 = x->scale * 1.4426950408889634f;
+  a.mass_log2 = x->qx * a.scale_log2;
+  a.q = x->q;
+  a.kn = x->k_new;
+  a.vn = x->v_new;
+  a.parents = x->parents;
+  a.pstride = x->parents_stride;
+  a.wide = x->parents_wide;
+  float* part = static_cast<float*>(workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (layout->dtype == LOGKV_DTYPE_BF16) {
+    switch (layout->dim) {
+      case 16: return launch_tree_bf16<16>(a, p, *prefix, *state, *x, part, st);
+      case 32: return launch_tree_bf16<32>(a, p, *prefix, *state, *x, part, st);
+      case 64: return launch_tree_bf16<64>(a, p, *prefix, *state, *x, part, st);
+      case 128: return launch_tree_bf16<128>(a, p, *prefix, *state, *x, part, st);
+      default: return launch_tree_bf16<256>(a, p, *prefix, *state, *x, part, st);
+    }
+  }
+  switch (layout->dim) {
+    case 16: return launch_tree_f32<16>(a, p, *prefix, *state, *x, part, st);
+    case 32: return launch_tree_f32<32>(a, p, *prefix, *state, *x, part, st);
+    case 64: return launch_tree_f32<64>(a, p, *prefix, *state, *x, part, st);
+    default: return launch_tree_f32<128>(a, p, *prefix, *state, *x, part, st);
+  }
+}
+
+}  // extern "C"

@@ -177,6 +177,33 @@ LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_sta
                                    const logkv_prefix_t* prefix, const logkv_tree_args_t* args, void* workspace,
                                    size_t workspace_bytes, void* stream);
 
+/*
+ * Beam search: batch row b of the cache becomes the old row index[b], in place (no reference
+ * counterpart).  index is [B] on the device, int32 or int64 (index_wide); any map is allowed (one row
+ * taken over by several, swaps, cycles).  An entry outside [0, B) leaves its row as it is and sets bit
+ * 19 of `status` (device int32, may be NULL).  Rows with index[b] = b are not touched.
+ *
+ * window_from = -1: the whole rows: ladder, clusters, exact pool, span bookkeeping, s_h, the window's
+ * rows [0, recent_count) and, when `prefix` is not NULL, the packed prefix.  K and V past a level's
+ * count (zero in every row), prefix rows past their length and window rows from recent_count on
+ * are not moved.
+ * window_from >= 0: only the window's rows [window_from, recent_count), for a caller whose rows b and
+ * index[b] hold the same ladder, pool and earlier window rows (hypotheses forked from one row since
+ * the last flush).  batch <= 2048.
+ */
+LOGKV_API int logkv_reorder_batch(const logkv_layout_t* layout, const logkv_state_t* state,
+                                  const logkv_prefix_t* prefix, int32_t recent_count, int32_t window_from,
+                                  const void* index, int32_t index_wide, int32_t* status, void* stream);
+
+/* The same for up to 40 contiguous [batch, ...] buffers of row_bytes bytes per row (a decoder's own
+ * per-row state). */
+typedef struct logkv_rows {
+  void* base;
+  int64_t row_bytes;
+} logkv_rows_t;
+LOGKV_API int logkv_reorder_rows(const logkv_rows_t* buffers, int32_t n, int32_t batch, const void* index,
+                                 int32_t index_wide, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

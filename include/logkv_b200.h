@@ -223,6 +223,19 @@ typedef struct logkv_chunk {
 } logkv_chunk_t;
 
 /*
+ * Append the accepted path of a tree of drafted tokens (no reference counterpart): committed row t of
+ * batch row b is the chunk's token path[b, t].  chunk->k, k_raw, v, positions and ends hold `tokens`
+ * drafted tokens per batch row ([B, G, tokens, D], [B, tokens]); chunk->n rows are appended (NULL
+ * positions: pos0 + t).  path is [B, n] on the device, int32 or int64 (path_wide), path_stride elements
+ * between batch rows (0: one path for all); an entry outside [0, tokens) takes token 0 and sets bit 19
+ * of `status` (device int32, may be NULL).  One kernel.
+ */
+LOGKV_API int logkv_window_append_path(const logkv_layout_t* layout, const logkv_state_t* state,
+                                       const logkv_chunk_t* chunk, int32_t tokens, const void* path,
+                                       int64_t path_stride, int32_t path_wide, int32_t recent_count,
+                                       int32_t* status, void* stream);
+
+/*
  * _semantic_add_recent of a chunk whose append overflows the window by exactly one flush of
  * the flush_tokens oldest rows (log_kv_cache.py:5668-5718 with one pass of the flush loop),
  * when those rows are all rows already in the window: recent_count (the fill before the

@@ -104,6 +104,11 @@ class TreeArgs(ctypes.Structure):
                 ("qx", ctypes.c_float), ("status", ctypes.c_void_p)]
 
 
+class Rows(ctypes.Structure):
+    """logkv_rows_t (include/logkv_attention.h)."""
+    _fields_ = [("base", ctypes.c_void_p), ("row_bytes", ctypes.c_int64)]
+
+
 TREE_MAX_TOKENS = 256   # LOGKV_TREE_MAX_TOKENS
 
 _lib = None
@@ -141,6 +146,10 @@ def lib() -> ctypes.CDLL:
         handle.logkv_window_append.argtypes = [P(Layout), P(State), ctypes.c_void_p, I64, ctypes.c_void_p, I64,
                                                ctypes.c_void_p, I64, ctypes.c_void_p, I64, ctypes.c_int64,
                                                ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
+        handle.logkv_window_append_path.restype = ctypes.c_int
+        handle.logkv_window_append_path.argtypes = [P(Layout), P(State), P(Chunk), ctypes.c_int32, ctypes.c_void_p,
+                                                    ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                                    ctypes.c_void_p]
         handle.logkv_flush_chunk.restype = ctypes.c_int
         handle.logkv_flush_chunk.argtypes = [P(Layout), P(State), ctypes.c_int32, ctypes.c_int32, P(Chunk),
                                              ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
@@ -199,6 +208,12 @@ def lib() -> ctypes.CDLL:
         handle.logkv_tree_attention.restype = ctypes.c_int
         handle.logkv_tree_attention.argtypes = [P(Layout), P(State), P(Prefix), P(TreeArgs), ctypes.c_void_p,
                                                 ctypes.c_size_t, ctypes.c_void_p]
+        handle.logkv_reorder_batch.restype = ctypes.c_int
+        handle.logkv_reorder_batch.argtypes = [P(Layout), P(State), P(Prefix), ctypes.c_int32, ctypes.c_int32,
+                                               ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]
+        handle.logkv_reorder_rows.restype = ctypes.c_int
+        handle.logkv_reorder_rows.argtypes = [P(Rows), ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                              ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]
         _lib = handle
     return _lib
 

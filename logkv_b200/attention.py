@@ -327,7 +327,7 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
     Returns [B, H, T, D]; ``out`` may be given.  The scratch is allocated per call, so calls on
     different streams, or captured graphs, never share it.  Forward-only.
 
-    After verification the accepted path is committed with ``cache.add_recent``.
+    After verification ``cache.add_recent_path`` commits the accepted path.
     """
     if q.dim() != 4:
         raise ValueError(f"q must be [B, H, T, D], got {tuple(q.shape)}")

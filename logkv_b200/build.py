@@ -4,6 +4,7 @@ Translation units with different numerics:
   flush.cu      -fmad=false: every float expression of the flush is rounded
                  exactly as written (bit-exact with the reference's CPU path);
   attention.cu, tree_attention.cu  default contraction (FMA) for the attention math;
+  reorder.cu    moves rows, no arithmetic;
   plugin.cu, unified.cu  -fmad=false: the operator-level plugin functions, same contract as flush.cu.
 Run ``python -m logkv_b200.build`` (or ``__graft_entry__.build()``).
 """
@@ -26,6 +27,7 @@ UNITS = [
     ("flush.cu", ["-fmad=false"]),
     ("attention.cu", []),
     ("tree_attention.cu", []),
+    ("reorder.cu", []),
     ("plugin.cu", ["-fmad=false"]),
     ("unified.cu", ["-fmad=false"]),
 ]

@@ -261,6 +261,7 @@ class LogStructuredKVCache(nn.Module):
         self._route_ready_capture = 0
         self._route_done = None
         self._deferred_take = None   # flush started by add_recent_deferred, committed by commit_deferred
+        self._read = None            # read side: plan, packed prefix (logkv_b200.attention)
 
     # ------------------------------------------------------------------ C-ABI state
     def _apply(self, fn, *args, **kwargs):
@@ -562,6 +563,70 @@ class LogStructuredKVCache(nn.Module):
             return
         self._append_window(*chunk)
         self.recent_count += chunk[-1]
+        self._run_flushes(record_op_log, replaying)
+
+    def add_recent_path(self, k, v, path, *, k_raw, input_pos=None, span_ends=None, span_ends_device=None,
+                        record_op_log=False) -> None:
+        """Commit the accepted path of a tree of drafted tokens: add_recent of the drafted rows that
+        ``path`` names, gathered by the window write itself (no reference counterpart).
+
+        k, v, k_raw [B, G, T, D], input_pos ([T] or [B, T]) and the span-end flags ([B][T] host rows, or
+        ``span_ends_device`` uint8 [B, T]) are those of the T drafted tokens; ``path`` ([n], or [B, n];
+        int32 or int64, on the device or a host list) lists the n accepted tokens from the root down.
+        Every batch row commits n tokens, since the window's fill is one number: with different
+        accepted lengths commit the shortest and draft the rest again.  A bad device value commits token
+        0 and sets bit 19 of the read status (when the cache has been attended over).  Without input_pos the positions continue the sequence.
+        """
+        if self._deferred_take is not None:
+            raise RuntimeError("commit_deferred must follow add_recent_deferred")
+        dev = self.recent_k.device
+        shape = (self.batch_size, self.n_groups)
+        for name, t in (("k", k), ("v", v), ("k_raw", k_raw)):
+            if t is None or t.dim() != 4 or t.shape[:2] != shape or t.shape != (*shape, k.size(2), self.k_dim):
+                raise ValueError(f"{name} must be [{shape[0]}, {shape[1]}, T, {self.k_dim}]")
+        T = k.size(2)
+        p = path if isinstance(path, torch.Tensor) else torch.as_tensor(path)
+        if p.dtype not in (torch.int32, torch.int64) and p.numel():
+            raise ValueError(f"path must hold integers (int32 or int64), got {p.dtype}")
+        if p.dim() not in (1, 2) or (p.dim() == 2 and p.size(0) != self.batch_size):
+            raise ValueError(f"path must be [n] or [{self.batch_size}, n], got {tuple(p.shape)}")
+        n = p.size(-1)
+        if n == 0:
+            return
+        if p.device.type == "cpu":
+            if bool(((p < 0) | (p >= T)).any()):
+                raise ValueError(f"path entries must be drafted tokens in [0, {T})")
+            p = p.to(dev)
+        elif p.device != dev:
+            raise ValueError(f"path must be on {dev}, got {p.device}")
+        p = p if p.stride(-1) == 1 else p.contiguous()
+        if span_ends_device is not None:
+            if tuple(span_ends_device.shape) != (self.batch_size, T):
+                raise ValueError("AlphaLogKV span boundaries must match the input batch and token count")
+            ends = span_ends_device.to(device=dev, dtype=torch.uint8).contiguous()
+        elif span_ends is None or len(span_ends) != self.batch_size or any(len(r) != T for r in span_ends):
+            raise ValueError("AlphaLogKV span boundaries must match the input batch and token count")
+        else:
+            ends = torch.tensor(span_ends, dtype=torch.uint8).to(dev)
+        positions = self._positions(T, input_pos)
+        self._check_room(n)
+        from .attention import _rows16
+        with torch.cuda.device(dev):
+            k, k_raw, v = (_rows16(t.to(device=dev, dtype=self.recent_k.dtype)) for t in (k, k_raw, v))
+            self.token_count += n
+            c, keep = self._chunk_struct(k, k_raw, v, positions, ends, n)
+            state = self._state_struct()
+            status = self._read.status.data_ptr() if self._read is not None else None
+            _lib.check(_lib.lib().logkv_window_append_path(
+                ctypes.byref(self._layout), ctypes.byref(state), ctypes.byref(c), T, p.data_ptr(),
+                p.stride(0) if p.dim() == 2 else 0, int(p.dtype == torch.int64), int(self.recent_count), status,
+                ctypes.c_void_p(_lib.stream_ptr(dev))), "logkv_window_append_path")
+            del keep
+            self.recent_count += n
+            self._run_flushes(record_op_log, False)
+
+    def _run_flushes(self, record_op_log: bool, replaying: bool) -> None:
+        """The flushes that the window's overflow needs, after an append."""
         for take in self._pending_flushes():
             if self._active_updates is None and replaying:
                 # As the reference's Alpha flush (log_kv_cache.py:5060-5061): an op-log alone cannot
@@ -664,12 +729,7 @@ class LogStructuredKVCache(nn.Module):
         if span_ends is None or len(span_ends) != self.batch_size or any(len(r) != n for r in span_ends):
             raise ValueError("AlphaLogKV span boundaries must match the input batch and token count")
         positions = self._positions(n, input_pos)
-        if self.token_count + n > self.max_seq_length:
-            raise RuntimeError(f"LogStructuredKVCache: token overflow! token_count={self.token_count}, n={n}, "
-                               f"max_seq_length={self.max_seq_length}.")
-        if self.recent_count + n > self.recent_capacity:
-            raise RuntimeError(f"semantic LogKV recent buffer overflow: recent_count={self.recent_count}, n={n}, "
-                               f"capacity={self.recent_capacity}")
+        self._check_room(n)
         self.token_count += n
         if span_ends_device is not None:
             ends = span_ends_device.to(device=self.recent_pos.device, dtype=torch.uint8).contiguous()
@@ -678,6 +738,16 @@ class LogStructuredKVCache(nn.Module):
             ends = self._ends_stage[:self.batch_size * n].view(self.batch_size, n)
             ends.copy_(host.pin_memory() if self.recent_pos.is_cuda else host, non_blocking=True)
         return k, k_raw, v, positions, ends, n
+
+    def _check_room(self, n: int) -> None:
+        if n > self.recent_size:
+            raise ValueError(f"chunk size {n} exceeds recent_size {self.recent_size}")
+        if self.token_count + n > self.max_seq_length:
+            raise RuntimeError(f"LogStructuredKVCache: token overflow! token_count={self.token_count}, n={n}, "
+                               f"max_seq_length={self.max_seq_length}.")
+        if self.recent_count + n > self.recent_capacity:
+            raise RuntimeError(f"semantic LogKV recent buffer overflow: recent_count={self.recent_count}, n={n}, "
+                               f"capacity={self.recent_capacity}")
 
     def _pending_flushes(self):
         """Sizes of the flushes the window overflow needs (_semantic_add_recent :5708-5718)."""
@@ -740,6 +810,58 @@ class LogStructuredKVCache(nn.Module):
             c.pos_strides if c.positions else None, c.pos0, ctypes.c_void_p(c.ends), c.n, int(self.recent_count),
             ctypes.c_void_p(_lib.stream_ptr(self.recent_k.device))), "logkv_window_append")
         del keep
+
+    # ------------------------------------------------------------------ hypotheses
+    def _row_index(self, index):
+        """[batch] row indices as an integer tensor on the cache's device; host values are checked."""
+        dev = self.level_k.device
+        t = index if isinstance(index, torch.Tensor) else torch.as_tensor(index)
+        if t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"row indices must be integers (int32 or int64), got {t.dtype}")
+        if tuple(t.shape) != (self.batch_size,):
+            raise ValueError(f"row indices must be [{self.batch_size}], got {tuple(t.shape)}")
+        if t.device.type == "cpu":
+            if bool(((t < 0) | (t >= self.batch_size)).any()):
+                raise ValueError(f"row indices must be in [0, {self.batch_size})")
+            t = t.to(dev)
+        elif t.device != dev:
+            raise ValueError(f"row indices must be on {dev}, got {t.device}")
+        return t.contiguous()
+
+    def reorder_batch(self, index, *, window_from=None) -> None:
+        """Beam search: batch row b takes over the old row index[b], in place (no reference counterpart).
+
+        ``index`` ([B], int32 or int64; on the device or a host list) may name a row several times, swap
+        rows and move them in cycles; a bad device value leaves its row as it is and sets bit 19 of the
+        read status.  The ladder, clusters, exact pool, window and packed prefix move; rows that stay are
+        not touched.  ``window_from``: move only the window's rows [window_from, recent_count), when row b
+        and row index[b] are known to agree in everything else (beams forked from one row, no flush
+        since).  Not while an update tape or an op-log is bound or a deferred flush is open: their
+        records name rows.
+        """
+        if self._active_updates is not None:
+            raise RuntimeError("reorder_batch is not recorded by update tapes")
+        if self.op_log is not None:
+            raise RuntimeError("reorder_batch cannot reorder the rows of a bound op-log")
+        if self._deferred_take is not None:
+            raise RuntimeError("commit_deferred must follow add_recent_deferred")
+        if window_from is not None and not 0 <= window_from <= self.recent_count:
+            raise ValueError(f"window_from must be in [0, recent_count={self.recent_count}], got {window_from}")
+        index = self._row_index(index)
+        from .attention import _read_state
+        dev = self.level_k.device
+        with torch.cuda.device(dev):
+            # The prefix moves whether or not it is current, so that a captured call does not depend on
+            # what was current when it was captured; its buffers therefore exist from here on.
+            if self._read is None and _lib.capture_id(dev):
+                raise RuntimeError("capture reorder_batch only after the cache has been attended over once")
+            rs = _read_state(self)
+            state, pre = self._state_struct(), rs.prefix_struct()
+            _lib.check(_lib.lib().logkv_reorder_batch(
+                ctypes.byref(self._layout), ctypes.byref(state), ctypes.byref(pre), int(self.recent_count),
+                -1 if window_from is None else int(window_from), index.data_ptr(), int(index.dtype == torch.int64),
+                rs.status.data_ptr(), ctypes.c_void_p(_lib.stream_ptr(dev))), "logkv_reorder_batch")
+        self._route_ready = None     # the next flush's decisions must wait for the moved rows
 
     # ------------------------------------------------------------------ read side
     def _semantic_attention_plan(self):

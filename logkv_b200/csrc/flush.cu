@@ -270,7 +270,24 @@ struct AppendArgs {
   long long pos0;
   const uint8_t* ends;              // [B, n] contiguous
   int n, recent_count;
+  // logkv_window_append_path: row t is the chunk's row path[b, t] of `tokens` (also of pos and ends).
+  const void* path;
+  long long path_stride;
+  int path_wide, tokens;
+  int32_t* status;
 };
+
+constexpr int32_t kStatusBadPath = 1 << 19;
+
+// Chunk row of committed row t: path[b, t], or row 0 (and the status bit) where that is no chunk row.
+__device__ __forceinline__ int path_row(const AppendArgs& a, int b, int t) {
+  const size_t at = (size_t)b * a.path_stride + t;
+  const long long p = a.path_wide ? static_cast<const long long*>(a.path)[at]
+                                  : (long long)static_cast<const int32_t*>(a.path)[at];
+  if (p >= 0 && p < a.tokens) return (int)p;
+  set_status(a.status, kStatusBadPath);
+  return 0;
+}
 
 // Chunk row t, 16-byte unit v of lane (b, grp) into window row `row` (K, pre-RoPE K, V).
 template <typename T>
@@ -286,7 +303,7 @@ __device__ __forceinline__ void put_chunk_unit(const Geo& g, const logkv_state_t
   *reinterpret_cast<uint4*>(static_cast<T*>(s.recent_v) + d) = *reinterpret_cast<const uint4*>(sv);
 }
 
-template <typename T>
+template <typename T, bool PATH>
 __global__ void window_append_kernel(Geo g, logkv_state_t s, AppendArgs a) {
   pdl_entry();
   constexpr int VN = Vec<T>::N;
@@ -294,13 +311,14 @@ __global__ void window_append_kernel(Geo g, logkv_state_t s, AppendArgs a) {
   const int units = a.n * DV;   // <= 8192 rows x 256 units
   for (int u = blockIdx.x * blockDim.x + threadIdx.x; u < units; u += gridDim.x * blockDim.x) {
     const int t = u / DV;
-    put_chunk_unit<T>(g, s, a, b, grp, t, u - t * DV, a.recent_count + t);
+    put_chunk_unit<T>(g, s, a, b, grp, PATH ? path_row(a, b, t) : t, u - t * DV, a.recent_count + t);
   }
   if (grp == 0 && blockIdx.x == 0)
     for (int t = threadIdx.x; t < a.n; t += blockDim.x) {
       const size_t r = (size_t)b * g.cap2R + a.recent_count + t;
-      s.recent_pos[r] = a.pos ? a.pos[b * a.ps[0] + t * a.ps[1]] : a.pos0 + t;
-      s.recent_ends[r] = a.ends[(size_t)b * a.n + t];
+      const int c = PATH ? path_row(a, b, t) : t;
+      s.recent_pos[r] = a.pos ? a.pos[b * a.ps[0] + c * a.ps[1]] : a.pos0 + t;
+      s.recent_ends[r] = a.ends[(size_t)b * (PATH ? a.tokens : a.n) + c];
     }
 }
 
@@ -932,9 +950,38 @@ extern "C" int logkv_window_append(const logkv_layout_t* layout, const logkv_sta
   const int per = std::max(1, std::min(64, (int)(((size_t)n * g.D / (16 / esize) + 255) / 256)));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (layout->dtype == LOGKV_DTYPE_BF16)
-    launch_pdl(window_append_kernel<__nv_bfloat16>, dim3(per, g.G, g.B), 256, 0, st, g, *state, a);
+    launch_pdl(window_append_kernel<__nv_bfloat16, false>, dim3(per, g.G, g.B), 256, 0, st, g, *state, a);
   else
-    launch_pdl(window_append_kernel<float>, dim3(per, g.G, g.B), 256, 0, st, g, *state, a);
+    launch_pdl(window_append_kernel<float, false>, dim3(per, g.G, g.B), 256, 0, st, g, *state, a);
+  return (int)cudaGetLastError();
+}
+
+extern "C" int logkv_window_append_path(const logkv_layout_t* layout, const logkv_state_t* state,
+                                        const logkv_chunk_t* chunk, int32_t tokens, const void* path,
+                                        int64_t path_stride, int32_t path_wide, int32_t recent_count, int32_t* status,
+                                        void* stream) {
+  const int val = validate(layout, 1);
+  if (val != LOGKV_OK) return val;
+  if (!chunk || !path) return LOGKV_E_POINTER;
+  if (tokens < 1) return LOGKV_E_SHAPE;
+  AppendArgs a{};
+  const int rc = make_append(layout, state, chunk->k, chunk->k_strides, chunk->k_raw, chunk->k_raw_strides, chunk->v,
+                             chunk->v_strides, chunk->positions, chunk->pos_strides, chunk->pos0, chunk->ends, chunk->n,
+                             recent_count, &a);
+  if (rc != LOGKV_OK) return rc;
+  a.path = path;
+  a.path_stride = path_stride;
+  a.path_wide = path_wide;
+  a.tokens = tokens;
+  a.status = status;
+  const size_t esize = layout->dtype == LOGKV_DTYPE_BF16 ? 2 : 4;
+  const Geo g = make_geo(*layout, 1, recent_count);
+  const int per = std::max(1, std::min(64, (int)(((size_t)a.n * g.D / (16 / esize) + 255) / 256)));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (layout->dtype == LOGKV_DTYPE_BF16)
+    launch_pdl(window_append_kernel<__nv_bfloat16, true>, dim3(per, g.G, g.B), 256, 0, st, g, *state, a);
+  else
+    launch_pdl(window_append_kernel<float, true>, dim3(per, g.G, g.B), 256, 0, st, g, *state, a);
   return (int)cudaGetLastError();
 }
 

@@ -79,3 +79,69 @@ def test_tree_c_abi_checks(lib):
     assert call(args, 1 << 30) == -1
     args.recent_count, args.heads = 0, 15
     assert call(args, 1 << 30) == -1
+
+
+def test_reorder_refusals(cache):
+    for index, match in [([0], "row indices must be"), ([[0, 1]], "row indices must be"), ([0.0, 1.0], "integers"),
+                         ([0, 2], "in \\[0, 2\\)"), ([-1, 0], "in \\[0, 2\\)"),
+                         (torch.tensor([0, 1], dtype=torch.uint8), "integers")]:
+        with pytest.raises(ValueError, match=match):
+            cache.reorder_batch(index)
+    for w in (-1, 6):
+        with pytest.raises(ValueError, match="window_from"):
+            cache.reorder_batch([0, 1], window_from=w)
+    from logkv_b200 import _SemanticReplayUpdates
+    with cache._semantic_update_context(_SemanticReplayUpdates()):
+        with pytest.raises(RuntimeError, match="update tapes"):
+            cache.reorder_batch([0, 1])
+    cache._deferred_take = 4
+    with pytest.raises(RuntimeError, match="commit_deferred"):
+        cache.reorder_batch([0, 1])
+    k = torch.zeros(2, 2, 3, 64)
+    with pytest.raises(RuntimeError, match="commit_deferred"):
+        cache.add_recent_path(k, k, [0], k_raw=k, span_ends=[[0, 0, 0]] * 2)
+
+
+def test_path_refusals(cache):
+    k = torch.zeros(2, 2, 3, 64)
+    ends = [[False] * 3] * 2
+    f = lambda *a, **kw: cache.add_recent_path(*a, **{"k_raw": k, "span_ends": ends, **kw})  # noqa: E731
+    for args, kw, match in [((k[:1], k, [0]), {}, "k must be"), ((k, k[:, :, :2], [0]), {}, "v must be"),
+                            ((k, k, [0]), {"k_raw": k[..., :32]}, "k_raw must be"), ((k, k, [0.5]), {}, "integers"),
+                            ((k, k, [[0]]), {}, "path must be"), ((k, k, torch.zeros(1, 2, 1).long()), {}, "path must be"),
+                            ((k, k, [3]), {}, "path entries"), ((k, k, [-1]), {}, "path entries"),
+                            ((k, k, [0]), {"span_ends": None}, "boundaries"), ((k, k, [0]), {"span_ends": ends[:1]}, "boundaries"),
+                            ((k, k, [0]), {"span_ends_device": torch.zeros(2, 1)}, "boundaries"),
+                            ((k, k, [0]), {"input_pos": torch.zeros(2)}, "input_pos length"),
+                            ((k, k, [0] * 257), {}, "exceeds recent_size")]:
+        with pytest.raises(ValueError, match=match):
+            f(*args, **kw)
+    before = cache.recent_count
+    f(k, k, [])
+    assert cache.recent_count == before
+    cache.token_count = cache.max_seq_length
+    with pytest.raises(RuntimeError, match="token overflow"):
+        f(k, k, [0])
+
+
+def test_reorder_c_abi_checks(lib):
+    from logkv_b200 import _lib
+    layout = _lib.Layout(4, 8, 128, 12, 7, 125, 4096, 256, 64, 1, 1, 1.0, 2048.0, 1.0)
+    state = _lib.State(**{n: 1 << 20 for n in _lib.STATE_FIELDS})
+    call = lambda lay, st, rc, w, idx: lib.logkv_reorder_batch(  # noqa: E731
+        ctypes.byref(lay), ctypes.byref(st), None, rc, w, idx, 1, None, None)
+    assert call(layout, state, 10, -1, None) == -4
+    assert call(layout, _lib.State(), 10, -1, 1 << 20) == -4
+    assert call(layout, state, 4097, -1, 1 << 20) == -1 and call(layout, state, 10, 11, 1 << 20) == -1
+    assert call(layout, state, 10, -2, 1 << 20) == -1
+    big = _lib.Layout(4096, 8, 128, 12, 7, 125, 4096, 256, 64, 1, 1, 1.0, 2048.0, 1.0)
+    assert call(big, state, 10, -1, 1 << 20) == -1
+    rows = (_lib.Rows * 2)(_lib.Rows(None, 8), _lib.Rows(1 << 20, 8))
+    assert lib.logkv_reorder_rows(rows, 2, 4, 1 << 20, 1, None, None) == -4
+    assert lib.logkv_reorder_rows(rows, 41, 4, 1 << 20, 1, None, None) == -1
+    assert lib.logkv_reorder_rows(None, 1, 4, 1 << 20, 1, None, None) == -4
+    chunk = _lib.Chunk()
+    assert lib.logkv_window_append_path(ctypes.byref(layout), ctypes.byref(state), ctypes.byref(chunk), 4, None, 0, 1,
+                                        0, None, None) == -4
+    assert lib.logkv_window_append_path(ctypes.byref(layout), ctypes.byref(state), ctypes.byref(chunk), 0, 1 << 20, 0,
+                                        1, 0, None, None) == -1

@@ -109,6 +109,15 @@ class Rows(ctypes.Structure):
     _fields_ = [("base", ctypes.c_void_p), ("row_bytes", ctypes.c_int64)]
 
 
+class BeamArgs(ctypes.Structure):
+    """logkv_beam_args_t (include/logkv_beam.h)."""
+    _fields_ = [("logits", ctypes.c_void_p), ("scores", ctypes.c_void_p), ("out_scores", ctypes.c_void_p),
+                ("out_rows", ctypes.c_void_p), ("out_tokens", ctypes.c_void_p), ("n_stride", ctypes.c_int64),
+                ("w_stride", ctypes.c_int64), ("dtype", ctypes.c_int32), ("requests", ctypes.c_int32),
+                ("width", ctypes.c_int32), ("vocab", ctypes.c_int32), ("k", ctypes.c_int32),
+                ("keep_places", ctypes.c_int32)]
+
+
 TREE_MAX_TOKENS = 256   # LOGKV_TREE_MAX_TOKENS
 
 _lib = None
@@ -214,6 +223,10 @@ def lib() -> ctypes.CDLL:
         handle.logkv_reorder_rows.restype = ctypes.c_int
         handle.logkv_reorder_rows.argtypes = [P(Rows), ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
                                               ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]
+        handle.logkv_beam_workspace_bytes.restype = ctypes.c_size_t
+        handle.logkv_beam_workspace_bytes.argtypes = [ctypes.c_int32] * 4
+        handle.logkv_beam_select.restype = ctypes.c_int
+        handle.logkv_beam_select.argtypes = [P(BeamArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         _lib = handle
     return _lib
 

@@ -5,6 +5,7 @@ Translation units with different numerics:
                  exactly as written (bit-exact with the reference's CPU path);
   attention.cu, tree_attention.cu  default contraction (FMA) for the attention math;
   reorder.cu    moves rows, no arithmetic;
+  beam.cu       default contraction (its float64 scores decide);
   plugin.cu, unified.cu  -fmad=false: the operator-level plugin functions, same contract as flush.cu.
 Run ``python -m logkv_b200.build`` (or ``__graft_entry__.build()``).
 """
@@ -28,6 +29,7 @@ UNITS = [
     ("attention.cu", []),
     ("tree_attention.cu", []),
     ("reorder.cu", []),
+    ("beam.cu", []),
     ("plugin.cu", ["-fmad=false"]),
     ("unified.cu", ["-fmad=false"]),
 ]

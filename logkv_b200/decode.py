@@ -6,12 +6,20 @@ the next token's single query attends over the cache plus [pending, itself] (``c
 and the pair is committed with ``add_recent``, which flushes ``semantic_flush_granularity``
 tokens when the window overflows (the first pair after a full window does).  ``LogKVDecoder``
 keeps the pending token in preallocated two-token buffers, so a step allocates nothing.
+
+``LogKVBeams`` runs beam search over such decoders, one per layer: it selects every step's
+continuations and lets the rows of the beams that go on be taken over, in the decoders and their
+caches.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
+from . import _lib
 from .attention import log_kv_chunk_attention
+from .beam import beam_select
 
 
 class LogKVDecoder:
@@ -33,6 +41,26 @@ class LogKVDecoder:
     def reset(self) -> None:
         """Forget the pending token (the reference clears it with the cache, model.py:1180-1182)."""
         self.pending = False
+
+    def reorder(self, index, *, window_from=None) -> None:
+        """Row b takes over the old row index[b]: the cache's rows (``LogStructuredKVCache.reorder_batch``,
+        same arguments) and the pending token's.  A pending token's span-end flags must be on the device
+        (``span_ends_device``): host lists cannot follow a device index."""
+        if self.pending and self._ends_host is not None:
+            raise RuntimeError("reordering a pending token needs its span-end flags on the device (span_ends_device)")
+        cache = self.cache
+        index = cache._row_index(index)
+        cache.reorder_batch(index, window_from=window_from)
+        if not self.pending:
+            return
+        bufs = (self._k, self._v, self._kr, self._pos, self._ends)
+        rows = (_lib.Rows * len(bufs))(*[_lib.Rows(t.data_ptr(), t.numel() * t.element_size() // cache.batch_size)
+                                         for t in bufs])
+        dev = self._k.device
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().logkv_reorder_rows(
+                rows, len(bufs), cache.batch_size, index.data_ptr(), int(index.dtype == torch.int64),
+                cache._read.status.data_ptr(), ctypes.c_void_p(_lib.stream_ptr(dev))), "logkv_reorder_rows")
 
     def step(self, q, k, v, *, k_raw, input_pos=None, span_ends=None, span_ends_device=None, out=None):
         """One token: q [B, H, 1, D], k / v / k_raw [B, G, 1, D]; returns the attention output
@@ -68,3 +96,52 @@ class LogKVDecoder:
                               span_ends=ends, span_ends_device=self._ends if span_ends_device is not None else None)
         self.pending = False
         return y
+
+
+class LogKVBeams:
+    """Beam search over ``decoders`` (one LogKVDecoder per layer) whose batch rows are `requests` x
+    `beams`, a request's beams next to each other.
+
+    After the prompt, ``fork()`` gives every beam its request's first row; then each step is the
+    decoders' ``step`` for the beams' last tokens, the model's logits, and ``advance``.
+    """
+
+    def __init__(self, decoders, requests: int, beams: int):
+        self.decoders = list(decoders)
+        if not self.decoders or requests < 1 or beams < 1:
+            raise ValueError("at least one decoder, request and beam")
+        for d in self.decoders:
+            if d.cache.batch_size != requests * beams:
+                raise ValueError(f"a decoder's cache has {d.cache.batch_size} rows, not {requests} x {beams}")
+        self.requests, self.beams = int(requests), int(beams)
+        dev = self.decoders[0].cache.level_k.device
+        self.scores = torch.full((self.requests, self.beams), float("-inf"), dtype=torch.float32, device=dev)
+        self.scores[:, 0] = 0.0
+        self._forked = None
+
+    def fork(self) -> None:
+        """Every beam takes over its request's first row; the scores start again (only that beam alive)."""
+        dev = self.scores.device
+        first = torch.arange(self.requests, device=dev).mul_(self.beams).repeat_interleave(self.beams)
+        for d in self.decoders:
+            d.reorder(first)
+        self.scores.fill_(float("-inf"))
+        self.scores[:, 0] = 0.0
+        # Until a cache's next flush its rows of one request differ in the window behind this fill only.
+        self._forked = [(d.cache._flush_cursor, d.cache.recent_count) for d in self.decoders]
+
+    def advance(self, logits):
+        """Select the next tokens from the logits [requests, beams, V] (or [requests * beams, V]) of the
+        beams' last tokens and let the rows follow.  Returns (tokens, rows), each [requests * beams]:
+        the token of every row and the old row it continues; ``scores`` holds their scores.  The best
+        continuation of a beam stays in the beam's row, so rows are in no order of score."""
+        if logits.dim() == 2:
+            logits = logits.view(self.requests, self.beams, -1)
+        if logits.shape[:2] != (self.requests, self.beams):
+            raise ValueError(f"logits must be [{self.requests}, {self.beams}, V], got {tuple(logits.shape)}")
+        self.scores, rows, tokens = beam_select(logits, self.scores, self.beams, keep_places=True)
+        rows = rows.view(-1)
+        for i, d in enumerate(self.decoders):
+            forked = self._forked[i] if self._forked else (None, 0)
+            d.reorder(rows, window_from=forked[1] if forked[0] == d.cache._flush_cursor else None)
+        return tokens.view(-1), rows

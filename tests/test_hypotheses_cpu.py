@@ -145,3 +145,38 @@ def test_reorder_c_abi_checks(lib):
                                         0, None, None) == -4
     assert lib.logkv_window_append_path(ctypes.byref(layout), ctypes.byref(state), ctypes.byref(chunk), 0, 1 << 20, 0,
                                         1, 0, None, None) == -1
+
+
+def test_beam_refusals(lib):
+    from logkv_b200 import beam_select
+    x, r = torch.zeros(2, 3, 10), torch.zeros(2, 3)
+    for args, kw, match in [((x[0], r, 1), {}, "logits must be"), ((x.double(), r, 1), {}, "not supported"),
+                            ((x, r[:1], 1), {}, "scores must be"), ((x, r.double(), 1), {}, "scores must be"),
+                            ((x, r, 0), {}, "k must be"), ((x, r, 31), {}, "k must be"),
+                            ((torch.zeros(1, 1, 500), torch.zeros(1, 1), 129), {}, "k must be"),
+                            ((x, r, 2), {"keep_places": True}, "keep_places"),
+                            ((torch.zeros(1, 257, 2), torch.zeros(1, 257), 2), {}, "supported range"),
+                            ((x[:, :, :0], r, 1), {}, "k must be"), ((x, r, 3), {}, "CUDA")]:
+        with pytest.raises(ValueError, match=match):
+            beam_select(*args, **kw)
+
+
+def test_beam_c_abi_checks(lib):
+    from logkv_b200 import _lib
+    size = lib.logkv_beam_workspace_bytes
+    assert size(2, 4, 32000, 8) > 0 and size(1, 1, 1, 1) > 0
+    for bad in [(0, 4, 10, 1), (1, 0, 10, 1), (1, 257, 10, 1), (1, 1, 0, 1), (1, 1, 4, 5), (1, 4, 1000, 129),
+                (1, 4, 1000, 0), (16384, 4, 10, 1), (1, 4, 1 << 29, 1)]:
+        assert size(*bad) == 0, bad
+    a = _lib.BeamArgs()
+    call = lambda n: lib.logkv_beam_select(ctypes.byref(a), 1 << 20, n, None)  # noqa: E731
+    assert lib.logkv_beam_select(None, None, 0, None) == -4
+    assert call(1 << 30) == -1
+    a.requests, a.width, a.vocab, a.k = 2, 4, 100, 8
+    assert call(1 << 30) == -4
+    a.logits = a.scores = a.out_scores = a.out_rows = a.out_tokens = 1 << 20
+    assert call(16) == -3
+    a.keep_places = 1
+    assert call(1 << 30) == -1
+    a.keep_places, a.dtype = 0, 7
+    assert call(1 << 30) == -2

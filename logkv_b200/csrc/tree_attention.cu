@@ -6,6 +6,7 @@
 // maximum and sum of its rows' softmax in float32 and leaves (m, l, O) per row, which
 // tree_combine_kernel joins in split order.
 #include <algorithm>
+#include <cstring>
 
 #include "attn_common.cuh"
 
@@ -354,6 +355,374 @@ __global__ void __launch_bounds__(kTreeWarps * 32, D <= 128 ? 2 : 1)
   }
 }
 
+// ---------------------------------------------------------------- bf16: tcgen05, up to 128 query rows per CTA
+// Head dims 64 and 128.  The query rows (padded to the 128 rows of tcgen05.mma.cta_group::1.kind::f16)
+// stay in shared memory; the CTA streams its split of the lane's keys in units of 64 slots:
+//   warps 0-3  softmax, thread = query row = TMEM lane (warps past the last row leave at once);
+//   warp 4     one thread issues S(r) = Q K(r)^T, then O += P(r-1) V(r-1);
+//   warp 5     loads K and V: full tiles by TMA (128-byte swizzle, no multicast), a segment's last
+//              tile and the drafted tokens' (strided) by cp.async with zero fill.
+// Tensor memory, 256 columns: two 64-column score buffers (P as bf16 over the first half of its own
+// scores) and O.  K and V have rings of their own: K(r) is free once its scores are done, V(r) once
+// its product is; the loader asks in the order in which the tensor core gives them back.  Every wait
+// is bounded; on expiry a role stops and the status gets bit 17.
+constexpr int32_t kStatusTreeTimeout = 1 << 17;
+constexpr long long kTreeWaitBudget = 4000000000LL;   // clock cycles (about 2 s)
+constexpr int kTreeTcThreads = 192;
+
+template <int D>
+struct TreeTcShape {
+  static constexpr int TS = kTcTS, ST = D == 128 ? 2 : 4;
+  static constexpr int Q_BYTES = (D / 64) * 128 * 128, KV_BYTES = (D / 64) * TS * 128;
+  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + ST * KV_BYTES, OFF_M = OFF_V + ST * KV_BYTES;
+  static constexpr size_t smem = OFF_M + ST * TS * 4 + 1024;   // + alignment slack
+  static constexpr uint32_t COLS = 256;
+};
+
+// K/V rows of the prefix and the window as tensor maps (64 x 64 boxes).
+struct TreeMaps {
+  CUtensorMap k[2];
+  CUtensorMap v[2];
+};
+
+template <int D>
+__global__ void __launch_bounds__(kTreeTcThreads, 2)
+    tree_tc_kernel(TreeGeo a, logkv_prefix_t pre, const __nv_bfloat16* rk, const __nv_bfloat16* rv, float* part,
+                   int32_t* status, const __grid_constant__ TreeMaps maps, int tma_mask, int tile_rows) {
+  using S = TreeTcShape<D>;
+  using B16 = __nv_bfloat16;
+  constexpr int TS = S::TS, ST = S::ST, CPR = D / 8;
+  extern __shared__ uint4 smem4[];
+  __shared__ uint32_t masks[kTreeMaxTokens][kTreeWords];
+  __shared__ int up_[kTreeMaxTokens];
+  __shared__ uint64_t q_full, k_full[ST], v_full[ST], k_empty[ST], v_empty[ST], s_full[2], p_full[2], pv_done[2];
+  __shared__ uint32_t sh_tmem;
+  __shared__ uint32_t sh_poison[ST][2];   // drafted tokens of the stage whose V is not finite
+  pdl_entry();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int ln = blockIdx.x, split = blockIdx.y, g = ln % a.G, b = ln / a.G, T = a.T;
+  const int row0 = blockIdx.z * tile_rows, NQ = min(tile_rows, a.rf * T - row0);
+  const int Lp = prefix_length(pre, ln), R = a.rcount;
+  const int up = (Lp + TS - 1) / TS, ur = (R + TS - 1) / TS, U = up + ur + (T + TS - 1) / TS;
+  const int ns = tree_splits(a, U);
+  if (split >= ns) return;
+  const int u0 = (int)((long long)U * split / ns), n = (int)((long long)U * (split + 1) / ns) - u0;
+  unsigned char* raw = reinterpret_cast<unsigned char*>(smem4);
+  unsigned char* base = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
+  const uint32_t base_s = tc::smem_u32(base);
+  const int live = (NQ + 31) / 32;   // softmax warps with rows
+  if (tid == 0) {
+    tc::mbar_init(&q_full, 32 * live);
+    for (int i = 0; i < ST; ++i) {
+      tc::mbar_init(&k_full[i], 1);
+      tc::mbar_init(&v_full[i], 1);
+      tc::mbar_init(&k_empty[i], 1);
+      tc::mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&p_full[i], 32 * live);
+      tc::mbar_init(&pv_done[i], 1);
+    }
+    tc::mbar_fence_init();
+  }
+  if (warp == 0) {
+    tc::tmem_alloc(&sh_tmem, S::COLS);
+    tc::tmem_relinquish();
+  }
+  if (u0 + n > up + ur) tree_masks(a, b, masks, up_, status);   // uniform over the block
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = sh_tmem, t_o = tmem + 128u;
+  auto t_s = [&](int r) { return tmem + 64u * (r & 1); };
+  auto unit = [&](int u, int& first, int& rows) {
+    if (u < up) {
+      first = u * TS;
+      rows = min(TS, Lp - first);
+      return 0;
+    }
+    if (u < up + ur) {
+      first = (u - up) * TS;
+      rows = min(TS, R - first);
+      return 1;
+    }
+    first = (u - up - ur) * TS;
+    rows = min(TS, T - first);
+    return 2;
+  };
+  auto fail = [&]() {
+    if (status) atomicOr(status, kStatusTreeTimeout);
+  };
+
+  if (warp == 5) {
+    // ------------------------------------------------ loader
+    auto row_of = [&](int cls, int first) { return cls == 0 ? (size_t)ln * pre.capacity + first : (size_t)ln * a.rcap + first; };
+    auto mass_of = [&](int r, int j) {   // slot j's term of unit r in the log2 domain
+      int first, rows;
+      const int cls = unit(u0 + r, first, rows);
+      return cls == 0 && j < rows ? pre.mass[row_of(0, first) + j] * a.mass_log2 : 0.f;
+    };
+    auto copy_rows = [&](unsigned char* dst, const B16* src, long long stride, int rows) {
+      for (int flat = lane; flat < TS * CPR; flat += 32) {
+        const int r = flat / CPR, c = flat % CPR;
+        unsigned char* d = dst + (c >> 3) * (TS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        if (r < rows) cp_async16(d, src + r * stride + c * 8);
+        else *reinterpret_cast<uint4*>(d) = make_uint4(0, 0, 0, 0);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      __syncwarp();
+    };
+    auto load = [&](int r, bool is_v) {
+      const int st = r % ST;
+      uint64_t* empty = is_v ? &v_empty[st] : &k_empty[st];
+      uint64_t* full = is_v ? &v_full[st] : &k_full[st];
+      if (r >= ST && !tc::mbar_wait(empty, (r / ST - 1) & 1, kTreeWaitBudget)) return false;
+      int first, rows;
+      const int cls = unit(u0 + r, first, rows);
+      unsigned char* dst = base + (is_v ? S::OFF_V : S::OFF_K) + st * S::KV_BYTES;
+      if (rows == TS && cls < 2 && (tma_mask >> cls & 1)) {
+        if (lane == 0) {
+          tc::fence_proxy_async();   // earlier plain stores to this stage before the asynchronous ones
+          tc::mbar_arrive_expect_tx(full, S::KV_BYTES);
+          const CUtensorMap* map = is_v ? &maps.v[cls] : &maps.k[cls];
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tc::tma_load_2d(tc::smem_u32(dst) + c * (TS * 128), map, c * 64, (int)row_of(cls, first), full);
+        }
+        return true;
+      }
+      const B16* src;
+      long long stride = D;
+      if (cls == 2) {
+        stride = is_v ? a.vs[2] : a.ks[2];
+        src = is_v ? static_cast<const B16*>(a.vn) + b * a.vs[0] + g * a.vs[1]
+                   : static_cast<const B16*>(a.kn) + b * a.ks[0] + g * a.ks[1];
+        src += first * stride;
+      } else {
+        src = (cls == 0 ? static_cast<const B16*>(is_v ? pre.v : pre.k) : is_v ? rv : rk) + row_of(cls, first) * D;
+      }
+      copy_rows(dst, src, stride, rows);
+      if (is_v && cls == 2) {
+        // Drafted tokens whose V is not finite leave the product; the rows that see them get a NaN sum.
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r_ = 32 * h + lane;
+          bool bad = false;
+          for (int c = 0; c < CPR; ++c) {
+            uint4* p = reinterpret_cast<uint4*>(dst + (c >> 3) * (TS * 128) + r_ * 128 + (((c & 7) ^ (r_ & 7)) << 4));
+            uint4 x = *p;
+            unsigned* w = reinterpret_cast<unsigned*>(&x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool lo = (w[i] & 0x7f80u) == 0x7f80u, hi = (w[i] & 0x7f800000u) == 0x7f800000u;
+              bad |= lo | hi;
+              w[i] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
+            }
+            *p = x;
+          }
+          const unsigned m = __ballot_sync(0xffffffffu, bad);
+          if (lane == 0) sh_poison[st][h] = m;
+        }
+      }
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(full);
+      return true;
+    };
+    float m0 = mass_of(0, lane), m1 = mass_of(0, lane + 32);
+    bool ok = load(0, false);
+    for (int r = 0; ok && r < n; ++r) {
+      if (r + 1 < n) ok = load(r + 1, false);
+      if (!ok) break;
+      // The stage's mass terms: read by the softmax of unit r - ST before its V was given back.
+      const int st = r % ST;
+      if (r >= ST && !tc::mbar_wait(&v_empty[st], (r / ST - 1) & 1, kTreeWaitBudget)) {
+        ok = false;
+        break;
+      }
+      float* sm = reinterpret_cast<float*>(base + S::OFF_M) + st * TS;
+      sm[lane] = m0;
+      sm[lane + 32] = m1;
+      __syncwarp();
+      ok = load(r, true);
+      if (r + 1 < n) {
+        m0 = mass_of(r + 1, lane);
+        m1 = mass_of(r + 1, lane + 32);
+      }
+    }
+    if (!ok && lane == 0) fail();
+  } else if (warp == 4) {
+    // ------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = tc::f16_idesc(128, TS, 0, 0), idesc_o = tc::f16_idesc(128, D, 0, 1);
+      bool ok = tc::mbar_wait(&q_full, 0, kTreeWaitBudget);
+      for (int r = 0; ok && r <= n; ++r) {
+        if (r < n) {
+          const int st = r % ST;
+          // Scores r overwrite P(r - 2): its product is done.
+          ok = tc::mbar_wait(&k_full[st], (r / ST) & 1, kTreeWaitBudget) &&
+               (r < 2 || tc::mbar_wait(&pv_done[r & 1], (r / 2 - 1) & 1, kTreeWaitBudget));
+          if (!ok) break;
+          tc::fence_proxy_async();
+          tc::fence_after();
+          const uint32_t kbs = base_s + S::OFF_K + st * S::KV_BYTES;
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint64_t da = tc::sw128_desc(base_s + (ks >> 2) * (128 * 128) + (ks & 3) * 32, 16, 1024);
+            const uint64_t db = tc::sw128_desc(kbs + (ks >> 2) * (TS * 128) + (ks & 3) * 32, 16, 1024);
+            tc::umma_f16(t_s(r), da, db, idesc_s, ks > 0 ? 1u : 0u);
+          }
+          tc::umma_commit(&k_empty[st]);
+          tc::umma_commit(&s_full[r & 1]);
+        }
+        if (r >= 1) {
+          const int v = r - 1, st = v % ST;
+          ok = tc::mbar_wait(&v_full[st], (v / ST) & 1, kTreeWaitBudget) &&
+               tc::mbar_wait(&p_full[v & 1], (v / 2) & 1, kTreeWaitBudget);
+          if (!ok) break;
+          tc::fence_proxy_async();
+          tc::fence_after();
+          const uint32_t vbs = base_s + S::OFF_V + st * S::KV_BYTES;
+#pragma unroll
+          for (int ks = 0; ks < TS / 16; ++ks) {
+            const uint64_t db = tc::sw128_desc(vbs + ks * 16 * 128, TS * 128, 1024);
+            tc::umma_f16_ts(t_o, t_s(v) + ks * 8, db, idesc_o, (v > 0 || ks > 0) ? 1u : 0u);
+          }
+          tc::umma_commit(&v_empty[st]);
+          tc::umma_commit(&pv_done[v & 1]);
+        }
+      }
+      if (!ok) fail();
+    }
+  } else if (warp < live) {
+    // ------------------------------------------------ softmax, row `tid`
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    const bool in = tid < NQ;
+    const int row = row0 + min(tid, NQ - 1), t = row % T, hh = row / T;
+    {
+      const B16* qp = static_cast<const B16*>(a.q) + b * a.qs[0] + (g * a.rf + hh) * a.qs[1] + t * a.qs[2];
+#pragma unroll
+      for (int c = 0; c < CPR; ++c) {
+        unsigned char* d = base + (c >> 3) * (128 * 128) + tid * 128 + (((c & 7) ^ (tid & 7)) << 4);
+        if (in) cp_async16(d, qp + c * 8);
+        else *reinterpret_cast<uint4*>(d) = make_uint4(0, 0, 0, 0);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      tc::fence_proxy_async();
+      tc::mbar_arrive(&q_full);
+    }
+    float m_used = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int r = 0; r < n; ++r) {
+      const int st = r % ST;
+      ok = __all_sync(0xffffffffu, tc::mbar_wait(&v_full[st], (r / ST) & 1, kTreeWaitBudget) &&
+                                       tc::mbar_wait(&s_full[r & 1], (r / 2) & 1, kTreeWaitBudget));
+      if (!ok) break;
+      tc::fence_after();
+      int first, rows;
+      const int cls = unit(u0 + r, first, rows);
+      const float* sm = reinterpret_cast<const float*>(base + S::OFF_M) + st * TS;
+      float sv[TS];
+      {
+        uint32_t r64[64];
+        tc::tmem_ld64(t_s(r) + lane_off, r64);
+#pragma unroll
+        for (int j = 0; j < TS; ++j) sv[j] = __uint_as_float(r64[j]);
+      }
+      float mt = -INFINITY;
+      const uint64_t c2 = tc::f2pack(a.scale_log2, a.scale_log2);
+#pragma unroll
+      for (int j = 0; j < TS; j += 4) {
+        const float4 m4 = *reinterpret_cast<const float4*>(sm + j);
+        tc::f2unpack(tc::ffma2(tc::f2pack(sv[j], sv[j + 1]), c2, tc::f2pack(m4.x, m4.y)), sv[j], sv[j + 1]);
+        tc::f2unpack(tc::ffma2(tc::f2pack(sv[j + 2], sv[j + 3]), c2, tc::f2pack(m4.z, m4.w)), sv[j + 2], sv[j + 3]);
+      }
+      float spoil = 0.f;
+      if (rows < TS || cls == 2) {
+        uint32_t lo = rows >= 32 ? ~0u : (1u << rows) - 1, hi = rows >= 64 ? ~0u : rows > 32 ? (1u << (rows - 32)) - 1 : 0u;
+        if (cls == 2) {
+          lo &= masks[t][first >> 5];
+          hi &= masks[t][(first >> 5) + 1];
+          if ((lo & sh_poison[st][0]) | (hi & sh_poison[st][1])) spoil = NAN;
+        }
+#pragma unroll
+        for (int j = 0; j < TS; ++j) sv[j] = (j < 32 ? lo >> (j & 31) : hi >> (j & 31)) & 1 ? sv[j] : -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < TS; j += 4) mt = fmaxf(mt, fmaxf(fmaxf(sv[j], sv[j + 1]), fmaxf(sv[j + 2], sv[j + 3])));
+      // The running maximum moves only when a unit exceeds it by more than 2^8 (then O is rescaled).
+      float alpha = 1.f;
+      if (mt > m_used + 8.f || (m_used == -INFINITY && mt != -INFINITY)) {
+        alpha = m_used == -INFINITY ? 0.f : tc::ex2(m_used - mt);
+        m_used = mt;
+      }
+      const float msub = m_used == -INFINITY ? 0.f : m_used;
+      const uint64_t nm2 = tc::f2pack(-msub, -msub);
+      uint64_t ps2 = tc::f2pack(0.f, 0.f);
+      uint32_t pk[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        float x0, x1;
+        tc::f2unpack(tc::fadd2(tc::f2pack(sv[2 * j], sv[2 * j + 1]), nm2), x0, x1);
+        const float p0 = tc::ex2(x0), p1 = tc::ex2(x1);
+        ps2 = tc::fadd2(ps2, tc::f2pack(p0, p1));
+        pk[j] = pack_bf16x2(p0, p1);   // the matrix instruction's operand type; l sums the unrounded values
+      }
+      float ps0, ps1;
+      tc::f2unpack(ps2, ps0, ps1);
+      l = l * alpha + (ps0 + ps1) + spoil;
+      if (r > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(&pv_done[(r - 1) & 1], ((r - 1) / 2) & 1, kTreeWaitBudget));
+        if (!ok) break;
+        tc::fence_after();
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t r32[32];
+          tc::tmem_ld32(t_o + lane_off + c0, r32);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r32[j] = __float_as_uint(__uint_as_float(r32[j]) * alpha);
+          tc::tmem_st32(t_o + lane_off + c0, r32);
+        }
+      }
+      tc::tmem_st32(t_s(r) + lane_off, pk);
+      tc::fence_before();
+      tc::mbar_arrive(&p_full[r & 1]);
+    }
+    if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(&pv_done[(n - 1) & 1], ((n - 1) / 2) & 1, kTreeWaitBudget));
+    if (!ok) {
+      if (lane == 0) fail();
+    } else {
+      tc::fence_after();
+      float* pp = tree_part(part, a, split, (size_t)ln * a.rf * T + row);
+      if (in) {
+        pp[0] = m_used;
+        pp[1] = l;
+      }
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t r32[32];
+        tc::tmem_ld32(t_o + lane_off + c0, r32);
+        if (in) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(pp + 4 + c0 + j) =
+                make_float4(__uint_as_float(r32[j]), __uint_as_float(r32[j + 1]), __uint_as_float(r32[j + 2]),
+                            __uint_as_float(r32[j + 3]));
+        }
+      }
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc::fence_after();
+    tc::tmem_dealloc(tmem, S::COLS);
+  }
+}
+
 // ---------------------------------------------------------------- float32: CUDA cores, 32 query rows per CTA
 // Q, K and V tiles in shared memory (rows padded by one 16-byte chunk), every thread a 4 x 4 block of
 // the 32 x 64 scores and a 4 x (D / 16) block of O.
@@ -608,16 +977,24 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeGeo a, logkv_pref
 // ---------------------------------------------------------------- host side
 struct TreePlan {
   int tile_rows, ts, nsplit, nsmin, upw;   // query rows per CTA, key tile, splits
+  bool tc;
 };
+
+static bool tree_tc(const logkv_layout_t& l, long long rows) {
+  return l.dtype == LOGKV_DTYPE_BF16 && (l.dim == 64 || l.dim == 128) && rows > 16;
+}
 
 // Splits: two CTAs per SM over all lanes and row tiles, at least a key tile per warp each.
 static TreePlan tree_plan(const logkv_layout_t& l, int heads, int tokens, int prefix_capacity) {
   TreePlan p;
   const bool f32 = l.dtype == LOGKV_DTYPE_F32;
-  p.tile_rows = f32 ? kF32Rows : 16;
-  p.ts = f32 ? kF32TS : 16;
-  p.upw = f32 ? 1 : kTreeWarps;
-  const long long rows = (long long)(heads / l.groups) * tokens, tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  const long long rows = (long long)(heads / l.groups) * tokens;
+  p.tc = tree_tc(l, rows);
+  const int most = p.tc ? 128 : f32 ? kF32Rows : 16;
+  const long long tiles = (rows + most - 1) / most;
+  p.tile_rows = p.tc ? (int)((rows + tiles - 1) / tiles) : most;
+  p.ts = p.tc ? kTcTS : f32 ? kF32TS : 16;
+  p.upw = p.tc ? 2 : f32 ? 1 : kTreeWarps;
   const long long ctas = (long long)l.batch * l.groups * tiles;
   const int units = (prefix_capacity + l.recent_capacity + tokens) / p.ts + 3;
   p.nsmin = (int)std::max(1LL, 296 / ctas);
@@ -660,6 +1037,34 @@ static int launch_tree_bf16(const TreeGeo& a, const TreePlan& p, const logkv_pre
              static_cast<const B16*>(s.recent_k), static_cast<const B16*>(s.recent_v), static_cast<B16*>(x.out), part,
              x.status);
   launch_tree_combine<B16, D, 16>(a, pre, part, x.out, st);
+  return launch_status();
+}
+
+// tcgen05: head dims 64 and 128.
+template <int D>
+static int launch_tree_tc(const TreeGeo& a, const TreePlan& p, const logkv_prefix_t& pre, const logkv_state_t& s,
+                          const logkv_tree_args_t& x, float* part, cudaStream_t st) {
+  using S = TreeTcShape<D>;
+  using B16 = __nv_bfloat16;
+  auto kern = tree_tc_kernel<D>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
+  if (e != cudaSuccess) return (int)e;
+  TreeMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  const size_t lanes = (size_t)a.B * a.G;
+  int mask = 0;
+  // Rows are 32-bit coordinates; larger buffers take the cp.async path.
+  if (lanes * pre.capacity < (1ull << 31) && encode_rows_map(&maps.k[0], pre.k, lanes * pre.capacity, D) &&
+      encode_rows_map(&maps.v[0], pre.v, lanes * pre.capacity, D))
+    mask |= 1;
+  if (lanes * a.rcap < (1ull << 31) && encode_rows_map(&maps.k[1], s.recent_k, lanes * a.rcap, D) &&
+      encode_rows_map(&maps.v[1], s.recent_v, lanes * a.rcap, D))
+    mask |= 2;
+  const unsigned tiles = (unsigned)((a.rf * a.T + p.tile_rows - 1) / p.tile_rows);
+  launch_pdl(kern, dim3(a.B * a.G, p.nsplit, tiles), kTreeTcThreads, S::smem, st, a, pre,
+             static_cast<const B16*>(s.recent_k), static_cast<const B16*>(s.recent_v), part, x.status, maps, mask,
+             p.tile_rows);
+  launch_tree_combine<B16, D, kTcTS>(a, pre, part, x.out, st);
   return launch_status();
 }
 
@@ -733,6 +1138,10 @@ LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_sta
   a.wide = x->parents_wide;
   float* part = static_cast<float*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p.tc) {
+    if (layout->dim == 64) return launch_tree_tc<64>(a, p, *prefix, *state, *x, part, st);
+    return launch_tree_tc<128>(a, p, *prefix, *state, *x, part, st);
+  }
   if (layout->dtype == LOGKV_DTYPE_BF16) {
     switch (layout->dim) {
       case 16: return launch_tree_bf16<16>(a, p, *prefix, *state, *x, part, st);

@@ -66,6 +66,16 @@ def test_tree_lane_counts(dtype, B, G):
     check(cache, q, k, v, p, run(cache, q, k, v, p))
 
 
+@pytest.mark.parametrize("dtype,D,T,rf", [(BF16, 128, 40, 2), (BF16, 64, 60, 2), (BF16, 128, 200, 1), (BF16, 32, 10, 2),
+                                          (BF16, 128, 8, 2), (F32, 64, 20, 2)])
+def test_long_splits(dtype, D, T, rf):
+    """One split per lane, many key tiles each (the stages are used over and over)."""
+    cache = make_cache(dtype, B=40, G=8, D=D, R=1999, recent=2048, seed=21)
+    q, k, v = drafts(cache, rf, T)
+    p = random_tree(np.random.RandomState(22), 40, T, absent=5)
+    check(cache, q, k, v, p, run(cache, q, k, v, p))
+
+
 @pytest.mark.parametrize("dtype,D", [(BF16, 64), (BF16, 32), (F32, 64)])
 def test_special_trees(dtype, D):
     """A chain (every token sees all before it), a star (none sees another), a batch row without any

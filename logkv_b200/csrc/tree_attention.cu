@@ -90,7 +90,12 @@ __device__ void tree_masks(const TreeGeo& a, int b, uint32_t (*mask)[kTreeWords]
   __syncthreads();
 }
 
-// Partial of one row and split: [m, l, -, -, O[D]], O relative to 2^m.
+__device__ __forceinline__ bool tree_absent(const uint32_t (*mask)[kTreeWords], int t) {
+  return !(mask[t][t >> 5] >> (t & 31) & 1);   // a token that is there sees itself
+}
+
+// Partial of one row and split: [m, l, -, -, O[D]], O relative to 2^m; l = -1 marks a row of an absent
+// token (written by the splits that hold drafted tokens).
 __device__ __forceinline__ float* tree_part(float* part, const TreeGeo& a, int split, size_t row) {
   return part + ((size_t)split * a.B * a.H * a.T + row) * (a.D + 4);
 }
@@ -349,7 +354,7 @@ __global__ void __launch_bounds__(kTreeWarps * 32, D <= 128 ? 2 : 1)
     float* pp = tree_part(part, a, split, row);
     if (d == 0) {
       pp[0] = mx;
-      pp[1] = l;
+      pp[1] = u1 > up + ur && tree_absent(masks, (row0 + r) % T) ? -1.f : l;
     }
     pp[4 + d] = ov;
   }
@@ -373,9 +378,10 @@ constexpr int kTreeTcThreads = 192;
 template <int D>
 struct TreeTcShape {
   static constexpr int TS = kTcTS, ST = D == 128 ? 2 : 4;
+  static constexpr int MR = 2 * ST;   // mass stages, at least ST + 2
   static constexpr int Q_BYTES = (D / 64) * 128 * 128, KV_BYTES = (D / 64) * TS * 128;
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + ST * KV_BYTES, OFF_M = OFF_V + ST * KV_BYTES;
-  static constexpr size_t smem = OFF_M + ST * TS * 4 + 1024;   // + alignment slack
+  static constexpr size_t smem = OFF_M + MR * TS * 4 + 1024;   // + alignment slack
   static constexpr uint32_t COLS = 256;
 };
 
@@ -387,15 +393,16 @@ struct TreeMaps {
 
 template <int D>
 __global__ void __launch_bounds__(kTreeTcThreads, 2)
-    tree_tc_kernel(TreeGeo a, logkv_prefix_t pre, const __nv_bfloat16* rk, const __nv_bfloat16* rv, float* part,
-                   int32_t* status, const __grid_constant__ TreeMaps maps, int tma_mask, int tile_rows) {
+    tree_tc_kernel(TreeGeo a, logkv_prefix_t pre, const __nv_bfloat16* rk, const __nv_bfloat16* rv, __nv_bfloat16* out,
+                   float* part, int32_t* status, const __grid_constant__ TreeMaps maps, int tma_mask, int tile_rows) {
   using S = TreeTcShape<D>;
   using B16 = __nv_bfloat16;
-  constexpr int TS = S::TS, ST = S::ST, CPR = D / 8;
+  constexpr int TS = S::TS, ST = S::ST, MR = S::MR, CPR = D / 8;
   extern __shared__ uint4 smem4[];
   __shared__ uint32_t masks[kTreeMaxTokens][kTreeWords];
   __shared__ int up_[kTreeMaxTokens];
-  __shared__ uint64_t q_full, k_full[ST], v_full[ST], k_empty[ST], v_empty[ST], s_full[2], p_full[2], pv_done[2];
+  __shared__ uint64_t q_full, k_full[ST], v_full[ST], k_empty[ST], v_empty[ST], m_full[MR], s_full[2], p_full[2],
+      pv_done[2];
   __shared__ uint32_t sh_tmem;
   __shared__ uint32_t sh_poison[ST][2];   // drafted tokens of the stage whose V is not finite
   pdl_entry();
@@ -419,6 +426,7 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
       tc::mbar_init(&k_empty[i], 1);
       tc::mbar_init(&v_empty[i], 1);
     }
+    for (int i = 0; i < MR; ++i) tc::mbar_init(&m_full[i], 1);
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&s_full[i], 1);
       tc::mbar_init(&p_full[i], 32 * live);
@@ -458,10 +466,11 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
   if (warp == 5) {
     // ------------------------------------------------ loader
     auto row_of = [&](int cls, int first) { return cls == 0 ? (size_t)ln * pre.capacity + first : (size_t)ln * a.rcap + first; };
-    auto mass_of = [&](int r, int j) {   // slot j's term of unit r in the log2 domain
+    // Slot j's mass of unit r: read a unit ahead and not touched (so not waited for) until it is stored.
+    auto mass_of = [&](int r, int j) {
       int first, rows;
       const int cls = unit(u0 + r, first, rows);
-      return cls == 0 && j < rows ? pre.mass[row_of(0, first) + j] * a.mass_log2 : 0.f;
+      return cls == 0 && j < rows ? pre.mass[row_of(0, first) + j] : 0.f;
     };
     auto copy_rows = [&](unsigned char* dst, const B16* src, long long stride, int rows) {
       for (int flat = lane; flat < TS * CPR; flat += 32) {
@@ -531,26 +540,25 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
       if (lane == 0) tc::mbar_arrive(full);
       return true;
     };
+    // The mass terms have a longer ring: K(r) may be loaded once the scores of unit r - ST are done, so
+    // once P of unit r - ST - 2 has been written and its mass terms read.
     float m0 = mass_of(0, lane), m1 = mass_of(0, lane + 32);
-    bool ok = load(0, false);
-    for (int r = 0; ok && r < n; ++r) {
-      if (r + 1 < n) ok = load(r + 1, false);
-      if (!ok) break;
-      // The stage's mass terms: read by the softmax of unit r - ST before its V was given back.
-      const int st = r % ST;
-      if (r >= ST && !tc::mbar_wait(&v_empty[st], (r / ST - 1) & 1, kTreeWaitBudget)) {
-        ok = false;
-        break;
+    bool ok = true;
+    for (int r = 0; ok && r <= n; ++r) {
+      if (r < n) {
+        ok = load(r, false);
+        if (!ok) break;
+        float* sm = reinterpret_cast<float*>(base + S::OFF_M) + (r % MR) * TS;
+        sm[lane] = m0 * a.mass_log2;
+        sm[lane + 32] = m1 * a.mass_log2;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&m_full[r % MR]);
+        if (r + 1 < n) {
+          m0 = mass_of(r + 1, lane);
+          m1 = mass_of(r + 1, lane + 32);
+        }
       }
-      float* sm = reinterpret_cast<float*>(base + S::OFF_M) + st * TS;
-      sm[lane] = m0;
-      sm[lane + 32] = m1;
-      __syncwarp();
-      ok = load(r, true);
-      if (r + 1 < n) {
-        m0 = mass_of(r + 1, lane);
-        m1 = mass_of(r + 1, lane + 32);
-      }
+      if (r > 0) ok = load(r - 1, true);
     }
     if (!ok && lane == 0) fail();
   } else if (warp == 4) {
@@ -618,13 +626,14 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
     bool ok = true;
     for (int r = 0; r < n; ++r) {
       const int st = r % ST;
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(&v_full[st], (r / ST) & 1, kTreeWaitBudget) &&
-                                       tc::mbar_wait(&s_full[r & 1], (r / 2) & 1, kTreeWaitBudget));
-      if (!ok) break;
-      tc::fence_after();
       int first, rows;
       const int cls = unit(u0 + r, first, rows);
-      const float* sm = reinterpret_cast<const float*>(base + S::OFF_M) + st * TS;
+      ok = __all_sync(0xffffffffu, tc::mbar_wait(&m_full[r % MR], (r / MR) & 1, kTreeWaitBudget) &&
+                                       tc::mbar_wait(&s_full[r & 1], (r / 2) & 1, kTreeWaitBudget) &&
+                                       (cls < 2 || tc::mbar_wait(&v_full[st], (r / ST) & 1, kTreeWaitBudget)));
+      if (!ok) break;
+      tc::fence_after();
+      const float* sm = reinterpret_cast<const float*>(base + S::OFF_M) + (r % MR) * TS;
       float sv[TS];
       {
         uint32_t r64[64];
@@ -696,16 +705,30 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
       if (lane == 0) fail();
     } else {
       tc::fence_after();
-      float* pp = tree_part(part, a, split, (size_t)ln * a.rf * T + row);
-      if (in) {
-        pp[0] = m_used;
-        pp[1] = l;
-      }
+      const size_t orow = (size_t)ln * a.rf * T + row;
+      const bool absent = u0 + n > up + ur && tree_absent(masks, t);
+      const bool whole = a.nsplit == 1;   // no partials, no combine
+      float* pp = tree_part(part, a, split, orow);
+      const float inv = 1.f / l;
+      if (in && !whole) *reinterpret_cast<float2*>(pp) = make_float2(m_used, absent ? -1.f : l);
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 32) {
         uint32_t r32[32];
         tc::tmem_ld32(t_o + lane_off + c0, r32);
-        if (in) {
+        if (!in) continue;
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (!absent) {
+              w.x = pack_bf16x2(__uint_as_float(r32[j]) * inv, __uint_as_float(r32[j + 1]) * inv);
+              w.y = pack_bf16x2(__uint_as_float(r32[j + 2]) * inv, __uint_as_float(r32[j + 3]) * inv);
+              w.z = pack_bf16x2(__uint_as_float(r32[j + 4]) * inv, __uint_as_float(r32[j + 5]) * inv);
+              w.w = pack_bf16x2(__uint_as_float(r32[j + 6]) * inv, __uint_as_float(r32[j + 7]) * inv);
+            }
+            *reinterpret_cast<uint4*>(out + orow * D + c0 + j) = w;
+          }
+        } else {
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
             *reinterpret_cast<float4*>(pp + 4 + c0 + j) =
@@ -904,7 +927,7 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(TreeGeo a, logkv_
     float* pp = tree_part(part, a, split, (size_t)ln * a.rf * T + row0 + r);
     if (tx == 0) {
       pp[0] = rm[r];
-      pp[1] = rl[r];
+      pp[1] = u1 > up + ur && tree_absent(masks, (row0 + r) % T) ? -1.f : rl[r];
     }
 #pragma unroll
     for (int j = 0; j < (DC + 3) / 4; ++j) {
@@ -915,61 +938,108 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(TreeGeo a, logkv_
 }
 
 // ---------------------------------------------------------------- combine
-// One warp per output row: the splits' partials weighted by 2^(m_s - max m), in split order.  TS: the
-// key tile of the kernel that wrote them.  Rows of absent tokens are zero.
-template <typename T, int D, int TS>
-__global__ void __launch_bounds__(256) tree_combine_kernel(TreeGeo a, logkv_prefix_t pre, const float* part, T* out) {
+// WPR warps per output row (1 or 4): each joins its share of the splits' partials, 32 at a time (lane s
+// holds split s's m and l; the O loads of 4 or 16 splits in flight), then the warps in order.  TS: the key
+// tile of the kernel that wrote the partials.  The order of the sums is fixed by the split count.
+template <typename T, int D, int TS, int WPR>
+__global__ void __launch_bounds__(128) tree_combine_kernel(TreeGeo a, logkv_prefix_t pre, const float* part, T* out) {
+  constexpr int PER = (D + 127) / 128, NB = WPR > 1 ? 16 : 4;
+  __shared__ float sh[4][2 + D];
   pdl_entry();
-  const int lane = threadIdx.x & 31;
-  const size_t row = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (row >= (size_t)a.B * a.H * a.T) return;
-  const int ln = (int)(row / ((size_t)a.rf * a.T)), b = ln / a.G;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
+  const size_t row = (size_t)blockIdx.x * (4 / WPR) + warp / WPR;
+  if (WPR == 1 && row >= (size_t)a.B * a.H * a.T) return;
+  const int ln = (int)(row / ((size_t)a.rf * a.T));
   const int units = (prefix_length(pre, ln) + TS - 1) / TS + (a.rcount + TS - 1) / TS + (a.T + TS - 1) / TS;
   const int ns = tree_splits(a, units);
-  // Absent, or under an absent token: walk up the tree.
-  long long t = (long long)(row % a.T);
-  for (int i = 0; i < a.T && t >= 0; ++i) {
-    const size_t at = (size_t)b * a.pstride + t;
-    const long long p = a.wide ? static_cast<const long long*>(a.parents)[at]
-                               : (long long)static_cast<const int32_t*>(a.parents)[at];
-    t = p < -2 || p >= t ? -2 : p;
-  }
   const size_t stride = (size_t)a.B * a.H * a.T * (D + 4);
   const float* p0 = part + row * (D + 4);
-  float mx = -INFINITY;
-  for (int s = 0; s < ns; ++s) mx = fmaxf(mx, p0[s * stride]);
-  float l = 0.f;
-  constexpr int PER = (D + 127) / 128;
+  float m = -INFINITY, l = 0.f;
+  bool absent = false;
   float4 o[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < ns; ++s) {
-    const float* pp = p0 + s * stride;
-    const float m = pp[0], w = m == -INFINITY ? 0.f : exp2f(m - mx);
-    l += pp[1] * w;
+  const int share = (ns + WPR - 1) / WPR, end = min(ns, (sub + 1) * share);
+  for (int s0 = sub * share; s0 < end; s0 += 32) {
+    const int cnt = min(32, end - s0);
+    const float2 ml = lane < cnt ? *reinterpret_cast<const float2*>(p0 + (s0 + lane) * stride) : make_float2(-INFINITY, 0.f);
+    float mc = ml.x;
+#pragma unroll
+    for (int off = 16; off; off >>= 1) mc = fmaxf(mc, __shfl_xor_sync(0xffffffffu, mc, off));
+    const float mn = fmaxf(m, mc), al = m == -INFINITY ? 0.f : exp2f(m - mn);
+    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
+    absent |= __any_sync(0xffffffffu, ml.y < 0.f);
+    float lw = ml.y * w;
+#pragma unroll
+    for (int off = 16; off; off >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, off);
+    l = l * al + lw;
+    m = mn;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) o[k] = make_float4(o[k].x * al, o[k].y * al, o[k].z * al, o[k].w * al);
+    for (int t0 = 0; t0 < cnt; t0 += NB) {
+      float4 v[NB][PER];
+#pragma unroll
+      for (int s = 0; s < NB; ++s)
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int c = 4 * (lane + 32 * k);
+          v[s][k] = t0 + s < cnt && c < D ? *reinterpret_cast<const float4*>(p0 + (s0 + t0 + s) * stride + 4 + c)
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+      for (int s = 0; s < NB; ++s) {
+        const float ws = __shfl_sync(0xffffffffu, w, (t0 + s) & 31);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          o[k].x = fmaf(v[s][k].x, ws, o[k].x);
+          o[k].y = fmaf(v[s][k].y, ws, o[k].y);
+          o[k].z = fmaf(v[s][k].z, ws, o[k].z);
+          o[k].w = fmaf(v[s][k].w, ws, o[k].w);
+        }
+      }
+    }
+  }
+  if (WPR > 1) {
+    if (lane == 0) {
+      sh[warp][0] = m;
+      sh[warp][1] = absent ? -1.f : l;
+    }
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       const int c = 4 * (lane + 32 * k);
       if (c < D) {
-        const float4 v = *reinterpret_cast<const float4*>(pp + 4 + c);
-        o[k].x += v.x * w;
-        o[k].y += v.y * w;
-        o[k].z += v.z * w;
-        o[k].w += v.w * w;
+        float* d = &sh[warp][2 + c];
+        d[0] = o[k].x, d[1] = o[k].y, d[2] = o[k].z, d[3] = o[k].w;
       }
     }
+    __syncthreads();
+    m = -INFINITY;
+    for (int w = 0; w < WPR; ++w) {
+      m = fmaxf(m, sh[w][0]);
+      absent |= sh[w][1] < 0.f;
+    }
+    for (int d = threadIdx.x; d < D; d += 128) {
+      float L = 0.f, x = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) {
+        const float f = sh[w][0] == -INFINITY ? 0.f : exp2f(sh[w][0] - m);
+        L += sh[w][1] * f;
+        x += sh[w][2 + d] * f;
+      }
+      Elem<T>::store(out + row * D + d, absent ? 0.f : x / L);
+    }
+    return;
   }
-  const bool gone = t == -2;
   const float inv = 1.f / l;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int c = 4 * (lane + 32 * k);
     if (c < D) {
       T* dst = out + row * D + c;
-      Elem<T>::store(dst, gone ? 0.f : o[k].x * inv);
-      Elem<T>::store(dst + 1, gone ? 0.f : o[k].y * inv);
-      Elem<T>::store(dst + 2, gone ? 0.f : o[k].z * inv);
-      Elem<T>::store(dst + 3, gone ? 0.f : o[k].w * inv);
+      Elem<T>::store(dst, absent ? 0.f : o[k].x * inv);
+      Elem<T>::store(dst + 1, absent ? 0.f : o[k].y * inv);
+      Elem<T>::store(dst + 2, absent ? 0.f : o[k].z * inv);
+      Elem<T>::store(dst + 3, absent ? 0.f : o[k].w * inv);
     }
   }
 }
@@ -1020,8 +1090,9 @@ template <typename T, int D, int TS>
 static void launch_tree_combine(const TreeGeo& a, const logkv_prefix_t& pre, const float* part, void* out,
                                 cudaStream_t st) {
   const size_t rows = (size_t)a.B * a.H * a.T;
-  launch_pdl(tree_combine_kernel<T, D, TS>, dim3((unsigned)((rows + 7) / 8)), 256, 0, st, a, pre, part,
-             static_cast<T*>(out));
+  T* o = static_cast<T*>(out);
+  if (a.nsplit > 8) launch_pdl(tree_combine_kernel<T, D, TS, 4>, dim3((unsigned)rows), 128, 0, st, a, pre, part, o);
+  else launch_pdl(tree_combine_kernel<T, D, TS, 1>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, a, pre, part, o);
 }
 
 template <int D>
@@ -1062,9 +1133,9 @@ static int launch_tree_tc(const TreeGeo& a, const TreePlan& p, const logkv_prefi
     mask |= 2;
   const unsigned tiles = (unsigned)((a.rf * a.T + p.tile_rows - 1) / p.tile_rows);
   launch_pdl(kern, dim3(a.B * a.G, p.nsplit, tiles), kTreeTcThreads, S::smem, st, a, pre,
-             static_cast<const B16*>(s.recent_k), static_cast<const B16*>(s.recent_v), part, x.status, maps, mask,
-             p.tile_rows);
-  launch_tree_combine<B16, D, kTcTS>(a, pre, part, x.out, st);
+             static_cast<const B16*>(s.recent_k), static_cast<const B16*>(s.recent_v), static_cast<B16*>(x.out), part,
+             x.status, maps, mask, p.tile_rows);
+  if (p.nsplit > 1) launch_tree_combine<B16, D, kTcTS>(a, pre, part, x.out, st);
   return launch_status();
 }
 

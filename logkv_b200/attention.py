@@ -55,8 +55,12 @@ class _ReadState:
         self.mass = torch.zeros(B, G, self.capacity, dtype=torch.float32, device=dev)
         self.length = torch.zeros(B, G, **i32)
         self.status = torch.zeros(1, **i32)
+        self.status_ptr = self.status.data_ptr()
         self.epoch = -1
         self.workspaces: dict = {}
+        self.tree_bytes: dict = {}   # scratch bytes of log_kv_tree_attention by (heads, tokens)
+        self.qx: dict = {}           # query_extra by scale
+        self._prefix = None
 
     def plan_struct(self, full: bool) -> _lib.Plan:
         p = lambda t: t.data_ptr()  # noqa: E731
@@ -65,8 +69,10 @@ class _ReadState:
                          p(self.vanchor), p(self.nvalid), p(self.exact_rows), p(self.nexact))
 
     def prefix_struct(self) -> _lib.Prefix:
-        return _lib.Prefix(self.pk.data_ptr(), self.pv.data_ptr(), self.mass.data_ptr(), self.length.data_ptr(),
-                           self.capacity)
+        if self._prefix is None:
+            self._prefix = _lib.Prefix(self.pk.data_ptr(), self.pv.data_ptr(), self.mass.data_ptr(),
+                                       self.length.data_ptr(), self.capacity)
+        return self._prefix
 
     def workspace(self, cache, heads: int, q_tokens: int) -> torch.Tensor:
         key = (heads, q_tokens)
@@ -292,20 +298,20 @@ def log_kv_chunk_attention(cache, q_b, k_b, v_b, scale, second_order_scale=1.0, 
 
 def _rows16(t):
     """``t`` with its head dim contiguous and every row 16-byte aligned (a copy where it is not)."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * t.element_size() % 16 == 0 for s in t.stride()[:3]):
+    s = t.stride()
+    if s[3] == 1 and not (t.data_ptr() | (s[0] | s[1] | s[2]) * t.element_size()) & 15:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _tree_parents(cache, parents, T: int):
+def _tree_parents(parents, B: int, T: int, dev):
     """Parents as an integer tensor on the cache's device ([T] or [B, T]); host values are checked."""
-    dev = cache.level_k.device
     p = parents if isinstance(parents, torch.Tensor) else torch.as_tensor(parents)
-    if p.dtype not in (torch.int32, torch.int64):
+    if p.dtype != torch.int32 and p.dtype != torch.int64:
         raise ValueError(f"parents must be integers (int32 or int64), got {p.dtype}")
-    if tuple(p.shape) not in ((T,), (cache.batch_size, T)):
-        raise ValueError(f"parents must be [{T}] or [{cache.batch_size}, {T}], got {tuple(p.shape)}")
-    if p.device.type == "cpu":
+    if tuple(p.shape) not in ((T,), (B, T)):
+        raise ValueError(f"parents must be [{T}] or [{B}, {T}], got {tuple(p.shape)}")
+    if not p.is_cuda:
         if bool(((p < -2) | (p >= torch.arange(T))).any()):
             raise ValueError("a token's parent must be an earlier token, -1 (the committed tokens) or -2 (no token)")
         p = p.to(dev)
@@ -332,43 +338,50 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
     if q.dim() != 4:
         raise ValueError(f"q must be [B, H, T, D], got {tuple(q.shape)}")
     B, H, T, kd = q.shape
-    dev = cache.level_k.device
-    if B != cache.batch_size or kd != cache.k_dim or q.dtype != cache.level_k.dtype:
+    rs = _read_state(cache)
+    dev, dt, G = rs.pk.device, rs.pk.dtype, cache.n_groups
+    if B != cache.batch_size or kd != cache.k_dim or q.dtype != dt:
         raise ValueError(f"q must be [B={cache.batch_size}, H, T, {cache.k_dim}] in the cache dtype")
     _check_kv(cache, k, v)
     if k.size(2) != T:
         raise ValueError("q, k and v must cover the same drafted tokens")
-    if H < 1 or H % cache.n_groups:
-        raise ValueError(f"query heads {H} must be a multiple of KV groups {cache.n_groups}")
-    if any(t.device != dev for t in (q, k, v)):
+    if H < 1 or H % G:
+        raise ValueError(f"query heads {H} must be a multiple of KV groups {G}")
+    if q.device != dev or k.device != dev or v.device != dev:
         raise ValueError(f"q, k and v must be on the cache's device {dev}")
     if T > _lib.TREE_MAX_TOKENS:
         raise ValueError(f"{T} drafted tokens: at most {_lib.TREE_MAX_TOKENS}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError("logkv_b200 attention is forward-only")
     if out is None:
-        out = torch.empty(B, H, T, cache.v_dim, dtype=q.dtype, device=dev)
-    elif out.shape != (B, H, T, cache.v_dim) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous [{B}, {H}, {T}, {cache.v_dim}] tensor in the cache dtype on {dev}")
+        out = torch.empty((B, H, T, kd), dtype=dt, device=dev)
+    elif out.shape != (B, H, T, kd) or out.dtype != dt or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous [{B}, {H}, {T}, {kd}] tensor in the cache dtype on {dev}")
     if T == 0:
         return out
-    p = _tree_parents(cache, parents, T)
-    with torch.cuda.device(dev):
-        rs = refresh_prefix(cache)
+    p = _tree_parents(parents, B, T, dev)
+    with _lib.on_device(dev):
+        if rs.epoch < 0 or rs.epoch != getattr(cache, "_ladder_epoch", None):
+            refresh_prefix(cache)
         layout, state = _structs(cache)
+        lib = _lib.lib()
+        n = rs.tree_bytes.get((H, T))
+        if n is None:
+            n = lib.logkv_tree_attention_workspace_bytes(ctypes.byref(layout), H, T, rs.capacity)
+            if not n:
+                raise ValueError(f"tree attention shape outside the supported range (heads={H}, tokens={T}, "
+                                 f"head dim {kd}, {dt})")
+            rs.tree_bytes[H, T] = n
+        scale = float(scale)
+        qx = rs.qx.get(scale)
+        if qx is None:
+            qx = rs.qx[scale] = query_extra(scale, dt)
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        n = _lib.lib().logkv_tree_attention_workspace_bytes(ctypes.byref(layout), H, T, rs.capacity)
-        if not n:
-            raise ValueError(f"tree attention shape outside the supported range (heads={H}, tokens={T}, "
-                             f"head dim {kd}, {q.dtype})")
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        i64x3 = ctypes.c_int64 * 3
-        args = _lib.TreeArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p.data_ptr(),
-                             i64x3(*q.stride()[:3]), i64x3(*k.stride()[:3]), i64x3(*v.stride()[:3]),
-                             p.stride(0) if p.dim() == 2 else 0, int(p.dtype == torch.int64), H, T,
-                             int(cache.recent_count), float(scale), query_extra(scale, q.dtype), rs.status.data_ptr())
-        pre = rs.prefix_struct()
-        _lib.check(_lib.lib().logkv_tree_attention(ctypes.byref(layout), ctypes.byref(state), ctypes.byref(pre),
-                                                   ctypes.byref(args), ws.data_ptr(), n, _stream(cache)),
-                   "logkv_tree_attention")
+        args = _lib.TreeArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p.data_ptr(), q.stride()[:3],
+                             k.stride()[:3], v.stride()[:3], p.stride(0) if p.dim() == 2 else 0,
+                             p.dtype == torch.int64, H, T, cache.recent_count, scale, qx, rs.status_ptr)
+        _lib.check(lib.logkv_tree_attention(ctypes.byref(layout), ctypes.byref(state),
+                                            ctypes.byref(rs.prefix_struct()), ctypes.byref(args), ws.data_ptr(), n,
+                                            _lib.stream_ptr(dev)), "logkv_tree_attention")
     return out

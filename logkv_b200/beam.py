@@ -49,18 +49,20 @@ def beam_select(logits, scores, k: int, *, keep_places: bool = False):
     dev = logits.device
     if dev.type != "cuda" or scores.device != dev:
         raise ValueError("logits and scores must be CUDA tensors on one device")
-    out = (torch.empty(N, k, dtype=torch.float32, device=dev), torch.empty(N, k, dtype=torch.int64, device=dev),
-           torch.empty(N, k, dtype=torch.int64, device=dev))
+    out_scores = torch.empty((N, k), dtype=torch.float32, device=dev)
+    out_rows, out_tokens = torch.empty((2, N, k), dtype=torch.int64, device=dev).unbind(0)
     if N == 0:
-        return out
-    with torch.cuda.device(dev):
-        if V > 1 and logits.stride(-1) != 1:
+        return out_scores, out_rows, out_tokens
+    with _lib.on_device(dev):
+        if V > 1 and logits.stride(2) != 1:
             logits = logits.contiguous()
         scores = scores.contiguous()
-        n = _lib.lib().logkv_beam_workspace_bytes(N, W, V, k)
+        lib = _lib.lib()
+        n = lib.logkv_beam_workspace_bytes(N, W, V, k)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        args = _lib.BeamArgs(logits.data_ptr(), scores.data_ptr(), *[t.data_ptr() for t in out], logits.stride(0),
-                             logits.stride(1), _lib.DTYPE_CODES[logits.dtype], N, W, V, k, int(keep_places))
-        _lib.check(_lib.lib().logkv_beam_select(ctypes.byref(args), ws.data_ptr(), n,
-                                                ctypes.c_void_p(_lib.stream_ptr(dev))), "logkv_beam_select")
-    return out
+        args = _lib.BeamArgs(logits.data_ptr(), scores.data_ptr(), out_scores.data_ptr(), out_rows.data_ptr(),
+                             out_tokens.data_ptr(), logits.stride(0), logits.stride(1),
+                             _lib.DTYPE_CODES[logits.dtype], N, W, V, k, keep_places)
+        _lib.check(lib.logkv_beam_select(ctypes.byref(args), ws.data_ptr(), n, _lib.stream_ptr(dev)),
+                   "logkv_beam_select")
+    return out_scores, out_rows, out_tokens

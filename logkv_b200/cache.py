@@ -270,8 +270,8 @@ class LogStructuredKVCache(nn.Module):
 
     def _state_struct(self) -> _lib.State:
         """Device pointers of every state buffer (built once; rebuilt when the buffers move)."""
-        st = self._state
-        if st is not None and st.level_k == self.level_k.data_ptr() and st.recent_k == self.recent_k.data_ptr():
+        st, bufs = self._state, self._buffers
+        if st is not None and st.level_k == bufs["level_k"].data_ptr() and st.recent_k == bufs["recent_k"].data_ptr():
             return st
         views = dict(level_k=self.level_k, level_v=self.level_v, level_w=self.level_w,
                      level_p_lo=self.level_p_lo, level_p_hi=self.level_p_hi, level_sum_wp=self.level_sum_wp,
@@ -611,7 +611,7 @@ class LogStructuredKVCache(nn.Module):
         positions = self._positions(T, input_pos)
         self._check_room(n)
         from .attention import _rows16
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             k, k_raw, v = (_rows16(t.to(device=dev, dtype=self.recent_k.dtype)) for t in (k, k_raw, v))
             self.token_count += n
             c, keep = self._chunk_struct(k, k_raw, v, positions, ends, n)
@@ -814,18 +814,20 @@ class LogStructuredKVCache(nn.Module):
     # ------------------------------------------------------------------ hypotheses
     def _row_index(self, index):
         """[batch] row indices as an integer tensor on the cache's device; host values are checked."""
-        dev = self.level_k.device
+        dev = self._buffers["level_k"].device
         t = index if isinstance(index, torch.Tensor) else torch.as_tensor(index)
-        if t.dtype not in (torch.int32, torch.int64):
+        if t.dtype != torch.int64 and t.dtype != torch.int32:
             raise ValueError(f"row indices must be integers (int32 or int64), got {t.dtype}")
-        if tuple(t.shape) != (self.batch_size,):
+        if t.dim() != 1 or t.size(0) != self.batch_size:
             raise ValueError(f"row indices must be [{self.batch_size}], got {tuple(t.shape)}")
-        if t.device.type == "cpu":
+        if t.device != dev:
+            if t.device.type != "cpu":
+                raise ValueError(f"row indices must be on {dev}, got {t.device}")
             if bool(((t < 0) | (t >= self.batch_size)).any()):
                 raise ValueError(f"row indices must be in [0, {self.batch_size})")
             t = t.to(dev)
-        elif t.device != dev:
-            raise ValueError(f"row indices must be on {dev}, got {t.device}")
+        elif dev.type == "cpu" and bool(((t < 0) | (t >= self.batch_size)).any()):
+            raise ValueError(f"row indices must be in [0, {self.batch_size})")
         return t.contiguous()
 
     def reorder_batch(self, index, *, window_from=None) -> None:
@@ -848,19 +850,20 @@ class LogStructuredKVCache(nn.Module):
         if window_from is not None and not 0 <= window_from <= self.recent_count:
             raise ValueError(f"window_from must be in [0, recent_count={self.recent_count}], got {window_from}")
         index = self._row_index(index)
-        from .attention import _read_state
-        dev = self.level_k.device
-        with torch.cuda.device(dev):
+        dev = self._buffers["level_k"].device
+        with _lib.on_device(dev):
             # The prefix moves whether or not it is current, so that a captured call does not depend on
             # what was current when it was captured; its buffers therefore exist from here on.
-            if self._read is None and _lib.capture_id(dev):
-                raise RuntimeError("capture reorder_batch only after the cache has been attended over once")
-            rs = _read_state(self)
-            state, pre = self._state_struct(), rs.prefix_struct()
+            rs = self._read
+            if rs is None:
+                if _lib.capture_id(dev):
+                    raise RuntimeError("capture reorder_batch only after the cache has been attended over once")
+                from .attention import _read_state
+                rs = _read_state(self)
             _lib.check(_lib.lib().logkv_reorder_batch(
-                ctypes.byref(self._layout), ctypes.byref(state), ctypes.byref(pre), int(self.recent_count),
-                -1 if window_from is None else int(window_from), index.data_ptr(), int(index.dtype == torch.int64),
-                rs.status.data_ptr(), ctypes.c_void_p(_lib.stream_ptr(dev))), "logkv_reorder_batch")
+                ctypes.byref(self._layout), ctypes.byref(self._state_struct()), ctypes.byref(rs.prefix_struct()),
+                self.recent_count, -1 if window_from is None else int(window_from), index.data_ptr(),
+                index.dtype == torch.int64, rs.status_ptr, _lib.stream_ptr(dev)), "logkv_reorder_batch")
         self._route_ready = None     # the next flush's decisions must wait for the moved rows
 
     # ------------------------------------------------------------------ read side

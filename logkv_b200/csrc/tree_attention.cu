@@ -42,52 +42,61 @@ __device__ __forceinline__ int prefix_length(const logkv_prefix_t& pre, int ln) 
 }
 
 // Ancestor masks of batch row b: bit j of mask[t] = token t sees token j; 0 for an absent token.
-// Pointer doubling: after round i the mask covers the 2^i nearest tokens of the chain and `up` is
-// the next one (-1: the committed tokens, -2: an absent token).  Called by the whole block.
-__device__ void tree_masks(const TreeGeo& a, int b, uint32_t (*mask)[kTreeWords], int* up, int32_t* status) {
-  const int T = a.T, words = (T + 31) >> 5;
-  for (int t = threadIdx.x; t < T; t += blockDim.x) {
+// Pointer jumping without rounds: up[t] is the next token of t's chain that its mask does not cover
+// yet (-1: the committed tokens, -2: an absent token).  A step joins that token's mask and takes over
+// its `up`; reading `up` before the mask, and writing the mask before `up`, leaves no gap whatever the
+// other tokens' threads have done by then, and a chain ends after about log2 of its length steps.
+// Called by `threads` threads, tid in [0, threads), with their barrier, after tree_parents by the same
+// threads has landed.
+struct TreeSmem {
+  uint32_t mask[kTreeMaxTokens][kTreeWords];
+  int up[kTreeMaxTokens];
+  long long raw[kTreeMaxTokens];   // parents as given (int32 ones packed)
+};
+
+// Batch row b's parents into `m.raw` by cp.async, asked for at a kernel's start: under a full memory
+// system they take microseconds to come.
+__device__ __forceinline__ void tree_parents(const TreeGeo& a, int b, TreeSmem& m, int tid, int threads) {
+  for (int t = tid; t < a.T; t += threads) {
     const size_t at = (size_t)b * a.pstride + t;
-    const long long p = a.wide ? static_cast<const long long*>(a.parents)[at]
-                               : (long long)static_cast<const int32_t*>(a.parents)[at];
+    if (a.wide) cp_async8(&m.raw[t], static_cast<const long long*>(a.parents) + at);
+    else cp_async4(reinterpret_cast<int*>(m.raw) + t, static_cast<const int*>(a.parents) + at);
+  }
+}
+
+template <typename Sync>
+__device__ __forceinline__ void tree_masks(const TreeGeo& a, TreeSmem& m, int32_t* status, int tid, int threads,
+                                           Sync sync) {
+  const int T = a.T, words = (T + 31) >> 5;
+  uint32_t(*mask)[kTreeWords] = m.mask;
+  int* up = m.up;
+  for (int t = tid; t < T; t += threads) {
+    const long long p = a.wide ? m.raw[t] : (long long)reinterpret_cast<const int*>(m.raw)[t];
     const bool bad = p < -2 || p >= t;
     if (bad) set_status(status, kStatusBadParent);
     up[t] = bad ? -2 : (int)p;
     for (int w = 0; w < words; ++w) mask[t][w] = (t >> 5) == w ? 1u << (t & 31) : 0u;
   }
-  __syncthreads();
-  for (int len = 1; len < T; len *= 2) {
-    uint32_t add[2][kTreeWords];   // blockDim.x >= kTreeMaxTokens / 2
-    int next[2];
-    bool more = false;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = threadIdx.x + i * blockDim.x;
-      next[i] = -1;
-      if (t < T && up[t] >= 0) {
-        more = true;
-        next[i] = up[up[t]];
-#pragma unroll
-        for (int w = 0; w < kTreeWords; ++w) add[i][w] = w < words ? mask[up[t]][w] : 0u;
-      }
+  sync();
+  volatile int* vup = up;
+  for (int t = tid; t < T; t += threads) {
+    volatile uint32_t* mine = mask[t];
+    int u = up[t];
+    while (u >= 0) {   // u falls with every step
+      const int next = vup[u];
+      __threadfence_block();
+      volatile uint32_t* theirs = mask[u];
+      for (int w = 0; w <= u >> 5; ++w) mine[w] = mine[w] | theirs[w];
+      __threadfence_block();
+      vup[t] = next;
+      u = next;
     }
-    if (!__syncthreads_or(more)) break;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = threadIdx.x + i * blockDim.x;
-      if (t < T && up[t] >= 0) {
-#pragma unroll
-        for (int w = 0; w < kTreeWords; ++w)
-          if (w < words) mask[t][w] |= add[i][w];
-        up[t] = next[i];
-      }
-    }
-    __syncthreads();
   }
-  for (int t = threadIdx.x; t < T; t += blockDim.x)
+  sync();
+  for (int t = tid; t < T; t += threads)
     if (up[t] == -2)
       for (int w = 0; w < words; ++w) mask[t][w] = 0u;
-  __syncthreads();
+  sync();
 }
 
 __device__ __forceinline__ bool tree_absent(const uint32_t (*mask)[kTreeWords], int t) {
@@ -125,26 +134,16 @@ __global__ void __launch_bounds__(kTreeWarps * 32, D <= 128 ? 2 : 1)
   using B16 = __nv_bfloat16;
   constexpr int TS = S::TS, CPR = S::CPR, KS = S::KS, DT = S::DT, ST = kTreeStages;
   extern __shared__ uint4 smem4[];
-  __shared__ uint32_t masks[kTreeMaxTokens][kTreeWords];
-  __shared__ int up_[kTreeMaxTokens];
+  __shared__ TreeSmem tree;
   __shared__ float wm_[kTreeWarps][16], wl_[kTreeWarps][16];
   pdl_entry();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int g8 = lane >> 2, t4 = lane & 3;
   const int ln = blockIdx.x, split = blockIdx.y, row0 = blockIdx.z * 16, g = ln % a.G, b = ln / a.G;
   const int NQ = min(16, a.rf * a.T - row0), T = a.T;
+  tree_parents(a, b, tree, tid, kTreeWarps * 32);
+  cp_async_commit();
   const int Lp = prefix_length(pre, ln), R = a.rcount;
-  const int up = (Lp + TS - 1) / TS, ur = (R + TS - 1) / TS, uc = (T + TS - 1) / TS, U = up + ur + uc;
-  const int ns = tree_splits(a, U);
-  if (split >= ns) return;
-  const int u0 = (int)((long long)U * split / ns), u1 = (int)((long long)U * (split + 1) / ns);
-  const int mine = (u1 - u0) > warp ? (u1 - u0 - warp + kTreeWarps - 1) / kTreeWarps : 0;
-  if (u1 > up + ur) tree_masks(a, b, masks, up_, status);   // uniform over the block
-  unsigned char* wbase = reinterpret_cast<unsigned char*>(smem4) + (size_t)warp * ST * S::STAGE_BYTES;
-  const unsigned wbase_s = (unsigned)__cvta_generic_to_shared(wbase);
-  const B16* kn = static_cast<const B16*>(a.kn) + b * a.ks[0] + g * a.ks[1];
-  const B16* vn = static_cast<const B16*>(a.vn) + b * a.vs[0] + g * a.vs[1];
-
   int tok[2];   // tokens of the lane's rows g8 and g8 + 8
   unsigned qa[KS][4];
 #pragma unroll
@@ -158,6 +157,18 @@ __global__ void __launch_bounds__(kTreeWarps * 32, D <= 128 ? 2 : 1)
       qa[ks][2 + hr] = r < NQ ? *reinterpret_cast<const unsigned*>(qp + ks * 16 + 2 * t4 + 8) : 0u;
     }
   }
+  const int up = (Lp + TS - 1) / TS, ur = (R + TS - 1) / TS, uc = (T + TS - 1) / TS, U = up + ur + uc;
+  const int ns = tree_splits(a, U);
+  if (split >= ns) {
+    cp_async_wait<0>();
+    return;
+  }
+  const int u0 = (int)((long long)U * split / ns), u1 = (int)((long long)U * (split + 1) / ns);
+  const int mine = (u1 - u0) > warp ? (u1 - u0 - warp + kTreeWarps - 1) / kTreeWarps : 0;
+  unsigned char* wbase = reinterpret_cast<unsigned char*>(smem4) + (size_t)warp * ST * S::STAGE_BYTES;
+  const unsigned wbase_s = (unsigned)__cvta_generic_to_shared(wbase);
+  const B16* kn = static_cast<const B16*>(a.kn) + b * a.ks[0] + g * a.ks[1];
+  const B16* vn = static_cast<const B16*>(a.vn) + b * a.vs[0] + g * a.vs[1];
 
   // Tile u: its segment, first row and row count.
   auto tile = [&](int u, int& first, int& rows) {
@@ -214,6 +225,10 @@ __global__ void __launch_bounds__(kTreeWarps * 32, D <= 128 ? 2 : 1)
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
   for (int k = 0; k < ST - 1; ++k) issue(k, k);
+  if (u1 > up + ur) {   // uniform over the block; the parents' copies are the oldest group
+    cp_async_wait<ST - 1>();
+    tree_masks(a, tree, status, tid, kTreeWarps * 32, [] { __syncthreads(); });
+  }
   for (int k = 0; k < mine; ++k) {
     issue(k + ST - 1, (k + ST - 1) % ST);
     cp_async_wait<ST - 1>();
@@ -227,8 +242,8 @@ __global__ void __launch_bounds__(kTreeWarps * 32, D <= 128 ? 2 : 1)
     // Columns each row sees; drafted tokens whose V is not finite, taken out of the product below.
     unsigned see0 = (1u << rows) - 1, see1 = see0, poison = 0;
     if (cls == 2) {
-      see0 = masks[tok[0]][first >> 5] >> (first & 31) & see0;
-      see1 = masks[tok[1]][first >> 5] >> (first & 31) & see1;
+      see0 = tree.mask[tok[0]][first >> 5] >> (first & 31) & see0;
+      see1 = tree.mask[tok[1]][first >> 5] >> (first & 31) & see1;
       unsigned char* v = st + TS * D * 2;
       const int r = lane & 15;   // two lanes per row of V
       bool bad = false;
@@ -339,24 +354,44 @@ __global__ void __launch_bounds__(kTreeWarps * 32, D <= 128 ? 2 : 1)
     *reinterpret_cast<float2*>(wacc + (g8 + 8) * D + c0) = make_float2(o[jd][2], o[jd][3]);
   }
   __syncthreads();
-  for (int x = tid; x < NQ * D; x += blockDim.x) {
-    const int r = x / D, d = x % D;
+  const size_t orow = (size_t)ln * a.rf * T + row0;
+  const bool whole = a.nsplit == 1;   // no partials, no combine
+  if (tid < NQ) {
     float mx = -INFINITY;
-    for (int w = 0; w < kTreeWarps; ++w) mx = fmaxf(mx, wm_[w][r]);
-    float l = 0.f, ov = 0.f;
+#pragma unroll
+    for (int w = 0; w < kTreeWarps; ++w) mx = fmaxf(mx, wm_[w][tid]);
+    float l = 0.f, f[kTreeWarps];
+#pragma unroll
     for (int w = 0; w < kTreeWarps; ++w) {
-      const float f = wm_[w][r] == -INFINITY ? 0.f : exp2f(wm_[w][r] - mx);
-      l += wl_[w][r] * f;
-      ov += reinterpret_cast<const float*>(reinterpret_cast<unsigned char*>(smem4) +
-                                           (size_t)w * ST * S::STAGE_BYTES)[r * D + d] * f;
+      f[w] = wm_[w][tid] == -INFINITY ? 0.f : exp2f(wm_[w][tid] - mx);
+      l += wl_[w][tid] * f[w];
     }
-    const size_t row = (size_t)ln * a.rf * T + row0 + r;
-    float* pp = tree_part(part, a, split, row);
-    if (d == 0) {
-      pp[0] = mx;
-      pp[1] = u1 > up + ur && tree_absent(masks, (row0 + r) % T) ? -1.f : l;
+    const bool absent = u1 > up + ur && tree_absent(tree.mask, (row0 + tid) % T);
+#pragma unroll
+    for (int w = 0; w < kTreeWarps; ++w) wm_[w][tid] = whole ? f[w] / l : f[w];
+    wl_[0][tid] = absent ? 1.f : 0.f;
+    if (!whole) *reinterpret_cast<float2*>(tree_part(part, a, split, orow + tid)) = make_float2(mx, absent ? -1.f : l);
+  }
+  __syncthreads();
+  for (int x = tid; x < NQ * (D / 4); x += blockDim.x) {
+    const int r = x / (D / 4), c = x % (D / 4) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!whole || wl_[0][r] == 0.f) {
+#pragma unroll
+      for (int w = 0; w < kTreeWarps; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<unsigned char*>(smem4) +
+                                                          (size_t)w * ST * S::STAGE_BYTES + (r * D + c) * 4);
+        const float f = wm_[w][r];
+        v.x = fmaf(y.x, f, v.x);
+        v.y = fmaf(y.y, f, v.y);
+        v.z = fmaf(y.z, f, v.z);
+        v.w = fmaf(y.w, f, v.w);
+      }
     }
-    pp[4 + d] = ov;
+    if (whole)
+      *reinterpret_cast<uint2*>(out + (orow + r) * D + c) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    else
+      *reinterpret_cast<float4*>(tree_part(part, a, split, orow + r) + 4 + c) = v;
   }
 }
 
@@ -399,12 +434,12 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
   using B16 = __nv_bfloat16;
   constexpr int TS = S::TS, ST = S::ST, MR = S::MR, CPR = D / 8;
   extern __shared__ uint4 smem4[];
-  __shared__ uint32_t masks[kTreeMaxTokens][kTreeWords];
-  __shared__ int up_[kTreeMaxTokens];
+  __shared__ TreeSmem tree;
   __shared__ uint64_t q_full, k_full[ST], v_full[ST], k_empty[ST], v_empty[ST], m_full[MR], s_full[2], p_full[2],
       pv_done[2];
   __shared__ uint32_t sh_tmem;
   __shared__ uint32_t sh_poison[ST][2];   // drafted tokens of the stage whose V is not finite
+  if (threadIdx.x < 4) tc::prefetch_tensormap(threadIdx.x < 2 ? &maps.k[threadIdx.x] : &maps.v[threadIdx.x - 2]);
   pdl_entry();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ln = blockIdx.x, split = blockIdx.y, g = ln % a.G, b = ln / a.G, T = a.T;
@@ -413,7 +448,10 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
   const int up = (Lp + TS - 1) / TS, ur = (R + TS - 1) / TS, U = up + ur + (T + TS - 1) / TS;
   const int ns = tree_splits(a, U);
   if (split >= ns) return;
-  const int u0 = (int)((long long)U * split / ns), n = (int)((long long)U * (split + 1) / ns) - u0;
+  // The drafted tokens' units cost about four more (copied and checked by one warp, masks): the last
+  // split gets that many fewer.  pad < U / ns, so no split is empty.
+  const int pad = min(4, U / ns - 1), W = U + (ns > 1 ? max(pad, 0) : 0);
+  const int u0 = (int)((long long)W * split / ns), n = min(U, (int)((long long)W * (split + 1) / ns)) - u0;
   unsigned char* raw = reinterpret_cast<unsigned char*>(smem4);
   unsigned char* base = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
   const uint32_t base_s = tc::smem_u32(base);
@@ -438,7 +476,6 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
     tc::tmem_alloc(&sh_tmem, S::COLS);
     tc::tmem_relinquish();
   }
-  if (u0 + n > up + ur) tree_masks(a, b, masks, up_, status);   // uniform over the block
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -617,11 +654,16 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
         if (in) cp_async16(d, qp + c * 8);
         else *reinterpret_cast<uint4*>(d) = make_uint4(0, 0, 0, 0);
       }
+      if (u0 + n > up + ur) tree_parents(a, b, tree, tid, 32 * live);
       cp_async_commit();
       cp_async_wait<0>();
       tc::fence_proxy_async();
       tc::mbar_arrive(&q_full);
     }
+    // The tree's masks while the first keys are on their way.
+    if (u0 + n > up + ur)
+      tree_masks(a, tree, status, tid, 32 * live,
+                 [&] { asm volatile("bar.sync 1, %0;\n" ::"r"(32 * live) : "memory"); });
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int r = 0; r < n; ++r) {
@@ -653,8 +695,8 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
       if (rows < TS || cls == 2) {
         uint32_t lo = rows >= 32 ? ~0u : (1u << rows) - 1, hi = rows >= 64 ? ~0u : rows > 32 ? (1u << (rows - 32)) - 1 : 0u;
         if (cls == 2) {
-          lo &= masks[t][first >> 5];
-          hi &= masks[t][(first >> 5) + 1];
+          lo &= tree.mask[t][first >> 5];
+          hi &= tree.mask[t][(first >> 5) + 1];
           if ((lo & sh_poison[st][0]) | (hi & sh_poison[st][1])) spoil = NAN;
         }
 #pragma unroll
@@ -706,7 +748,7 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
     } else {
       tc::fence_after();
       const size_t orow = (size_t)ln * a.rf * T + row;
-      const bool absent = u0 + n > up + ur && tree_absent(masks, t);
+      const bool absent = u0 + n > up + ur && tree_absent(tree.mask, t);
       const bool whole = a.nsplit == 1;   // no partials, no combine
       float* pp = tree_part(part, a, split, orow);
       const float inv = 1.f / l;
@@ -747,96 +789,110 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
 }
 
 // ---------------------------------------------------------------- float32: CUDA cores, 32 query rows per CTA
-// Q, K and V tiles in shared memory (rows padded by one 16-byte chunk), every thread a 4 x 4 block of
-// the 32 x 64 scores and a 4 x (D / 16) block of O.
+// Q, K, V and P tiles in shared memory (rows padded by one 16-byte chunk), every thread a 4 x 4 block of
+// the 32 x 64 scores and a 4 x (D / 16) block of O; four elements of the inner index per step, so that
+// the shared-memory reads (12 wavefronts per 64 fused products of a warp) stay below the products.
+// The next K tile is on its way during this tile's softmax and value product, the next V tile during
+// the next scores.
 constexpr int kF32Rows = 32, kF32TS = 64, kF32Threads = 128;
 
 template <int D>
 struct TreeF32Shape {
   static constexpr int LD = D + 4, LDP = kF32TS + 4;
-  static constexpr size_t smem = sizeof(float) * (kF32Rows * LD + 2 * kF32TS * LD + kF32Rows * LDP + kF32TS + 2 * kF32Rows);
+  static constexpr size_t smem = sizeof(float) * (kF32Rows * LD + 2 * kF32TS * LD + kF32Rows * LDP + 2 * kF32TS + 2 * kF32Rows);
 };
 
 template <int D>
-__global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(TreeGeo a, logkv_prefix_t pre, const float* rk,
+__global__ void __launch_bounds__(kF32Threads, 2) tree_f32_kernel(TreeGeo a, logkv_prefix_t pre, const float* rk,
                                                               const float* rv, float* part, int32_t* status) {
   using S = TreeF32Shape<D>;
-  constexpr int LD = S::LD, LDP = S::LDP, TS = kF32TS, NR = kF32Rows, C4 = D / 4, DC = D / 16;
+  constexpr int LD = S::LD, LDP = S::LDP, TS = kF32TS, NR = kF32Rows, C4 = D / 4, J = (D + 63) / 64;
   extern __shared__ uint4 smem4[];
-  __shared__ uint32_t masks[kTreeMaxTokens][kTreeWords];
-  __shared__ int up_[kTreeMaxTokens];
+  __shared__ TreeSmem tree;
   __shared__ int sh_poison[2];
   float* sq = reinterpret_cast<float*>(smem4);
   float* sk = sq + NR * LD;
   float* sv = sk + TS * LD;
   float* sp = sv + TS * LD;
-  float* sm = sp + NR * LDP;
-  float* rm = sm + TS;   // [NR] running maximum and sum
+  float* sm = sp + NR * LDP;   // [2][TS] masses of this tile and the next
+  float* rm = sm + 2 * TS;     // [NR] running maximum and sum
   float* rl = rm + NR;
   pdl_entry();
   const int tid = threadIdx.x;
   const int ln = blockIdx.x, split = blockIdx.y, row0 = blockIdx.z * NR, g = ln % a.G, b = ln / a.G;
   const int T = a.T, NQ = min(NR, a.rf * T - row0);
+  tree_parents(a, b, tree, tid, kF32Threads);
+  for (int x = tid; x < NR * C4; x += kF32Threads) {
+    const int r = x / C4, c = x % C4, row = row0 + r;
+    if (r < NQ)
+      cp_async16(sq + r * LD + 4 * c, static_cast<const float*>(a.q) + b * a.qs[0] + (g * a.rf + row / T) * a.qs[1] +
+                                          (row % T) * a.qs[2] + 4 * c);
+    else
+      *reinterpret_cast<float4*>(sq + r * LD + 4 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  cp_async_commit();
   const int Lp = prefix_length(pre, ln), R = a.rcount;
   const int up = (Lp + TS - 1) / TS, ur = (R + TS - 1) / TS, uc = (T + TS - 1) / TS, U = up + ur + uc;
   const int ns = tree_splits(a, U);
-  if (split >= ns) return;
-  const int u0 = (int)((long long)U * split / ns), u1 = (int)((long long)U * (split + 1) / ns);
-  if (u1 > up + ur) tree_masks(a, b, masks, up_, status);
-  for (int x = tid; x < NR * C4; x += kF32Threads) {
-    const int r = x / C4, c = x % C4, row = row0 + r;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < NQ)
-      v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + b * a.qs[0] +
-                                           (g * a.rf + row / T) * a.qs[1] + (row % T) * a.qs[2] + 4 * c);
-    *reinterpret_cast<float4*>(sq + r * LD + 4 * c) = v;
+  if (split >= ns) {
+    cp_async_wait<0>();
+    return;
   }
+  const int u0 = (int)((long long)U * split / ns), u1 = (int)((long long)U * (split + 1) / ns);
+  const bool drafts = u1 > up + ur;
   if (tid < NR) {
     rm[tid] = -INFINITY;
     rl[tid] = 0.f;
   }
+  auto unit = [&](int u, int& first, int& rows) {
+    const int cls = u < up ? 0 : u < up + ur ? 1 : 2;
+    first = (cls == 0 ? u : cls == 1 ? u - up : u - up - ur) * TS;
+    rows = min(TS, (cls == 0 ? Lp : cls == 1 ? R : T) - first);
+    return cls;
+  };
+  // Tile u of K (with its masses) or V by cp.async; rows past the segment's end are zeros.
+  auto load = [&](int u, bool is_v) {
+    int first, rows;
+    const int cls = unit(u, first, rows);
+    const size_t r0 = cls == 0 ? (size_t)ln * pre.capacity + first : (size_t)ln * a.rcap + first;
+    const long long* st = is_v ? a.vs : a.ks;
+    const float* src = cls == 0   ? static_cast<const float*>(is_v ? pre.v : pre.k) + r0 * D
+                       : cls == 1 ? (is_v ? rv : rk) + r0 * D
+                                  : static_cast<const float*>(is_v ? a.vn : a.kn) + b * st[0] + g * st[1] + first * st[2];
+    const long long stride = cls == 2 ? st[2] : D;
+    float* dst = is_v ? sv : sk;
+    for (int x = tid; x < TS * C4; x += kF32Threads) {
+      const int r = x / C4, c = x % C4;
+      if (r < rows) cp_async16(dst + r * LD + 4 * c, src + r * stride + 4 * c);
+      else *reinterpret_cast<float4*>(dst + r * LD + 4 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (!is_v && tid < TS) {
+      float* m = sm + (u & 1) * TS + tid;
+      if (cls == 0 && tid < rows) cp_async4(m, pre.mass + r0 + tid);
+      else *m = 0.f;
+    }
+    cp_async_commit();
+  };
+  load(u0, false);
+  load(u0, true);
   const int ty = tid >> 4, tx = tid & 15;   // rows 4 ty .. 4 ty + 3; keys tx + 16 j; columns 4 (tx + 16 j)
-  float o[4][DC < 4 ? 4 : DC];
+  float o[4][4 * J];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < (DC < 4 ? 4 : DC); ++j) o[i][j] = 0.f;
-  const float* kn = static_cast<const float*>(a.kn) + b * a.ks[0] + g * a.ks[1];
-  const float* vn = static_cast<const float*>(a.vn) + b * a.vs[0] + g * a.vs[1];
+    for (int j = 0; j < 4 * J; ++j) o[i][j] = 0.f;
+  if (drafts) {   // uniform over the block; the oldest group holds Q and the parents
+    cp_async_wait<2>();
+    tree_masks(a, tree, status, tid, kF32Threads, [] { __syncthreads(); });
+  }
+  int tok[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tok[i] = (row0 + min(4 * ty + i, NQ - 1)) % T;
   for (int u = u0; u < u1; ++u) {
-    const int cls = u < up ? 0 : u < up + ur ? 1 : 2;
-    const int first = (cls == 0 ? u : cls == 1 ? u - up : u - up - ur) * TS;
-    const int rows = min(TS, (cls == 0 ? Lp : cls == 1 ? R : T) - first);
-    const size_t r0 = cls == 0 ? (size_t)ln * pre.capacity + first : (size_t)ln * a.rcap + first;
-    const float* kb = cls == 0 ? static_cast<const float*>(pre.k) + r0 * D : cls == 1 ? rk + r0 * D : kn + first * a.ks[2];
-    const float* vb = cls == 0 ? static_cast<const float*>(pre.v) + r0 * D : cls == 1 ? rv + r0 * D : vn + first * a.vs[2];
-    const long long kst = cls == 2 ? a.ks[2] : D, vst = cls == 2 ? a.vs[2] : D;
-    __syncthreads();   // the previous tile's K, V and P have been read
-    if (tid < 2) sh_poison[tid] = 0;
-    for (int x = tid; x < TS * C4; x += kF32Threads) {
-      const int r = x / C4, c = x % C4;
-      if (r < rows) {
-        cp_async16(sk + r * LD + 4 * c, kb + r * kst + 4 * c);
-        cp_async16(sv + r * LD + 4 * c, vb + r * vst + 4 * c);
-      } else {
-        *reinterpret_cast<float4*>(sk + r * LD + 4 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
-        *reinterpret_cast<float4*>(sv + r * LD + 4 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-    }
-    if (tid < TS) sm[tid] = cls == 0 && tid < rows ? pre.mass[r0 + tid] * a.mass_log2 : 0.f;
-    cp_async_commit();
-    cp_async_wait<0>();
-    __syncthreads();
-    if (cls == 2) {   // drafted tokens whose V is not finite leave the product; their rows' sums become NaN
-      for (int x = tid; x < rows * D; x += kF32Threads) {
-        float* v = sv + x / D * LD + x % D;
-        if (!isfinite(*v)) {
-          *v = 0.f;
-          atomicOr(&sh_poison[x / D >> 5], 1 << (x / D & 31));
-        }
-      }
-      __syncthreads();
-    }
+    int first, rows;
+    const int cls = unit(u, first, rows);
+    cp_async_wait<1>();
+    __syncthreads();   // K and the masses are here
     float s[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -859,9 +915,27 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(TreeGeo a, logkv_
           s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
         }
     }
+    __syncthreads();   // K has been read
+    if (u + 1 < u1) load(u + 1, false);
+    if (cls == 2) {
+      // Drafted tokens whose V is not finite leave the product; the rows that see them get a NaN sum.
+      if (tid < 2) sh_poison[tid] = 0;
+      if (u + 1 < u1) cp_async_wait<1>();
+      else cp_async_wait<0>();
+      __syncthreads();
+      for (int x = tid; x < rows * D; x += kF32Threads) {
+        float* v = sv + x / D * LD + x % D;
+        if (!isfinite(*v)) {
+          *v = 0.f;
+          atomicOr(&sh_poison[x / D >> 5], 1 << (x / D & 31));
+        }
+      }
+      __syncthreads();
+    }
+    const float* mass = sm + (u & 1) * TS;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = 4 * ty + i, t = (row0 + min(r, NQ - 1)) % T;
+      const int r = 4 * ty + i;
       float mt = -INFINITY;
       bool bad = false;
 #pragma unroll
@@ -869,10 +943,10 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(TreeGeo a, logkv_
         const int col = tx + 16 * j;
         bool see = col < rows;
         if (cls == 2 && see) {
-          see = masks[t][(first + col) >> 5] >> ((first + col) & 31) & 1;
+          see = tree.mask[tok[i]][(first + col) >> 5] >> ((first + col) & 31) & 1;
           bad |= see && (sh_poison[col >> 5] >> (col & 31) & 1);
         }
-        s[i][j] = see ? fmaf(s[i][j], a.scale_log2, sm[col]) : -INFINITY;
+        s[i][j] = see ? fmaf(s[i][j], a.scale_log2, mass[col] * a.mass_log2) : -INFINITY;
         mt = fmaxf(mt, s[i][j]);
       }
 #pragma unroll
@@ -895,42 +969,47 @@ __global__ void __launch_bounds__(kF32Threads) tree_f32_kernel(TreeGeo a, logkv_
       }
       // The row's 16 threads also own its columns of O.
 #pragma unroll
-      for (int j = 0; j < (DC < 4 ? 4 : DC); ++j) o[i][j] *= al;
+      for (int j = 0; j < 4 * J; ++j) o[i][j] *= al;
     }
-    __syncwarp();   // P of rows 4 ty .. 4 ty + 3 is written and read by the same half warp
-#pragma unroll 4
-    for (int n = 0; n < TS; ++n) {
-      float p[4];
+    if (u + 1 < u1) cp_async_wait<1>();
+    else cp_async_wait<0>();
+    __syncthreads();   // V is here (P of rows 4 ty .. 4 ty + 3 is written and read by the same half warp)
+#pragma unroll 2
+    for (int n = 0; n < TS; n += 4) {
+      float4 p[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = sp[(4 * ty + i) * LDP + n];
+      for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4*>(sp + (4 * ty + i) * LDP + n);
 #pragma unroll
-      for (int j = 0; j < (DC + 3) / 4; ++j) {
+      for (int j = 0; j < J; ++j) {
         const int c = 4 * (tx + 16 * j);
         if (c < D) {
-          const float4 v = *reinterpret_cast<const float4*>(sv + n * LD + c);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            o[i][4 * j] = fmaf(p[i], v.x, o[i][4 * j]);
-            o[i][4 * j + 1] = fmaf(p[i], v.y, o[i][4 * j + 1]);
-            o[i][4 * j + 2] = fmaf(p[i], v.z, o[i][4 * j + 2]);
-            o[i][4 * j + 3] = fmaf(p[i], v.w, o[i][4 * j + 3]);
+          for (int e = 0; e < 4; ++e) {
+            const float4 v = *reinterpret_cast<const float4*>(sv + (n + e) * LD + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float pe = e == 0 ? p[i].x : e == 1 ? p[i].y : e == 2 ? p[i].z : p[i].w;
+              o[i][4 * j] = fmaf(pe, v.x, o[i][4 * j]);
+              o[i][4 * j + 1] = fmaf(pe, v.y, o[i][4 * j + 1]);
+              o[i][4 * j + 2] = fmaf(pe, v.z, o[i][4 * j + 2]);
+              o[i][4 * j + 3] = fmaf(pe, v.w, o[i][4 * j + 3]);
+            }
           }
         }
       }
     }
+    __syncthreads();   // V has been read
+    if (u + 1 < u1) load(u + 1, true);
   }
-  __syncwarp();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = 4 * ty + i;
     if (r >= NQ) continue;
     float* pp = tree_part(part, a, split, (size_t)ln * a.rf * T + row0 + r);
-    if (tx == 0) {
-      pp[0] = rm[r];
-      pp[1] = u1 > up + ur && tree_absent(masks, (row0 + r) % T) ? -1.f : rl[r];
-    }
+    if (tx == 0)
+      *reinterpret_cast<float2*>(pp) = make_float2(rm[r], drafts && tree_absent(tree.mask, tok[i]) ? -1.f : rl[r]);
 #pragma unroll
-    for (int j = 0; j < (DC + 3) / 4; ++j) {
+    for (int j = 0; j < J; ++j) {
       const int c = 4 * (tx + 16 * j);
       if (c < D) *reinterpret_cast<float4*>(pp + 4 + c) = make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
     }
@@ -1107,7 +1186,7 @@ static int launch_tree_bf16(const TreeGeo& a, const TreePlan& p, const logkv_pre
   launch_pdl(kern, dim3(a.B * a.G, p.nsplit, tiles), kTreeWarps * 32, S::smem, st, a, pre,
              static_cast<const B16*>(s.recent_k), static_cast<const B16*>(s.recent_v), static_cast<B16*>(x.out), part,
              x.status);
-  launch_tree_combine<B16, D, 16>(a, pre, part, x.out, st);
+  if (p.nsplit > 1) launch_tree_combine<B16, D, 16>(a, pre, part, x.out, st);
   return launch_status();
 }
 

@@ -57,10 +57,10 @@ class LogKVDecoder:
         rows = (_lib.Rows * len(bufs))(*[_lib.Rows(t.data_ptr(), t.numel() * t.element_size() // cache.batch_size)
                                          for t in bufs])
         dev = self._k.device
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             _lib.check(_lib.lib().logkv_reorder_rows(
-                rows, len(bufs), cache.batch_size, index.data_ptr(), int(index.dtype == torch.int64),
-                cache._read.status.data_ptr(), ctypes.c_void_p(_lib.stream_ptr(dev))), "logkv_reorder_rows")
+                rows, len(bufs), cache.batch_size, index.data_ptr(), index.dtype == torch.int64,
+                cache._read.status_ptr, _lib.stream_ptr(dev)), "logkv_reorder_rows")
 
     def step(self, q, k, v, *, k_raw, input_pos=None, span_ends=None, span_ends_device=None, out=None):
         """One token: q [B, H, 1, D], k / v / k_raw [B, G, 1, D]; returns the attention output

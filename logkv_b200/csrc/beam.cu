@@ -21,6 +21,7 @@ namespace logkv {
 constexpr int kBeamThreads = 256;
 constexpr int kBeamCand = 1024;    // gathered candidates at most
 constexpr int kBeamVecs = 4;       // 16-byte vectors per thread and chunk
+constexpr int kBeamGroups = 16;    // groups of chunks whose maxima a thread keeps
 
 struct BeamGeo {
   const void* logits;
@@ -31,7 +32,7 @@ struct BeamGeo {
   long long n_stride, w_stride;
   int W, V, k, S, keep;
   int chunks;     // chunks (kBeamThreads x kBeamVecs vectors) of a beam's vocabulary, divided among S slices
-  // Scratch: per (request, beam, slice) the sum of 2^((x - top) e') and top; per request [k][W * S] lists.
+  // Scratch per (request, beam, slice): the sum of 2^((x - top) e') and top; the k best logits, sorted.
   double* sum;
   float* top;
   float* val;
@@ -140,11 +141,10 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
 // (below 2e-7), the same way for every beam.
 constexpr float kLog2e = 1.44269502f;
 
-// A CTA walks its slice in chunks, the next chunk's loads in flight.  Every thread keeps the running
-// maximum and sum of its own terms.  Candidates above the running threshold go to a buffer; a buffer
-// that fills up is cut to its k best, which raises the threshold.  The first chunk's threshold comes from
-// the groups' maxima.  Later elements equal to the threshold are not needed: k elements at or above it
-// have lower indices.
+// A CTA walks its slice in chunks, the next chunk's loads in flight and no barrier in between: every
+// thread keeps the running maximum and sum of its own terms, and the maximum of every group of chunks.
+// The threads' maxima give the threshold; the few (thread, group) pairs that reach it read their
+// logits again (from L2) and gather.
 template <typename T>
 __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) {
   using U64 = unsigned long long;
@@ -153,12 +153,12 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
   __shared__ unsigned gm[kBeamThreads];
   __shared__ unsigned sh_t;
   __shared__ U64 cand[kBeamCand];
+  __shared__ float tops[kBeamGroups][kBeamThreads];
   __shared__ float wmax[kBeamThreads / 32];
   __shared__ double wsum[kBeamThreads / 32];
   __shared__ int isum[kBeamThreads / 32];
-  __shared__ int sh_n;
-  __shared__ float sh_cut;
-  __shared__ unsigned xs[NW * kBeamThreads];
+  __shared__ int sh_n, sh_h;
+  __shared__ unsigned short hits[kBeamGroups * kBeamThreads];
   pdl_entry();
   const int tid = threadIdx.x, slice = blockIdx.x, w = blockIdx.y % a.W, n = blockIdx.y / a.W, k = a.k;
   // The row from the 16-byte boundary at or below its start: element e of it is logit e - lead.
@@ -167,53 +167,20 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
   const uint4* vec = reinterpret_cast<const uint4*>(row - lead);
   const int nvec = (a.V + lead + VN - 1) / VN;
   const int c0 = (int)((long long)a.chunks * slice / a.S), c1 = (int)((long long)a.chunks * (slice + 1) / a.S);
-  // Cut the buffer's m entries (m >= 1) to the k best, sorted; the k-th's value is the new threshold.
-  auto cut = [&](int m) {
-    U64 mine[kBeamCand / kBeamThreads];
-    int rank[kBeamCand / kBeamThreads];
-#pragma unroll
-    for (int i = 0; i < kBeamCand / kBeamThreads; ++i) {
-      const int at = tid + i * kBeamThreads;
-      mine[i] = at < m ? cand[at] : 0ull;
-      rank[i] = at < m ? 0 : k;
-      if (at < m) {
-#pragma unroll 8
-        for (int j = 0; j < m; ++j) rank[i] += cand[j] > mine[i];
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kBeamCand / kBeamThreads; ++i)
-      if (rank[i] < k) {
-        cand[rank[i]] = mine[i];
-        if (rank[i] == k - 1) sh_cut = key_value(mine[i]);
-      }
-    if (tid == 0) sh_n = min(m, k);
-    __syncthreads();
-  };
-  unsigned next[NW], x[NW];
-  auto fetch = [&](int c) {
+  const int per = (c1 - c0 + kBeamGroups - 1) / kBeamGroups;   // chunks per group
+  // Vocabulary index of element e of the thread's word i in chunk c.
+  auto index = [&](int c, int i, int e) { return (c * CH + i / 4 * kBeamThreads + tid) * VN + i % 4 * WN + e - lead; };
+  auto fetch = [&](int c, unsigned* x) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = c * CH + i * kBeamThreads + tid;
       uint4 v = make_uint4(Word::kNone, Word::kNone, Word::kNone, Word::kNone);
-      if (j < nvec) v = __ldcs(vec + j);
-      next[4 * i] = v.x, next[4 * i + 1] = v.y, next[4 * i + 2] = v.z, next[4 * i + 3] = v.w;
+      if (j < nvec) v = __ldg(vec + j);
+      x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
     }
   };
-  // Vocabulary index of element e of the thread's word i in chunk c.
-  auto index = [&](int c, int i, int e) { return (c * CH + i / 4 * kBeamThreads + tid) * VN + i % 4 * WN + e - lead; };
-  if (tid == 0) {
-    sh_n = 0;
-    sh_cut = -INFINITY;
-  }
-  const int full = max(4 * k, 128);   // entries that call for a cut
-  float cutoff = -INFINITY, m = -INFINITY, s = 0.f;
-  fetch(c0);
-  for (int c = c0; c < c1; ++c) {
-#pragma unroll
-    for (int i = 0; i < NW; ++i) x[i] = next[i];
-    if (c == 0 || (c + 1) * CH >= nvec) {   // the row's first and last vectors may hold a neighbour's logits
+  auto edges = [&](int c, unsigned* x) {   // the row's first and last vectors may hold a neighbour's logits
+    if (c == 0 || (c + 1) * CH >= nvec) {
 #pragma unroll
       for (int i = 0; i < NW; ++i)
 #pragma unroll
@@ -222,7 +189,16 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
           if (v < 0 || v >= a.V) x[i] = Word::mask(x[i], e);
         }
     }
-    if (c + 1 < c1) fetch(c + 1);
+  };
+  float m = -INFINITY, s = 0.f, mg = -INFINITY;
+  unsigned next[NW];
+  fetch(c0, next);
+  for (int c = c0; c < c1; ++c) {
+    unsigned x[NW];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) x[i] = next[i];
+    edges(c, x);
+    if (c + 1 < c1) fetch(c + 1, next);
     unsigned mx = x[0];
 #pragma unroll
     for (int i = 1; i < NW; ++i) mx = Word::max(mx, x[i]);
@@ -230,6 +206,12 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
     if (mt > m) {
       s = m == -INFINITY ? s : s * tc::ex2((m - mt) * kLog2e);   // s without a finite maximum: 0 or NaN
       m = mt;
+    }
+    mg = fmaxf(mg, mt);
+    const int in = (c - c0) % per;
+    if (in == per - 1 || c == c1 - 1) {
+      tops[(c - c0) / per][tid] = mg;
+      mg = -INFINITY;
     }
     const float ref = m == -INFINITY ? 0.f : m;
     const uint64_t e2 = tc::f2pack(kLog2e, kLog2e), m2 = tc::f2pack(-ref, -ref);
@@ -244,103 +226,94 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
     float s0, s1;
     tc::f2unpack(s2, s0, s1);
     s += s0 + s1;
-    // Candidates of this chunk: above the threshold, in the first chunk at or above the groups'.
-    bool first = c == c0;
-    if (first) {
-      const unsigned none = order32(-INFINITY);
-      const unsigned t = max(group_threshold<unsigned>(order32(mt), k, gm, &sh_t), none);
-      cutoff = t == none ? -INFINITY : __uint_as_float(t & 0x80000000u ? t & 0x7fffffffu : ~t);
-      first = t != none;
-    }
-    int last = -1;
-    if (first ? mt >= cutoff : mt > cutoff) {
-#pragma unroll
-      for (int i = 0; i < NW; ++i)
-#pragma unroll
-        for (int e = 0; e < WN; ++e) {
-          const float v = Word::get(x[i], e);
-          if (first ? v >= cutoff : v > cutoff) {
-            last = atomicAdd(&sh_n, 1);
-            if (last < kBeamCand) cand[last] = beam_key(v, index(c, i, e));
-          }
-        }
-    }
-    if (!__syncthreads_or(last >= full)) continue;
-    const int got = sh_n;
-    if (got <= kBeamCand) {
-      cut(got);
-    } else {
-      // More than the buffer holds: the k-th largest key of the buffer's earlier entries and this chunk,
-      // bit by bit.
-      const int begin = c * CH * VN - lead;   // earlier entries have lower indices
-      U64 old[kBeamCand / kBeamThreads];
-#pragma unroll
-      for (int i = 0; i < kBeamCand / kBeamThreads; ++i) {
-        old[i] = cand[tid + i * kBeamThreads];
-        if ((int)(0xffffffffu - (unsigned)old[i]) >= begin) old[i] = 0ull;
-      }
-      // (From shared memory: unrolled over registers, the keys would be kept over the 64 rounds.)
-#pragma unroll
-      for (int i = 0; i < NW; ++i) xs[i * kBeamThreads + tid] = x[i];
-      auto key = [&](int q) {
-        const int i = q / WN, e = q % WN;
-        const float v = Word::get(xs[i * kBeamThreads + tid], e);
-        return v > -INFINITY ? beam_key(v, index(c, i, e)) : 0ull;
-      };
-      U64 kt = 0;
-      for (int bit = 63; bit >= 0; --bit) {
-        const U64 test = kt | 1ull << bit;
-        int cnt = 0;
-#pragma unroll 1
-        for (int q = 0; q < NW * WN; ++q) cnt += key(q) >= test;
-#pragma unroll
-        for (int i = 0; i < kBeamCand / kBeamThreads; ++i) cnt += old[i] >= test;
-        if (block_sum(cnt, isum) >= k) kt = test;
-      }
-      if (tid == 0) sh_n = 0;
-      __syncthreads();
-#pragma unroll 1
-      for (int q = 0; q < NW * WN; ++q)
-        if (key(q) >= kt) cand[atomicAdd(&sh_n, 1)] = key(q);
-#pragma unroll
-      for (int i = 0; i < kBeamCand / kBeamThreads; ++i)
-        if (old[i] >= kt) cand[atomicAdd(&sh_n, 1)] = old[i];
-      __syncthreads();
-      cut(k);
-    }
-    cutoff = sh_cut;
   }
-  __syncthreads();
-  const int nc = sh_n;
-  if (nc) cut(nc);   // sorted
+  if (tid == 0) sh_n = sh_h = 0;
+  // The slice's sum: the threads' maxima and float32 sums, joined in float64.
   const float mw = warp_max(m);
   if ((tid & 31) == 0) wmax[tid >> 5] = mw;
-  __syncthreads();
-  float t = wmax[0];
+  const unsigned none = order32(-INFINITY);
+  const unsigned t = max(group_threshold<unsigned>(order32(m), k, gm, &sh_t), none);   // its barriers publish wmax
+  float top = wmax[0];
 #pragma unroll
-  for (int i = 1; i < kBeamThreads / 32; ++i) t = fmaxf(t, wmax[i]);
-  double sd = m == -INFINITY ? (double)s : (double)s * exp2f((m - t) * kLog2e);   // s is 0 or NaN without a maximum
+  for (int i = 1; i < kBeamThreads / 32; ++i) top = fmaxf(top, wmax[i]);
+  double sd = m == -INFINITY ? (double)s : (double)s * exp2f((m - top) * kLog2e);
 #pragma unroll
   for (int off = 16; off; off >>= 1) sd += __shfl_xor_sync(0xffffffffu, sd, off);
   if ((tid & 31) == 0) wsum[tid >> 5] = sd;
+  // Gather the logits at or above the threshold (all above -inf when fewer than k groups hold any): the
+  // (thread, group) pairs that reach it in a list, a warp to each, a lane to each of its logits.
+  const float least = t == none ? -INFINITY : __uint_as_float(t & 0x80000000u ? t & 0x7fffffffu : ~t);
+  for (int g = 0; g * per < c1 - c0; ++g)
+    if (tops[g][tid] >= least && tops[g][tid] > -INFINITY) hits[atomicAdd(&sh_h, 1)] = (unsigned short)(g << 8 | tid);
   __syncthreads();
+  const T* base = row - lead;
+  for (int h = tid >> 5; h < sh_h; h += kBeamThreads / 32) {
+    const int g = hits[h] >> 8, th = hits[h] & 255;
+    for (int c = c0 + g * per; c < min(c1, c0 + (g + 1) * per); ++c)
+      for (int q = tid & 31; q < NV * VN; q += 32) {
+        const int e = (c * CH + q / VN * kBeamThreads + th) * VN + q % VN, v = e - lead;
+        if (v >= 0 && v < a.V) {
+          const float f = (float)base[e];
+          if (f >= least && f > -INFINITY) {
+            const int at = atomicAdd(&sh_n, 1);
+            if (at < kBeamCand) cand[at] = beam_key(f, v);
+          }
+        }
+      }
+  }
+  __syncthreads();
+  int nc = sh_n;
   const size_t at = (size_t)blockIdx.y * a.S + slice;
   if (tid == 0) {
     double total = 0.0;
     for (int i = 0; i < kBeamThreads / 32; ++i) total += wsum[i];
     a.sum[at] = total;
-    a.top[at] = t;
+    a.top[at] = top;
   }
-  const int L = a.W * a.S;
-  float* val = a.val + (size_t)n * k * L + w * a.S + slice;
-  int* idx = a.idx + (size_t)n * k * L + w * a.S + slice;
-  for (int i = tid; i < k; i += kBeamThreads) {
-    val[(size_t)i * L] = i < nc ? key_value(cand[i]) : 0.f;
-    idx[(size_t)i * L] = i < nc ? (int)(0xffffffffu - (unsigned)cand[i]) : -1;
+  if (nc > kBeamCand) {
+    // More than the buffer holds: the k-th largest key bit by bit, the logits read again each time.
+    auto visit = [&](auto take) {
+      for (int c = c0; c < c1; ++c)
+#pragma unroll 1
+        for (int i = 0; i < NV * VN; ++i) {
+          const int e = (c * CH + i / VN * kBeamThreads + tid) * VN + i % VN, v = e - lead;
+          if (v >= 0 && v < a.V && (float)base[e] > -INFINITY) take(beam_key((float)base[e], v));
+        }
+    };
+    U64 kt = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const U64 test = kt | 1ull << bit;
+      int cnt = 0;
+      visit([&](U64 key) { cnt += key >= test; });
+      if (block_sum(cnt, isum) >= k) kt = test;
+    }
+    if (tid == 0) sh_n = 0;
+    __syncthreads();
+    visit([&](U64 key) {
+      if (key >= kt) cand[atomicAdd(&sh_n, 1)] = key;
+    });
+    __syncthreads();
+    nc = k;
   }
+  float* val = a.val + at * k;
+  int* idx = a.idx + at * k;
+  for (int i = tid; i < nc; i += kBeamThreads) {
+    const U64 me = cand[i];
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < nc; ++j) above += cand[j] > me;
+    if (above < k) {
+      val[above] = key_value(me);
+      idx[above] = (int)(0xffffffffu - (unsigned)me);
+    }
+  }
+  for (int i = nc + tid; i < k; i += kBeamThreads) idx[i] = -1;
 }
 
 // ---------------------------------------------------------------- B2
+// The candidates in rounds of up to kBeamRound, the k best so far among each round's.
+constexpr int kBeamRound = 2048, kBeamEach = kBeamRound / kBeamThreads;
+
 __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
   using U64 = unsigned long long;
   __shared__ U64 gm[kBeamThreads];
@@ -348,98 +321,135 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
   __shared__ U64 cand[kBeamCand];
   __shared__ int cidx[kBeamCand];
   __shared__ double lse[LOGKV_BEAM_MAX_WIDTH];
+  __shared__ float prior[LOGKV_BEAM_MAX_WIDTH];
   __shared__ int isum[kBeamThreads / 32];
   __shared__ int sh_n;
   __shared__ U64 best[LOGKV_BEAM_MAX_K];
   __shared__ int bflat[LOGKV_BEAM_MAX_K];
   __shared__ short place[LOGKV_BEAM_MAX_K];
   pdl_entry();
-  const int tid = threadIdx.x, lane = tid & 31, n = blockIdx.x, W = a.W, S = a.S, k = a.k, L = W * S;
+  const int tid = threadIdx.x, lane = tid & 31, n = blockIdx.x, W = a.W, S = a.S, k = a.k;
+  const float* val = a.val + (size_t)n * W * S * k;
+  const int* idx = a.idx + (size_t)n * W * S * k;
+  // Candidate i is place i / L of list i % L, so that every group of threads sees a mix of lists.
+  const int L = W * S, all = L * k;
+  // The first round's candidates are on their way while the beams' sums are joined.
+  float v[kBeamEach];
+  int vi[kBeamEach];
+  auto fetch = [&](int from, int upto) {
+#pragma unroll
+    for (int i = 0; i < kBeamEach; ++i) {
+      const int at = from + i * kBeamThreads + tid;
+      const int where = at % L * k + at / L;
+      vi[i] = at < upto ? idx[where] : -1;
+      v[i] = at < upto ? val[where] : 0.f;
+    }
+  };
+  int upto = min(all, kBeamRound);
+  fetch(0, upto);
   // log sum exp of each beam in float64; NaN for a beam that offers nothing.
   for (int w = tid >> 5; w < W; w += kBeamThreads / 32) {
     const size_t at = (size_t)(n * W + w) * S;
-    float m = -INFINITY;
-    for (int i = lane; i < S; i += 32) m = fmaxf(m, a.sum[at + i] > 0.0 ? a.top[at + i] : -INFINITY);
+    const float r = a.scores[n * W + w];
+    double si = lane < S ? a.sum[at + lane] : 0.0;
+    float ti = lane < S ? a.top[at + lane] : -INFINITY;
+    float m = si > 0.0 ? ti : -INFINITY;
+    for (int i = lane + 32; i < S; i += 32) m = fmaxf(m, a.sum[at + i] > 0.0 ? a.top[at + i] : -INFINITY);
     m = warp_max(m);
-    double s = 0.0;
-    for (int i = lane; i < S; i += 32) {
-      const double si = a.sum[at + i];
-      if (si != 0.0) s += si * exp2(((double)a.top[at + i] - (double)m) * kLog2e);   // a NaN stays
+    double s = si != 0.0 ? si * exp2(((double)ti - (double)m) * kLog2e) : 0.0;   // a NaN stays
+    for (int i = lane + 32; i < S; i += 32) {
+      si = a.sum[at + i];
+      if (si != 0.0) s += si * exp2(((double)a.top[at + i] - (double)m) * kLog2e);
     }
 #pragma unroll
     for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
     if (lane == 0) {
-      const float r = a.scores[n * W + w];
       const double z = (double)m + log2(s) / (double)kLog2e;
       lse[w] = isfinite(r) && isfinite(z) ? z : nan("");
+      prior[w] = r;
     }
   }
-  if (tid == 0) sh_n = 0;
   __syncthreads();
-  const float* val = a.val + (size_t)n * k * L;
-  const int* idx = a.idx + (size_t)n * k * L;
-  // Candidate i = place * L + list.  Score key, 0 for none.
-  auto key = [&](int i, int& flat) -> U64 {
-    const int v = idx[i], w = i % L / S;
-    flat = w * a.V + v;
-    if (v < 0 || isnan(lse[w])) return 0ull;
-    return order64((double)a.scores[n * W + w] + ((double)val[i] - lse[w]));
-  };
-  const int all = k * L;
-  U64 mine = 0;
-  int flat;
-  for (int i = tid; i < all; i += kBeamThreads) {
-    const U64 q = key(i, flat);
-    mine = q > mine ? q : mine;
-  }
-  U64 t = group_threshold<U64>(mine, k, gm, &sh_t);
-  t = t ? t : 1;
-  int cnt = 0;
-  for (int i = tid; i < all; i += kBeamThreads) cnt += key(i, flat) >= t;
-  int total = block_sum(cnt, isum);
-  int tf = 0x7fffffff;   // flat indices taken at the threshold itself
-  if (total > kBeamCand) {
-    t = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const U64 test = t | 1ull << bit;
-      cnt = 0;
-      for (int i = tid; i < all; i += kBeamThreads) cnt += key(i, flat) >= test;
-      if (block_sum(cnt, isum) >= k) t = test;
+  int found = 0;
+  for (int from = 0; from < all;) {
+    // Keys (score, 0 for none) and flat indices of the round; the best so far take the last places.
+    U64 key[kBeamEach];
+    int flat[kBeamEach];
+    U64 mine = 0;
+#pragma unroll
+    for (int i = 0; i < kBeamEach; ++i) {
+      const int at = from + i * kBeamThreads + tid;
+      key[i] = 0;
+      flat[i] = 0x7fffffff;
+      if (vi[i] >= 0) {
+        const int w = at % L / S;
+        if (!isnan(lse[w])) {
+          key[i] = order64((double)prior[w] + ((double)v[i] - lse[w]));
+          flat[i] = w * a.V + vi[i];
+        }
+      } else if (at >= upto && at - upto < found) {
+        key[i] = best[at - upto];
+        flat[i] = bflat[at - upto];
+      }
+      mine = key[i] > mine ? key[i] : mine;
     }
+    if (tid == 0) sh_n = 0;
+    U64 t = group_threshold<U64>(mine, k, gm, &sh_t);
     t = t ? t : 1;
-    cnt = 0;
-    for (int i = tid; i < all; i += kBeamThreads) cnt += key(i, flat) > t;
-    const int need = k - block_sum(cnt, isum);
-    int low = 0;   // the `need` lowest flat indices among the ties: flat <= tf
-    for (int bit = 30; bit >= 0; --bit) {
-      const int test = low | 1 << bit;
+    const int next = upto, step = min(all, upto + kBeamRound - k);
+    if (next < all) fetch(next, step);
+    int cnt = 0;
+#pragma unroll
+    for (int i = 0; i < kBeamEach; ++i) cnt += key[i] >= t;
+    int tf = 0x7fffffff;   // flat indices taken at the threshold itself
+    if (block_sum(cnt, isum) > kBeamCand) {
+      t = 0;
+      for (int bit = 63; bit >= 0; --bit) {
+        const U64 test = t | 1ull << bit;
+        cnt = 0;
+#pragma unroll
+        for (int i = 0; i < kBeamEach; ++i) cnt += key[i] >= test;
+        if (block_sum(cnt, isum) >= k) t = test;
+      }
       cnt = 0;
-      for (int i = tid; i < all; i += kBeamThreads) cnt += key(i, flat) == t && flat < test;
-      if (block_sum(cnt, isum) < need) low = test;
+#pragma unroll
+      for (int i = 0; i < kBeamEach; ++i) cnt += key[i] > t;
+      const int need = k - block_sum(cnt, isum);
+      int low = 0;   // the `need` lowest flat indices among the ties: flat <= low
+      for (int bit = 30; bit >= 0; --bit) {
+        const int test = low | 1 << bit;
+        cnt = 0;
+#pragma unroll
+        for (int i = 0; i < kBeamEach; ++i) cnt += key[i] == t && flat[i] < test;
+        if (block_sum(cnt, isum) < need) low = test;
+      }
+      tf = low;
     }
-    tf = low;
-  }
-  for (int i = tid; i < all; i += kBeamThreads) {
-    const U64 q = key(i, flat);
-    if (q > t || (q == t && flat <= tf)) {
-      const int at = atomicAdd(&sh_n, 1);
-      cand[at] = q;
-      cidx[at] = flat;
+#pragma unroll
+    for (int i = 0; i < kBeamEach; ++i)
+      if (key[i] > t || (key[i] == t && flat[i] <= tf)) {
+        const int at = atomicAdd(&sh_n, 1);
+        cand[at] = key[i];
+        cidx[at] = flat[i];
+      }
+    __syncthreads();
+    const int nc = sh_n;
+    for (int i = tid; i < nc; i += kBeamThreads) {
+      const U64 me = cand[i];
+      const int mf = cidx[i];
+      int above = 0;
+#pragma unroll 4
+      for (int j = 0; j < nc; ++j) above += cand[j] > me || (cand[j] == me && cidx[j] < mf);
+      if (above < k) {
+        best[above] = me;
+        bflat[above] = mf;
+      }
     }
+    found = min(nc, k);
+    from = next;
+    upto = step;
+    __syncthreads();
   }
-  __syncthreads();
-  const int nc = sh_n, found = min(nc, k);
-  for (int i = tid; i < nc; i += kBeamThreads) {
-    const U64 me = cand[i];
-    const int mf = cidx[i];
-    int above = 0;
-    for (int j = 0; j < nc; ++j) above += cand[j] > me || (cand[j] == me && cidx[j] < mf);
-    if (above < k) {
-      best[above] = me;
-      bflat[above] = mf;
-    }
-  }
-  __syncthreads();
   if (!a.keep) {
     for (int i = tid; i < k; i += kBeamThreads) place[i] = (short)i;
   } else if (tid == 0) {

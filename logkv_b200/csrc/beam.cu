@@ -21,7 +21,8 @@ namespace logkv {
 constexpr int kBeamThreads = 256;
 constexpr int kBeamCand = 1024;    // gathered candidates at most
 constexpr int kBeamVecs = 4;       // 16-byte vectors per thread and chunk
-constexpr int kBeamGroups = 16;    // groups of chunks whose maxima a thread keeps
+constexpr int kBeamGroups = 32;    // groups of chunks whose maxima a thread keeps
+constexpr int kBeamHits = 1024;    // (thread, group) pairs that reach the threshold, at most
 
 struct BeamGeo {
   const void* logits;
@@ -30,8 +31,10 @@ struct BeamGeo {
   long long* out_rows;
   long long* out_tokens;
   long long n_stride, w_stride;
-  int W, V, k, S, keep;
-  int chunks;     // chunks (kBeamThreads x kBeamVecs vectors) of a beam's vocabulary, divided among S slices
+  int W, V, k, keep;
+  int rows;       // beams in all
+  int chunks;     // chunks (kBeamThreads x kBeamVecs vectors) of a beam's vocabulary
+  int S;          // slices of a beam at most
   // Scratch per (request, beam, slice): the sum of 2^((x - top) e') and top; the k best logits, sorted.
   double* sum;
   float* top;
@@ -76,6 +79,7 @@ __device__ __forceinline__ int block_sum(int v, int* sh) {
 // 2 k.  `gm`: one entry per thread.
 template <typename K>
 __device__ __forceinline__ K group_threshold(K mine, int k, K* gm, K* sh) {
+  constexpr int N = 16 / sizeof(K);   // keys per shared-memory read
   const int gs = k <= 32 ? 4 : k <= 64 ? 2 : 1, ng = kBeamThreads / gs, tid = threadIdx.x;
   for (int off = 1; off < gs; off <<= 1) {
     const K o = __shfl_xor_sync(0xffffffffu, mine, off);
@@ -86,13 +90,33 @@ __device__ __forceinline__ K group_threshold(K mine, int k, K* gm, K* sh) {
   __syncthreads();
   if (tid < ng) {
     const K me = gm[tid];
-    int above = 0;
-#pragma unroll 8
-    for (int g = 0; g < ng; ++g) above += gm[g] > me || (gm[g] == me && g < tid);
-    if (above == k - 1) *sh = me;
+    int above = 0, same = 0;
+#pragma unroll 4
+    for (int g = 0; g < ng; g += N) {
+      K q[N];
+      *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(gm + g);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        above += q[e] > me;
+        same += q[e] == me;
+      }
+    }
+    if (above < k && above + same >= k) *sh = me;   // equal maxima write the same value
   }
   __syncthreads();
   return *sh;
+}
+
+// Number of the n keys (16-byte aligned, an even number of places) that are above `me`.
+__device__ __forceinline__ int keys_above(const unsigned long long* keys, int n, unsigned long long me) {
+  int above = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; j += 2) {
+    const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(keys + j);
+    above += q.x > me;
+    above += q.y > me && j + 1 < n;
+  }
+  return above;
 }
 
 // ---------------------------------------------------------------- B1
@@ -141,64 +165,63 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
 // (below 2e-7), the same way for every beam.
 constexpr float kLog2e = 1.44269502f;
 
-// A CTA walks its slice in chunks, the next chunk's loads in flight and no barrier in between: every
-// thread keeps the running maximum and sum of its own terms, and the maximum of every group of chunks.
-// The threads' maxima give the threshold; the few (thread, group) pairs that reach it read their
-// logits again (from L2) and gather.
+// The chunks of all beams are divided evenly among the CTAs, so a CTA's share may end in one beam and go
+// on in the next; each part is a slice.  A slice is walked with the next chunks' loads in flight and no
+// barrier in between: every thread keeps the running maximum and sum of its own terms, and the maximum
+// of every group of chunks.  The threads' maxima give the threshold; the few (thread, group) pairs that
+// reach it have their logits read again (from L2) and gathered.
 template <typename T>
 __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) {
   using U64 = unsigned long long;
   using Word = BeamWord<T>;
   constexpr int WN = Word::N, VN = 4 * WN, NV = kBeamVecs, NW = 4 * NV, CH = kBeamThreads * NV;
-  __shared__ unsigned gm[kBeamThreads];
+  __shared__ __align__(16) unsigned gm[kBeamThreads];
   __shared__ unsigned sh_t;
-  __shared__ U64 cand[kBeamCand];
+  __shared__ __align__(16) U64 cand[kBeamCand];
   __shared__ float tops[kBeamGroups][kBeamThreads];
   __shared__ float wmax[kBeamThreads / 32];
   __shared__ double wsum[kBeamThreads / 32];
   __shared__ int isum[kBeamThreads / 32];
   __shared__ int sh_n, sh_h;
-  __shared__ unsigned short hits[kBeamGroups * kBeamThreads];
+  __shared__ unsigned short hits[kBeamHits];
   pdl_entry();
-  const int tid = threadIdx.x, slice = blockIdx.x, w = blockIdx.y % a.W, n = blockIdx.y / a.W, k = a.k;
+  const int tid = threadIdx.x, k = a.k;
+  const long long all = (long long)a.rows * a.chunks, ctas = gridDim.x;
+  const long long end = all * (blockIdx.x + 1) / ctas;
+  long long at_chunk = all * blockIdx.x / ctas;
+ next_slice:
+  if (at_chunk >= end) return;
+  const int rw = (int)(at_chunk / a.chunks), w = rw % a.W, n = rw / a.W;
+  const int c0 = (int)(at_chunk - (long long)rw * a.chunks), c1 = (int)min((long long)a.chunks, c0 + (end - at_chunk));
+  at_chunk += c1 - c0;
   // The row from the 16-byte boundary at or below its start: element e of it is logit e - lead.
   const T* row = static_cast<const T*>(a.logits) + n * a.n_stride + w * a.w_stride;
   const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-  const uint4* vec = reinterpret_cast<const uint4*>(row - lead);
+  const T* base = row - lead;
+  const uint4* vec = reinterpret_cast<const uint4*>(base);
   const int nvec = (a.V + lead + VN - 1) / VN;
-  const int c0 = (int)((long long)a.chunks * slice / a.S), c1 = (int)((long long)a.chunks * (slice + 1) / a.S);
   const int per = (c1 - c0 + kBeamGroups - 1) / kBeamGroups;   // chunks per group
-  // Vocabulary index of element e of the thread's word i in chunk c.
-  auto index = [&](int c, int i, int e) { return (c * CH + i / 4 * kBeamThreads + tid) * VN + i % 4 * WN + e - lead; };
   auto fetch = [&](int c, unsigned* x) {
+    const int j0 = c * CH + tid;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = c * CH + i * kBeamThreads + tid;
       uint4 v = make_uint4(Word::kNone, Word::kNone, Word::kNone, Word::kNone);
-      if (j < nvec) v = __ldg(vec + j);
+      if (j0 + i * kBeamThreads < nvec) v = __ldg(vec + j0 + i * kBeamThreads);
       x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
     }
   };
-  auto edges = [&](int c, unsigned* x) {   // the row's first and last vectors may hold a neighbour's logits
-    if (c == 0 || (c + 1) * CH >= nvec) {
+  float m = -INFINITY, s = 0.f, mg = -INFINITY;
+  int left = per, group = 0;
+  auto step = [&](int c, unsigned* x) {
+    if (c == 0 || (c + 1) * CH >= nvec) {   // the row's first and last vectors may hold a neighbour's logits
 #pragma unroll
       for (int i = 0; i < NW; ++i)
 #pragma unroll
         for (int e = 0; e < WN; ++e) {
-          const int v = index(c, i, e);
+          const int v = (c * CH + i / 4 * kBeamThreads + tid) * VN + i % 4 * WN + e - lead;
           if (v < 0 || v >= a.V) x[i] = Word::mask(x[i], e);
         }
     }
-  };
-  float m = -INFINITY, s = 0.f, mg = -INFINITY;
-  unsigned next[NW];
-  fetch(c0, next);
-  for (int c = c0; c < c1; ++c) {
-    unsigned x[NW];
-#pragma unroll
-    for (int i = 0; i < NW; ++i) x[i] = next[i];
-    edges(c, x);
-    if (c + 1 < c1) fetch(c + 1, next);
     unsigned mx = x[0];
 #pragma unroll
     for (int i = 1; i < NW; ++i) mx = Word::max(mx, x[i]);
@@ -208,25 +231,53 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
       m = mt;
     }
     mg = fmaxf(mg, mt);
-    const int in = (c - c0) % per;
-    if (in == per - 1 || c == c1 - 1) {
-      tops[(c - c0) / per][tid] = mg;
+    if (--left == 0) {
+      tops[group++][tid] = mg;
       mg = -INFINITY;
+      left = per;
     }
     const float ref = m == -INFINITY ? 0.f : m;
-    const uint64_t e2 = tc::f2pack(kLog2e, kLog2e), m2 = tc::f2pack(-ref, -ref);
+    const uint64_t e2 = tc::f2pack(kLog2e, kLog2e);
     uint64_t s2 = tc::f2pack(0.f, 0.f);
+    if (fabsf(ref) < 1e38f) {
+      // (x - ref) e' as one fused product with the offset rounded; the sum is put right below.
+      const float off = ref * kLog2e;
+      const uint64_t o2 = tc::f2pack(-off, -off);
 #pragma unroll
-    for (int i = 0; i < NW; i += 2 / WN) {
-      const float x0 = Word::get(x[i], 0), x1 = WN == 2 ? Word::get(x[i], 1) : Word::get(x[(i + 1) % NW], 0);
-      float y0, y1;
-      tc::f2unpack(tc::fmul2(tc::fadd2(tc::f2pack(x0, x1), m2), e2), y0, y1);
-      s2 = tc::fadd2(s2, tc::f2pack(tc::ex2(y0), tc::ex2(y1)));
+      for (int i = 0; i < NW; i += 2 / WN) {
+        const float x0 = Word::get(x[i], 0), x1 = WN == 2 ? Word::get(x[i], 1) : Word::get(x[(i + 1) % NW], 0);
+        float y0, y1;
+        tc::f2unpack(tc::ffma2(tc::f2pack(x0, x1), e2, o2), y0, y1);
+        s2 = tc::fadd2(s2, tc::f2pack(tc::ex2(y0), tc::ex2(y1)));
+      }
+      float s0, s1;
+      tc::f2unpack(s2, s0, s1);
+      s += (s0 + s1) * tc::ex2(fmaf(-ref, kLog2e, off));   // the offset's rounding error
+    } else {   // x e' may overflow: the difference first
+      float t = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < NW; ++i) {
+        unsigned word = 0;
+#pragma unroll
+        for (int q = 0; q < NW; ++q) word = q == i ? x[q] : word;
+#pragma unroll
+        for (int e = 0; e < WN; ++e) t += tc::ex2((Word::get(word, e) - ref) * kLog2e);
+      }
+      s += t;
     }
-    float s0, s1;
-    tc::f2unpack(s2, s0, s1);
-    s += s0 + s1;
+  };
+  unsigned xa[NW], xb[NW];
+  fetch(c0, xa);
+  if (c0 + 1 < c1) fetch(c0 + 1, xb);
+  for (int c = c0; c < c1; c += 2) {
+    step(c, xa);
+    if (c + 2 < c1) fetch(c + 2, xa);
+    if (c + 1 < c1) {
+      step(c + 1, xb);
+      if (c + 3 < c1) fetch(c + 3, xb);
+    }
   }
+  if (left != per) tops[group][tid] = mg;
   if (tid == 0) sh_n = sh_h = 0;
   // The slice's sum: the threads' maxima and float32 sums, joined in float64.
   const float mw = warp_max(m);
@@ -243,35 +294,49 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
   // Gather the logits at or above the threshold (all above -inf when fewer than k groups hold any): the
   // (thread, group) pairs that reach it in a list, a warp to each, a lane to each of its logits.
   const float least = t == none ? -INFINITY : __uint_as_float(t & 0x80000000u ? t & 0x7fffffffu : ~t);
-  for (int g = 0; g * per < c1 - c0; ++g)
-    if (tops[g][tid] >= least && tops[g][tid] > -INFINITY) hits[atomicAdd(&sh_h, 1)] = (unsigned short)(g << 8 | tid);
-  __syncthreads();
-  const T* base = row - lead;
-  for (int h = tid >> 5; h < sh_h; h += kBeamThreads / 32) {
-    const int g = hits[h] >> 8, th = hits[h] & 255;
-    for (int c = c0 + g * per; c < min(c1, c0 + (g + 1) * per); ++c)
-      for (int q = tid & 31; q < NV * VN; q += 32) {
-        const int e = (c * CH + q / VN * kBeamThreads + th) * VN + q % VN, v = e - lead;
-        if (v >= 0 && v < a.V) {
-          const float f = (float)base[e];
-          if (f >= least && f > -INFINITY) {
-            const int at = atomicAdd(&sh_n, 1);
-            if (at < kBeamCand) cand[at] = beam_key(f, v);
-          }
-        }
-      }
+  for (int g = 0; g * per < c1 - c0; ++g) {
+    const float f = tops[g][tid];
+    if (f >= least && f > -INFINITY) {
+      const int h = atomicAdd(&sh_h, 1);
+      if (h < kBeamHits) hits[h] = (unsigned short)(g << 8 | tid);
+    }
   }
   __syncthreads();
+  // Four pairs of a warp at a time, so that their loads wait together.
+  static_assert(NV * VN <= 32, "a lane per logit of a chunk");
+  constexpr int WARPS = kBeamThreads / 32;
+  const int nh = min(sh_h, kBeamHits), lane = tid & 31;
+  for (int c = 0; c < per; ++c)
+    for (int h0 = tid >> 5; h0 < nh; h0 += 4 * WARPS) {
+      float f[4];
+      int v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int h = h0 + i * WARPS, hit = h < nh ? hits[h] : 0, ch = c0 + (hit >> 8) * per + c;
+        const int e = (ch * CH + lane / VN * kBeamThreads + (hit & 255)) * VN + lane % VN;
+        v[i] = e - lead;
+        f[i] = h < nh && ch < c1 && lane < NV * VN && v[i] >= 0 && v[i] < a.V ? (float)base[e] : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (f[i] >= least && f[i] > -INFINITY) {
+          const int at = atomicAdd(&sh_n, 1);
+          if (at < kBeamCand) cand[at] = beam_key(f[i], v[i]);
+        }
+    }
+  __syncthreads();
   int nc = sh_n;
-  const size_t at = (size_t)blockIdx.y * a.S + slice;
+  // The slice's place among its beam's: counted from the CTA that holds the beam's first chunk.
+  const int slot = (int)(blockIdx.x - (((long long)rw * a.chunks + 1) * ctas - 1) / all);
+  const size_t at = (size_t)rw * a.S + slot;
   if (tid == 0) {
     double total = 0.0;
     for (int i = 0; i < kBeamThreads / 32; ++i) total += wsum[i];
     a.sum[at] = total;
     a.top[at] = top;
   }
-  if (nc > kBeamCand) {
-    // More than the buffer holds: the k-th largest key bit by bit, the logits read again each time.
+  if (nc > kBeamCand || sh_h > kBeamHits) {
+    // More than the buffers hold: the k-th largest key bit by bit, the logits read again each time.
     auto visit = [&](auto take) {
       for (int c = c0; c < c1; ++c)
 #pragma unroll 1
@@ -299,15 +364,22 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
   int* idx = a.idx + at * k;
   for (int i = tid; i < nc; i += kBeamThreads) {
     const U64 me = cand[i];
-    int above = 0;
-#pragma unroll 8
-    for (int j = 0; j < nc; ++j) above += cand[j] > me;
+    const int above = keys_above(cand, nc, me);
     if (above < k) {
       val[above] = key_value(me);
       idx[above] = (int)(0xffffffffu - (unsigned)me);
     }
   }
   for (int i = nc + tid; i < k; i += kBeamThreads) idx[i] = -1;
+  if (c1 == a.chunks) {   // the beam's last slice: the places behind it hold nothing
+    for (int i = tid; i < (a.S - 1 - slot) * k; i += kBeamThreads) idx[k + i] = -1;
+    for (int i = slot + 1 + tid; i < a.S; i += kBeamThreads) {
+      a.sum[(size_t)rw * a.S + i] = 0.0;
+      a.top[(size_t)rw * a.S + i] = -INFINITY;
+    }
+  }
+  __syncthreads();   // before the next slice uses the shared memory again
+  goto next_slice;
 }
 
 // ---------------------------------------------------------------- B2
@@ -316,9 +388,9 @@ constexpr int kBeamRound = 2048, kBeamEach = kBeamRound / kBeamThreads;
 
 __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
   using U64 = unsigned long long;
-  __shared__ U64 gm[kBeamThreads];
+  __shared__ __align__(16) U64 gm[kBeamThreads];
   __shared__ U64 sh_t;
-  __shared__ U64 cand[kBeamCand];
+  __shared__ __align__(16) U64 cand[kBeamCand];
   __shared__ int cidx[kBeamCand];
   __shared__ double lse[LOGKV_BEAM_MAX_WIDTH];
   __shared__ float prior[LOGKV_BEAM_MAX_WIDTH];
@@ -328,7 +400,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
   __shared__ int bflat[LOGKV_BEAM_MAX_K];
   __shared__ short place[LOGKV_BEAM_MAX_K];
   pdl_entry();
-  const int tid = threadIdx.x, lane = tid & 31, n = blockIdx.x, W = a.W, S = a.S, k = a.k;
+  const int tid = threadIdx.x, n = blockIdx.x, W = a.W, S = a.S, k = a.k;
   const float* val = a.val + (size_t)n * W * S * k;
   const int* idx = a.idx + (size_t)n * W * S * k;
   // Candidate i is place i / L of list i % L, so that every group of threads sees a mix of lists.
@@ -347,23 +419,22 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
   };
   int upto = min(all, kBeamRound);
   fetch(0, upto);
-  // log sum exp of each beam in float64; NaN for a beam that offers nothing.
-  for (int w = tid >> 5; w < W; w += kBeamThreads / 32) {
-    const size_t at = (size_t)(n * W + w) * S;
-    const float r = a.scores[n * W + w];
-    double si = lane < S ? a.sum[at + lane] : 0.0;
-    float ti = lane < S ? a.top[at + lane] : -INFINITY;
-    float m = si > 0.0 ? ti : -INFINITY;
-    for (int i = lane + 32; i < S; i += 32) m = fmaxf(m, a.sum[at + i] > 0.0 ? a.top[at + i] : -INFINITY);
-    m = warp_max(m);
-    double s = si != 0.0 ? si * exp2(((double)ti - (double)m) * kLog2e) : 0.0;   // a NaN stays
-    for (int i = lane + 32; i < S; i += 32) {
-      si = a.sum[at + i];
-      if (si != 0.0) s += si * exp2(((double)a.top[at + i] - (double)m) * kLog2e);
-    }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if (lane == 0) {
+  // log sum exp of each beam in float64; NaN for a beam that offers nothing.  A lane to a slice: 2 to 32
+  // lanes to a beam.
+  int lanes = 2;
+  while (lanes < S && lanes < 32) lanes *= 2;
+  for (int w0 = 0; w0 < W; w0 += kBeamThreads / lanes) {
+    const int w = w0 + tid / lanes, first = tid % lanes;
+    const size_t at = (size_t)(n * W + min(w, W - 1)) * S;
+    float m = -INFINITY;
+    for (int q = first; q < S; q += lanes) m = fmaxf(m, a.sum[at + q] > 0.0 ? a.top[at + q] : -INFINITY);
+    for (int off = 1; off < lanes; off *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    double s = 0.0;
+    for (int q = first; q < S; q += lanes)
+      if (a.sum[at + q] != 0.0) s += a.sum[at + q] * exp2f((a.top[at + q] - m) * kLog2e);   // a NaN stays
+    for (int off = 1; off < lanes; off *= 2) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if (first == 0 && w < W) {
+      const float r = a.scores[n * W + w];
       const double z = (double)m + log2(s) / (double)kLog2e;
       lse[w] = isfinite(r) && isfinite(z) ? z : nan("");
       prior[w] = r;
@@ -437,9 +508,9 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
     for (int i = tid; i < nc; i += kBeamThreads) {
       const U64 me = cand[i];
       const int mf = cidx[i];
-      int above = 0;
-#pragma unroll 4
-      for (int j = 0; j < nc; ++j) above += cand[j] > me || (cand[j] == me && cidx[j] < mf);
+      int above = keys_above(cand, nc, me);
+      if (above < k)   // equal scores: the lower flat index first
+        for (int j = 0; j < nc; ++j) above += cand[j] == me && cidx[j] < mf;
       if (above < k) {
         best[above] = me;
         bflat[above] = mf;
@@ -485,9 +556,11 @@ static int beam_chunks(int vocab, int esize) {   // the row may start up to 15 b
   const long long per = kBeamThreads * kBeamVecs * (16 / esize);
   return (int)((vocab + 16 / esize - 1 + per - 1) / per);
 }
-// Slices of a beam: six CTAs per SM over all beams, a chunk each at least.
+// CTAs: four per SM (as many as run at once), a chunk each at least; a beam's slices at most.
+static long long beam_ctas(long long rows, int chunks) { return std::min<long long>(rows * chunks, 592); }
 static int beam_slices(long long rows, int chunks) {
-  return (int)std::max(1LL, std::min<long long>(chunks, (888 + rows - 1) / rows));
+  const long long each = rows * chunks / beam_ctas(rows, chunks);
+  return (int)((chunks - 1 + each - 1) / each + 1);
 }
 
 static bool beam_ok(int requests, int width, int vocab, int k) {
@@ -504,8 +577,9 @@ extern "C" {
 
 LOGKV_API size_t logkv_beam_workspace_bytes(int32_t requests, int32_t width, int32_t vocab, int32_t k) {
   if (!beam_ok(requests, width, vocab, k)) return 0;
-  // Of either logits type: bf16 has no more chunks than float32.
-  const size_t rows = (size_t)requests * width, lists = rows * beam_slices(rows, beam_chunks(vocab, 4));
+  // Of either logits type.
+  const size_t rows = (size_t)requests * width;
+  const size_t lists = rows * std::max(beam_slices(rows, beam_chunks(vocab, 4)), beam_slices(rows, beam_chunks(vocab, 2)));
   return lists * (sizeof(double) + sizeof(float)) + lists * k * (sizeof(float) + sizeof(int));
 }
 
@@ -532,6 +606,7 @@ LOGKV_API int logkv_beam_select(const logkv_beam_args_t* x, void* workspace, siz
   a.k = x->k;
   a.keep = x->keep_places;
   a.chunks = beam_chunks(x->vocab, x->dtype == LOGKV_DTYPE_F32 ? 4 : 2);
+  a.rows = rows;
   a.S = beam_slices(rows, a.chunks);
   const size_t lists = (size_t)rows * a.S;
   a.sum = static_cast<double*>(workspace);
@@ -539,8 +614,9 @@ LOGKV_API int logkv_beam_select(const logkv_beam_args_t* x, void* workspace, siz
   a.val = a.top + lists;
   a.idx = reinterpret_cast<int*>(a.val + lists * x->k);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (x->dtype == LOGKV_DTYPE_F32) launch_pdl(beam_slice_kernel<float>, dim3(a.S, rows), kBeamThreads, 0, st, a);
-  else launch_pdl(beam_slice_kernel<__nv_bfloat16>, dim3(a.S, rows), kBeamThreads, 0, st, a);
+  const dim3 grid((unsigned)beam_ctas(rows, a.chunks));
+  if (x->dtype == LOGKV_DTYPE_F32) launch_pdl(beam_slice_kernel<float>, grid, kBeamThreads, 0, st, a);
+  else launch_pdl(beam_slice_kernel<__nv_bfloat16>, grid, kBeamThreads, 0, st, a);
   launch_pdl(beam_merge_kernel, dim3(x->requests), kBeamThreads, 0, st, a);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? LOGKV_OK : (int)e;

@@ -1,14 +1,16 @@
 // Batch rows of a cache taken over by the hypotheses that go on (C ABI in include/logkv_b200.h):
 // row b of every state buffer becomes the old row index[b], in place.
 //
-// A buffer's batch row is `segs` segments of bytes.  A CTA takes one column (up to C bytes of one
-// segment) of every row that is a source into shared memory, waits, and writes it to the rows that
-// take it over; no other CTA touches that column, so chains, swaps and cycles of rows need no order
-// and no second copy of the state.  Rows that stay are neither read nor written.
+// A buffer's batch row is `segs` segments of bytes; rows that stay are neither read nor written.
+//
+// Where every source row stays itself (beams that go on keep their places), a CTA copies up to 16 KB of
+// one segment of one source to all rows that take it over, through registers.  Where a source row is
+// itself taken over (swaps, chains, cycles), a CTA takes the same column of all sources into shared
+// memory, waits, and then writes it; no other CTA touches that column, so no order among the rows and
+// no second copy of the state is needed.
 #include <algorithm>
 
-#include "common.cuh"
-#include "../../include/logkv_attention.h"
+#include "attn_common.cuh"
 
 namespace logkv {
 
@@ -17,6 +19,7 @@ constexpr int kRowBuffers = 40;
 constexpr int kReorderThreads = 256;
 constexpr int kReorderBatch = 2048;
 constexpr int kReorderStage = 32 * 1024;   // staged bytes per CTA (more above 512 source rows)
+constexpr int kReorderTile = 16 * 1024;    // bytes a CTA copies at a time when nothing is staged
 
 // Segment i of row b: base + b * stride + i * seg_stride, seg_bytes long.  With counts (of element
 // size count_size, [B, segs]) only the first unit * max(count of the source, count of the row) bytes
@@ -42,117 +45,242 @@ __device__ __forceinline__ int row_count(const RowBuffer& r, int b, int seg) {
   return r.count_size == 2 ? static_cast<const int16_t*>(r.counts)[at] : static_cast<const int32_t*>(r.counts)[at];
 }
 
-template <typename V>
-__device__ __forceinline__ void stage_in(const RowBuffer& r, long long off, int C, int nsrc, const short* ssrc,
-                                         const int* lim, char* stage) {
-  const int per = C / (int)sizeof(V);
-  for (int x = threadIdx.x; x < nsrc * per; x += blockDim.x) {
-    const int s = x / per, c = (x - s * per) * (int)sizeof(V);
-    if (c < lim[s]) *reinterpret_cast<V*>(stage + s * C + c) = *reinterpret_cast<const V*>(r.base + ssrc[s] * r.stride + off + c);
-  }
+// Who takes over whom: sources (distinct, ascending) and, grouped by source, the rows that go on from them.
+struct RowLists {
+  short* src;     // [nsrc] source rows
+  short* first;   // [nsrc + 1] their rows' places in dst
+  short* dst;     // [nmov]
+  int nsrc, nmov;
+  bool chained;   // some source is itself taken over
+};
+
+__device__ __forceinline__ int source_of(const RowArgs& a, int b) {
+  const long long v = a.wide ? static_cast<const long long*>(a.index)[b] : (long long)static_cast<const int32_t*>(a.index)[b];
+  if (v >= 0 && v < a.B) return (int)v;
+  if (blockIdx.x == 0) set_status(a.status, kStatusBadIndex);
+  return b;
 }
+
+// By the whole block; from[B] and num[B] are scratch.
+__device__ RowLists row_lists(const RowArgs& a, short* src, short* first, short* dst, short* from, int* num) {
+  __shared__ int wsum[32];
+  __shared__ int sh[3];
+  RowLists r{src, first, dst, 0, 0, false};
+  const int tid = threadIdx.x, B = a.B;
+  if (B <= 32) {   // a warp, by ballots
+    if (tid < 32) {
+      const int s = tid < B ? source_of(a, tid) : tid;
+      const bool moved = s != tid;
+      const unsigned need = __reduce_or_sync(0xffffffffu, moved ? 1u << s : 0u);
+      const unsigned mv = __ballot_sync(0xffffffffu, moved);
+      int at = 0, n = 0;
+      for (unsigned left = need; left; left &= left - 1) {
+        const int x = __ffs(left) - 1;
+        const unsigned who = __ballot_sync(0xffffffffu, moved && s == x);
+        if (tid == 0) {
+          src[n] = (short)x;
+          first[n] = (short)at;
+        }
+        if (who >> tid & 1) dst[at + __popc(who & ((1u << tid) - 1))] = (short)tid;
+        at += __popc(who);
+        ++n;
+      }
+      if (tid == 0) {
+        first[n] = (short)at;
+        sh[0] = n;
+        sh[1] = at;
+        sh[2] = (need & mv) != 0;
+      }
+    }
+    __syncthreads();
+  } else {
+    for (int b = tid; b < B; b += blockDim.x) {
+      from[b] = (short)source_of(a, b);
+      num[b] = 0;
+    }
+    if (tid == 0) sh[2] = 0;
+    __syncthreads();
+    for (int b = tid; b < B; b += blockDim.x)
+      if (from[b] != b) atomicAdd(&num[from[b]], 1);
+    __syncthreads();
+    int nsrc = 0, nmov = 0;
+    for (int b0 = 0; b0 < B; b0 += blockDim.x) {
+      const int b = b0 + tid, c = b < B ? num[b] : 0;
+      const int i = block_inclusive_scan(c > 0, wsum), j = block_inclusive_scan(c, wsum);
+      if (c > 0) {
+        src[nsrc + i - 1] = (short)b;
+        first[nsrc + i - 1] = (short)(nmov + j - c);
+        num[b] = nmov + j - c;   // where the next of its rows goes
+        if (from[b] != b) sh[2] = 1;
+      }
+      if (tid == blockDim.x - 1) {
+        sh[0] = i;
+        sh[1] = j;
+      }
+      __syncthreads();
+      nsrc += sh[0];
+      nmov += sh[1];
+      __syncthreads();
+    }
+    for (int b = tid; b < B; b += blockDim.x)
+      if (from[b] != b) dst[atomicAdd(&num[from[b]], 1)] = (short)b;
+    if (tid == 0) {
+      first[nsrc] = (short)nmov;
+      sh[0] = nsrc;
+      sh[1] = nmov;
+    }
+    __syncthreads();
+  }
+  r.nsrc = sh[0];
+  r.nmov = sh[1];
+  r.chained = sh[2] != 0;
+  return r;
+}
+
+// Bytes of segment `seg`, from c0 on and at most `bytes`, that a row taken over from source s needs.
+__device__ __forceinline__ int row_limit(const RowBuffer& r, int s, int d, int seg, int c0, int bytes) {
+  if (!r.counts) return bytes;
+  return max(0, min(bytes, max(row_count(r, s, seg), row_count(r, d, seg)) * r.unit - c0));
+}
+
+// `bytes` of one source from offset `off` to the rows dst[0..n) (each as far as it needs).
 template <typename V>
-__device__ __forceinline__ void stage_out(const RowBuffer& r, long long off, int C, int nmov, const short* mdst,
-                                          const short* mslot, const int* mlim, const char* stage) {
-  const int per = C / (int)sizeof(V);
-  for (int x = threadIdx.x; x < nmov * per; x += blockDim.x) {
-    const int m = x / per, c = (x - m * per) * (int)sizeof(V);
-    if (c < mlim[m]) *reinterpret_cast<V*>(r.base + mdst[m] * r.stride + off + c) = *reinterpret_cast<const V*>(stage + mslot[m] * C + c);
+__device__ __forceinline__ void copy_rows(const RowBuffer& r, long long off, int seg, int c0, int bytes, int s,
+                                          const short* dst, int n) {
+  constexpr int W = (int)sizeof(V);
+  int most = 0;
+  for (int i = 0; i < n; ++i) most = max(most, row_limit(r, s, dst[i], seg, c0, bytes));
+  const char* from = r.base + s * r.stride + off;
+  for (int x = threadIdx.x * W; x < most; x += 4 * kReorderThreads * W) {
+    V v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (x + j * kReorderThreads * W < most) v[j] = *reinterpret_cast<const V*>(from + x + j * kReorderThreads * W);
+    for (int i = 0; i < n; ++i) {
+      const int d = dst[i], lim = row_limit(r, s, d, seg, c0, bytes);
+      char* to = r.base + d * r.stride + off;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (x + j * kReorderThreads * W < lim) *reinterpret_cast<V*>(to + x + j * kReorderThreads * W) = v[j];
+    }
   }
 }
 
-__global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_constant__ RowArgs a, int stage_bytes) {
+// A column of all sources (C bytes each) into the stage, a warp to a source.
+template <typename V>
+__device__ __forceinline__ void stage_in(const RowBuffer& r, long long off, int C, int nsrc, const short* src,
+                                         const int* lim, char* stage) {
+  for (int s = threadIdx.x >> 5; s < nsrc; s += kReorderThreads / 32) {
+    const char* from = r.base + src[s] * r.stride + off;
+    for (int c = (threadIdx.x & 31) * (int)sizeof(V); c < lim[s]; c += 32 * (int)sizeof(V)) {
+      if (sizeof(V) == 16) cp_async16(stage + s * C + c, from + c);
+      else *reinterpret_cast<V*>(stage + s * C + c) = *reinterpret_cast<const V*>(from + c);
+    }
+  }
+}
+template <typename V>
+__device__ __forceinline__ void stage_out(const RowBuffer& r, long long off, int C, int nsrc, const short* src,
+                                          const short* first, const short* dst, int seg, int c0, int bytes,
+                                          const char* stage) {
+  for (int s = threadIdx.x >> 5; s < nsrc; s += kReorderThreads / 32)
+    for (int i = first[s]; i < first[s + 1]; ++i) {
+      char* to = r.base + dst[i] * r.stride + off;
+      const int lim = row_limit(r, src[s], dst[i], seg, c0, bytes);
+      for (int c = (threadIdx.x & 31) * (int)sizeof(V); c < lim; c += 32 * (int)sizeof(V))
+        *reinterpret_cast<V*>(to + c) = *reinterpret_cast<const V*>(stage + s * C + c);
+    }
+}
+
+template <typename F>
+__device__ __forceinline__ void by_width(int width, F f) {
+  switch (width) {
+    case 16: f(uint4{}); break;
+    case 8: f(uint2{}); break;
+    case 4: f(0u); break;
+    case 2: f((unsigned short)0); break;
+    default: f((unsigned char)0); break;
+  }
+}
+
+__global__ void __launch_bounds__(kReorderThreads, 4) reorder_kernel(const __grid_constant__ RowArgs a, int stage_bytes) {
   extern __shared__ uint4 smem4[];
-  __shared__ int wsum[32];
-  __shared__ int sh_n[2];
   char* stage = reinterpret_cast<char*>(smem4);
-  int* mlim = reinterpret_cast<int*>(stage + stage_bytes);   // [B] bytes of the column each taken-over row needs
-  int* slim = mlim + a.B;                                    // [B] and each source
-  short* mdst = reinterpret_cast<short*>(slim + a.B);        // [B] rows taken over
-  short* mslot = mdst + a.B;                                 // [B] their source's place in the stage
-  short* ssrc = mslot + a.B;                                 // [B] source rows
-  short* slot = ssrc + a.B;                                  // [B] place of a source row, -1: none
-  const int tid = threadIdx.x, B = a.B;
+  int* num = reinterpret_cast<int*>(stage + stage_bytes);   // [B]
+  short* src = reinterpret_cast<short*>(num + a.B);         // [B]
+  short* first = src + a.B;                                 // [B + 1]
+  short* dst = first + a.B + 1;                             // [B]
+  short* from = dst + a.B;                                  // [B]
   pdl_entry();
-  auto source = [&](int b) {
-    const long long v = a.wide ? static_cast<const long long*>(a.index)[b] : (long long)static_cast<const int32_t*>(a.index)[b];
-    if (v >= 0 && v < B) return (int)v;
-    if (blockIdx.x == 0) set_status(a.status, kStatusBadIndex);
-    return b;
-  };
-  for (int b = tid; b < B; b += blockDim.x) slot[b] = -1;
-  __syncthreads();
-  for (int b = tid; b < B; b += blockDim.x) {
-    const int s = source(b);
-    if (s != b) slot[s] = 0;
+  const RowLists l = row_lists(a, src, first, dst, from, num);
+  if (l.nmov == 0) return;
+  const int tid = threadIdx.x;
+  // Tiles: (buffer, segment, column, source), or all sources of a column together when they are staged.
+  const int C = l.chained ? min(stage_bytes / l.nsrc, kReorderTile) & ~63 : kReorderTile;
+  const int split = l.chained ? 1 : l.nsrc;
+  // Tiles before each buffer (fewer than 2^31: each moves 64 bytes or more of every source).
+  __shared__ int begin[kRowBuffers + 1], cols[kRowBuffers];
+  if (tid == 0) begin[0] = 0;
+  if (tid < 64) {
+    const int c = tid < a.n ? (a.buf[tid].seg_bytes + C - 1) / C : 0;
+    int v = tid < a.n ? c * a.buf[tid].segs * split : 0;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, v, off);
+      if ((tid & 31) >= off) v += y;
+    }
+    if (tid < a.n) {
+      cols[tid] = c;
+      begin[tid + 1] = v;
+    }
   }
   __syncthreads();
-  int nsrc = 0, nmov = 0;
-  for (int b0 = 0; b0 < B; b0 += blockDim.x) {
-    const int b = b0 + tid;
-    const bool is = b < B && slot[b] == 0, mv = b < B && source(b) != b;
-    const int i = block_inclusive_scan(is, wsum), j = block_inclusive_scan(mv, wsum);
-    if (is) {
-      ssrc[nsrc + i - 1] = (short)b;
-      slot[b] = (short)(nsrc + i - 1);
-    }
-    if (mv) mdst[nmov + j - 1] = (short)b;
-    if (tid == blockDim.x - 1) {
-      sh_n[0] = i;
-      sh_n[1] = j;
-    }
-    __syncthreads();
-    nsrc += sh_n[0];
-    nmov += sh_n[1];
-    __syncthreads();
-  }
-  if (nmov == 0) return;
-  for (int m = tid; m < nmov; m += blockDim.x) mslot[m] = slot[source(mdst[m])];
-  const int C = min(stage_bytes / nsrc, 16 * 1024) & ~63;
+  if (tid >= 32 && tid < a.n) begin[tid + 1] += begin[32];
+  __syncthreads();
   int i = 0;
-  long long first = 0;   // first tile of buffer i
-  for (long long id = blockIdx.x;; id += gridDim.x) {
-    int cols = 0;
-    while (i < a.n) {
-      cols = (a.buf[i].seg_bytes + C - 1) / C;
-      const long long tiles = (long long)cols * a.buf[i].segs;
-      if (id - first < tiles) break;
-      first += tiles;
-      ++i;
-    }
-    if (i >= a.n) return;
+  for (int id = blockIdx.x; id < begin[a.n]; id += gridDim.x) {
+    while (id >= begin[i + 1]) ++i;
     const RowBuffer& r = a.buf[i];
-    const int seg = (int)((id - first) / cols), c0 = (int)((id - first) % cols) * C;
+    const int t = id - begin[i], at = t / split, s = t - at * split, seg = at / cols[i], c0 = (at - seg * cols[i]) * C;
     const int bytes = min(C, r.seg_bytes - c0);
-    __syncthreads();   // the stage and the limits of the previous tile have been read
-    for (int s = tid; s < nsrc; s += blockDim.x) slim[s] = r.counts ? 0 : bytes;
-    __syncthreads();
-    for (int m = tid; m < nmov; m += blockDim.x) {
-      int lim = bytes;
-      if (r.counts) {
-        const int n = max(row_count(r, mdst[m], seg), row_count(r, ssrc[mslot[m]], seg));
-        lim = max(0, min(bytes, n * r.unit - c0));
-        atomicMax(&slim[mslot[m]], lim);
-      }
-      mlim[m] = lim;
-    }
-    __syncthreads();
     const long long off = (long long)seg * r.seg_stride + c0;
-    switch (r.width) {
-      case 16: stage_in<uint4>(r, off, C, nsrc, ssrc, slim, stage); break;
-      case 8: stage_in<uint2>(r, off, C, nsrc, ssrc, slim, stage); break;
-      case 4: stage_in<unsigned>(r, off, C, nsrc, ssrc, slim, stage); break;
-      case 2: stage_in<unsigned short>(r, off, C, nsrc, ssrc, slim, stage); break;
-      default: stage_in<unsigned char>(r, off, C, nsrc, ssrc, slim, stage); break;
+    if (!l.chained) {
+      by_width(r.width, [&](auto v) {
+        copy_rows<decltype(v)>(r, off, seg, c0, bytes, l.src[s], l.dst + l.first[s], l.first[s + 1] - l.first[s]);
+      });
+      continue;
+    }
+    __syncthreads();   // the stage and the limits of the previous tile have been read
+    for (int x = tid; x < l.nsrc; x += kReorderThreads) {
+      int lim = 0;
+      for (int j = l.first[x]; j < l.first[x + 1]; ++j) lim = max(lim, row_limit(r, l.src[x], l.dst[j], seg, c0, bytes));
+      num[x] = lim;
     }
     __syncthreads();
-    switch (r.width) {
-      case 16: stage_out<uint4>(r, off, C, nmov, mdst, mslot, mlim, stage); break;
-      case 8: stage_out<uint2>(r, off, C, nmov, mdst, mslot, mlim, stage); break;
-      case 4: stage_out<unsigned>(r, off, C, nmov, mdst, mslot, mlim, stage); break;
-      case 2: stage_out<unsigned short>(r, off, C, nmov, mdst, mslot, mlim, stage); break;
-      default: stage_out<unsigned char>(r, off, C, nmov, mdst, mslot, mlim, stage); break;
-    }
+    by_width(r.width, [&](auto v) { stage_in<decltype(v)>(r, off, C, l.nsrc, l.src, num, stage); });
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
+    by_width(r.width, [&](auto v) {
+      stage_out<decltype(v)>(r, off, C, l.nsrc, l.src, l.first, l.dst, seg, c0, bytes, stage);
+    });
+  }
+}
+
+// The counts themselves, once nothing reads them any more: whole rows of the (small) buffers through shared
+// memory, 64 bytes of every row per CTA.
+__global__ void __launch_bounds__(kReorderThreads) reorder_counts_kernel(const __grid_constant__ RowArgs a) {
+  extern __shared__ uint4 smem4[];
+  unsigned short* old = reinterpret_cast<unsigned short*>(smem4);   // [B][32]
+  pdl_entry();
+  const RowBuffer& r = a.buf[blockIdx.y];
+  const int lane = threadIdx.x & 31, c = (blockIdx.x * 32 + lane) * 2;
+  if (c < r.seg_bytes)
+    for (int b = threadIdx.x >> 5; b < a.B; b += kReorderThreads / 32)
+      old[b * 32 + lane] = *reinterpret_cast<const unsigned short*>(r.base + b * r.stride + c);
+  __syncthreads();
+  for (int b = threadIdx.x >> 5; b < a.B; b += kReorderThreads / 32) {
+    const int s = source_of(a, b);
+    if (s != b && c < r.seg_bytes) *reinterpret_cast<unsigned short*>(r.base + b * r.stride + c) = old[s * 32 + lane];
   }
 }
 
@@ -178,24 +306,38 @@ static void add_rows(RowArgs* a, void* base, long long stride, int segs, long lo
 
 static size_t reorder_stage(int B) { return std::max<size_t>(kReorderStage, (size_t)B * 64); }
 
-static int launch_reorder(RowArgs& a, int B, const void* index, int wide, int32_t* status, cudaStream_t st) {
-  if (a.n == 0) return LOGKV_OK;
+static void set_index(RowArgs& a, int B, const void* index, int wide, int32_t* status) {
   a.B = B;
   a.index = index;
   a.wide = wide;
   a.status = status;
-  const size_t stage = reorder_stage(B), smem = stage + (size_t)B * 16;
+}
+
+static int launch_reorder(RowArgs& a, int B, const void* index, int wide, int32_t* status, cudaStream_t st) {
+  if (a.n == 0) return LOGKV_OK;
+  set_index(a, B, index, wide, status);
+  const size_t stage = reorder_stage(B), smem = stage + (size_t)B * 12 + 16;
   const cudaError_t e = cudaFuncSetAttribute(reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
-  // The CTAs loop over columns of about stage / B bytes or more; no more CTAs than columns.
+  // The CTAs loop over the tiles; no more CTAs than a source per row would need.
   long long tiles = 0;
-  const long long c = std::max<long long>(64, (long long)(stage / B) & ~63LL);
-  for (int i = 0; i < a.n; ++i) tiles += (a.buf[i].seg_bytes + c - 1) / c * a.buf[i].segs;
-  const int per_sm = (int)std::max<size_t>(1, (220 * 1024) / (smem + 1024));
-  launch_pdl(reorder_kernel, dim3((unsigned)std::max(1LL, std::min<long long>(tiles, 148LL * std::min(per_sm, 6)))),
+  for (int i = 0; i < a.n; ++i)
+    tiles += (long long)(a.buf[i].seg_bytes + kReorderTile - 1) / kReorderTile * a.buf[i].segs * B;
+  const int per_sm = (int)std::max<size_t>(1, std::min<size_t>(4, (220 * 1024) / (smem + 1024)));
+  launch_pdl(reorder_kernel, dim3((unsigned)std::max(1LL, std::min<long long>(tiles, 148LL * per_sm))),
              kReorderThreads, smem, st, a, (int)stage);
-  const cudaError_t r = cudaGetLastError();
-  return r == cudaSuccess ? LOGKV_OK : (int)r;
+  return launch_status();
+}
+
+static int launch_counts(RowArgs& a, int B, const void* index, int wide, int32_t* status, cudaStream_t st) {
+  set_index(a, B, index, wide, status);
+  int cols = 1;
+  for (int i = 0; i < a.n; ++i) cols = std::max(cols, (a.buf[i].seg_bytes + 63) / 64);
+  const size_t smem = (size_t)B * 64;
+  const cudaError_t e = cudaFuncSetAttribute(reorder_counts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  launch_pdl(reorder_counts_kernel, dim3(cols, a.n), kReorderThreads, smem, st, a);
+  return launch_status();
 }
 
 }  // namespace logkv
@@ -272,7 +414,7 @@ LOGKV_API int logkv_reorder_batch(const logkv_layout_t* layout, const logkv_stat
   RowArgs c{};
   add_rows(&c, s.level_count, G * KL * 2, 1, 0, G * KL * 2);
   if (prefix) add_rows(&c, prefix->length, G * 4, 1, 0, G * 4);
-  return launch_reorder(c, l.batch, index, index_wide, status, st);
+  return launch_counts(c, l.batch, index, index_wide, status, st);
 }
 
 LOGKV_API int logkv_reorder_rows(const logkv_rows_t* buffers, int32_t n, int32_t batch, const void* index,

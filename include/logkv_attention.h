@@ -189,13 +189,13 @@ LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_sta
  * are not moved.
  * window_from >= 0: only the window's rows [window_from, recent_count), for a caller whose rows b and
  * index[b] hold the same ladder, pool and earlier window rows (hypotheses forked from one row since
- * the last flush).  batch <= 2048.
+ * the last flush).  batch <= 512.
  */
 LOGKV_API int logkv_reorder_batch(const logkv_layout_t* layout, const logkv_state_t* state,
                                   const logkv_prefix_t* prefix, int32_t recent_count, int32_t window_from,
                                   const void* index, int32_t index_wide, int32_t* status, void* stream);
 
-/* The same for up to 40 contiguous [batch, ...] buffers of row_bytes bytes per row (a decoder's own
+/* The same for up to 30 contiguous [batch, ...] buffers of row_bytes bytes per row (a decoder's own
  * per-row state). */
 typedef struct logkv_rows {
   void* base;

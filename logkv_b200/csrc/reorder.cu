@@ -1,13 +1,14 @@
 // Batch rows of a cache taken over by the hypotheses that go on (C ABI in include/logkv_b200.h):
 // row b of every state buffer becomes the old row index[b], in place.
 //
-// A buffer's batch row is `segs` segments of bytes; rows that stay are neither read nor written.
-//
-// Where every source row stays itself (beams that go on keep their places), a CTA copies up to 16 KB of
-// one segment of one source to all rows that take it over, through registers.  Where a source row is
-// itself taken over (swaps, chains, cycles), a CTA takes the same column of all sources into shared
-// memory, waits, and then writes it; no other CTA touches that column, so no order among the rows and
-// no second copy of the state is needed.
+// A buffer's batch row is `segs` segments of bytes; rows that stay are neither read nor written.  A warp
+// moves a column of up to 8 KB of a segment at a time by bulk copies, through a ring of shared-memory
+// slots: source rows in, every row that takes one over out, four columns on their way in while earlier
+// ones go out, so one CTA of four warps keeps 190 KB of an SM in motion and issues next to nothing.  Where
+// every source row stays itself (beams that go on keep their places) a column is of one source.  Where a
+// source row is itself taken over (swaps, chains, cycles) it is of all sources: they are in shared
+// memory before any row is written and no other warp touches the column, so the rows need no order and
+// the state no second copy.
 #include <algorithm>
 
 #include "attn_common.cuh"
@@ -15,15 +16,18 @@
 namespace logkv {
 
 constexpr int32_t kStatusBadIndex = 1 << 19;
-constexpr int kRowBuffers = 40;
-constexpr int kReorderThreads = 256;
-constexpr int kReorderBatch = 2048;
-constexpr int kReorderStage = 32 * 1024;   // staged bytes per CTA (more above 512 source rows)
-constexpr int kReorderTile = 16 * 1024;    // bytes a CTA copies at a time when nothing is staged
+constexpr int kRowBuffers = 60;
+constexpr int kReorderWarps = 4;
+constexpr int kReorderBatch = 512;
+constexpr int kReorderSlots = 6, kReorderAhead = 4;   // slots of a warp's ring; columns on their way in
+constexpr int kReorderSlot = 8 * 1024;                // bytes of a slot
+constexpr int kReorderTileBatch = 32;                 // tiles whose places a warp works out together
+constexpr long long kReorderWaitBudget = 4000000000LL;   // clock cycles (about 2 s)
+constexpr int32_t kStatusReorderTimeout = 1 << 20;
 
 // Segment i of row b: base + b * stride + i * seg_stride, seg_bytes long.  With counts (of element
 // size count_size, [B, segs]) only the first unit * max(count of the source, count of the row) bytes
-// move: K and V past a level's count are zero in every row (a flush clears what it vacates), and
+// (rounded up to whole accesses) move: K and V past a level's count are zero in every row (a flush clears what it vacates), and
 // prefix rows past the length are never read.
 struct RowBuffer {
   char* base;
@@ -137,58 +141,56 @@ __device__ RowLists row_lists(const RowArgs& a, short* src, short* first, short*
   return r;
 }
 
-// Bytes of segment `seg`, from c0 on and at most `bytes`, that a row taken over from source s needs.
-__device__ __forceinline__ int row_limit(const RowBuffer& r, int s, int d, int seg, int c0, int bytes) {
-  if (!r.counts) return bytes;
-  return max(0, min(bytes, max(row_count(r, s, seg), row_count(r, d, seg)) * r.unit - c0));
+__device__ __forceinline__ void bulk_in(void* dst, const void* src, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
+                   tc::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
 }
+__device__ __forceinline__ void bulk_out(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(dst), "r"(tc::smem_u32(src)),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {   // all but the last N groups have read their source
+  asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 
-// `bytes` of one source from offset `off` to the rows dst[0..n) (each as far as it needs).
+// A column of one segment: bytes [0, len) at `base` + row * stride, of the sources [s0, s1).
+struct RowTile {
+  char* base;
+  long long stride;
+  int len;          // 0: nothing to move
+  short s0, s1;
+  short width, pad;
+};
+
+// Elements of V between the rows and a slot, a lane to an element (buffers too narrow for bulk copies).
 template <typename V>
-__device__ __forceinline__ void copy_rows(const RowBuffer& r, long long off, int seg, int c0, int bytes, int s,
-                                          const short* dst, int n) {
-  constexpr int W = (int)sizeof(V);
-  int most = 0;
-  for (int i = 0; i < n; ++i) most = max(most, row_limit(r, s, dst[i], seg, c0, bytes));
-  const char* from = r.base + s * r.stride + off;
-  for (int x = threadIdx.x * W; x < most; x += 4 * kReorderThreads * W) {
-    V v[4];
+__device__ __forceinline__ void narrow_copy(const RowTile& t, const RowLists& l, int C, char* slot, int lane) {
+  const int per = t.len / (int)sizeof(V);
+  for (int s = t.s0; s < t.s1; ++s) {
+    const V* from = reinterpret_cast<const V*>(t.base + l.src[s] * t.stride);
+    V* to = reinterpret_cast<V*>(slot + (s - t.s0) * C);
+    for (int x0 = lane; x0 < per; x0 += 8 * 32) {
+      V v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (x + j * kReorderThreads * W < most) v[j] = *reinterpret_cast<const V*>(from + x + j * kReorderThreads * W);
-    for (int i = 0; i < n; ++i) {
-      const int d = dst[i], lim = row_limit(r, s, d, seg, c0, bytes);
-      char* to = r.base + d * r.stride + off;
+      for (int j = 0; j < 8; ++j)
+        if (x0 + 32 * j < per) v[j] = from[x0 + 32 * j];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (x + j * kReorderThreads * W < lim) *reinterpret_cast<V*>(to + x + j * kReorderThreads * W) = v[j];
+      for (int j = 0; j < 8; ++j)
+        if (x0 + 32 * j < per) to[x0 + 32 * j] = v[j];
     }
   }
-}
-
-// A column of all sources (C bytes each) into the stage, a warp to a source.
-template <typename V>
-__device__ __forceinline__ void stage_in(const RowBuffer& r, long long off, int C, int nsrc, const short* src,
-                                         const int* lim, char* stage) {
-  for (int s = threadIdx.x >> 5; s < nsrc; s += kReorderThreads / 32) {
-    const char* from = r.base + src[s] * r.stride + off;
-    for (int c = (threadIdx.x & 31) * (int)sizeof(V); c < lim[s]; c += 32 * (int)sizeof(V)) {
-      if (sizeof(V) == 16) cp_async16(stage + s * C + c, from + c);
-      else *reinterpret_cast<V*>(stage + s * C + c) = *reinterpret_cast<const V*>(from + c);
-    }
-  }
-}
-template <typename V>
-__device__ __forceinline__ void stage_out(const RowBuffer& r, long long off, int C, int nsrc, const short* src,
-                                          const short* first, const short* dst, int seg, int c0, int bytes,
-                                          const char* stage) {
-  for (int s = threadIdx.x >> 5; s < nsrc; s += kReorderThreads / 32)
-    for (int i = first[s]; i < first[s + 1]; ++i) {
-      char* to = r.base + dst[i] * r.stride + off;
-      const int lim = row_limit(r, src[s], dst[i], seg, c0, bytes);
-      for (int c = (threadIdx.x & 31) * (int)sizeof(V); c < lim; c += 32 * (int)sizeof(V))
-        *reinterpret_cast<V*>(to + c) = *reinterpret_cast<const V*>(stage + s * C + c);
-    }
+  __syncwarp();
+  for (int s = t.s0; s < t.s1; ++s)
+    for (int i = l.first[s]; i < l.first[s + 1]; ++i)
+      for (int x = lane; x < per; x += 32)
+        reinterpret_cast<V*>(t.base + l.dst[i] * t.stride)[x] = reinterpret_cast<const V*>(slot + (s - t.s0) * C)[x];
+  __syncwarp();
 }
 
 template <typename F>
@@ -202,23 +204,26 @@ __device__ __forceinline__ void by_width(int width, F f) {
   }
 }
 
-__global__ void __launch_bounds__(kReorderThreads, 4) reorder_kernel(const __grid_constant__ RowArgs a, int stage_bytes) {
-  extern __shared__ uint4 smem4[];
-  char* stage = reinterpret_cast<char*>(smem4);
-  int* num = reinterpret_cast<int*>(stage + stage_bytes);   // [B]
-  short* src = reinterpret_cast<short*>(num + a.B);         // [B]
-  short* first = src + a.B;                                 // [B + 1]
-  short* dst = first + a.B + 1;                             // [B]
-  short* from = dst + a.B;                                  // [B]
+__global__ void __launch_bounds__(kReorderWarps * 32, 1) reorder_kernel(const __grid_constant__ RowArgs a) {
+  extern __shared__ __align__(128) uint4 smem4[];
+  char* ring = reinterpret_cast<char*>(smem4);
+  int* num = reinterpret_cast<int*>(ring + kReorderWarps * kReorderSlots * kReorderSlot);   // [B]
+  short* src = reinterpret_cast<short*>(num + a.B);                                         // [B]
+  short* first = src + a.B;                                                                 // [B + 1]
+  short* dst = first + a.B + 1;                                                             // [B]
+  short* from = dst + a.B;                                                                  // [B]
+  __shared__ uint64_t full[kReorderWarps][kReorderSlots];
+  __shared__ RowTile tiles[kReorderWarps][kReorderTileBatch];
+  __shared__ int begin[kRowBuffers + 1], cols[kRowBuffers];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid < kReorderWarps * kReorderSlots) tc::mbar_init(&full[0][0] + tid, 1);
+  tc::mbar_fence_init();
   pdl_entry();
   const RowLists l = row_lists(a, src, first, dst, from, num);
   if (l.nmov == 0) return;
-  const int tid = threadIdx.x;
-  // Tiles: (buffer, segment, column, source), or all sources of a column together when they are staged.
-  const int C = l.chained ? min(stage_bytes / l.nsrc, kReorderTile) & ~63 : kReorderTile;
-  const int split = l.chained ? 1 : l.nsrc;
-  // Tiles before each buffer (fewer than 2^31: each moves 64 bytes or more of every source).
-  __shared__ int begin[kRowBuffers + 1], cols[kRowBuffers];
+  // Tiles: (buffer, segment, column, source), or all sources of a column together.
+  const int each = l.chained ? l.nsrc : 1, split = l.chained ? 1 : l.nsrc, C = kReorderSlot / each & ~15;
+  // Tiles before each buffer (fewer than 2^31: each moves 16 bytes or more of every source).
   if (tid == 0) begin[0] = 0;
   if (tid < 64) {
     const int c = tid < a.n ? (a.buf[tid].seg_bytes + C - 1) / C : 0;
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(kReorderThreads, 4) reorder_kernel(const __gri
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, v, off);
-      if ((tid & 31) >= off) v += y;
+      if (lane >= off) v += y;
     }
     if (tid < a.n) {
       cols[tid] = c;
@@ -236,49 +241,100 @@ __global__ void __launch_bounds__(kReorderThreads, 4) reorder_kernel(const __gri
   __syncthreads();
   if (tid >= 32 && tid < a.n) begin[tid + 1] += begin[32];
   __syncthreads();
-  int i = 0;
-  for (int id = blockIdx.x; id < begin[a.n]; id += gridDim.x) {
-    while (id >= begin[i + 1]) ++i;
-    const RowBuffer& r = a.buf[i];
-    const int t = id - begin[i], at = t / split, s = t - at * split, seg = at / cols[i], c0 = (at - seg * cols[i]) * C;
-    const int bytes = min(C, r.seg_bytes - c0);
-    const long long off = (long long)seg * r.seg_stride + c0;
-    if (!l.chained) {
-      by_width(r.width, [&](auto v) {
-        copy_rows<decltype(v)>(r, off, seg, c0, bytes, l.src[s], l.dst + l.first[s], l.first[s + 1] - l.first[s]);
-      });
-      continue;
+  char* slots = ring + warp * kReorderSlots * kReorderSlot;
+  RowTile* mine = tiles[warp];
+  const int stride = gridDim.x * kReorderWarps, total = begin[a.n];
+  int in = 0, out = 0;   // columns asked for and written so far
+  bool ok = true;
+  // One column: wait for its sources, write the rows that take them over.
+  auto finish = [&](const RowTile& t) {
+    const int slot = out % kReorderSlots;
+    ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&full[warp][slot], (out / kReorderSlots) & 1, kReorderWaitBudget));
+    if (ok)
+      for (int s = t.s0; s < t.s1; ++s)
+        for (int i = l.first[s] + lane; i < l.first[s + 1]; i += 32)
+          bulk_out(t.base + l.dst[i] * t.stride, slots + slot * kReorderSlot + (s - t.s0) * C, t.len);
+    bulk_commit();
+    ++out;
+  };
+  for (int id0 = blockIdx.x * kReorderWarps + warp; id0 < total && ok; id0 += stride * kReorderTileBatch) {
+    // A lane to a tile: its place, and how far its rows go.
+    const int id = id0 + lane * stride;
+    RowTile t{};
+    if (id < total) {
+      int i = 0;
+      while (id >= begin[i + 1]) ++i;
+      const RowBuffer& r = a.buf[i];
+      const int q = id - begin[i], at = q / split, s = q - at * split, seg = at / cols[i], c0 = (at - seg * cols[i]) * C;
+      t.s0 = (short)(l.chained ? 0 : s);
+      t.s1 = (short)(l.chained ? l.nsrc : s + 1);
+      t.len = min(C, r.seg_bytes - c0);
+      if (r.counts) {
+        int n = 0;
+        for (int x = t.s0; x < t.s1; ++x) {
+          n = max(n, row_count(r, l.src[x], seg));
+          for (int j = l.first[x]; j < l.first[x + 1]; ++j) n = max(n, row_count(r, l.dst[j], seg));
+        }
+        t.len = max(0, min(t.len, (n * r.unit + r.width - 1) / r.width * r.width - c0));
+      }
+      t.base = r.base + (long long)seg * r.seg_stride + c0;
+      t.stride = r.stride;
+      t.width = r.width;
     }
-    __syncthreads();   // the stage and the limits of the previous tile have been read
-    for (int x = tid; x < l.nsrc; x += kReorderThreads) {
-      int lim = 0;
-      for (int j = l.first[x]; j < l.first[x + 1]; ++j) lim = max(lim, row_limit(r, l.src[x], l.dst[j], seg, c0, bytes));
-      num[x] = lim;
+    mine[lane] = t;
+    __syncwarp();
+    const unsigned bulk = __ballot_sync(0xffffffffu, t.len > 0 && t.width == 16);
+    unsigned narrow = __ballot_sync(0xffffffffu, t.len > 0 && t.width < 16);
+    unsigned ask = bulk, done = bulk;
+    while (done && ok) {
+      if (ask && in - out < kReorderAhead) {
+        const RowTile& n = mine[__ffs(ask) - 1];
+        ask &= ask - 1;
+        const int slot = in % kReorderSlots;
+        // The column that had the slot before was written kReorderSlots - kReorderAhead columns ago or more.
+        bulk_wait_read<kReorderSlots - kReorderAhead - 1>();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_expect_tx(&full[warp][slot], n.len * (n.s1 - n.s0));
+        __syncwarp();
+        for (int s = n.s0 + lane; s < n.s1; s += 32)
+          bulk_in(slots + slot * kReorderSlot + (s - n.s0) * C, n.base + l.src[s] * n.stride, n.len, &full[warp][slot]);
+        ++in;
+      } else {
+        finish(mine[__ffs(done) - 1]);
+        done &= done - 1;
+      }
     }
-    __syncthreads();
-    by_width(r.width, [&](auto v) { stage_in<decltype(v)>(r, off, C, l.nsrc, l.src, num, stage); });
-    cp_async_commit();
-    cp_async_wait<0>();
-    __syncthreads();
-    by_width(r.width, [&](auto v) {
-      stage_out<decltype(v)>(r, off, C, l.nsrc, l.src, l.first, l.dst, seg, c0, bytes, stage);
-    });
+    if (narrow && ok) {
+      bulk_wait_read<0>();   // the ring is idle: the first slot serves
+      __syncwarp();
+      for (; narrow; narrow &= narrow - 1) {
+        const RowTile& n = mine[__ffs(narrow) - 1];
+        by_width(n.width, [&](auto v) { narrow_copy<decltype(v)>(n, l, C, slots, lane); });
+      }
+      tc::fence_proxy_async();   // before a bulk copy writes the slot again
+    }
+    __syncwarp();
+  }
+  bulk_wait();
+  if (!ok) {   // (copies that are late may still land in the ring)
+    for (; out < in; ++out) tc::mbar_wait(&full[warp][out % kReorderSlots], (out / kReorderSlots) & 1, kReorderWaitBudget);
+    if (lane == 0) set_status(a.status, kStatusReorderTimeout);
   }
 }
 
 // The counts themselves, once nothing reads them any more: whole rows of the (small) buffers through shared
 // memory, 64 bytes of every row per CTA.
-__global__ void __launch_bounds__(kReorderThreads) reorder_counts_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(256) reorder_counts_kernel(const __grid_constant__ RowArgs a) {
   extern __shared__ uint4 smem4[];
   unsigned short* old = reinterpret_cast<unsigned short*>(smem4);   // [B][32]
   pdl_entry();
   const RowBuffer& r = a.buf[blockIdx.y];
   const int lane = threadIdx.x & 31, c = (blockIdx.x * 32 + lane) * 2;
   if (c < r.seg_bytes)
-    for (int b = threadIdx.x >> 5; b < a.B; b += kReorderThreads / 32)
+    for (int b = threadIdx.x >> 5; b < a.B; b += 8)
       old[b * 32 + lane] = *reinterpret_cast<const unsigned short*>(r.base + b * r.stride + c);
   __syncthreads();
-  for (int b = threadIdx.x >> 5; b < a.B; b += kReorderThreads / 32) {
+  for (int b = threadIdx.x >> 5; b < a.B; b += 8) {
     const int s = source_of(a, b);
     if (s != b && c < r.seg_bytes) *reinterpret_cast<unsigned short*>(r.base + b * r.stride + c) = old[s * 32 + lane];
   }
@@ -288,6 +344,14 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_counts_kernel(const _
 static void add_rows(RowArgs* a, void* base, long long stride, int segs, long long seg_stride, long long seg_bytes,
                      const void* counts = nullptr, int count_size = 0, int unit = 0) {
   if (segs < 1 || seg_bytes < 1) return;
+  unsigned long long all = (unsigned long long)reinterpret_cast<uintptr_t>(base) | (unsigned long long)stride |
+                           (segs > 1 ? (unsigned long long)seg_stride : 0ull);
+  if (!counts && all % 16 == 0 && seg_bytes > 16 && seg_bytes % 16) {   // the odd end apart
+    const long long main = seg_bytes & ~15LL;
+    add_rows(a, base, stride, segs, seg_stride, main);
+    add_rows(a, static_cast<char*>(base) + main, stride, segs, seg_stride, seg_bytes - main);
+    return;
+  }
   RowBuffer& r = a->buf[a->n++];
   r.base = static_cast<char*>(base);
   r.counts = counts;
@@ -297,14 +361,10 @@ static void add_rows(RowArgs* a, void* base, long long stride, int segs, long lo
   r.seg_bytes = (int)seg_bytes;
   r.unit = unit;
   r.count_size = (short)count_size;
-  const unsigned long long all = (unsigned long long)reinterpret_cast<uintptr_t>(base) | (unsigned long long)stride |
-                                 (segs > 1 ? (unsigned long long)seg_stride : 0ull) | (unsigned long long)seg_bytes |
-                                 (unsigned long long)unit;
+  all |= (unsigned long long)seg_bytes;
   r.width = 16;
   while (all % r.width) r.width /= 2;
 }
-
-static size_t reorder_stage(int B) { return std::max<size_t>(kReorderStage, (size_t)B * 64); }
 
 static void set_index(RowArgs& a, int B, const void* index, int wide, int32_t* status) {
   a.B = B;
@@ -316,16 +376,15 @@ static void set_index(RowArgs& a, int B, const void* index, int wide, int32_t* s
 static int launch_reorder(RowArgs& a, int B, const void* index, int wide, int32_t* status, cudaStream_t st) {
   if (a.n == 0) return LOGKV_OK;
   set_index(a, B, index, wide, status);
-  const size_t stage = reorder_stage(B), smem = stage + (size_t)B * 12 + 16;
+  const size_t smem = (size_t)kReorderWarps * kReorderSlots * kReorderSlot + (size_t)B * 12 + 16;
   const cudaError_t e = cudaFuncSetAttribute(reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
-  // The CTAs loop over the tiles; no more CTAs than a source per row would need.
+  // One CTA per SM; no more warps than a source per row would have tiles.
   long long tiles = 0;
   for (int i = 0; i < a.n; ++i)
-    tiles += (long long)(a.buf[i].seg_bytes + kReorderTile - 1) / kReorderTile * a.buf[i].segs * B;
-  const int per_sm = (int)std::max<size_t>(1, std::min<size_t>(4, (220 * 1024) / (smem + 1024)));
-  launch_pdl(reorder_kernel, dim3((unsigned)std::max(1LL, std::min<long long>(tiles, 148LL * per_sm))),
-             kReorderThreads, smem, st, a, (int)stage);
+    tiles += (long long)(a.buf[i].seg_bytes + kReorderSlot - 1) / kReorderSlot * a.buf[i].segs * B;
+  const unsigned grid = (unsigned)std::max(1LL, std::min<long long>((tiles + kReorderWarps - 1) / kReorderWarps, 148LL));
+  launch_pdl(reorder_kernel, dim3(grid), kReorderWarps * 32, smem, st, a);
   return launch_status();
 }
 
@@ -336,7 +395,7 @@ static int launch_counts(RowArgs& a, int B, const void* index, int wide, int32_t
   const size_t smem = (size_t)B * 64;
   const cudaError_t e = cudaFuncSetAttribute(reorder_counts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
-  launch_pdl(reorder_counts_kernel, dim3(cols, a.n), kReorderThreads, smem, st, a);
+  launch_pdl(reorder_counts_kernel, dim3(cols, a.n), 256, smem, st, a);
   return launch_status();
 }
 
@@ -420,7 +479,7 @@ LOGKV_API int logkv_reorder_batch(const logkv_layout_t* layout, const logkv_stat
 LOGKV_API int logkv_reorder_rows(const logkv_rows_t* buffers, int32_t n, int32_t batch, const void* index,
                                  int32_t index_wide, int32_t* status, void* stream) {
   if (!buffers || !index) return LOGKV_E_POINTER;
-  if (n < 0 || n > kRowBuffers || batch < 1 || batch > kReorderBatch) return LOGKV_E_SHAPE;
+  if (n < 0 || n > 30 || batch < 1 || batch > kReorderBatch) return LOGKV_E_SHAPE;
   RowArgs a{};
   for (int i = 0; i < n; ++i) {
     if (!buffers[i].base) return LOGKV_E_POINTER;

@@ -255,7 +255,7 @@ class on_device:
     """``torch.cuda.device(device)``, at the cost of one comparison when it is current already."""
 
     def __init__(self, device: torch.device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        self.guard = None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
     def __enter__(self):
         if self.guard is not None:

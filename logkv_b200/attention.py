@@ -297,11 +297,12 @@ def log_kv_chunk_attention(cache, q_b, k_b, v_b, scale, second_order_scale=1.0, 
 
 
 def _rows16(t):
-    """``t`` with its head dim contiguous and every row 16-byte aligned (a copy where it is not)."""
+    """(``t`` with its head dim contiguous and every row 16-byte aligned, a copy where it is not; strides)."""
     s = t.stride()
     if s[3] == 1 and not (t.data_ptr() | (s[0] | s[1] | s[2]) * t.element_size()) & 15:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+        return t, s[:3]
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()[:3]
 
 
 def _tree_parents(parents, B: int, T: int, dev):
@@ -309,7 +310,7 @@ def _tree_parents(parents, B: int, T: int, dev):
     p = parents if isinstance(parents, torch.Tensor) else torch.as_tensor(parents)
     if p.dtype != torch.int32 and p.dtype != torch.int64:
         raise ValueError(f"parents must be integers (int32 or int64), got {p.dtype}")
-    if tuple(p.shape) not in ((T,), (B, T)):
+    if p.shape != (B, T) and p.shape != (T,):
         raise ValueError(f"parents must be [{T}] or [{B}, {T}], got {tuple(p.shape)}")
     if not p.is_cuda:
         if bool(((p < -2) | (p >= torch.arange(T))).any()):
@@ -335,15 +336,18 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
 
     After verification ``cache.add_recent_path`` commits the accepted path.
     """
+    rs = _read_state(cache)
+    pk = rs.pk
+    dev, dt = pk.device, pk.dtype
+    B, G, _, kd = pk.shape
     if q.dim() != 4:
         raise ValueError(f"q must be [B, H, T, D], got {tuple(q.shape)}")
-    B, H, T, kd = q.shape
-    rs = _read_state(cache)
-    dev, dt, G = rs.pk.device, rs.pk.dtype, cache.n_groups
-    if B != cache.batch_size or kd != cache.k_dim or q.dtype != dt:
-        raise ValueError(f"q must be [B={cache.batch_size}, H, T, {cache.k_dim}] in the cache dtype")
-    _check_kv(cache, k, v)
-    if k.size(2) != T:
+    H, T = q.size(1), q.size(2)
+    if q.size(0) != B or q.size(3) != kd or q.dtype != dt:
+        raise ValueError(f"q must be [B={B}, H, T, {kd}] in the cache dtype")
+    want = (B, G, T, kd)
+    if k.shape != want or v.shape != want or k.dtype != dt or v.dtype != dt:
+        _check_kv(cache, k, v)
         raise ValueError("q, k and v must cover the same drafted tokens")
     if H < 1 or H % G:
         raise ValueError(f"query heads {H} must be a multiple of KV groups {G}")
@@ -354,7 +358,7 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError("logkv_b200 attention is forward-only")
     if out is None:
-        out = torch.empty((B, H, T, kd), dtype=dt, device=dev)
+        out = pk.new_empty((B, H, T, kd))
     elif out.shape != (B, H, T, kd) or out.dtype != dt or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous [{B}, {H}, {T}, {kd}] tensor in the cache dtype on {dev}")
     if T == 0:
@@ -376,11 +380,11 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
         qx = rs.qx.get(scale)
         if qx is None:
             qx = rs.qx[scale] = query_extra(scale, dt)
-        q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        args = _lib.TreeArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p.data_ptr(), q.stride()[:3],
-                             k.stride()[:3], v.stride()[:3], p.stride(0) if p.dim() == 2 else 0,
-                             p.dtype == torch.int64, H, T, cache.recent_count, scale, qx, rs.status_ptr)
+        (q, qs), (k, ks), (v, vs) = _rows16(q), _rows16(k), _rows16(v)
+        ws = rs.mass.new_empty(n >> 2)
+        args = _lib.TreeArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p.data_ptr(), qs, ks, vs,
+                             p.stride(0) if p.dim() == 2 else 0, p.dtype == torch.int64, H, T, cache.recent_count,
+                             scale, qx, rs.status_ptr)
         _lib.check(lib.logkv_tree_attention(ctypes.byref(layout), ctypes.byref(state),
                                             ctypes.byref(rs.prefix_struct()), ctypes.byref(args), ws.data_ptr(), n,
                                             _lib.stream_ptr(dev)), "logkv_tree_attention")

@@ -49,8 +49,8 @@ def beam_select(logits, scores, k: int, *, keep_places: bool = False):
     dev = logits.device
     if dev.type != "cuda" or scores.device != dev:
         raise ValueError("logits and scores must be CUDA tensors on one device")
-    out_scores = torch.empty((N, k), dtype=torch.float32, device=dev)
-    out_rows, out_tokens = torch.empty((2, N, k), dtype=torch.int64, device=dev).unbind(0)
+    out_scores = scores.new_empty((N, k))
+    out_rows, out_tokens = scores.new_empty((N, k), dtype=torch.int64), scores.new_empty((N, k), dtype=torch.int64)
     if N == 0:
         return out_scores, out_rows, out_tokens
     with _lib.on_device(dev):
@@ -59,7 +59,7 @@ def beam_select(logits, scores, k: int, *, keep_places: bool = False):
         scores = scores.contiguous()
         lib = _lib.lib()
         n = lib.logkv_beam_workspace_bytes(N, W, V, k)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        ws = scores.new_empty((n + 7) >> 3, dtype=torch.float64)
         args = _lib.BeamArgs(logits.data_ptr(), scores.data_ptr(), out_scores.data_ptr(), out_rows.data_ptr(),
                              out_tokens.data_ptr(), logits.stride(0), logits.stride(1),
                              _lib.DTYPE_CODES[logits.dtype], N, W, V, k, keep_places)

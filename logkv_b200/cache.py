@@ -612,7 +612,7 @@ class LogStructuredKVCache(nn.Module):
         self._check_room(n)
         from .attention import _rows16
         with _lib.on_device(dev):
-            k, k_raw, v = (_rows16(t.to(device=dev, dtype=self.recent_k.dtype)) for t in (k, k_raw, v))
+            k, k_raw, v = (_rows16(t.to(device=dev, dtype=self.recent_k.dtype))[0] for t in (k, k_raw, v))
             self.token_count += n
             c, keep = self._chunk_struct(k, k_raw, v, positions, ends, n)
             state = self._state_struct()

@@ -115,6 +115,73 @@ __device__ __forceinline__ float* tree_part(float* part, const TreeGeo& a, int s
 constexpr int kTreeWarps = 4;
 constexpr int kTreeStages = 3;
 
+// The four warps' results of a CTA's 16 rows, joined in warp order: the split's partial, or the output
+// where a lane has one split.  `ring`: each warp's own shared memory, ring_bytes apart.
+template <typename T, int D, int DT>
+__device__ __forceinline__ void tree_join_warps(const TreeGeo& a, unsigned char* ring, size_t ring_bytes,
+                                                float (*wm_)[16], float (*wl_)[16], float (&o)[DT][4], float m0,
+                                                float m1, float l0, float l1, int ln, int split, int row0, int NQ,
+                                                bool drafts, const TreeSmem& tree, T* out, float* part) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3, T_ = a.T;
+  unsigned char* wbase = ring + warp * ring_bytes;
+  float* wacc = reinterpret_cast<float*>(wbase);
+  if (t4 == 0) {
+    wm_[warp][g8] = m0;
+    wl_[warp][g8] = l0;
+    wm_[warp][g8 + 8] = m1;
+    wl_[warp][g8 + 8] = l1;
+  }
+#pragma unroll
+  for (int jd = 0; jd < DT; ++jd) {
+    const int c0 = jd * 8 + 2 * t4;
+    *reinterpret_cast<float2*>(wacc + g8 * D + c0) = make_float2(o[jd][0], o[jd][1]);
+    *reinterpret_cast<float2*>(wacc + (g8 + 8) * D + c0) = make_float2(o[jd][2], o[jd][3]);
+  }
+  __syncthreads();
+  const size_t orow = (size_t)ln * a.rf * T_ + row0;
+  const bool whole = a.nsplit == 1;   // no partials, no combine
+  if (tid < NQ) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kTreeWarps; ++w) mx = fmaxf(mx, wm_[w][tid]);
+    float l = 0.f, f[kTreeWarps];
+#pragma unroll
+    for (int w = 0; w < kTreeWarps; ++w) {
+      f[w] = wm_[w][tid] == -INFINITY ? 0.f : exp2f(wm_[w][tid] - mx);
+      l += wl_[w][tid] * f[w];
+    }
+    const bool absent = drafts && tree_absent(tree.mask, (row0 + tid) % T_);
+#pragma unroll
+    for (int w = 0; w < kTreeWarps; ++w) wm_[w][tid] = whole ? f[w] / l : f[w];
+    wl_[0][tid] = absent ? 1.f : 0.f;
+    if (!whole) *reinterpret_cast<float2*>(tree_part(part, a, split, orow + tid)) = make_float2(mx, absent ? -1.f : l);
+  }
+  __syncthreads();
+  for (int x = tid; x < NQ * (D / 4); x += blockDim.x) {
+    const int r = x / (D / 4), c = x % (D / 4) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!whole || wl_[0][r] == 0.f) {
+#pragma unroll
+      for (int w = 0; w < kTreeWarps; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(ring + w * ring_bytes + (r * D + c) * 4);
+        const float f = wm_[w][r];
+        v.x = fmaf(y.x, f, v.x);
+        v.y = fmaf(y.y, f, v.y);
+        v.z = fmaf(y.z, f, v.z);
+        v.w = fmaf(y.w, f, v.w);
+      }
+    }
+    if (whole) {
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(out + (orow + r) * D + c) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+      else
+        *reinterpret_cast<float4*>(out + (orow + r) * D + c) = v;
+    } else {
+      *reinterpret_cast<float4*>(tree_part(part, a, split, orow + r) + 4 + c) = v;
+    }
+  }
+}
+
 template <int D>
 struct TreeShape {
   static constexpr int TS = 16, CPR = D / 8, KS = D / 16, DT = D / 8;
@@ -339,60 +406,8 @@ __global__ void __launch_bounds__(kTreeWarps * 32, D <= 128 ? 2 : 1)
     l0 += __shfl_xor_sync(0xffffffffu, l0, off);
     l1 += __shfl_xor_sync(0xffffffffu, l1, off);
   }
-  // The warps' results of the 16 rows in shared memory (each in its own ring), joined in warp order.
-  float* wacc = reinterpret_cast<float*>(wbase);
-  if (t4 == 0) {
-    wm_[warp][g8] = m0;
-    wl_[warp][g8] = l0;
-    wm_[warp][g8 + 8] = m1;
-    wl_[warp][g8 + 8] = l1;
-  }
-#pragma unroll
-  for (int jd = 0; jd < DT; ++jd) {
-    const int c0 = jd * 8 + 2 * t4;
-    *reinterpret_cast<float2*>(wacc + g8 * D + c0) = make_float2(o[jd][0], o[jd][1]);
-    *reinterpret_cast<float2*>(wacc + (g8 + 8) * D + c0) = make_float2(o[jd][2], o[jd][3]);
-  }
-  __syncthreads();
-  const size_t orow = (size_t)ln * a.rf * T + row0;
-  const bool whole = a.nsplit == 1;   // no partials, no combine
-  if (tid < NQ) {
-    float mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kTreeWarps; ++w) mx = fmaxf(mx, wm_[w][tid]);
-    float l = 0.f, f[kTreeWarps];
-#pragma unroll
-    for (int w = 0; w < kTreeWarps; ++w) {
-      f[w] = wm_[w][tid] == -INFINITY ? 0.f : exp2f(wm_[w][tid] - mx);
-      l += wl_[w][tid] * f[w];
-    }
-    const bool absent = u1 > up + ur && tree_absent(tree.mask, (row0 + tid) % T);
-#pragma unroll
-    for (int w = 0; w < kTreeWarps; ++w) wm_[w][tid] = whole ? f[w] / l : f[w];
-    wl_[0][tid] = absent ? 1.f : 0.f;
-    if (!whole) *reinterpret_cast<float2*>(tree_part(part, a, split, orow + tid)) = make_float2(mx, absent ? -1.f : l);
-  }
-  __syncthreads();
-  for (int x = tid; x < NQ * (D / 4); x += blockDim.x) {
-    const int r = x / (D / 4), c = x % (D / 4) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!whole || wl_[0][r] == 0.f) {
-#pragma unroll
-      for (int w = 0; w < kTreeWarps; ++w) {
-        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<unsigned char*>(smem4) +
-                                                          (size_t)w * ST * S::STAGE_BYTES + (r * D + c) * 4);
-        const float f = wm_[w][r];
-        v.x = fmaf(y.x, f, v.x);
-        v.y = fmaf(y.y, f, v.y);
-        v.z = fmaf(y.z, f, v.z);
-        v.w = fmaf(y.w, f, v.w);
-      }
-    }
-    if (whole)
-      *reinterpret_cast<uint2*>(out + (orow + r) * D + c) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-    else
-      *reinterpret_cast<float4*>(tree_part(part, a, split, orow + r) + 4 + c) = v;
-  }
+  tree_join_warps<B16, D, DT>(a, reinterpret_cast<unsigned char*>(smem4), (size_t)ST * S::STAGE_BYTES, wm_, wl_, o, m0, m1,
+                              l0, l1, ln, split, row0, NQ, u1 > up + ur, tree, out, part);
 }
 
 // ---------------------------------------------------------------- bf16: tcgen05, up to 128 query rows per CTA
@@ -788,50 +803,76 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
   }
 }
 
-// ---------------------------------------------------------------- float32: CUDA cores, 32 query rows per CTA
-// Q, K, V and P tiles in shared memory (rows padded by one 16-byte chunk), every thread a 4 x 4 block of
-// the 32 x 64 scores and a 4 x (D / 16) block of O; four elements of the inner index per step, so that
-// the shared-memory reads (12 wavefronts per 64 fused products of a warp) stay below the products.
-// The next K tile is on its way during this tile's softmax and value product, the next V tile during
-// the next scores.
-constexpr int kF32Rows = 32, kF32TS = 64, kF32Threads = 128;
-
+// ---------------------------------------------------------------- float32: mma.sync in three tf32 products
+// As the bf16 kernel, with mma.sync.m16n8k8 (tf32): every float32 operand is split into a tf32 part and
+// the tf32 part of the rest (22 bits together), and a product is hi hi + hi lo + lo hi, summed in
+// float32; what is left out is below 2^-21 of it.  (Float32 fused products from shared memory, four rows by
+// four keys a thread, were bound by shared-memory reads: 23.7 us against 14.6 for 39 rows over 2.2K keys.)
+// K and V rows are padded by 16 bytes, so that the fragments' reads fall into 32 different banks.
 template <int D>
 struct TreeF32Shape {
-  static constexpr int LD = D + 4, LDP = kF32TS + 4;
-  static constexpr size_t smem = sizeof(float) * (kF32Rows * LD + 2 * kF32TS * LD + kF32Rows * LDP + 2 * kF32TS + 2 * kF32Rows);
+  static constexpr int TS = 16, LD = D + 4, KS = D / 8, DT = D / 8, CPR = D / 4;
+  static constexpr int ST = D == 64 ? 2 : 3;   // two CTAs per SM up to 64 features, one at 128
+  static constexpr int STAGE_BYTES = 2 * TS * LD * 4 + TS * 4;   // K, V, mass
+  static constexpr size_t smem = (size_t)kTreeWarps * ST * STAGE_BYTES;
+  static constexpr int CTAS = D <= 64 ? 2 : 1;   // per SM
 };
 
+__device__ __forceinline__ void mma_tf32(float* c, const unsigned* a, unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void split_tf32(float x, unsigned& hi, unsigned& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(hi) : "f"(x));
+  asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+// The same, not moved out of a loop (Q's parts of 128 features would not fit the registers).
+__device__ __forceinline__ void split_tf32_here(float x, unsigned& hi, unsigned& lo) {
+  asm volatile("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(hi) : "f"(x));
+  asm volatile("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+// c += a b for one n8 tile, the operands split.
+__device__ __forceinline__ void mma_split(float* c, const unsigned* ah, const unsigned* al, float x0, float x1) {
+  unsigned h0, l0, h1, l1;
+  split_tf32(x0, h0, l0);
+  split_tf32(x1, h1, l1);
+  mma_tf32(c, al, h0, h1);
+  mma_tf32(c, ah, l0, l1);
+  mma_tf32(c, ah, h0, h1);
+}
+
 template <int D>
-__global__ void __launch_bounds__(kF32Threads, 2) tree_f32_kernel(TreeGeo a, logkv_prefix_t pre, const float* rk,
-                                                              const float* rv, float* part, int32_t* status) {
+__global__ void __launch_bounds__(kTreeWarps * 32, TreeF32Shape<D>::CTAS)
+    tree_f32_kernel(TreeGeo a, logkv_prefix_t pre, const float* rk, const float* rv, float* out, float* part,
+                    int32_t* status) {
   using S = TreeF32Shape<D>;
-  constexpr int LD = S::LD, LDP = S::LDP, TS = kF32TS, NR = kF32Rows, C4 = D / 4, J = (D + 63) / 64;
+  constexpr int TS = S::TS, LD = S::LD, KS = S::KS, DT = S::DT, CPR = S::CPR, ST = S::ST;
   extern __shared__ uint4 smem4[];
   __shared__ TreeSmem tree;
-  __shared__ int sh_poison[2];
-  float* sq = reinterpret_cast<float*>(smem4);
-  float* sk = sq + NR * LD;
-  float* sv = sk + TS * LD;
-  float* sp = sv + TS * LD;
-  float* sm = sp + NR * LDP;   // [2][TS] masses of this tile and the next
-  float* rm = sm + 2 * TS;     // [NR] running maximum and sum
-  float* rl = rm + NR;
+  __shared__ float wm_[kTreeWarps][16], wl_[kTreeWarps][16];
   pdl_entry();
-  const int tid = threadIdx.x;
-  const int ln = blockIdx.x, split = blockIdx.y, row0 = blockIdx.z * NR, g = ln % a.G, b = ln / a.G;
-  const int T = a.T, NQ = min(NR, a.rf * T - row0);
-  tree_parents(a, b, tree, tid, kF32Threads);
-  for (int x = tid; x < NR * C4; x += kF32Threads) {
-    const int r = x / C4, c = x % C4, row = row0 + r;
-    if (r < NQ)
-      cp_async16(sq + r * LD + 4 * c, static_cast<const float*>(a.q) + b * a.qs[0] + (g * a.rf + row / T) * a.qs[1] +
-                                          (row % T) * a.qs[2] + 4 * c);
-    else
-      *reinterpret_cast<float4*>(sq + r * LD + 4 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int g8 = lane >> 2, t4 = lane & 3;
+  const int ln = blockIdx.x, split = blockIdx.y, row0 = blockIdx.z * 16, g = ln % a.G, b = ln / a.G;
+  const int NQ = min(16, a.rf * a.T - row0), T = a.T;
+  tree_parents(a, b, tree, tid, kTreeWarps * 32);
   cp_async_commit();
   const int Lp = prefix_length(pre, ln), R = a.rcount;
+  int tok[2];   // tokens of the lane's rows g8 and g8 + 8
+  float qf[KS][4];   // A fragments: (g8, t4), (g8 + 8, t4), (g8, t4 + 4), (g8 + 8, t4 + 4)
+#pragma unroll
+  for (int hr = 0; hr < 2; ++hr) {
+    const int r = g8 + 8 * hr, row = row0 + min(r, NQ - 1);
+    tok[hr] = row % T;
+    const float* qp = static_cast<const float*>(a.q) + b * a.qs[0] + (g * a.rf + row / T) * a.qs[1] + tok[hr] * a.qs[2];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks][hr] = r < NQ ? qp[ks * 8 + t4] : 0.f;
+      qf[ks][2 + hr] = r < NQ ? qp[ks * 8 + t4 + 4] : 0.f;
+    }
+  }
   const int up = (Lp + TS - 1) / TS, ur = (R + TS - 1) / TS, uc = (T + TS - 1) / TS, U = up + ur + uc;
   const int ns = tree_splits(a, U);
   if (split >= ns) {
@@ -839,181 +880,173 @@ __global__ void __launch_bounds__(kF32Threads, 2) tree_f32_kernel(TreeGeo a, log
     return;
   }
   const int u0 = (int)((long long)U * split / ns), u1 = (int)((long long)U * (split + 1) / ns);
-  const bool drafts = u1 > up + ur;
-  if (tid < NR) {
-    rm[tid] = -INFINITY;
-    rl[tid] = 0.f;
-  }
-  auto unit = [&](int u, int& first, int& rows) {
-    const int cls = u < up ? 0 : u < up + ur ? 1 : 2;
-    first = (cls == 0 ? u : cls == 1 ? u - up : u - up - ur) * TS;
-    rows = min(TS, (cls == 0 ? Lp : cls == 1 ? R : T) - first);
-    return cls;
-  };
-  // Tile u of K (with its masses) or V by cp.async; rows past the segment's end are zeros.
-  auto load = [&](int u, bool is_v) {
-    int first, rows;
-    const int cls = unit(u, first, rows);
-    const size_t r0 = cls == 0 ? (size_t)ln * pre.capacity + first : (size_t)ln * a.rcap + first;
-    const long long* st = is_v ? a.vs : a.ks;
-    const float* src = cls == 0   ? static_cast<const float*>(is_v ? pre.v : pre.k) + r0 * D
-                       : cls == 1 ? (is_v ? rv : rk) + r0 * D
-                                  : static_cast<const float*>(is_v ? a.vn : a.kn) + b * st[0] + g * st[1] + first * st[2];
-    const long long stride = cls == 2 ? st[2] : D;
-    float* dst = is_v ? sv : sk;
-    for (int x = tid; x < TS * C4; x += kF32Threads) {
-      const int r = x / C4, c = x % C4;
-      if (r < rows) cp_async16(dst + r * LD + 4 * c, src + r * stride + 4 * c);
-      else *reinterpret_cast<float4*>(dst + r * LD + 4 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int mine = (u1 - u0) > warp ? (u1 - u0 - warp + kTreeWarps - 1) / kTreeWarps : 0;
+  unsigned char* wbase = reinterpret_cast<unsigned char*>(smem4) + (size_t)warp * ST * S::STAGE_BYTES;
+  const float* kn = static_cast<const float*>(a.kn) + b * a.ks[0] + g * a.ks[1];
+  const float* vn = static_cast<const float*>(a.vn) + b * a.vs[0] + g * a.vs[1];
+  auto tile = [&](int u, int& first, int& rows) {
+    if (u < up) {
+      first = u * TS;
+      rows = min(TS, Lp - first);
+      return 0;
     }
-    if (!is_v && tid < TS) {
-      float* m = sm + (u & 1) * TS + tid;
-      if (cls == 0 && tid < rows) cp_async4(m, pre.mass + r0 + tid);
-      else *m = 0.f;
+    if (u < up + ur) {
+      first = (u - up) * TS;
+      rows = min(TS, R - first);
+      return 1;
+    }
+    first = (u - up - ur) * TS;
+    rows = min(TS, T - first);
+    return 2;
+  };
+  auto issue = [&](int k, int stage) {
+    if (k < mine) {
+      int first, rows;
+      const int cls = tile(u0 + warp + k * kTreeWarps, first, rows);
+      const size_t r0 = cls == 0 ? (size_t)ln * pre.capacity + first : (size_t)ln * a.rcap + first;
+      const float* kb = cls == 0 ? static_cast<const float*>(pre.k) + r0 * D : cls == 1 ? rk + r0 * D : kn + first * a.ks[2];
+      const float* vb = cls == 0 ? static_cast<const float*>(pre.v) + r0 * D : cls == 1 ? rv + r0 * D : vn + first * a.vs[2];
+      const long long kst = cls == 2 ? a.ks[2] : D, vst = cls == 2 ? a.vs[2] : D;
+      float* sk = reinterpret_cast<float*>(wbase + (size_t)stage * S::STAGE_BYTES);
+      float* sv = sk + TS * LD;
+      float* sm = sv + TS * LD;
+#pragma unroll 8
+      for (int flat = lane; flat < TS * CPR; flat += 32) {
+        const int r = flat / CPR, c = flat % CPR;
+        if (r < rows) {
+          cp_async16(sk + r * LD + c * 4, kb + r * kst + c * 4);
+          cp_async16(sv + r * LD + c * 4, vb + r * vst + c * 4);
+        } else {
+          *reinterpret_cast<float4*>(sk + r * LD + c * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+          *reinterpret_cast<float4*>(sv + r * LD + c * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      if (lane < TS) {
+        if (cls == 0 && lane < rows) cp_async4(sm + lane, pre.mass + r0 + lane);
+        else sm[lane] = 0.f;
+      }
     }
     cp_async_commit();
   };
-  load(u0, false);
-  load(u0, true);
-  const int ty = tid >> 4, tx = tid & 15;   // rows 4 ty .. 4 ty + 3; keys tx + 16 j; columns 4 (tx + 16 j)
-  float o[4][4 * J];
+  float o[DT][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int j = 0; j < DT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4 * J; ++j) o[i][j] = 0.f;
-  if (drafts) {   // uniform over the block; the oldest group holds Q and the parents
-    cp_async_wait<2>();
-    tree_masks(a, tree, status, tid, kF32Threads, [] { __syncthreads(); });
+  for (int k = 0; k < ST - 1; ++k) issue(k, k);
+  if (u1 > up + ur) {   // uniform over the block; the parents' copies are the oldest group
+    cp_async_wait<ST - 1>();
+    tree_masks(a, tree, status, tid, kTreeWarps * 32, [] { __syncthreads(); });
   }
-  int tok[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) tok[i] = (row0 + min(4 * ty + i, NQ - 1)) % T;
-  for (int u = u0; u < u1; ++u) {
+  for (int k = 0; k < mine; ++k) {
+    issue(k + ST - 1, (k + ST - 1) % ST);
+    cp_async_wait<ST - 1>();
+    __syncwarp();
     int first, rows;
-    const int cls = unit(u, first, rows);
-    cp_async_wait<1>();
-    __syncthreads();   // K and the masses are here
-    float s[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-#pragma unroll 4
-    for (int c = 0; c < C4; ++c) {
-      float4 x[4], y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(sq + (4 * ty + i) * LD + 4 * c);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * LD + 4 * c);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
-          s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
-          s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
-          s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
-        }
-    }
-    __syncthreads();   // K has been read
-    if (u + 1 < u1) load(u + 1, false);
+    const int cls = tile(u0 + warp + k * kTreeWarps, first, rows);
+    float* sk = reinterpret_cast<float*>(wbase + (size_t)(k % ST) * S::STAGE_BYTES);
+    float* sv = sk + TS * LD;
+    const float* sm = sv + TS * LD;
+    // Columns each row sees; drafted tokens whose V is not finite, taken out of the product below.
+    unsigned see0 = (1u << rows) - 1, see1 = see0, poison = 0;
     if (cls == 2) {
-      // Drafted tokens whose V is not finite leave the product; the rows that see them get a NaN sum.
-      if (tid < 2) sh_poison[tid] = 0;
-      if (u + 1 < u1) cp_async_wait<1>();
-      else cp_async_wait<0>();
-      __syncthreads();
-      for (int x = tid; x < rows * D; x += kF32Threads) {
-        float* v = sv + x / D * LD + x % D;
-        if (!isfinite(*v)) {
-          *v = 0.f;
-          atomicOr(&sh_poison[x / D >> 5], 1 << (x / D & 31));
-        }
-      }
-      __syncthreads();
-    }
-    const float* mass = sm + (u & 1) * TS;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 4 * ty + i;
-      float mt = -INFINITY;
+      see0 = tree.mask[tok[0]][first >> 5] >> (first & 31) & see0;
+      see1 = tree.mask[tok[1]][first >> 5] >> (first & 31) & see1;
+      const int r = lane & 15;   // two lanes per row of V
       bool bad = false;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int col = tx + 16 * j;
-        bool see = col < rows;
-        if (cls == 2 && see) {
-          see = tree.mask[tok[i]][(first + col) >> 5] >> ((first + col) & 31) & 1;
-          bad |= see && (sh_poison[col >> 5] >> (col & 31) & 1);
+      for (int c = lane >> 4; c < D; c += 2)
+        if (!isfinite(sv[r * LD + c])) {
+          sv[r * LD + c] = 0.f;
+          bad = true;
         }
-        s[i][j] = see ? fmaf(s[i][j], a.scale_log2, mass[col] * a.mass_log2) : -INFINITY;
-        mt = fmaxf(mt, s[i][j]);
-      }
-#pragma unroll
-      for (int off = 1; off < 16; off <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, off));
-      const float mo = rm[r], mn = fmaxf(mo, mt);
-      const float al = mn == -INFINITY ? 1.f : exp2f(mo - mn);
-      float sum = bad ? NAN : 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float p = s[i][j] == -INFINITY ? 0.f : exp2f(s[i][j] - mn);
-        sp[r * LDP + tx + 16 * j] = p;
-        sum += p;
-      }
-#pragma unroll
-      for (int off = 1; off < 16; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      __syncwarp();   // every lane of the row has read its running maximum
-      if (tx == 0) {
-        rm[r] = mn;
-        rl[r] = rl[r] * al + sum;
-      }
-      // The row's 16 threads also own its columns of O.
-#pragma unroll
-      for (int j = 0; j < 4 * J; ++j) o[i][j] *= al;
+      poison = __ballot_sync(0xffffffffu, bad);
+      poison = (poison | poison >> 16) & 0xffffu;
+      __syncwarp();
     }
-    if (u + 1 < u1) cp_async_wait<1>();
-    else cp_async_wait<0>();
-    __syncthreads();   // V is here (P of rows 4 ty .. 4 ty + 3 is written and read by the same half warp)
-#pragma unroll 2
-    for (int n = 0; n < TS; n += 4) {
-      float4 p[4];
+    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4*>(sp + (4 * ty + i) * LDP + n);
+    for (int ks = 0; ks < KS; ++ks) {
+      unsigned ah[4], al[4];
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int c = 4 * (tx + 16 * j);
-        if (c < D) {
+      for (int i = 0; i < 4; ++i) {
+        if (D > 64) split_tf32_here(qf[ks][i], ah[i], al[i]);
+        else split_tf32(qf[ks][i], ah[i], al[i]);
+      }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 v = *reinterpret_cast<const float4*>(sv + (n + e) * LD + c);
+      for (int j = 0; j < 2; ++j)
+        mma_split(sc[j], ah, al, sk[(8 * j + g8) * LD + 8 * ks + t4], sk[(8 * j + g8) * LD + 8 * ks + t4 + 4]);
+    }
+    float mt0 = -INFINITY, mt1 = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float pe = e == 0 ? p[i].x : e == 1 ? p[i].y : e == 2 ? p[i].z : p[i].w;
-              o[i][4 * j] = fmaf(pe, v.x, o[i][4 * j]);
-              o[i][4 * j + 1] = fmaf(pe, v.y, o[i][4 * j + 1]);
-              o[i][4 * j + 2] = fmaf(pe, v.z, o[i][4 * j + 2]);
-              o[i][4 * j + 3] = fmaf(pe, v.w, o[i][4 * j + 3]);
-            }
-          }
-        }
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int col = 8 * j + 2 * t4 + e;
+        const float mass = sm[col] * a.mass_log2;
+        sc[j][e] = see0 >> col & 1 ? fmaf(sc[j][e], a.scale_log2, mass) : -INFINITY;
+        sc[j][2 + e] = see1 >> col & 1 ? fmaf(sc[j][2 + e], a.scale_log2, mass) : -INFINITY;
+        mt0 = fmaxf(mt0, sc[j][e]);
+        mt1 = fmaxf(mt1, sc[j][2 + e]);
       }
     }
-    __syncthreads();   // V has been read
-    if (u + 1 < u1) load(u + 1, true);
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      mt0 = fmaxf(mt0, __shfl_xor_sync(0xffffffffu, mt0, off));
+      mt1 = fmaxf(mt1, __shfl_xor_sync(0xffffffffu, mt1, off));
+    }
+    const float mn0 = fmaxf(m0, mt0), mn1 = fmaxf(m1, mt1);
+    const float al0 = mn0 == -INFINITY ? 1.f : exp2f(m0 - mn0);
+    const float al1 = mn1 == -INFINITY ? 1.f : exp2f(m1 - mn1);
+    m0 = mn0;
+    m1 = mn1;
+    float p[2][4], s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        p[j][e] = sc[j][e] == -INFINITY ? 0.f : exp2f(sc[j][e] - mn0);
+        p[j][2 + e] = sc[j][2 + e] == -INFINITY ? 0.f : exp2f(sc[j][2 + e] - mn1);
+        s0 += p[j][e];
+        s1 += p[j][2 + e];
+      }
+    }
+    if (poison & see0) s0 = NAN;
+    if (poison & see1) s1 = NAN;
+    l0 = l0 * al0 + s0;
+    l1 = l1 * al1 + s1;
+    if (__any_sync(0xffffffffu, al0 != 1.f || al1 != 1.f)) {
+#pragma unroll
+      for (int jd = 0; jd < DT; ++jd) {
+        o[jd][0] *= al0;
+        o[jd][1] *= al0;
+        o[jd][2] *= al1;
+        o[jd][3] *= al1;
+      }
+    }
+    // O += P V, eight slots at a time: slot 8 j + 2 t4 + e is index t4 + 4 e of the product, which makes the
+    // scores' fragment P's.
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      unsigned ph[4], pl[4];
+      split_tf32(p[j][0], ph[0], pl[0]);
+      split_tf32(p[j][2], ph[1], pl[1]);
+      split_tf32(p[j][1], ph[2], pl[2]);
+      split_tf32(p[j][3], ph[3], pl[3]);
+      const float* vr = sv + (8 * j + 2 * t4) * LD + g8;
+#pragma unroll
+      for (int jd = 0; jd < DT; ++jd) mma_split(o[jd], ph, pl, vr[8 * jd], vr[LD + 8 * jd]);
+    }
+    __syncwarp();
   }
+  cp_async_wait<0>();
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 4 * ty + i;
-    if (r >= NQ) continue;
-    float* pp = tree_part(part, a, split, (size_t)ln * a.rf * T + row0 + r);
-    if (tx == 0)
-      *reinterpret_cast<float2*>(pp) = make_float2(rm[r], drafts && tree_absent(tree.mask, tok[i]) ? -1.f : rl[r]);
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int c = 4 * (tx + 16 * j);
-      if (c < D) *reinterpret_cast<float4*>(pp + 4 + c) = make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
-    }
+  for (int off = 1; off < 4; off <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, off);
   }
+  tree_join_warps<float, D, DT>(a, reinterpret_cast<unsigned char*>(smem4), (size_t)ST * S::STAGE_BYTES, wm_, wl_, o, m0,
+                                m1, l0, l1, ln, split, row0, NQ, u1 > up + ur, tree, out, part);
 }
 
 // ---------------------------------------------------------------- combine
@@ -1133,20 +1166,21 @@ static bool tree_tc(const logkv_layout_t& l, long long rows) {
   return l.dtype == LOGKV_DTYPE_BF16 && (l.dim == 64 || l.dim == 128) && rows > 16;
 }
 
-// Splits: two CTAs per SM over all lanes and row tiles, at least a key tile per warp each.
+// Splits: as many CTAs over all lanes and row tiles as run at once, at least a key tile per warp each.
 static TreePlan tree_plan(const logkv_layout_t& l, int heads, int tokens, int prefix_capacity) {
   TreePlan p;
   const bool f32 = l.dtype == LOGKV_DTYPE_F32;
   const long long rows = (long long)(heads / l.groups) * tokens;
   p.tc = tree_tc(l, rows);
-  const int most = p.tc ? 128 : f32 ? kF32Rows : 16;
+  const int most = p.tc ? 128 : 16;
   const long long tiles = (rows + most - 1) / most;
   p.tile_rows = p.tc ? (int)((rows + tiles - 1) / tiles) : most;
-  p.ts = p.tc ? kTcTS : f32 ? kF32TS : 16;
-  p.upw = p.tc ? 2 : f32 ? 1 : kTreeWarps;
+  p.ts = p.tc ? kTcTS : 16;
+  p.upw = p.tc ? 2 : kTreeWarps;
   const long long ctas = (long long)l.batch * l.groups * tiles;
   const int units = (prefix_capacity + l.recent_capacity + tokens) / p.ts + 3;
-  p.nsmin = (int)std::max(1LL, 296 / ctas);
+  const int per_sm = (f32 && l.dim > 64) || l.dim > 128 ? 1 : 2;
+  p.nsmin = (int)std::max(1LL, 148 * per_sm / ctas);
   p.nsplit = std::max(1, std::min(p.nsmin, units / p.upw));
   return p;
 }
@@ -1226,9 +1260,10 @@ static int launch_tree_f32(const TreeGeo& a, const TreePlan& p, const logkv_pref
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
   if (e != cudaSuccess) return (int)e;
   const unsigned tiles = (unsigned)((a.rf * a.T + p.tile_rows - 1) / p.tile_rows);
-  launch_pdl(kern, dim3(a.B * a.G, p.nsplit, tiles), kF32Threads, S::smem, st, a, pre,
-             static_cast<const float*>(s.recent_k), static_cast<const float*>(s.recent_v), part, x.status);
-  launch_tree_combine<float, D, kF32TS>(a, pre, part, x.out, st);
+  launch_pdl(kern, dim3(a.B * a.G, p.nsplit, tiles), kTreeWarps * 32, S::smem, st, a, pre,
+             static_cast<const float*>(s.recent_k), static_cast<const float*>(s.recent_v), static_cast<float*>(x.out),
+             part, x.status);
+  if (p.nsplit > 1) launch_tree_combine<float, D, 16>(a, pre, part, x.out, st);
   return launch_status();
 }
 

@@ -338,12 +338,18 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
   if (nc > kBeamCand || sh_h > kBeamHits) {
     // More than the buffers hold: the k-th largest key bit by bit, the logits read again each time.
     auto visit = [&](auto take) {
-      for (int c = c0; c < c1; ++c)
-#pragma unroll 1
-        for (int i = 0; i < NV * VN; ++i) {
-          const int e = (c * CH + i / VN * kBeamThreads + tid) * VN + i % VN, v = e - lead;
-          if (v >= 0 && v < a.V && (float)base[e] > -INFINITY) take(beam_key((float)base[e], v));
-        }
+      for (int c = c0; c < c1; ++c) {
+        unsigned x[NW];
+        fetch(c, x);
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+#pragma unroll
+          for (int e = 0; e < WN; ++e) {
+            const float f = Word::get(x[i], e);
+            const int v = (c * CH + i / 4 * kBeamThreads + tid) * VN + i % 4 * WN + e - lead;
+            if (f > -INFINITY && v >= 0 && v < a.V) take(beam_key(f, v));
+          }
+      }
     };
     U64 kt = 0;
     for (int bit = 63; bit >= 0; --bit) {

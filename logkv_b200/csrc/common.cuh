@@ -71,6 +71,22 @@ static void launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
   cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
+// Dynamic shared memory limit of a kernel, set once per device (the attribute stays; setting it again is
+// harmless, so no lock).
+template <auto Kern>
+static int smem_limit_once(size_t smem) {
+  static unsigned long long done = 0;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (__atomic_load_n(&done, __ATOMIC_RELAXED) & bit) return 0;
+  e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+  return 0;
+}
+
 __device__ __forceinline__ void set_status(int32_t* status, int32_t bit) {
   if (status) atomicOr(status, bit);
 }

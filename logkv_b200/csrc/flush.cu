@@ -962,7 +962,7 @@ extern "C" int logkv_window_append_path(const logkv_layout_t* layout, const logk
                                         void* stream) {
   const int val = validate(layout, 1);
   if (val != LOGKV_OK) return val;
-  if (!chunk || !path) return LOGKV_E_POINTER;
+  if (!chunk || !path || (reinterpret_cast<uintptr_t>(path) & (path_wide ? 7 : 3))) return LOGKV_E_POINTER;
   if (tokens < 1) return LOGKV_E_SHAPE;
   AppendArgs a{};
   const int rc = make_append(layout, state, chunk->k, chunk->k_strides, chunk->k_raw, chunk->k_raw_strides, chunk->v,

@@ -373,12 +373,15 @@ static void set_index(RowArgs& a, int B, const void* index, int wide, int32_t* s
   a.status = status;
 }
 
+static size_t reorder_smem(int B) {
+  return (size_t)kReorderWarps * kReorderSlots * kReorderSlot + (size_t)B * 12 + 16;
+}
+
 static int launch_reorder(RowArgs& a, int B, const void* index, int wide, int32_t* status, cudaStream_t st) {
   if (a.n == 0) return LOGKV_OK;
   set_index(a, B, index, wide, status);
-  const size_t smem = (size_t)kReorderWarps * kReorderSlots * kReorderSlot + (size_t)B * 12 + 16;
-  const cudaError_t e = cudaFuncSetAttribute(reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
+  const size_t smem = reorder_smem(B);
+  if (const int e = smem_limit_once<reorder_kernel>(reorder_smem(kReorderBatch))) return e;
   // One CTA per SM; no more warps than a source per row would have tiles.
   long long tiles = 0;
   for (int i = 0; i < a.n; ++i)
@@ -393,8 +396,7 @@ static int launch_counts(RowArgs& a, int B, const void* index, int wide, int32_t
   int cols = 1;
   for (int i = 0; i < a.n; ++i) cols = std::max(cols, (a.buf[i].seg_bytes + 63) / 64);
   const size_t smem = (size_t)B * 64;
-  const cudaError_t e = cudaFuncSetAttribute(reorder_counts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
+  static_assert(kReorderBatch * 64 <= 48 * 1024, "within the default limit");
   launch_pdl(reorder_counts_kernel, dim3(cols, a.n), 256, smem, st, a);
   return launch_status();
 }
@@ -408,7 +410,7 @@ extern "C" {
 LOGKV_API int logkv_reorder_batch(const logkv_layout_t* layout, const logkv_state_t* state,
                                   const logkv_prefix_t* prefix, int32_t recent_count, int32_t window_from,
                                   const void* index, int32_t index_wide, int32_t* status, void* stream) {
-  if (!layout || !state || !index) return LOGKV_E_POINTER;
+  if (!layout || !state || !index || (reinterpret_cast<uintptr_t>(index) & (index_wide ? 7 : 3))) return LOGKV_E_POINTER;
   const logkv_layout_t& l = *layout;
   if (l.dtype != LOGKV_DTYPE_F32 && l.dtype != LOGKV_DTYPE_BF16) return LOGKV_E_DTYPE;
   if (l.batch < 1 || l.batch > kReorderBatch || l.groups < 1 || l.dim < 1 || l.clusters < 1 || l.levels < 1 ||
@@ -478,7 +480,7 @@ LOGKV_API int logkv_reorder_batch(const logkv_layout_t* layout, const logkv_stat
 
 LOGKV_API int logkv_reorder_rows(const logkv_rows_t* buffers, int32_t n, int32_t batch, const void* index,
                                  int32_t index_wide, int32_t* status, void* stream) {
-  if (!buffers || !index) return LOGKV_E_POINTER;
+  if (!buffers || !index || (reinterpret_cast<uintptr_t>(index) & (index_wide ? 7 : 3))) return LOGKV_E_POINTER;
   if (n < 0 || n > 30 || batch < 1 || batch > kReorderBatch) return LOGKV_E_SHAPE;
   RowArgs a{};
   for (int i = 0; i < n; ++i) {

@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
 // As the bf16 kernel, with mma.sync.m16n8k8 (tf32): every float32 operand is split into a tf32 part and
 // the tf32 part of the rest (22 bits together), and a product is hi hi + hi lo + lo hi, summed in
 // float32; what is left out is below 2^-21 of it.  (Float32 fused products from shared memory, four rows by
-// four keys a thread, were bound by shared-memory reads: 23.7 us against 14.6 for 39 rows over 2.2K keys.)
+// four keys a thread, were bound by shared-memory reads: 23.7 us against 16.8 for 39 rows over 2.2K keys.)
 // K and V rows are padded by 16 bytes, so that the fragments' reads fall into 32 different banks.
 template <int D>
 struct TreeF32Shape {
@@ -828,19 +828,24 @@ __device__ __forceinline__ void split_tf32(float x, unsigned& hi, unsigned& lo) 
   asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(hi) : "f"(x));
   asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
-// The same, not moved out of a loop (Q's parts of 128 features would not fit the registers).
+// The same, not moved out of a loop (Q's parts of 64 features and more would not fit the registers).
 __device__ __forceinline__ void split_tf32_here(float x, unsigned& hi, unsigned& lo) {
   asm volatile("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(hi) : "f"(x));
   asm volatile("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
-// c += a b for one n8 tile, the operands split.
+// c += a b for one n8 tile, the operands split.  The three products start from zero and are added to c by a
+// rounded float32 sum: the matrix instruction's own accumulation truncates, which over a long sum is a
+// bias (relative error 2e-6 where this has 2.5e-7).
 __device__ __forceinline__ void mma_split(float* c, const unsigned* ah, const unsigned* al, float x0, float x1) {
   unsigned h0, l0, h1, l1;
   split_tf32(x0, h0, l0);
   split_tf32(x1, h1, l1);
-  mma_tf32(c, al, h0, h1);
-  mma_tf32(c, ah, l0, l1);
-  mma_tf32(c, ah, h0, h1);
+  float d[4] = {0.f, 0.f, 0.f, 0.f};
+  mma_tf32(d, al, h0, h1);
+  mma_tf32(d, ah, l0, l1);
+  mma_tf32(d, ah, h0, h1);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] += d[i];
 }
 
 template <int D>
@@ -969,7 +974,7 @@ __global__ void __launch_bounds__(kTreeWarps * 32, TreeF32Shape<D>::CTAS)
       unsigned ah[4], al[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (D > 64) split_tf32_here(qf[ks][i], ah[i], al[i]);
+        if (D > 32) split_tf32_here(qf[ks][i], ah[i], al[i]);
         else split_tf32(qf[ks][i], ah[i], al[i]);
       }
 #pragma unroll
@@ -1214,8 +1219,7 @@ static int launch_tree_bf16(const TreeGeo& a, const TreePlan& p, const logkv_pre
   using S = TreeShape<D>;
   using B16 = __nv_bfloat16;
   auto kern = tree_mma_kernel<D>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
-  if (e != cudaSuccess) return (int)e;
+  if (const int e = smem_limit_once<tree_mma_kernel<D>>(S::smem)) return e;
   const unsigned tiles = (unsigned)((a.rf * a.T + p.tile_rows - 1) / p.tile_rows);
   launch_pdl(kern, dim3(a.B * a.G, p.nsplit, tiles), kTreeWarps * 32, S::smem, st, a, pre,
              static_cast<const B16*>(s.recent_k), static_cast<const B16*>(s.recent_v), static_cast<B16*>(x.out), part,
@@ -1231,8 +1235,7 @@ static int launch_tree_tc(const TreeGeo& a, const TreePlan& p, const logkv_prefi
   using S = TreeTcShape<D>;
   using B16 = __nv_bfloat16;
   auto kern = tree_tc_kernel<D>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
-  if (e != cudaSuccess) return (int)e;
+  if (const int e = smem_limit_once<tree_tc_kernel<D>>(S::smem)) return e;
   TreeMaps maps;
   memset(&maps, 0, sizeof(maps));
   const size_t lanes = (size_t)a.B * a.G;
@@ -1257,8 +1260,7 @@ static int launch_tree_f32(const TreeGeo& a, const TreePlan& p, const logkv_pref
                            const logkv_tree_args_t& x, float* part, cudaStream_t st) {
   using S = TreeF32Shape<D>;
   auto kern = tree_f32_kernel<D>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
-  if (e != cudaSuccess) return (int)e;
+  if (const int e = smem_limit_once<tree_f32_kernel<D>>(S::smem)) return e;
   const unsigned tiles = (unsigned)((a.rf * a.T + p.tile_rows - 1) / p.tile_rows);
   launch_pdl(kern, dim3(a.B * a.G, p.nsplit, tiles), kTreeWarps * 32, S::smem, st, a, pre,
              static_cast<const float*>(s.recent_k), static_cast<const float*>(s.recent_v), static_cast<float*>(x.out),
@@ -1287,9 +1289,11 @@ LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_sta
   const int rc = check_tree(layout, x->heads, x->tokens);
   if (rc) return rc;
   if (x->recent_count < 0 || x->recent_count > layout->recent_capacity || prefix->capacity < 0) return LOGKV_E_SHAPE;
-  auto a16 = [](const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  auto at = [](const void* p, uintptr_t n) { return p && (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  auto a16 = [&](const void* p) { return at(p, 16); };
   if (!a16(x->q) || !a16(x->k_new) || !a16(x->v_new) || !a16(x->out) || !a16(workspace) || !a16(state->recent_k) ||
-      !a16(state->recent_v) || !a16(prefix->k) || !a16(prefix->v) || !prefix->mass || !prefix->length || !x->parents)
+      !a16(state->recent_v) || !a16(prefix->k) || !a16(prefix->v) || !at(prefix->mass, 4) || !at(prefix->length, 4) ||
+      !at(x->parents, x->parents_wide ? 8 : 4))
     return LOGKV_E_POINTER;
   const long long e = (long long)esize_of(layout->dtype);
   TreeGeo a{};

@@ -100,6 +100,18 @@ def test_ties_go_to_the_lowest_index(dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+def test_flat_distributions(dtype):
+    """Uniform logits over many slices (every one ties), and two levels split in the middle of a slice."""
+    x = torch.full((2, 3, 151936), 1.5, device="cuda", dtype=dtype)
+    r = torch.tensor([[0.0, 0.0, 0.0], [-2.0, -1.0, -3.0]], device="cuda")
+    check(x, r, 32)
+    x[:, :, 70000:] = 1.75
+    check(x, r, 32)
+    x[0, 2, 151935] = 2.0
+    check(x, r, 3, True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_masked_and_broken_logits(dtype):
     low = torch.finfo(dtype).min
     x, r = draw(8, 4, 9001, dtype, seed=2)

@@ -5,6 +5,11 @@
 // the tree's ancestor mask.  The keys of a lane are split over CTAs; every CTA keeps the running
 // maximum and sum of its rows' softmax in float32 and leaves (m, l, O) per row, which
 // tree_combine_kernel joins in split order.
+//
+// Bound by HBM (keys and values are read once per 128 query rows) from a few MB per SM on; below that
+// by latency.  Measured on B200, device time: 7 drafts of one sequence over 8.3K slots x 8 groups (32 MB)
+// 14.8 us; 8 x 26 drafts (260 MB) 53 us, 0.76 of the measured copy bandwidth; 32 x 64 drafts (1.06 GB,
+// 131 GFLOP) 176-212 us, 0.77-0.93.
 #include <algorithm>
 #include <cstring>
 
@@ -112,6 +117,8 @@ __device__ __forceinline__ float* tree_part(float* part, const TreeGeo& a, int s
 // ---------------------------------------------------------------- bf16: mma.sync, 16 query rows per CTA
 // The 16 rows are the M of mma.sync.m16n8k16.  Each of the 4 warps streams 16-slot tiles of its own
 // through a private ring of cp.async stages (XOR-swizzled for ldmatrix); tiles do not cross segments.
+// Used up to 16 rows, where the tcgen05 kernel's start-up costs more (52 rows: 156 us here, 73 there), and
+// for the head dims that kernel has no shape for, in tiles of 16 rows.
 constexpr int kTreeWarps = 4;
 constexpr int kTreeStages = 3;
 
@@ -419,7 +426,8 @@ __global__ void __launch_bounds__(kTreeWarps * 32, D <= 128 ? 2 : 1)
 //              tile and the drafted tokens' (strided) by cp.async with zero fill.
 // Tensor memory, 256 columns: two 64-column score buffers (P as bf16 over the first half of its own
 // scores) and O.  K and V have rings of their own: K(r) is free once its scores are done, V(r) once
-// its product is; the loader asks in the order in which the tensor core gives them back.  Every wait
+// its product is; the loader asks in the order in which the tensor core gives them back.  Two CTAs per
+// SM cover each other's chain of scores, softmax and product (1.1 us a unit at 128 rows).  Every wait
 // is bounded; on expiry a role stops and the status gets bit 17.
 constexpr int32_t kStatusTreeTimeout = 1 << 17;
 constexpr long long kTreeWaitBudget = 4000000000LL;   // clock cycles (about 2 s)

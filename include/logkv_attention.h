@@ -139,7 +139,7 @@ LOGKV_API int logkv_attention(const logkv_layout_t* layout, const logkv_state_t*
  * where the ancestors of t are parents[t], parents[parents[t]], ...  parents[t] = -1: t follows the
  * last committed token; 0 <= parents[t] < t: t follows token parents[t]; -2: no token (rows of a
  * batch whose trees are smaller are padded so).  Any other value is treated as -2 and sets bit 18
- * of `status`.  A token that is absent, or whose chain of parents reaches an absent token, writes a
+ * of `status` (bit 17: a bounded wait expired, the output is not valid).  A token that is absent, or whose chain of parents reaches an absent token, writes a
  * zero output row and is seen by no token: its K and V may hold anything.  A token whose V holds a
  * NaN or an infinity makes the outputs of the tokens that see it NaN, and only those.
  *
@@ -181,7 +181,8 @@ LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_sta
  * Beam search: batch row b of the cache becomes the old row index[b], in place (no reference
  * counterpart).  index is [B] on the device, int32 or int64 (index_wide); any map is allowed (one row
  * taken over by several, swaps, cycles).  An entry outside [0, B) leaves its row as it is and sets bit
- * 19 of `status` (device int32, may be NULL).  Rows with index[b] = b are not touched.
+ * 19 of `status` (device int32, may be NULL); bit 20: a bounded wait for a copy expired.  Rows with
+ * index[b] = b are not touched.
  *
  * window_from = -1: the whole rows: ladder, clusters, exact pool, span bookkeeping, s_h, the window's
  * rows [0, recent_count) and, when `prefix` is not NULL, the packed prefix.  K and V past a level's

@@ -864,7 +864,8 @@ class LogStructuredKVCache(nn.Module):
                 ctypes.byref(self._layout), ctypes.byref(self._state_struct()), ctypes.byref(rs.prefix_struct()),
                 self.recent_count, -1 if window_from is None else int(window_from), index.data_ptr(),
                 index.dtype == torch.int64, rs.status_ptr, _lib.stream_ptr(dev)), "logkv_reorder_batch")
-        self._route_ready = None     # the next flush's decisions must wait for the moved rows
+        if self._route_ready is not None:
+            self._route_ready = None     # the next flush's decisions must wait for the moved rows
 
     # ------------------------------------------------------------------ read side
     def _semantic_attention_plan(self):

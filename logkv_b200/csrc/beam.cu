@@ -11,8 +11,8 @@
 // k-th largest key is found bit by bit instead.  Keys are (value, lower index first), so the choice is
 // unique whatever the order of the gathering.
 //
-// Bound by HBM at best (each logit is read once; two instructions and one exponential a logit would allow
-// 24 us for 32 x 16 beams x 151936 in bf16).  Measured: 44 us for B1's walk and selections and 8 for B2
+// Bound by HBM at best (each logit is read once; about five instructions and one exponential a logit leave room
+// for 24 us for 32 x 16 beams x 151936 in bf16).  Measured: 44 us for B1's walk and selections and 8 for B2
 // there, 18 us in all for 29 x 5 x 50021 in float32, 10 us for 4 x 32000.
 #include <algorithm>
 

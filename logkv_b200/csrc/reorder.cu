@@ -9,6 +9,9 @@
 // source row is itself taken over (swaps, chains, cycles) it is of all sources: they are in shared
 // memory before any row is written and no other warp touches the column, so the rows need no order and
 // the state no second copy.
+//
+// Bound by HBM: 4 of 8 rows of a 32K-token cache (369 MB to move) take 75 us, 0.76 of the measured copy
+// bandwidth (92 us through registers, bound by instructions); a window's tail of 27 of 64 rows 10.8 us, 0.93.
 #include <algorithm>
 
 #include "attn_common.cuh"
@@ -27,8 +30,8 @@ constexpr int32_t kStatusReorderTimeout = 1 << 20;
 
 // Segment i of row b: base + b * stride + i * seg_stride, seg_bytes long.  With counts (of element
 // size count_size, [B, segs]) only the first unit * max(count of the source, count of the row) bytes
-// (rounded up to whole accesses) move: K and V past a level's count are zero in every row (a flush clears what it vacates), and
-// prefix rows past the length are never read.
+// (rounded up to whole accesses) move: K and V past a level's count are zero in every row (a flush clears
+// what it vacates), and prefix rows past the length are never read.
 struct RowBuffer {
   char* base;
   const void* counts;

@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
       const int st = r % ST;
       uint64_t* empty = is_v ? &v_empty[st] : &k_empty[st];
       uint64_t* full = is_v ? &v_full[st] : &k_full[st];
-      if (r >= ST && !tc::mbar_wait(empty, (r / ST - 1) & 1, kTreeWaitBudget)) return false;
+      if (r >= ST && !__all_sync(0xffffffffu, tc::mbar_wait(empty, (r / ST - 1) & 1, kTreeWaitBudget))) return false;
       int first, rows;
       const int cls = unit(u0 + r, first, rows);
       unsigned char* dst = base + (is_v ? S::OFF_V : S::OFF_K) + st * S::KV_BYTES;

@@ -44,7 +44,7 @@ def maps(B, rs):
 
 @pytest.mark.parametrize("dtype,B,G,D,levels,R", [(BF16, 1, 2, 64, 3, 100), (BF16, 2, 2, 64, 3, 101), (F32, 3, 1, 16, 2, 7),
                                                   (BF16, 5, 3, 128, 4, 256), (F32, 8, 2, 64, 0, 0), (BF16, 19, 1, 32, 3, 1),
-                                                  (BF16, 70, 1, 16, 2, 33)])
+                                                  (BF16, 70, 1, 16, 2, 33), (BF16, 300, 1, 16, 1, 5), (F32, 33, 2, 32, 3, 255)])
 def test_reorder_equals_indexing(dtype, B, G, D, levels, R):
     from logkv_b200.attention import refresh_prefix
     cache = make_cache(dtype, B=B, G=G, D=D, levels=levels, R=R, seed=B)

@@ -46,7 +46,8 @@ def run(cache, q, k, v, p, **kw):
     (BF16, 128, 2, 65, 64, 0), (BF16, 128, 1, 256, 100, 3), (BF16, 128, 7, 130, 31, 3), (BF16, 64, 2, 5, 100, 3),
     (BF16, 64, 4, 40, 255, 3), (BF16, 64, 3, 100, 0, 0), (BF16, 64, 16, 16, 90, 3), (BF16, 32, 2, 9, 100, 3),
     (BF16, 32, 3, 50, 63, 3), (BF16, 16, 4, 21, 100, 3), (BF16, 16, 1, 1, 0, 0), (BF16, 256, 2, 20, 100, 3),
-    (BF16, 256, 1, 3, 17, 0),
+    (BF16, 256, 1, 3, 17, 0), (BF16, 128, 8, 256, 200, 3), (BF16, 64, 12, 256, 0, 2), (BF16, 32, 3, 256, 100, 3),
+    (F32, 128, 3, 256, 100, 3), (BF16, 128, 17, 1, 40, 3), (F32, 32, 9, 2, 40, 3),
     (F32, 64, 2, 1, 100, 3), (F32, 64, 3, 13, 100, 3), (F32, 128, 2, 40, 65, 3), (F32, 128, 5, 7, 0, 0),
     (F32, 32, 4, 33, 256, 2), (F32, 16, 2, 70, 31, 3), (F32, 16, 1, 2, 0, 3)])
 def test_tree_matches_64_bits(dtype, D, rf, T, R, levels):
@@ -235,3 +236,35 @@ def test_runs_agree_bit_for_bit():
     first = run(cache, q, k, v, p)
     for _ in range(5):
         assert torch.equal(run(cache, q, k, v, p), first)
+
+
+def test_two_threads_at_once():
+    """Two host threads on streams of their own, over one cache, tree attention and beam selection."""
+    import threading
+    from logkv_b200 import beam_select, log_kv_tree_attention
+    cache = make_cache(BF16, B=2, G=4, D=128, R=200, seed=23)
+    p = random_tree(np.random.RandomState(24), 2, 40, absent=6)
+    dev = torch.from_numpy(p).cuda()
+    sets = [drafts(cache, 2, 40, seed=s) for s in (25, 26)]
+    x = torch.randn(3, 4, 20000, device="cuda")
+    r = torch.zeros(3, 4, device="cuda")
+    want = [run(cache, *s, p) for s in sets]
+    best = beam_select(x, r, 6)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                a = log_kv_tree_attention(cache, *sets[i], 128 ** -0.5, dev)
+                b = beam_select(x, r, 6)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(a, want[i]) or not all(torch.equal(s, t) for s, t in zip(b, best)):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

@@ -231,6 +231,26 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_host = None
+
+
+def host():
+    """The CPython binding of the latency-bound calls, loaded once; raises if it was not built."""
+    global _host
+    if _host is None:
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise RuntimeError("logkv_b200 host binding missing; run `python -m logkv_b200.build`") from e
+        _host = module
+    return _host
+
+
+def address(name: str) -> int:
+    """Address of a library function, for the host binding."""
+    return ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value
+
+
 def check(code: int, what: str) -> None:
     if code != 0:
         reason = ERRORS.get(code, f"CUDA error {code}")

@@ -11,6 +11,7 @@ import torch
 
 from . import _lib
 
+_native = None   # (beam call, function addresses) of the host binding, once a call has gone through
 MAX_K, MAX_WIDTH = 128, 256   # LOGKV_BEAM_MAX_K, LOGKV_BEAM_MAX_WIDTH
 
 
@@ -32,6 +33,13 @@ def beam_select(logits, scores, k: int, *, keep_places: bool = False):
     k <= 128, W <= 256, N * W <= 65535.  The scratch is allocated per call, so calls on different streams,
     or captured graphs, never share it.
     """
+    global _native
+    if _native is not None:      # checks, allocations and launch in the host binding; None: not covered there
+        y = _native[0](_native[1], _native[2], logits, scores, k, keep_places)
+        if y is not None:
+            if type(y) is int:
+                _lib.check(y, "logkv_beam_select")
+            return y
     if logits.dim() != 3:
         raise ValueError(f"logits must be [N, W, V], got {tuple(logits.shape)}")
     N, W, V = logits.shape
@@ -58,6 +66,7 @@ def beam_select(logits, scores, k: int, *, keep_places: bool = False):
             logits = logits.contiguous()
         scores = scores.contiguous()
         lib = _lib.lib()
+        _native = (_lib.host().beam, _lib.address("logkv_beam_select"), _lib.address("logkv_beam_workspace_bytes"))
         n = lib.logkv_beam_workspace_bytes(N, W, V, k)
         ws = scores.new_empty((n + 7) >> 3, dtype=torch.float64)
         args = _lib.BeamArgs(logits.data_ptr(), scores.data_ptr(), out_scores.data_ptr(), out_rows.data_ptr(),

@@ -7,6 +7,7 @@ Translation units with different numerics:
   reorder.cu    moves rows, no arithmetic;
   beam.cu       default contraction (its float64 scores decide);
   plugin.cu, unified.cu  -fmad=false: the operator-level plugin functions, same contract as flush.cu.
+and ``logkv_b200/_host.so``, the CPython binding of the calls whose time is the host's (host.cpp, g++).
 Run ``python -m logkv_b200.build`` (or ``__graft_entry__.build()``).
 """
 from __future__ import annotations
@@ -20,6 +21,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblogkv_b200.so")
+HOST = os.path.join(HERE, "_host.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
           f"-I{ROOT}", "--expt-relaxed-constexpr"]
@@ -42,24 +44,43 @@ def nvcc() -> str:
     return path
 
 
-def sources_newer_than(target: str) -> bool:
+def sources_newer_than(target: str, suffixes=(".cu", ".cuh")) -> bool:
     if not os.path.exists(target):
         return True
     t = os.path.getmtime(target)
     for root in (CSRC, os.path.join(ROOT, "include")):
         for name in os.listdir(root):
-            if os.path.getmtime(os.path.join(root, name)) > t:
+            if name.endswith((".h", *suffixes)) and os.path.getmtime(os.path.join(root, name)) > t:
                 return True
     return False
 
 
+def build_host() -> None:
+    """The CPython binding against this interpreter's torch."""
+    import sysconfig
+
+    import torch
+    base = os.path.join(os.path.dirname(torch.__file__))
+    inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+           os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
+    tmp = HOST + ".tmp"
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                    "-I" + sysconfig.get_paths()["include"], *(x for i in inc for x in ("-isystem", i)),
+                    os.path.join(CSRC, "host.cpp"), "-o", tmp, "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_cuda",
+                    "-ltorch_cpu", "-ltorch_python"], check=True)
+    os.replace(tmp, HOST)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    if force or sources_newer_than(HOST, (".cpp",)):
+        build_host()
     if not force and not sources_newer_than(LIB):
         return LIB
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
-    objs = []
-    for unit, extra in UNITS:
+    objs, running = [], []
+    for unit, extra in UNITS:   # the units compile side by side
         src = os.path.join(CSRC, unit)
         if not os.path.exists(src):
             continue
@@ -68,8 +89,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
             print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+        running.append((cmd, subprocess.Popen(cmd)))
         objs.append(obj)
+    for cmd, p in running:
+        if p.wait():
+            for _, other in running:
+                other.wait()
+            raise subprocess.CalledProcessError(p.returncode, cmd)
     tmp = LIB + ".tmp"
     subprocess.run([nvcc(), *ARCH, "-shared", "-o", tmp, *objs, "-lcudart"], check=True)
     os.replace(tmp, LIB)

@@ -192,8 +192,14 @@ def test_no_requests_and_refusals():
     from logkv_b200 import beam_select
     x, r = draw(2, 3, 100, F32)
     assert [t.shape for t in beam_select(x[:0], r[:0], 4)] == [(0, 4)] * 3
-    with pytest.raises(ValueError, match="one device"):
-        beam_select(x, r.cpu(), 3)
+    beam_select(x, r, 3)                 # from here on the host binding takes the calls it covers
+    for args, kw, match in [((x, r.cpu(), 3), {}, "one device"), ((x.half(), r, 3), {}, "not supported"),
+                            ((x, r[:1], 3), {}, "scores must be"), ((x, r, 0), {}, "k must be"),
+                            ((x, r, 301), {}, "k must be"), ((x, r, 2), {"keep_places": True}, "keep_places"),
+                            ((x[0], r, 2), {}, "logits must be")]:
+        with pytest.raises(ValueError, match=match):
+            beam_select(*args, **kw)
+    assert [t.shape for t in beam_select(x[:0], r[:0], 4)] == [(0, 4)] * 3
 
 
 # ---------------------------------------------------------------- beam search over decoders

@@ -268,3 +268,34 @@ def test_two_threads_at_once():
     for t in threads:
         t.join()
     assert not bad
+
+
+def test_repeated_calls_are_checked_like_the_first():
+    """Once a call of a shape has gone through, the host binding takes over: same results, same refusals."""
+    from logkv_b200 import log_kv_tree_attention as f
+    cache = make_cache(BF16, B=2, D=64, R=40, seed=27)
+    q, k, v = drafts(cache, 2, 9)
+    p = random_tree(np.random.RandomState(28), 2, 9, absent=2)
+    dev = torch.from_numpy(p).cuda()
+    first = f(cache, q, k, v, 0.125, dev)
+    assert cache._read.native is not None
+    for parents in (dev, dev.int(), torch.from_numpy(p), p.tolist()):
+        assert torch.equal(f(cache, q, k, v, 0.125, parents), first)
+    assert torch.equal(f(cache, q, k, v, 0.125, dev, out=torch.empty_like(first)), first)
+    bad = p.copy()
+    bad[0, 3] = 5
+    for args, match in [((q[:1], k, v, 0.125, dev), "q must be"), ((q.float(), k, v, 0.125, dev), "q must be"),
+                        ((q, k[:, :1], v, 0.125, dev), "k must be"), ((q, k, v[:, :, :8], 0.125, dev), "v shape"),
+                        ((q[:, :3], k, v, 0.125, dev), "multiple"), ((q.cpu(), k, v, 0.125, dev), "device"),
+                        ((q, k, v, 0.125, dev[:, :8]), "parents must be"), ((q, k, v, 0.125, dev.float()), "integers"),
+                        ((q, k, v, 0.125, torch.from_numpy(bad)), "earlier token")]:
+        with pytest.raises(ValueError, match=match):
+            f(cache, *args)
+    with pytest.raises(NotImplementedError):
+        f(cache, q.detach().requires_grad_(), k, v, 0.125, dev)
+    # A flush changes the ladder: the prefix is packed again before the next call.
+    cache._ladder_epoch += 1
+    cache.level_w.mul_(2)
+    again = f(cache, q, k, v, 0.125, dev)
+    assert cache._read.epoch == cache._ladder_epoch and not torch.equal(again, first)
+    check(cache, q, k, v, p, again, scale=0.125)

@@ -205,27 +205,22 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
   const uint4* vec = reinterpret_cast<const uint4*>(base);
   const int nvec = (a.V + lead + VN - 1) / VN;
   const int per = (c1 - c0 + kBeamGroups - 1) / kBeamGroups;   // chunks per group
+  // The row's first and last vectors may hold a neighbour's logits: then they are left out here and their
+  // own logits come after the walk, one by one, from the thread that would have had the vector.
+  const int tail = nvec * VN - lead - a.V, lo = lead ? 1 : 0, hi = tail ? nvec - 1 : nvec;
   auto fetch = [&](int c, unsigned* x) {
     const int j0 = c * CH + tid;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       uint4 v = make_uint4(Word::kNone, Word::kNone, Word::kNone, Word::kNone);
-      if (j0 + i * kBeamThreads < nvec) v = __ldg(vec + j0 + i * kBeamThreads);
+      const int j = j0 + i * kBeamThreads;
+      if (j >= lo && j < hi) v = __ldg(vec + j);
       x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
     }
   };
   float m = -INFINITY, s = 0.f, mg = -INFINITY;
   int left = per, group = 0;
-  auto step = [&](int c, unsigned* x) {
-    if (c == 0 || (c + 1) * CH >= nvec) {   // the row's first and last vectors may hold a neighbour's logits
-#pragma unroll
-      for (int i = 0; i < NW; ++i)
-#pragma unroll
-        for (int e = 0; e < WN; ++e) {
-          const int v = (c * CH + i / 4 * kBeamThreads + tid) * VN + i % 4 * WN + e - lead;
-          if (v < 0 || v >= a.V) x[i] = Word::mask(x[i], e);
-        }
-    }
+  auto step = [&](const unsigned* x) {
     unsigned mx = x[0];
 #pragma unroll
     for (int i = 1; i < NW; ++i) mx = Word::max(mx, x[i]);
@@ -274,14 +269,33 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
   fetch(c0, xa);
   if (c0 + 1 < c1) fetch(c0 + 1, xb);
   for (int c = c0; c < c1; c += 2) {
-    step(c, xa);
+    step(xa);
     if (c + 2 < c1) fetch(c + 2, xa);
     if (c + 1 < c1) {
-      step(c + 1, xb);
+      step(xb);
       if (c + 3 < c1) fetch(c + 3, xb);
     }
   }
   if (left != per) tops[group][tid] = mg;
+  auto single = [&](int j) {   // the logits of vector j, one by one
+    const int c = j / CH;
+    if (tid != j % kBeamThreads || c < c0 || c >= c1) return;
+    float best = -INFINITY;
+#pragma unroll 1
+    for (int e = max(j * VN, lead); e < min((j + 1) * VN, lead + a.V); ++e) {
+      const float f = (float)base[e];
+      if (f > m) {
+        s = m == -INFINITY ? s : s * tc::ex2((m - f) * kLog2e);
+        m = f;
+      }
+      s += tc::ex2((f - (m == -INFINITY ? 0.f : m)) * kLog2e);
+      best = fmaxf(best, f);
+    }
+    float& top = tops[(c - c0) / per][tid];
+    top = fmaxf(top, best);
+  };
+  if (lead) single(0);
+  if (tail && !(lead && nvec == 1)) single(nvec - 1);
   if (tid == 0) sh_n = sh_h = 0;
   // The slice's sum: the threads' maxima and float32 sums, joined in float64.
   const float mw = warp_max(m);
@@ -342,18 +356,20 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
   if (nc > kBeamCand || sh_h > kBeamHits) {
     // More than the buffers hold: the k-th largest key bit by bit, the logits read again each time.
     auto visit = [&](auto take) {
-      for (int c = c0; c < c1; ++c) {
-        unsigned x[NW];
-        fetch(c, x);
+      for (int c = c0; c < c1; ++c)
+#pragma unroll 1
+        for (int i = 0; i < NV; ++i) {
+          const int j = c * CH + i * kBeamThreads + tid;
+          if (j >= nvec) break;
+          const uint4 q = __ldg(vec + j);
+          const unsigned x[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int i = 0; i < NW; ++i)
-#pragma unroll
-          for (int e = 0; e < WN; ++e) {
-            const float f = Word::get(x[i], e);
-            const int v = (c * CH + i / 4 * kBeamThreads + tid) * VN + i % 4 * WN + e - lead;
+          for (int e = 0; e < VN; ++e) {
+            const float f = Word::get(x[e / WN], e % WN);
+            const int v = j * VN + e - lead;
             if (f > -INFINITY && v >= 0 && v < a.V) take(beam_key(f, v));
           }
-      }
+        }
     };
     U64 kt = 0;
     for (int bit = 63; bit >= 0; --bit) {

@@ -60,9 +60,9 @@ def build_host() -> None:
     import sysconfig
 
     import torch
-    base = os.path.join(os.path.dirname(torch.__file__))
+    base = os.path.dirname(torch.__file__)
     inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
-           os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
+           os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")]
     tmp = HOST + ".tmp"
     subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",

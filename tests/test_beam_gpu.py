@@ -278,3 +278,44 @@ def test_pending_host_flags_cannot_be_reordered():
         d.reorder([1, 0])
     with pytest.raises(ValueError, match="rows"):
         LogKVBeams([d], 2, 2)
+
+
+# ---------------------------------------------------------------- large finite logits
+def masked_requests(dtype, V, low, seed):
+    """Four requests of three beams: few live tokens, beams masked throughout or but for one token, every
+    beam masked, and the first half masked."""
+    x, r = draw(4, 3, V, dtype, seed=seed)
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x[0, :, torch.randperm(V, generator=gen, device="cuda")[30:]] = low
+    x[1, 1] = low
+    x[1, 2, 1:] = low
+    x[2] = low
+    x[3, :, :V // 2] = low
+    return x, r
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("low", [-1e4, -1e9, -1e10, -1e20, -1e30, None])
+def test_logits_masked_with_large_numbers(dtype, low):
+    """Masks of every magnitude, over one slice and over many.  Scores near a mask's magnitude are rounded
+    in float64 (1e10: 2e-6), which the tolerance's 2^-18 covers."""
+    low = torch.finfo(dtype).min if low is None else low
+    for V in (520, 40000):
+        x, r = masked_requests(dtype, V, low, seed=31)
+        for k, keep in ((3, True), (8, False), (64, False)):
+            check(x, r, k, keep)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("high", [2e6, 5e9, 1e30, None])
+def test_large_maxima(dtype, high):
+    """A few logits far above the others, and beams of nothing else: the others count for nothing."""
+    high = torch.finfo(dtype).max if high is None else high
+    x, r = draw(3, 4, 40000, dtype, seed=32)
+    x[0, :, 7::5000] = high              # eight places
+    x[1, 1] = high
+    x[1, 3, 39999] = high
+    x[2, 0, :4] = high
+    x[2, 0, 30000:30002] = high / 2
+    for k, keep in ((4, True), (8, False)):
+        check(x, r, k, keep)

@@ -279,20 +279,22 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
     }
   }
   if (left != per) tops[group][tid] = mg;
-  auto single = [&](int j) {   // the logits of vector j, one by one
+  auto own = [&](int j, auto use) {   // the row's logits in vector j, one by one
+#pragma unroll 1
+    for (int e = max(j * VN, lead); e < min((j + 1) * VN, lead + a.V); ++e) use((float)base[e], e - lead);
+  };
+  auto single = [&](int j) {
     const int c = j / CH;
     if (tid != j % kBeamThreads || c < c0 || c >= c1) return;
     float best = -INFINITY;
-#pragma unroll 1
-    for (int e = max(j * VN, lead); e < min((j + 1) * VN, lead + a.V); ++e) {
-      const float f = (float)base[e];
+    own(j, [&](float f, int) {
       if (f > m) {
         s = m == -INFINITY ? s : s * tc::ex2((m - f) * kLog2e);
         m = f;
       }
       s += tc::ex2((f - (m == -INFINITY ? 0.f : m)) * kLog2e);
       best = fmaxf(best, f);
-    }
+    });
     float& top = tops[(c - c0) / per][tid];
     top = fmaxf(top, best);
   };
@@ -363,13 +365,18 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
         for (int i = 0; i < NV; ++i) {
           const int j = c * CH + i * kBeamThreads + tid;
           if (j >= nvec) break;
+          if (j < lo || j >= hi) {   // a ragged end, as in the walk
+            own(j, [&](float f, int v) {
+              if (f > -INFINITY) take(beam_key(f, v));
+            });
+            continue;
+          }
           const uint4 q = __ldg(vec + j);
           const unsigned x[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
           for (int e = 0; e < VN; ++e) {
             const float f = Word::get(x[e / WN], e % WN);
-            const int v = j * VN + e - lead;
-            if (f > -INFINITY && v >= 0 && v < a.V) take(beam_key(f, v));
+            if (f > -INFINITY) take(beam_key(f, j * VN + e - lead));
           }
         }
     };

@@ -319,3 +319,20 @@ def test_large_maxima(dtype, high):
     x[2, 0, 30000:30002] = high / 2
     for k, keep in ((4, True), (8, False)):
         check(x, r, k, keep)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [1500, 5003, 20007])
+def test_ties_at_every_alignment(dtype, V):
+    """More equal logits than are gathered, in views at every offset from a 16-byte boundary: larger values
+    in front of a row and behind it are not its own."""
+    r = torch.tensor([[0.0, -0.5, -0.25], [-1.0, 0.0, -2.0]], device="cuda")
+    for off in (*range(9), 24):          # 24: the last row ends where the buffer does
+        wide = torch.full((2, 3, V + 24), 7.0, device="cuda", dtype=dtype)
+        x = wide[:, :, off:off + V]
+        x.fill_(1.5)
+        x[1, 1, V - 1] = x[1, 2, 0] = 1.75
+        check(x, r, 7)
+        x.fill_(-1e30)
+        x[0, 0, ::400] = 1.0
+        check(x, r, 3, True)

@@ -421,13 +421,20 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
 // The candidates in rounds of up to kBeamRound, the k best so far among each round's.
 constexpr int kBeamRound = 2048, kBeamEach = kBeamRound / kBeamThreads;
 
+// Log-sum-exps of the same logits agree to within this: measured over alignments, slices and vocabularies of 37
+// to 151936 they are 2^-23 apart at most, and off by as much.  Scores of different beams as close as this
+// were in no reliable order before.
+constexpr double kBeamSame = 1.0 / (1 << 21);
+static_assert(LOGKV_BEAM_MAX_WIDTH <= kBeamThreads, "a thread per beam");
+
 __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
   using U64 = unsigned long long;
   __shared__ __align__(16) U64 gm[kBeamThreads];
   __shared__ U64 sh_t;
   __shared__ __align__(16) U64 cand[kBeamCand];
   __shared__ int cidx[kBeamCand];
-  __shared__ double lse[LOGKV_BEAM_MAX_WIDTH];
+  __shared__ double lse[LOGKV_BEAM_MAX_WIDTH], above_peak[LOGKV_BEAM_MAX_WIDTH];
+  __shared__ float peak[LOGKV_BEAM_MAX_WIDTH];
   __shared__ float prior[LOGKV_BEAM_MAX_WIDTH];
   __shared__ int isum[kBeamThreads / 32];
   __shared__ int sh_n;
@@ -469,11 +476,22 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
       if (a.sum[at + q] != 0.0) s += a.sum[at + q] * exp2f((a.top[at + q] - m) * kLog2e);   // a NaN stays
     for (int off = 1; off < lanes; off *= 2) s += __shfl_xor_sync(0xffffffffu, s, off);
     if (first == 0 && w < W) {
-      const float r = a.scores[n * W + w];
-      const double z = (double)m + log2(s) / (double)kLog2e;
-      lse[w] = isfinite(r) && isfinite(z) ? z : nan("");
-      prior[w] = r;
+      peak[w] = m;
+      above_peak[w] = log2(s) / (double)kLog2e;
+      prior[w] = a.scores[n * W + w];
     }
+  }
+  __syncthreads();
+  // Beams with the same logits tie, but their sums differ in the last bits where their rows' alignment or
+  // slices do: a beam takes over the log-sum-exp of the lowest one with its maximum and a sum within rounding.
+  if (tid < W) {   // W <= kBeamThreads
+    const float mine = peak[tid];
+    int lowest = tid;
+#pragma unroll 4
+    for (int w = tid - 1; w >= 0; --w)
+      if (peak[w] == mine && fabs(above_peak[w] - above_peak[tid]) <= kBeamSame) lowest = w;
+    const double z = (double)mine + above_peak[lowest];
+    lse[tid] = isfinite(prior[tid]) && isfinite(z) ? z : nan("");
   }
   __syncthreads();
   int found = 0;

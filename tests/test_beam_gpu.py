@@ -336,3 +336,20 @@ def test_ties_at_every_alignment(dtype, V):
         x.fill_(-1e30)
         x[0, 0, ::400] = 1.0
         check(x, r, 3, True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [37, 500, 5003, 16384, 50021, 151936])
+def test_equal_beams_tie(dtype, V):
+    """Beams with the same logits and score tie token by token, whatever their rows' alignment and slices:
+    the lower beam comes first."""
+    x, r = draw(5, 6, V, dtype, seed=33 + V)
+    x[:, 1] = x[:, 0]
+    x[:, 4] = x[:, 0]
+    x[:, 5] = x[:, 2]
+    r[:, 1] = r[:, 4] = r[:, 0]
+    r[:, 5] = r[:, 2]
+    for k, keep in ((6, True), (6, False), (24, False)):
+        check(x, r, k, keep)
+    same, _ = draw(7, 1, V, dtype, seed=34 + V)
+    check(same.expand(7, 16, V).contiguous(), torch.zeros(7, 16, device="cuda"), 33)

@@ -830,6 +830,20 @@ class LogStructuredKVCache(nn.Module):
             raise ValueError(f"row indices must be in [0, {self.batch_size})")
         return t.contiguous()
 
+    def _check_reorder(self, window_from=None) -> None:
+        """Raise if reorder_batch would be refused (but for its index)."""
+        if self._active_updates is not None:
+            raise RuntimeError("reorder_batch is not recorded by update tapes")
+        if self.op_log is not None:
+            raise RuntimeError("reorder_batch cannot reorder the rows of a bound op-log")
+        if self._deferred_take is not None:
+            raise RuntimeError("commit_deferred must follow add_recent_deferred")
+        if window_from is not None and not 0 <= window_from <= self.recent_count:
+            raise ValueError(f"window_from must be in [0, recent_count={self.recent_count}], got {window_from}")
+        dev = self._buffers["level_k"].device
+        if self._read is None and dev.type == "cuda" and _lib.capture_id(dev):
+            raise RuntimeError("capture reorder_batch only after the cache has been attended over once")
+
     def reorder_batch(self, index, *, window_from=None) -> None:
         """Beam search: batch row b takes over the old row index[b], in place (no reference counterpart).
 
@@ -841,29 +855,19 @@ class LogStructuredKVCache(nn.Module):
         since).  Not while an update tape or an op-log is bound or a deferred flush is open: their
         records name rows.
         """
-        if self._active_updates is not None:
-            raise RuntimeError("reorder_batch is not recorded by update tapes")
-        if self.op_log is not None:
-            raise RuntimeError("reorder_batch cannot reorder the rows of a bound op-log")
-        if self._deferred_take is not None:
-            raise RuntimeError("commit_deferred must follow add_recent_deferred")
-        if window_from is not None and not 0 <= window_from <= self.recent_count:
-            raise ValueError(f"window_from must be in [0, recent_count={self.recent_count}], got {window_from}")
+        self._check_reorder(window_from)
         index = self._row_index(index)
-        dev = self._buffers["level_k"].device
-        with _lib.on_device(dev):
+        with _lib.on_device(index.device):
             # The prefix moves whether or not it is current, so that a captured call does not depend on
             # what was current when it was captured; its buffers therefore exist from here on.
             rs = self._read
             if rs is None:
-                if _lib.capture_id(dev):
-                    raise RuntimeError("capture reorder_batch only after the cache has been attended over once")
                 from .attention import _read_state
                 rs = _read_state(self)
             _lib.check(_lib.lib().logkv_reorder_batch(
                 ctypes.byref(self._layout), ctypes.byref(self._state_struct()), ctypes.byref(rs.prefix_struct()),
                 self.recent_count, -1 if window_from is None else int(window_from), index.data_ptr(),
-                index.dtype == torch.int64, rs.status_ptr, _lib.stream_ptr(dev)), "logkv_reorder_batch")
+                index.dtype == torch.int64, rs.status_ptr, _lib.stream_ptr(index.device)), "logkv_reorder_batch")
         if self._route_ready is not None:
             self._route_ready = None     # the next flush's decisions must wait for the moved rows
 

@@ -46,8 +46,7 @@ class LogKVDecoder:
         """Row b takes over the old row index[b]: the cache's rows (``LogStructuredKVCache.reorder_batch``,
         same arguments) and the pending token's.  A pending token's span-end flags must be on the device
         (``span_ends_device``): host lists cannot follow a device index."""
-        if self.pending and self._ends_host is not None:
-            raise RuntimeError("reordering a pending token needs its span-end flags on the device (span_ends_device)")
+        self._check_reorder(window_from)
         cache = self.cache
         index = cache._row_index(index)
         cache.reorder_batch(index, window_from=window_from)
@@ -61,6 +60,12 @@ class LogKVDecoder:
             _lib.check(_lib.lib().logkv_reorder_rows(
                 rows, len(bufs), cache.batch_size, index.data_ptr(), index.dtype == torch.int64,
                 cache._read.status_ptr, _lib.stream_ptr(dev)), "logkv_reorder_rows")
+
+    def _check_reorder(self, window_from=None) -> None:
+        """Raise if reorder would be refused (but for its index)."""
+        if self.pending and self._ends_host is not None:
+            raise RuntimeError("reordering a pending token needs its span-end flags on the device (span_ends_device)")
+        self.cache._check_reorder(window_from)
 
     def step(self, q, k, v, *, k_raw, input_pos=None, span_ends=None, span_ends_device=None, out=None):
         """One token: q [B, H, 1, D], k / v / k_raw [B, G, 1, D]; returns the attention output
@@ -121,6 +126,8 @@ class LogKVBeams:
 
     def fork(self) -> None:
         """Every beam takes over its request's first row; the scores start again (only that beam alive)."""
+        for d in self.decoders:      # refused before any row has moved
+            d._check_reorder()
         dev = self.scores.device
         first = torch.arange(self.requests, device=dev).mul_(self.beams).repeat_interleave(self.beams)
         for d in self.decoders:
@@ -139,9 +146,14 @@ class LogKVBeams:
             logits = logits.view(self.requests, self.beams, -1)
         if logits.shape[:2] != (self.requests, self.beams):
             raise ValueError(f"logits must be [{self.requests}, {self.beams}, V], got {tuple(logits.shape)}")
-        self.scores, rows, tokens = beam_select(logits, self.scores, self.beams, keep_places=True)
-        rows = rows.view(-1)
-        for i, d in enumerate(self.decoders):
+        window = [None] * len(self.decoders)
+        for i, d in enumerate(self.decoders):      # refused before any row has moved
             forked = self._forked[i] if self._forked else (None, 0)
-            d.reorder(rows, window_from=forked[1] if forked[0] == d.cache._flush_cursor else None)
+            window[i] = forked[1] if forked[0] == d.cache._flush_cursor else None
+            d._check_reorder(window[i])
+        scores, rows, tokens = beam_select(logits, self.scores, self.beams, keep_places=True)
+        rows = rows.view(-1)
+        for d, w in zip(self.decoders, window):
+            d.reorder(rows, window_from=w)
+        self.scores = scores
         return tokens.view(-1), rows

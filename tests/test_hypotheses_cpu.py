@@ -180,3 +180,53 @@ def test_beam_c_abi_checks(lib):
     assert call(1 << 30) == -1
     a.keep_places, a.dtype = 0, 7
     assert call(1 << 30) == -2
+
+
+@pytest.fixture()
+def two_layers(lib, monkeypatch):
+    """Two decoders over host caches whose row moves are recorded in ``moves`` instead of launched, and a
+    selection that keeps every beam."""
+    from logkv_b200 import decode
+    moves = []
+    layers = [decode.LogKVDecoder(make_cache(torch.float32, B=4, G=2, D=64, levels=0, R=5, device="cpu", recent=32),
+                                  0.125) for _ in range(2)]
+    for i, d in enumerate(layers):
+        def move(index, *, window_from=None, i=i, c=d.cache):
+            c._check_reorder(window_from)
+            moves.append((i, window_from))
+        monkeypatch.setattr(d.cache, "reorder_batch", move)
+    monkeypatch.setattr(decode, "beam_select", lambda logits, scores, k, keep_places: (
+        scores - 1, torch.arange(4).view(2, 2), torch.zeros(2, 2, dtype=torch.int64)))
+    return decode.LogKVBeams(layers, 2, 2), moves
+
+
+@pytest.mark.parametrize("why,match", [("flags", "span_ends_device"), ("op_log", "op-log"), ("deferred", "commit_deferred")])
+def test_beams_refuse_before_anything_moves(two_layers, why, match):
+    """A layer that cannot be reordered leaves the scores and the other layers as they were."""
+    beams, moves = two_layers
+    last = beams.decoders[1]
+    if why == "flags":
+        last.pending, last._ends_host = True, [[False]] * 4
+    elif why == "op_log":
+        last.cache.op_log = torch.zeros(1)
+    else:
+        last.cache._deferred_take = 4
+    beams.scores[:] = torch.tensor([[0.0, -2.0], [-1.0, -3.0]])
+    before = beams.scores.clone()
+    for call in (beams.fork, lambda: beams.advance(torch.zeros(4, 10))):
+        with pytest.raises(RuntimeError, match=match):
+            call()
+        assert moves == [] and torch.equal(beams.scores, before) and beams._forked is None
+
+
+def test_beams_keep_the_scores_of_a_failed_step(two_layers):
+    beams, moves = two_layers
+    beams.fork()
+    assert moves == [(0, None), (1, None)]
+    beams.advance(torch.zeros(4, 10))
+    assert moves[2:] == [(0, 5), (1, 5)]
+    before = beams.scores.clone()
+    beams.decoders[1].cache.recent_count = 3         # fewer window rows than at the fork
+    with pytest.raises(ValueError, match="window_from"):
+        beams.advance(torch.zeros(4, 10))
+    assert torch.equal(beams.scores, before) and len(moves) == 4

@@ -134,8 +134,8 @@ class LogKVBeams:
             d.reorder(first)
         self.scores.fill_(float("-inf"))
         self.scores[:, 0] = 0.0
-        # Until a cache's next flush its rows of one request differ in the window behind this fill only.
-        self._forked = [(d.cache._flush_cursor, d.cache.recent_count) for d in self.decoders]
+        # Until a cache's next flush (or reset) its rows of one request differ in the window behind this fill only.
+        self._forked = [(d.cache._ladder_epoch, d.cache.recent_count) for d in self.decoders]
 
     def advance(self, logits):
         """Select the next tokens from the logits [requests, beams, V] (or [requests * beams, V]) of the
@@ -149,7 +149,7 @@ class LogKVBeams:
         window = [None] * len(self.decoders)
         for i, d in enumerate(self.decoders):      # refused before any row has moved
             forked = self._forked[i] if self._forked else (None, 0)
-            window[i] = forked[1] if forked[0] == d.cache._flush_cursor else None
+            window[i] = forked[1] if forked[0] == d.cache._ladder_epoch else None
             d._check_reorder(window[i])
         scores, rows, tokens = beam_select(logits, self.scores, self.beams, keep_places=True)
         rows = rows.view(-1)

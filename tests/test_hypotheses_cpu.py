@@ -230,3 +230,18 @@ def test_beams_keep_the_scores_of_a_failed_step(two_layers):
     with pytest.raises(ValueError, match="window_from"):
         beams.advance(torch.zeros(4, 10))
     assert torch.equal(beams.scores, before) and len(moves) == 4
+
+
+def test_a_reset_cache_moves_whole_rows(two_layers):
+    """What a fork said about the window holds until the cache is filled anew, whose rows may differ
+    anywhere."""
+    beams, moves = two_layers
+    beams.fork()
+    for d in beams.decoders:
+        d.cache.reset_parameters()
+        d.cache.recent_count = d.cache.token_count = 9
+    beams.advance(torch.zeros(4, 10))
+    assert moves[2:] == [(0, None), (1, None)]
+    beams.fork()
+    beams.advance(torch.zeros(4, 10))
+    assert moves[6:] == [(0, 9), (1, 9)]

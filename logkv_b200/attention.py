@@ -54,7 +54,8 @@ class _ReadState:
         self.pv = torch.zeros(B, G, self.capacity, cache.v_dim, dtype=cache.level_v.dtype, device=dev)
         self.mass = torch.zeros(B, G, self.capacity, dtype=torch.float32, device=dev)
         self.length = torch.zeros(B, G, **i32)
-        self.status = torch.zeros(1, **i32)
+        status = getattr(cache, "_read_status", None)   # a foreign cache has none
+        self.status = torch.zeros(1, **i32) if status is None else status
         self.status_ptr = self.status.data_ptr()
         self.epoch = -1
         self.workspaces: dict = {}
@@ -331,7 +332,7 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
     committed tokens, an earlier token's index, or -2 for no token (rows with smaller trees are
     padded so).  Token t attends over the frozen prefix, the window, its ancestors and itself; absent
     tokens, and tokens below one, are seen by nobody and give zero rows.  Parents on the host are
-    checked here; a bad value in a device tensor counts as -2 and sets bit 18 of the read status.
+    checked here; a bad value in a device tensor counts as -2 and sets bit 18 of ``cache.read_status()``.
     Returns [B, H, T, D]; ``out`` may be given.  The scratch is allocated per call, so calls on
     different streams, or captured graphs, never share it.  Forward-only.
 

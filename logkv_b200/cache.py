@@ -262,6 +262,7 @@ class LogStructuredKVCache(nn.Module):
         self._route_done = None
         self._deferred_take = None   # flush started by add_recent_deferred, committed by commit_deferred
         self._read = None            # read side: plan, packed prefix (logkv_b200.attention)
+        self._read_status = torch.zeros(1, dtype=torch.int32, **z)   # bits 16 and up of read_status
 
     # ------------------------------------------------------------------ C-ABI state
     def _apply(self, fn, *args, **kwargs):
@@ -519,11 +520,19 @@ class LogStructuredKVCache(nn.Module):
                 for e in out[:n]]
 
     def read_status(self) -> int:
+        """Status bits (synchronizes); 0 when all is well.
+
+        Bits 0 to 4, of the last flush: carry list, merge list or candidate capacity exceeded, cluster
+        choice failed, a wait for a copy expired.  Bits 16 and up, of every other call since the cache
+        was built or reset: 16 a position outside the rotary tables, 17 a wait in log_kv_tree_attention
+        expired (its output is not valid), 18 a bad parent there, 19 a bad row index
+        in reorder_batch or path entry in add_recent_path, 20 a wait for a copy of a reorder expired.
+        """
         out = ctypes.c_int32(0)
         _lib.check(_lib.lib().logkv_read_status(ctypes.c_void_p(self._workspace.data_ptr()), ctypes.byref(out),
                                                 ctypes.c_void_p(_lib.stream_ptr(self.level_k.device))),
                    "logkv_read_status")
-        return int(out.value)
+        return int(out.value) | int(self._read_status.item())
 
     # ------------------------------------------------------------------ window
     def _positions(self, n: int, input_pos):
@@ -575,7 +584,7 @@ class LogStructuredKVCache(nn.Module):
         int32 or int64, on the device or a host list) lists the n accepted tokens from the root down.
         Every batch row commits n tokens, since the window's fill is one number: with different
         accepted lengths commit the shortest and draft the rest again.  A bad device value commits token
-        0 and sets bit 19 of the read status (when the cache has been attended over).  Without input_pos the positions continue the sequence.
+        0 and sets bit 19 of ``read_status()``.  Without input_pos the positions continue the sequence.
         """
         if self._deferred_take is not None:
             raise RuntimeError("commit_deferred must follow add_recent_deferred")
@@ -616,11 +625,10 @@ class LogStructuredKVCache(nn.Module):
             self.token_count += n
             c, keep = self._chunk_struct(k, k_raw, v, positions, ends, n)
             state = self._state_struct()
-            status = self._read.status.data_ptr() if self._read is not None else None
             _lib.check(_lib.lib().logkv_window_append_path(
                 ctypes.byref(self._layout), ctypes.byref(state), ctypes.byref(c), T, p.data_ptr(),
-                p.stride(0) if p.dim() == 2 else 0, int(p.dtype == torch.int64), int(self.recent_count), status,
-                ctypes.c_void_p(_lib.stream_ptr(dev))), "logkv_window_append_path")
+                p.stride(0) if p.dim() == 2 else 0, int(p.dtype == torch.int64), int(self.recent_count),
+                self._read_status.data_ptr(), ctypes.c_void_p(_lib.stream_ptr(dev))), "logkv_window_append_path")
             del keep
             self.recent_count += n
             self._run_flushes(record_op_log, False)
@@ -848,8 +856,8 @@ class LogStructuredKVCache(nn.Module):
         """Beam search: batch row b takes over the old row index[b], in place (no reference counterpart).
 
         ``index`` ([B], int32 or int64; on the device or a host list) may name a row several times, swap
-        rows and move them in cycles; a bad device value leaves its row as it is and sets bit 19 of the
-        read status.  The ladder, clusters, exact pool, window and packed prefix move; rows that stay are
+        rows and move them in cycles; a bad device value leaves its row as it is and sets bit 19 of
+        ``read_status()``.  The ladder, clusters, exact pool, window and packed prefix move; rows that stay are
         not touched.  ``window_from``: move only the window's rows [window_from, recent_count), when row b
         and row index[b] are known to agree in everything else (beams forked from one row, no flush
         since).  Not while an update tape or an op-log is bound or a deferred flush is open: their
@@ -937,7 +945,7 @@ class LogStructuredKVCache(nn.Module):
         self.p_hi_c.fill_(-1)
         self.ward_cost.fill_(float("inf"))
         for t in (self._recent_ends, self._span_len, self._span_closed, self._span_count, self._row_count,
-                  self._alpha_count_dev):
+                  self._alpha_count_dev, self._read_status):
             t.zero_()
         self.token_count = 0
         self.recent_count = 0

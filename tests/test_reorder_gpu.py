@@ -248,3 +248,21 @@ def test_speculative_step_end_to_end():
         b.add_recent(pick(k), pick(v), k_raw=pick(kr), span_ends=np.take_along_axis(ends, paths, 1).tolist())
         torch.cuda.synchronize()
         same(state(a), state(b), step)
+
+
+def test_read_status_tells_of_bad_device_values():
+    """The public status word has the bits of every call, those before the first attention too, until the
+    cache is reset."""
+    from logkv_b200 import log_kv_tree_attention
+    cache = make_cache(BF16, B=2, G=2, D=64, R=5, seed=15)
+    assert cache.read_status() == 0
+    k, v, kr = drafted(cache, 6, 1)
+    path = torch.tensor([[1, 6, 2], [0, -1, 5]], device="cuda")
+    cache.add_recent_path(k, v, path, k_raw=kr, span_ends=[[False] * 6] * 2)
+    assert cache.read_status() == 1 << 19
+    log_kv_tree_attention(cache, k, k, v, 0.125, torch.tensor([-1, 0, 2, 0, 1, -1], device="cuda"))
+    assert cache.read_status() == 1 << 19 | 1 << 18
+    cache.reset_parameters()
+    assert cache.read_status() == 0
+    cache.reorder_batch(torch.tensor([1, 2], device="cuda"))
+    assert cache.read_status() == 1 << 19

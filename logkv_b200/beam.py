@@ -31,7 +31,7 @@ def beam_select(logits, scores, k: int, *, keep_places: bool = False):
     (``LogStructuredKVCache.reorder_batch(rows.view(-1))``).
 
     k <= 128, W <= 256, N * W <= 65535.  The scratch is allocated per call, so calls on different streams,
-    or captured graphs, never share it.
+    or captured graphs, never share it.  Forward-only.
     """
     global _native
     if _native is not None:      # checks, allocations and launch in the host binding; None: not covered there
@@ -54,6 +54,8 @@ def beam_select(logits, scores, k: int, *, keep_places: bool = False):
         raise ValueError(f"keep_places takes as many continuations as beams (k = {k}, W = {W})")
     if W > MAX_WIDTH or N * W > 65535 or W * V >= (1 << 31) - 32:
         raise ValueError(f"beam shape outside the supported range (N={N}, W={W}, V={V})")
+    if (logits.requires_grad or scores.requires_grad) and torch.is_grad_enabled():
+        raise NotImplementedError("beam_select is forward-only")
     dev = logits.device
     if dev.type != "cuda" or scores.device != dev:
         raise ValueError("logits and scores must be CUDA tensors on one device")

@@ -33,11 +33,13 @@ at::Tensor bytes(size_t n, const at::Tensor& like) {
 
 PyObject* failed(int rc) { return PyLong_FromLong(rc); }
 
+bool wants_gradient(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+
 // [B, heads, T, D] rows in dtype and on the device of `like`, 16-byte aligned, without a gradient to record.
 bool rows_ok(const at::Tensor& t, const at::Tensor& like, int64_t heads, int64_t tokens) {
   if (t.dim() != 4 || t.size(0) != like.size(0) || t.size(1) != heads || t.size(2) != tokens ||
       t.size(3) != like.size(3) || t.scalar_type() != like.scalar_type() || t.device() != like.device() ||
-      t.stride(3) != 1 || (t.requires_grad() && at::GradMode::is_enabled()))
+      t.stride(3) != 1 || wants_gradient(t))
     return false;
   const uint64_t e = t.element_size();
   return ((reinterpret_cast<uint64_t>(t.const_data_ptr()) | (uint64_t)t.stride(0) * e | (uint64_t)t.stride(1) * e |
@@ -111,7 +113,7 @@ PyObject* beam(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const bool f32 = x->scalar_type() == at::kFloat;
   if ((!f32 && x->scalar_type() != at::kBFloat16) || s->dim() != 2 || s->size(0) != N || s->size(1) != W ||
       s->scalar_type() != at::kFloat || s->device() != x->device() || !s->is_contiguous() || N < 1 || N * W > 65535 ||
-      V >= (1LL << 31) || k < 1 || k > LOGKV_BEAM_MAX_K || (keep && k != W) ||
+      V >= (1LL << 31) || k < 1 || k > LOGKV_BEAM_MAX_K || (keep && k != W) || wants_gradient(*x) || wants_gradient(*s) ||
       c10::cuda::current_device() != x->get_device())
     Py_RETURN_NONE;
   const size_t need = address<BeamBytesFn>(args[1])((int32_t)N, (int32_t)W, (int32_t)V, (int32_t)k);

@@ -353,3 +353,15 @@ def test_equal_beams_tie(dtype, V):
         check(x, r, k, keep)
     same, _ = draw(7, 1, V, dtype, seed=34 + V)
     check(same.expand(7, 16, V).contiguous(), torch.zeros(7, 16, device="cuda"), 33)
+
+
+def test_gradients_are_refused_not_dropped():
+    from logkv_b200 import beam_select
+    x, r = draw(2, 3, 100, F32)
+    want = beam_select(x, r, 3)          # from here on the host binding takes the calls it covers
+    for a, b in ((x.clone().requires_grad_(), r), (x, r.clone().requires_grad_())):
+        with pytest.raises(NotImplementedError, match="forward-only"):
+            beam_select(a, b, 3)
+        with torch.no_grad():
+            got = beam_select(a, b, 3)
+        assert not got[0].requires_grad and all(torch.equal(s, t) for s, t in zip(got, want))

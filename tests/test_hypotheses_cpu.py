@@ -245,3 +245,13 @@ def test_a_reset_cache_moves_whole_rows(two_layers):
     beams.fork()
     beams.advance(torch.zeros(4, 10))
     assert moves[6:] == [(0, 9), (1, 9)]
+
+
+def test_beam_gradients_are_refused(lib):
+    from logkv_b200 import beam_select
+    x, r = torch.zeros(2, 3, 10), torch.zeros(2, 3)
+    for a, b in ((x.clone().requires_grad_(), r), (x, r.clone().requires_grad_())):
+        with pytest.raises(NotImplementedError, match="forward-only"):
+            beam_select(a, b, 3)
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+            beam_select(a, b, 3)

@@ -139,9 +139,10 @@ LOGKV_API int logkv_attention(const logkv_layout_t* layout, const logkv_state_t*
  * where the ancestors of t are parents[t], parents[parents[t]], ...  parents[t] = -1: t follows the
  * last committed token; 0 <= parents[t] < t: t follows token parents[t]; -2: no token (rows of a
  * batch whose trees are smaller are padded so).  Any other value is treated as -2 and sets bit 18
- * of `status` (bit 17: a bounded wait expired, the output is not valid).  A token that is absent, or whose chain of parents reaches an absent token, writes a
- * zero output row and is seen by no token: its K and V may hold anything.  A token whose V holds a
- * NaN or an infinity makes the outputs of the tokens that see it NaN, and only those.
+ * of `status` (bit 17: a bounded wait expired, the output is not valid).  A token that is absent, or
+ * whose chain of parents reaches an absent token, writes a zero output row and is seen by no token: its
+ * K and V may hold anything.  A token whose V holds a NaN or an infinity makes the outputs of the tokens
+ * that see it NaN, and only those.
  *
  * q is [B,H,tokens,D], k_new and v_new are [B,G,tokens,D] (post-RoPE, storage dtype) with the given
  * element strides of their batch, head and token axes; the head dim is contiguous and every row
@@ -190,8 +191,9 @@ LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_sta
  * are not moved.
  * window_from >= 0: only the window's rows [window_from, recent_count), for a caller whose rows b and
  * index[b] hold the same ladder, pool and earlier window rows (hypotheses forked from one row since
- * the last flush).  batch <= 512.
+ * the last flush).  batch <= LOGKV_REORDER_MAX_BATCH.
  */
+#define LOGKV_REORDER_MAX_BATCH 512
 LOGKV_API int logkv_reorder_batch(const logkv_layout_t* layout, const logkv_state_t* state,
                                   const logkv_prefix_t* prefix, int32_t recent_count, int32_t window_from,
                                   const void* index, int32_t index_wide, int32_t* status, void* stream);

@@ -118,7 +118,8 @@ class BeamArgs(ctypes.Structure):
                 ("keep_places", ctypes.c_int32)]
 
 
-TREE_MAX_TOKENS = 256   # LOGKV_TREE_MAX_TOKENS
+TREE_MAX_TOKENS = 256     # LOGKV_TREE_MAX_TOKENS
+REORDER_MAX_BATCH = 512   # LOGKV_REORDER_MAX_BATCH
 
 _lib = None
 

@@ -846,6 +846,8 @@ class LogStructuredKVCache(nn.Module):
             raise RuntimeError("reorder_batch cannot reorder the rows of a bound op-log")
         if self._deferred_take is not None:
             raise RuntimeError("commit_deferred must follow add_recent_deferred")
+        if self.batch_size > _lib.REORDER_MAX_BATCH:
+            raise ValueError(f"{self.batch_size} batch rows: reorder_batch takes at most {_lib.REORDER_MAX_BATCH}")
         if window_from is not None and not 0 <= window_from <= self.recent_count:
             raise ValueError(f"window_from must be in [0, recent_count={self.recent_count}], got {window_from}")
         dev = self._buffers["level_k"].device
@@ -861,7 +863,7 @@ class LogStructuredKVCache(nn.Module):
         not touched.  ``window_from``: move only the window's rows [window_from, recent_count), when row b
         and row index[b] are known to agree in everything else (beams forked from one row, no flush
         since).  Not while an update tape or an op-log is bound or a deferred flush is open: their
-        records name rows.
+        records name rows.  At most 512 batch rows.
         """
         self._check_reorder(window_from)
         index = self._row_index(index)

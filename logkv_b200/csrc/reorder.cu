@@ -21,7 +21,7 @@ namespace logkv {
 constexpr int32_t kStatusBadIndex = 1 << 19;
 constexpr int kRowBuffers = 60;
 constexpr int kReorderWarps = 4;
-constexpr int kReorderBatch = 512;
+constexpr int kReorderBatch = LOGKV_REORDER_MAX_BATCH;
 constexpr int kReorderSlots = 6, kReorderAhead = 4;   // slots of a warp's ring; columns on their way in
 constexpr int kReorderSlot = 8 * 1024;                // bytes of a slot
 constexpr int kReorderTileBatch = 32;                 // tiles whose places a warp works out together

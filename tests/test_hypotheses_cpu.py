@@ -255,3 +255,13 @@ def test_beam_gradients_are_refused(lib):
             beam_select(a, b, 3)
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
             beam_select(a, b, 3)
+
+
+def test_reorder_of_too_many_rows(lib):
+    """More batch rows than one call takes are refused with the number, by the cache and before a beam step."""
+    from logkv_b200 import _lib, decode
+    cache = make_cache(torch.float32, B=514, G=1, D=16, K=2, levels=0, R=1, P=8, recent=8, max_seq=64, device="cpu")
+    for call in (lambda: cache.reorder_batch(list(range(514))),
+                 decode.LogKVBeams([decode.LogKVDecoder(cache, 0.25)], 257, 2).fork):
+        with pytest.raises(ValueError, match=f"514 batch rows.*{_lib.REORDER_MAX_BATCH}"):
+            call()

@@ -602,6 +602,8 @@ class LogStructuredKVCache(nn.Module):
         n = p.size(-1)
         if n == 0:
             return
+        if T == 0:
+            raise ValueError(f"path names {n} tokens, but none was drafted")
         if p.device.type == "cpu":
             if bool(((p < 0) | (p >= T)).any()):
                 raise ValueError(f"path entries must be drafted tokens in [0, {T})")

@@ -266,3 +266,13 @@ def test_read_status_tells_of_bad_device_values():
     assert cache.read_status() == 0
     cache.reorder_batch(torch.tensor([1, 2], device="cuda"))
     assert cache.read_status() == 1 << 19
+
+
+def test_path_without_drafted_tokens():
+    """Nothing drafted: refused before anything is counted, with a path on the device too."""
+    cache = make_cache(BF16, B=2, G=2, D=64, R=5, seed=16)
+    k = torch.empty(2, 2, 0, 64, dtype=BF16, device="cuda")
+    for path in ([0], torch.zeros(1, dtype=torch.int64, device="cuda")):
+        with pytest.raises(ValueError, match="drafted"):
+            cache.add_recent_path(k, k, path, k_raw=k, span_ends=[[], []])
+    assert cache.token_count == cache.recent_count == 5

@@ -7,6 +7,7 @@ fails loudly when the shared object is missing (build it with
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 
 import torch
@@ -236,13 +237,18 @@ _host = None
 
 
 def host():
-    """The CPython binding of the latency-bound calls, loaded once; raises if it was not built."""
+    """The CPython binding of the latency-bound calls, loaded once; raises if it was not built for this
+    interpreter and torch."""
     global _host
     if _host is None:
-        try:
-            from . import _host as module
-        except ImportError as e:
-            raise RuntimeError("logkv_b200 host binding missing; run `python -m logkv_b200.build`") from e
+        from .build import host_file
+        path = host_file()
+        if not os.path.exists(path):
+            raise RuntimeError(f"logkv_b200 host binding missing ({os.path.basename(path)}); "
+                               "run `python -m logkv_b200.build`")
+        spec = importlib.util.spec_from_file_location(f"{__package__}._host", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
         _host = module
     return _host
 

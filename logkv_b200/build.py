@@ -7,7 +7,7 @@ Translation units with different numerics:
   reorder.cu    moves rows, no arithmetic;
   beam.cu       default contraction (its float64 scores decide);
   plugin.cu, unified.cu  -fmad=false: the operator-level plugin functions, same contract as flush.cu.
-and ``logkv_b200/_host.so``, the CPython binding of the calls whose time is the host's (host.cpp, g++).
+and ``host_file()``, the CPython binding of the calls whose time is the host's (host.cpp, g++).
 Run ``python -m logkv_b200.build`` (or ``__graft_entry__.build()``).
 """
 from __future__ import annotations
@@ -16,12 +16,12 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblogkv_b200.so")
-HOST = os.path.join(HERE, "_host.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
           f"-I{ROOT}", "--expt-relaxed-constexpr"]
@@ -55,25 +55,30 @@ def sources_newer_than(target: str, suffixes=(".cu", ".cuh")) -> bool:
     return False
 
 
+def host_file() -> str:
+    """The binding's path, with the torch version and the interpreter's ABI it is built against: either's
+    C++ or C interface changes, so another one's file is neither loaded nor taken for built."""
+    import torch
+    return os.path.join(HERE, f"_host.torch{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
 def build_host() -> None:
     """The CPython binding against this interpreter's torch."""
-    import sysconfig
-
     import torch
     base = os.path.dirname(torch.__file__)
     inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
            os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")]
-    tmp = HOST + ".tmp"
+    tmp = host_file() + ".tmp"
     subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                     "-I" + sysconfig.get_paths()["include"], *(x for i in inc for x in ("-isystem", i)),
                     os.path.join(CSRC, "host.cpp"), "-o", tmp, "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_cuda",
                     "-ltorch_cpu", "-ltorch_python"], check=True)
-    os.replace(tmp, HOST)
+    os.replace(tmp, host_file())
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    if force or sources_newer_than(HOST, (".cpp",)):
+    if force or sources_newer_than(host_file(), (".cpp",)):
         build_host()
     if not force and not sources_newer_than(LIB):
         return LIB

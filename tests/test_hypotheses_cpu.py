@@ -265,3 +265,25 @@ def test_reorder_of_too_many_rows(lib):
                  decode.LogKVBeams([decode.LogKVDecoder(cache, 0.25)], 257, 2).fork):
         with pytest.raises(ValueError, match=f"514 batch rows.*{_lib.REORDER_MAX_BATCH}"):
             call()
+
+
+@pytest.mark.parametrize("what", ["torch", "python"])
+def test_host_binding_of_another_torch_or_python(lib, monkeypatch, what):
+    """A binding built for another torch or interpreter is not loaded, the error asks for a build, and the
+    build does one."""
+    import sysconfig
+    from logkv_b200 import _lib, build
+    assert _lib.host().__file__ == build.host_file()
+    built = []
+    monkeypatch.setattr(build, "build_host", lambda: built.append(build.host_file()))
+    build.build()
+    assert built == []
+    monkeypatch.setattr(_lib, "_host", None)
+    if what == "torch":
+        monkeypatch.setattr(torch, "__version__", "0.0.0+none")
+    else:
+        monkeypatch.setattr(sysconfig, "get_config_var", lambda name: ".cpython-000-none.so")
+    with pytest.raises(RuntimeError, match="logkv_b200.build"):
+        _lib.host()
+    build.build()
+    assert built == [build.host_file()]

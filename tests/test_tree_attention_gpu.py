@@ -299,3 +299,33 @@ def test_repeated_calls_are_checked_like_the_first():
     again = f(cache, q, k, v, 0.125, dev)
     assert cache._read.epoch == cache._ladder_epoch and not torch.equal(again, first)
     check(cache, q, k, v, p, again, scale=0.125)
+
+
+def test_first_calls_of_a_process_in_two_threads():
+    """The first calls of a process, from two threads at once, look up the driver's tensor-map encoder: the
+    same bits as later calls."""
+    import os
+    import subprocess
+    import sys
+    import textwrap
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = """
+        import threading, torch
+        import numpy as np
+        from hypotheses import make_cache, random_tree
+        from test_tree_attention_gpu import BF16, drafts
+        from logkv_b200 import log_kv_tree_attention
+        caches = [make_cache(BF16, B=2, G=2, D=128, R=200, seed=s) for s in (1, 2)]
+        sets = [drafts(c, 2, 40) for c in caches]
+        p = torch.from_numpy(random_tree(np.random.RandomState(3), 2, 40)).cuda()
+        start, out = threading.Barrier(2), [None, None]
+        def work(i):
+            start.wait()
+            out[i] = log_kv_tree_attention(caches[i], *sets[i], 0.1, p)
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+        [t.start() for t in threads], [t.join() for t in threads]
+        for i in range(2):
+            assert torch.equal(out[i], log_kv_tree_attention(caches[i], *sets[i], 0.1, p))
+    """
+    subprocess.run([sys.executable, "-c", textwrap.dedent(code)], check=True, timeout=300,
+                   cwd=here, env={**os.environ, "PYTHONPATH": os.path.dirname(here)})

@@ -58,6 +58,8 @@ class _ReadState:
         self.status = torch.zeros(1, **i32) if status is None else status
         self.status_ptr = self.status.data_ptr()
         self.epoch = -1
+        self.pack_stream = None      # stream of the last pack (None: in a graph), and the pack's end
+        self.pack_event = None
         self.workspaces: dict = {}
         self.tree_bytes: dict = {}   # scratch bytes of log_kv_tree_attention by (heads, tokens)
         self.qx: dict = {}           # query_extra by scale
@@ -75,6 +77,27 @@ class _ReadState:
             self._prefix = _lib.Prefix(self.pk.data_ptr(), self.pv.data_ptr(), self.mass.data_ptr(),
                                        self.length.data_ptr(), self.capacity)
         return self._prefix
+
+    def packed(self, epoch: int) -> None:
+        """The current stream was given a pack of the ladder of ``epoch``."""
+        dev = self.pk.device
+        if epoch < 0 or _lib.capture_id(dev):
+            self.pack_stream = None
+        else:
+            if self.pack_event is None:
+                self.pack_event = torch.cuda.Event()
+            self.pack_event.record(torch.cuda.current_stream(dev))
+            self.pack_stream = _lib.stream_ptr(dev)
+        self.epoch = epoch
+
+    def after_pack(self) -> None:
+        """Let the current stream wait for a pack that another one was given.  (Not while capturing, where
+        an event from outside cannot be waited for: what a graph reads is packed before it is replayed.)"""
+        dev = self.pk.device
+        if self.pack_stream is None or self.pack_stream == _lib.stream_ptr(dev) or _lib.capture_id(dev):
+            return
+        if not self.pack_event.query():
+            torch.cuda.current_stream(dev).wait_event(self.pack_event)
 
     def workspace(self, cache, heads: int, q_tokens: int) -> torch.Tensor:
         key = (heads, q_tokens)
@@ -167,6 +190,7 @@ def refresh_prefix(cache) -> _ReadState:
     rs = _read_state(cache)
     epoch = getattr(cache, "_ladder_epoch", None)   # None: a foreign cache, repack every call
     if epoch is not None and rs.epoch == epoch:
+        rs.after_pack()
         return rs
     _run_plan(cache, full=False)
     layout, state = _structs(cache)
@@ -174,7 +198,7 @@ def refresh_prefix(cache) -> _ReadState:
     _lib.check(_lib.lib().logkv_pack_prefix(ctypes.byref(layout), ctypes.byref(state), ctypes.byref(plan),
                                             ctypes.byref(rope), ctypes.byref(pre), rs.status.data_ptr(),
                                             _stream(cache)), "logkv_pack_prefix")
-    rs.epoch = epoch if epoch is not None else -1
+    rs.packed(epoch if epoch is not None else -1)
     return rs
 
 
@@ -344,6 +368,7 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
     if out is None and rs.native is not None and rs.epoch == cache._ladder_epoch and q.dim() == 4:
         # A call like one before: checks, allocations and launch in the host binding, which hands back
         # (None) what it does not cover.
+        rs.after_pack()
         n, qx = rs.tree_bytes.get((q.size(1), q.size(2))), rs.qx.get(scale)
         if n is not None and qx is not None:
             call, fn, layout, prefix = rs.native
@@ -380,8 +405,7 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
         return out
     p = _tree_parents(parents, B, T, dev)
     with _lib.on_device(dev):
-        if rs.epoch < 0 or rs.epoch != getattr(cache, "_ladder_epoch", None):
-            refresh_prefix(cache)
+        refresh_prefix(cache)
         layout, state = _structs(cache)
         lib = _lib.lib()
         n = rs.tree_bytes.get((H, T))

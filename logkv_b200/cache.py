@@ -876,6 +876,7 @@ class LogStructuredKVCache(nn.Module):
             if rs is None:
                 from .attention import _read_state
                 rs = _read_state(self)
+            rs.after_pack()
             _lib.check(_lib.lib().logkv_reorder_batch(
                 ctypes.byref(self._layout), ctypes.byref(self._state_struct()), ctypes.byref(rs.prefix_struct()),
                 self.recent_count, -1 if window_from is None else int(window_from), index.data_ptr(),

@@ -329,3 +329,43 @@ def test_first_calls_of_a_process_in_two_threads():
     """
     subprocess.run([sys.executable, "-c", textwrap.dedent(code)], check=True, timeout=300,
                    cwd=here, env={**os.environ, "PYTHONPATH": os.path.dirname(here)})
+
+
+def test_another_stream_waits_for_the_prefix():
+    """The first call after a flush packs the prefix, on its stream; a call on another stream that waits for
+    the flush alone still reads the packed prefix.  So does chunk attention, and a reorder moves it."""
+    from logkv_b200 import log_kv_chunk_attention, log_kv_tree_attention
+    cache, same = (make_cache(BF16, B=2, G=2, D=64, R=40, seed=29) for _ in range(2))
+    q, k, v = drafts(cache, 2, 9)
+    p = torch.arange(-1, 8, device="cuda")
+    tree = lambda c: log_kv_tree_attention(c, q, k, v, 0.125, p)  # noqa: E731
+    chunk = lambda c: log_kv_chunk_attention(c, q, k, v, 0.125, 0.0)  # noqa: E731
+    for c in (cache, same):
+        tree(c)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.no_grad():
+        for call in (tree, chunk):
+            for c in (cache, same):          # a flush, as far as the read side can tell
+                c.level_w.mul_(2)
+                c._ladder_epoch += 1
+            want = call(same)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(a):
+                torch.cuda._sleep(100_000_000)
+                tree(cache)
+            with torch.cuda.stream(b):
+                got = call(cache)
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+        cache._ladder_epoch += 1
+        cache.level_w.mul_(2)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(100_000_000)
+            tree(cache)
+        with torch.cuda.stream(b):
+            cache.reorder_batch([1, 0])
+        torch.cuda.synchronize()
+        moved = tree(cache)
+        cache._ladder_epoch += 1
+        assert torch.equal(moved, tree(cache))

@@ -58,8 +58,9 @@ class _ReadState:
         self.status = torch.zeros(1, **i32) if status is None else status
         self.status_ptr = self.status.data_ptr()
         self.epoch = -1
-        self.pack_stream = None      # stream of the last pack (None: in a graph), and the pack's end
+        self.pack_stream = None      # the last pack's stream, its end and the capture it was in (0: none)
         self.pack_event = None
+        self.pack_capture = 0
         self.workspaces: dict = {}
         self.tree_bytes: dict = {}   # scratch bytes of log_kv_tree_attention by (heads, tokens)
         self.qx: dict = {}           # query_extra by scale
@@ -79,24 +80,27 @@ class _ReadState:
         return self._prefix
 
     def packed(self, epoch: int) -> None:
-        """The current stream was given a pack of the ladder of ``epoch``."""
+        """The current stream was given a pack of the ladder of ``epoch`` (-1: not to be kept)."""
         dev = self.pk.device
-        if epoch < 0 or _lib.capture_id(dev):
-            self.pack_stream = None
-        else:
-            if self.pack_event is None:
-                self.pack_event = torch.cuda.Event()
-            self.pack_event.record(torch.cuda.current_stream(dev))
-            self.pack_stream = _lib.stream_ptr(dev)
+        if self.pack_event is None:
+            self.pack_event = torch.cuda.Event()
+        self.pack_event.record(torch.cuda.current_stream(dev))
+        self.pack_stream, self.pack_capture = _lib.stream_ptr(dev), _lib.capture_id(dev)
         self.epoch = epoch
 
+    def current(self, epoch) -> bool:
+        """Whether the prefix is packed for ``epoch``.  A pack that was captured is one for its graph alone:
+        nothing has run yet."""
+        return self.epoch == epoch and (not self.pack_capture or self.pack_capture == _lib.capture_id(self.pk.device))
+
     def after_pack(self) -> None:
-        """Let the current stream wait for a pack that another one was given.  (Not while capturing, where
-        an event from outside cannot be waited for: what a graph reads is packed before it is replayed.)"""
+        """Let the current stream wait for a pack that another one was given.  (A capture cannot wait for an
+        event from outside: what a graph reads is packed before it is replayed.)"""
         dev = self.pk.device
-        if self.pack_stream is None or self.pack_stream == _lib.stream_ptr(dev) or _lib.capture_id(dev):
+        if self.pack_stream is None or self.pack_stream == _lib.stream_ptr(dev):
             return
-        if not self.pack_event.query():
+        capture = _lib.capture_id(dev)
+        if capture == self.pack_capture and (capture or not self.pack_event.query()):
             torch.cuda.current_stream(dev).wait_event(self.pack_event)
 
     def workspace(self, cache, heads: int, q_tokens: int) -> torch.Tensor:
@@ -189,7 +193,7 @@ def refresh_prefix(cache) -> _ReadState:
     """Plan and pack the frozen prefix when a flush has changed the ladder since the last pack."""
     rs = _read_state(cache)
     epoch = getattr(cache, "_ladder_epoch", None)   # None: a foreign cache, repack every call
-    if epoch is not None and rs.epoch == epoch:
+    if epoch is not None and rs.current(epoch):
         rs.after_pack()
         return rs
     _run_plan(cache, full=False)
@@ -358,14 +362,16 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
     tokens, and tokens below one, are seen by nobody and give zero rows.  Parents on the host are
     checked here; a bad value in a device tensor counts as -2 and sets bit 18 of ``cache.read_status()``.
     Returns [B, H, T, D]; ``out`` may be given.  The scratch is allocated per call, so calls on
-    different streams, or captured graphs, never share it.  Forward-only.
+    different streams, or captured graphs, never share it.  A captured call is one for the window's fill
+    at its capture, and reads the prefix as packed when it is replayed: ``refresh_prefix(cache)`` after a
+    flush.  Forward-only.
 
     After verification ``cache.add_recent_path`` commits the accepted path.
     """
     rs = _read_state(cache)
     pk = rs.pk
     scale = float(scale)
-    if out is None and rs.native is not None and rs.epoch == cache._ladder_epoch and q.dim() == 4:
+    if out is None and rs.native is not None and rs.current(cache._ladder_epoch) and q.dim() == 4:
         # A call like one before: checks, allocations and launch in the host binding, which hands back
         # (None) what it does not cover.
         rs.after_pack()

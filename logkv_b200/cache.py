@@ -852,8 +852,7 @@ class LogStructuredKVCache(nn.Module):
             raise ValueError(f"{self.batch_size} batch rows: reorder_batch takes at most {_lib.REORDER_MAX_BATCH}")
         if window_from is not None and not 0 <= window_from <= self.recent_count:
             raise ValueError(f"window_from must be in [0, recent_count={self.recent_count}], got {window_from}")
-        dev = self._buffers["level_k"].device
-        if self._read is None and dev.type == "cuda" and _lib.capture_id(dev):
+        if self._read is None and self.level_k.is_cuda and _lib.capture_id(self.level_k.device):
             raise RuntimeError("capture reorder_batch only after the cache has been attended over once")
 
     def reorder_batch(self, index, *, window_from=None) -> None:
@@ -869,7 +868,8 @@ class LogStructuredKVCache(nn.Module):
         """
         self._check_reorder(window_from)
         index = self._row_index(index)
-        with _lib.on_device(index.device):
+        dev = index.device
+        with _lib.on_device(dev):
             # The prefix moves whether or not it is current, so that a captured call does not depend on
             # what was current when it was captured; its buffers therefore exist from here on.
             rs = self._read
@@ -880,7 +880,7 @@ class LogStructuredKVCache(nn.Module):
             _lib.check(_lib.lib().logkv_reorder_batch(
                 ctypes.byref(self._layout), ctypes.byref(self._state_struct()), ctypes.byref(rs.prefix_struct()),
                 self.recent_count, -1 if window_from is None else int(window_from), index.data_ptr(),
-                index.dtype == torch.int64, rs.status_ptr, _lib.stream_ptr(index.device)), "logkv_reorder_batch")
+                index.dtype == torch.int64, rs.status_ptr, _lib.stream_ptr(dev)), "logkv_reorder_batch")
         if self._route_ready is not None:
             self._route_ready = None     # the next flush's decisions must wait for the moved rows
 

@@ -369,3 +369,42 @@ def test_another_stream_waits_for_the_prefix():
         moved = tree(cache)
         cache._ladder_epoch += 1
         assert torch.equal(moved, tree(cache))
+
+
+def test_a_captured_pack_is_its_graphs_own():
+    """A call that is captured while the prefix is out of date packs it when its graph runs: calls outside
+    that graph, and other graphs, pack it themselves."""
+    from logkv_b200 import log_kv_chunk_attention, log_kv_tree_attention
+    q, k, v = drafts(make_cache(BF16, B=2, G=2, D=64, R=40, seed=30), 2, 9)
+    p = torch.arange(-1, 8, device="cuda")
+    tree = lambda c: log_kv_tree_attention(c, q, k, v, 0.125, p)  # noqa: E731
+    chunk = lambda c: log_kv_chunk_attention(c, q, k, v, 0.125, 0.0)  # noqa: E731
+    for call in (tree, chunk):
+        cache, same = (make_cache(BF16, B=2, G=2, D=64, R=40, seed=31) for _ in range(2))
+        with torch.no_grad():
+            for c in (cache, same):
+                call(c)
+                c.level_w.mul_(2)            # a flush, as far as the read side can tell
+                c._ladder_epoch += 1
+            want = call(same)
+            graphs, outs = [], []
+            for _ in range(2):
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    call(cache)
+                    outs.append(call(cache))
+                graphs.append(g)
+            graphs[1].replay()               # not the one captured first
+            torch.cuda.synchronize()
+            assert torch.equal(outs[1], want)
+            for c in (cache, same):
+                c.level_w.mul_(2)
+                c._ladder_epoch += 1
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                call(cache)
+            want = call(same)
+            assert torch.equal(call(cache), want)    # outside, before any replay
+            graphs[0].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[0], want)

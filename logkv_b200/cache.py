@@ -233,7 +233,9 @@ class LogStructuredKVCache(nn.Module):
         self._span_closed = torch.zeros(batch, P, dtype=torch.uint8, **z)
         self._span_count = torch.zeros(batch, dtype=torch.int32, **z)
         self._row_count = torch.zeros(batch, dtype=torch.int32, **z)
-        self._alpha_count_dev = torch.zeros(1, dtype=torch.int32, **z)
+        # One allocation, cleared at once: the pool's count and bits 16 and up of read_status.
+        self._words = torch.zeros(2, dtype=torch.int32, **z)
+        self._alpha_count_dev, self._read_status = self._words[:1], self._words[1:]
         self.op_log = None
         self.op_log_len = None
         self._layout = _lib.Layout(batch, groups, k_dim, K, L, Bs, R, P, self.alpha_span_max_tokens,
@@ -262,7 +264,6 @@ class LogStructuredKVCache(nn.Module):
         self._route_done = None
         self._deferred_take = None   # flush started by add_recent_deferred, committed by commit_deferred
         self._read = None            # read side: plan, packed prefix (logkv_b200.attention)
-        self._read_status = torch.zeros(1, dtype=torch.int32, **z)   # bits 16 and up of read_status
 
     # ------------------------------------------------------------------ C-ABI state
     def _apply(self, fn, *args, **kwargs):
@@ -950,7 +951,7 @@ class LogStructuredKVCache(nn.Module):
         self.p_hi_c.fill_(-1)
         self.ward_cost.fill_(float("inf"))
         for t in (self._recent_ends, self._span_len, self._span_closed, self._span_count, self._row_count,
-                  self._alpha_count_dev, self._read_status):
+                  self._words):
             t.zero_()
         self.token_count = 0
         self.recent_count = 0

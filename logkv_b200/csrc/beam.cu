@@ -11,9 +11,11 @@
 // k-th largest key is found bit by bit instead.  Keys are (value, lower index first), so the choice is
 // unique whatever the order of the gathering.
 //
-// Bound by HBM at best (each logit is read once; about five instructions and one exponential a logit leave room
-// for 24 us for 32 x 16 beams x 151936 in bf16).  Measured: 44 us for B1's walk and selections and 8 for B2
-// there, 18 us in all for 29 x 5 x 50021 in float32, 10 us for 4 x 32000.
+// Bound by HBM at best: each logit is read once, 24 us for 32 x 16 beams x 151936 in bf16.  Measured 53 us there:
+// 44 for B1 (31 for the walk, whose 7.7 instructions and one exponential a logit bound it, and the
+// selections) and 9 for B2; 19 us for 29 x 5 x 50021 in float32, 10 for 4 x 32000.  The search bit by bit
+// reads a slice 65 times: thousands of equal logits among a slice's k best (a finite mask over all but a few
+// tokens) cost 3.8 ms at 32 x 16 x 151936, where a mask of -inf costs 49 us.
 #include <algorithm>
 
 #include "common.cuh"

@@ -7,7 +7,7 @@
 // tree_combine_kernel joins in split order.
 //
 // Bound by HBM (keys and values are read once per 128 query rows) from a few MB per SM on; below that
-// by latency.  Measured on B200, device time: 7 drafts of one sequence over 8.3K slots x 8 groups (32 MB)
+// by latency.  Measured on B200, device time: 7 drafts of one sequence over 7.8K slots x 8 groups (32 MB)
 // 14.8 us; 8 x 26 drafts (260 MB) 53 us, 0.76 of the measured copy bandwidth; 32 x 64 drafts (1.06 GB,
 // 131 GFLOP) 176-212 us, 0.77-0.93.
 #include <algorithm>
@@ -117,8 +117,8 @@ __device__ __forceinline__ float* tree_part(float* part, const TreeGeo& a, int s
 // ---------------------------------------------------------------- bf16: mma.sync, 16 query rows per CTA
 // The 16 rows are the M of mma.sync.m16n8k16.  Each of the 4 warps streams 16-slot tiles of its own
 // through a private ring of cp.async stages (XOR-swizzled for ldmatrix); tiles do not cross segments.
-// Used up to 16 rows, where the tcgen05 kernel's start-up costs more (52 rows: 156 us here, 73 there), and
-// for the head dims that kernel has no shape for, in tiles of 16 rows.
+// Used up to 16 rows (tree_tc below has the measurements), and in tiles of 16 rows for the head dims that the
+// tcgen05 kernel has no shape for.
 constexpr int kTreeWarps = 4;
 constexpr int kTreeStages = 3;
 
@@ -815,7 +815,7 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2)
 // As the bf16 kernel, with mma.sync.m16n8k8 (tf32): every float32 operand is split into a tf32 part and
 // the tf32 part of the rest (22 bits together), and a product is hi hi + hi lo + lo hi, summed in
 // float32; what is left out is below 2^-21 of it.  (Float32 fused products from shared memory, four rows by
-// four keys a thread, were bound by shared-memory reads: 23.7 us against 16.8 for 39 rows over 2.2K keys.)
+// four keys a thread, were bound by shared-memory reads: 23.7 us against 16.5 for 39 rows over 2.2K keys.)
 // K and V rows are padded by 16 bytes, so that the fragments' reads fall into 32 different banks.
 template <int D>
 struct TreeF32Shape {
@@ -1175,6 +1175,15 @@ struct TreePlan {
   bool tc;
 };
 
+// tcgen05 or mma.sync in tiles of 16 rows.  Measured at D 128 in us, tcgen05 against mma.sync:
+//                          16 rows          17 rows          96 rows
+//   7.8K keys, 64 lanes    50.3 : 50.4      50.5 : 81.4      57.9 : 292
+//   7.8K keys, 8 lanes     15.1 : 15.2      15.3 : 18.7      21.5 : 37.1
+//   1.2K keys, 64 lanes    17.6 : 16.6      17.6 : 22.5      22.4 : 61.2
+//   1.2K keys, 8 lanes     14.0 : 11.9      14.1 : 12.3      18.7 : 16.7
+//   100 keys, 8 lanes      14.5 :  9.4      14.6 : 10.9      18.3 : 13.3
+// Up to 16 rows both read every key once and mma.sync starts up faster; from 17 on it reads them twice or more.
+// On short caches it would still win 2 to 5 us there, but the host knows only the prefix's capacity.
 static bool tree_tc(const logkv_layout_t& l, long long rows) {
   return l.dtype == LOGKV_DTYPE_BF16 && (l.dim == 64 || l.dim == 128) && rows > 16;
 }
@@ -1212,6 +1221,10 @@ static int check_tree(const logkv_layout_t* l, int heads, int tokens) {
   return LOGKV_OK;
 }
 
+// Four warps to a row from 9 splits on, which few lanes have: 14 rows over 7.8K keys take 14.9 us against 17.7
+// with one warp on 8 lanes (37 splits) and 11.6 against 24.5 on one lane; over 100 keys, where
+// two of the splits hold any, 9.4 against 9.0.  With few splits the extra warps only wait: 64 lanes (4 splits), 14 rows
+// 53.7 against 49.7 us, 52 rows 63.3 against 52.0.
 template <typename T, int D, int TS>
 static void launch_tree_combine(const TreeGeo& a, const logkv_prefix_t& pre, const float* part, void* out,
                                 cudaStream_t st) {

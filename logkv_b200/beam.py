@@ -22,9 +22,9 @@ def beam_select(logits, scores, k: int, *, keep_places: bool = False):
     logits [N, W, V] (float32 or bf16; any strides of N and W) are the next-token logits of W beams per
     request, ``scores`` [N, W] float32 their log-probabilities so far.  A continuation (w, v) scores
     scores[w] + log_softmax(logits[w])[v]; best first, ties to the lower (w, v).  ``rows`` are flat beam
-    rows n * W + w.  Scores are float64 sums over log-sum-exps that are off by about 1e-7, so continuations
-    of different beams may change places when their scores are that close; beams with the same logits tie
-    exactly.  Logits of -inf are never chosen (mask with it: finite masks are right too, but where few
+    rows n * W + w.  Scores are ordered as float64 sums order them: beams whose scores come closer than float32
+    sums of exponentials tell apart are summed again in float64 (equal beams above all, which tie exactly;
+    115 us a beam of 151936).  Logits of -inf are never chosen (mask with it: finite masks are right too, but where few
     tokens are left their ties are searched one bit at a time, up to 70 times slower); a beam whose score is not finite, or that has a NaN
     or +inf logit or no finite one, offers nothing; places without a continuation get score -inf, token
     0 and row n * W + min(place, W - 1).

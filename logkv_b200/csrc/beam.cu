@@ -11,9 +11,9 @@
 // k-th largest key is found bit by bit instead.  Keys are (value, lower index first), so the choice is
 // unique whatever the order of the gathering.
 //
-// Bound by HBM at best: each logit is read once, 24 us for 32 x 16 beams x 151936 in bf16.  Measured 53 us there:
+// Bound by HBM at best: each logit is read once, 24 us for 32 x 16 beams x 151936 in bf16.  Measured 53.5 us there:
 // 44 for B1 (31 for the walk, whose 7.7 instructions and one exponential a logit bound it, and the
-// selections) and 9 for B2; 19 us for 29 x 5 x 50021 in float32, 10 for 4 x 32000.  The search bit by bit
+// selections) and 10 for B2; 20 us for 29 x 5 x 50021 in float32, 11 for 4 x 32000.  The search bit by bit
 // reads a slice 65 times: thousands of equal logits among a slice's k best (a finite mask over all but a few
 // tokens) cost 3.8 ms at 32 x 16 x 151936, where a mask of -inf costs 49 us.
 #include <algorithm>
@@ -38,6 +38,7 @@ struct BeamGeo {
   long long* out_tokens;
   long long n_stride, w_stride;
   int W, V, k, keep;
+  int f32;        // logits are float32 (else bf16)
   int rows;       // beams in all
   int chunks;     // chunks (kBeamThreads x kBeamVecs vectors) of a beam's vocabulary
   int S;          // slices of a beam at most
@@ -423,11 +424,35 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamGeo a) 
 // The candidates in rounds of up to kBeamRound, the k best so far among each round's.
 constexpr int kBeamRound = 2048, kBeamEach = kBeamRound / kBeamThreads;
 
-// Log-sum-exps of the same logits agree to within this: measured over alignments, slices and vocabularies of 37
-// to 151936 they are 2^-23 apart at most, and off by as much.  Scores of different beams as close as this
-// were in no reliable order before.
-constexpr double kBeamSame = 1.0 / (1 << 21);
-static_assert(LOGKV_BEAM_MAX_WIDTH <= kBeamThreads, "a thread per beam");
+// The slices' sums are off by up to 1.2e-7 relative (measured over alignments, slices and vocabularies of 37 to
+// 151936), so continuations of different beams whose scores are further apart than this are in their order
+// (those of one beam always are).  Beams with closer ones, equal beams above all, have their logits summed in
+// float64, in an order that is the same for every alignment, and are merged again: 115 us a beam of 151936.
+constexpr double kBeamClose = 1.0 / (1 << 21);
+
+// What two roundings of a beam's scores to float64 may differ by, beside that.  (From 1e17 on the maximum
+// swallows the logarithm, and there is nothing to round.)
+__device__ __forceinline__ double beam_wobble(float peak) {
+  const double p = fabs((double)peak);
+  return p < 1e17 ? p * (1.0 / (1ull << 51)) : 0.0;
+}
+__device__ __forceinline__ double key_score(unsigned long long q) {
+  return __longlong_as_double((long long)(q >> 63 ? q & 0x7fffffffffffffffull : ~q));
+}
+
+// The thread's share of a row's sum of exponentials in float64 (not inlined: its registers stay out of the merge).
+template <typename T>
+__device__ __noinline__ double beam_sum(const T* row, unsigned V, double top) {
+  double sum = 0.0;
+  for (unsigned j0 = threadIdx.x; j0 < V; j0 += 8 * kBeamThreads) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = j0 + i * kBeamThreads < V ? (float)row[j0 + i * kBeamThreads] : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += exp((double)x[i] - top);
+  }
+  return sum;
+}
 
 __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
   using U64 = unsigned long long;
@@ -435,9 +460,10 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
   __shared__ U64 sh_t;
   __shared__ __align__(16) U64 cand[kBeamCand];
   __shared__ int cidx[kBeamCand];
-  __shared__ double lse[LOGKV_BEAM_MAX_WIDTH], above_peak[LOGKV_BEAM_MAX_WIDTH];
-  __shared__ float peak[LOGKV_BEAM_MAX_WIDTH];
-  __shared__ float prior[LOGKV_BEAM_MAX_WIDTH];
+  __shared__ double lse[LOGKV_BEAM_MAX_WIDTH];
+  __shared__ float prior[LOGKV_BEAM_MAX_WIDTH], peak[LOGKV_BEAM_MAX_WIDTH];
+  __shared__ unsigned close_beams[LOGKV_BEAM_MAX_WIDTH / 32];
+  __shared__ double wsum[kBeamThreads / 32];
   __shared__ int isum[kBeamThreads / 32];
   __shared__ int sh_n;
   __shared__ U64 best[LOGKV_BEAM_MAX_K];
@@ -467,6 +493,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
   // lanes to a beam.
   int lanes = 2;
   while (lanes < S && lanes < 32) lanes *= 2;
+  bool wobbles = false;
   for (int w0 = 0; w0 < W; w0 += kBeamThreads / lanes) {
     const int w = w0 + tid / lanes, first = tid % lanes;
     const size_t at = (size_t)(n * W + min(w, W - 1)) * S;
@@ -478,42 +505,43 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
       if (a.sum[at + q] != 0.0) s += a.sum[at + q] * exp2f((a.top[at + q] - m) * kLog2e);   // a NaN stays
     for (int off = 1; off < lanes; off *= 2) s += __shfl_xor_sync(0xffffffffu, s, off);
     if (first == 0 && w < W) {
+      wobbles |= beam_wobble(m) > kBeamClose;
+      const float r = a.scores[n * W + w];
+      const double z = (double)m + log2(s) / (double)kLog2e;
+      lse[w] = isfinite(r) && isfinite(z) ? z : nan("");
+      prior[w] = r;
       peak[w] = m;
-      above_peak[w] = log2(s) / (double)kLog2e;
-      prior[w] = a.scores[n * W + w];
     }
   }
-  __syncthreads();
-  // Beams with the same logits tie, but their sums differ in the last bits where their rows' alignment or
-  // slices do: a beam takes over the log-sum-exp of the lowest one with its maximum and a sum within rounding.
-  if (tid < W) {   // W <= kBeamThreads
-    const float mine = peak[tid];
-    int lowest = tid;
-#pragma unroll 4
-    for (int w = tid - 1; w >= 0; --w)
-      if (peak[w] == mine && fabs(above_peak[w] - above_peak[tid]) <= kBeamSame) lowest = w;
-    const double z = (double)mine + above_peak[lowest];
-    lse[tid] = isfinite(prior[tid]) && isfinite(z) ? z : nan("");
-  }
-  __syncthreads();
-  int found = 0;
-  for (int from = 0; from < all;) {
-    // Keys (score, 0 for none) and flat indices of the round; the best so far take the last places.
-    U64 key[kBeamEach];
-    int flat[kBeamEach];
-    U64 mine = 0;
+  wobbles = __syncthreads_or(wobbles);
+  bool exact = W == 1;
+  int found;
+  // Keys (score, 0 for none) and flat indices of the candidates fetched.
+  U64 key[kBeamEach];
+  int flat[kBeamEach];
+  auto rate = [&](int from) {
 #pragma unroll
     for (int i = 0; i < kBeamEach; ++i) {
-      const int at = from + i * kBeamThreads + tid;
       key[i] = 0;
       flat[i] = 0x7fffffff;
       if (vi[i] >= 0) {
-        const int w = at % L / S;
+        const int w = (from + i * kBeamThreads + tid) % L / S;
         if (!isnan(lse[w])) {
           key[i] = order64((double)prior[w] + ((double)v[i] - lse[w]));
           flat[i] = w * a.V + vi[i];
         }
-      } else if (at >= upto && at - upto < found) {
+      }
+    }
+  };
+ merge:
+  found = 0;
+  for (int from = 0; from < all;) {
+    rate(from);
+    U64 mine = 0;
+#pragma unroll
+    for (int i = 0; i < kBeamEach; ++i) {
+      const int at = from + i * kBeamThreads + tid;
+      if (at >= upto && at - upto < found) {   // the best so far take the last places
         key[i] = best[at - upto];
         flat[i] = bflat[at - upto];
       }
@@ -576,6 +604,62 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
     upto = step;
     __syncthreads();
   }
+  if (!exact) {
+    // Beams that have a continuation close to another beam's, among those chosen or at their border.
+    if (tid < LOGKV_BEAM_MAX_WIDTH / 32) close_beams[tid] = 0;
+    __syncthreads();
+    auto mark = [&](int w) { atomicOr(&close_beams[w >> 5], 1u << (w & 31)); };
+    auto compare = [&](double higher, int w, double lower, int x) {
+      if (w != x && higher - lower <= kBeamClose + beam_wobble(peak[w]) + beam_wobble(peak[x])) {
+        mark(w);
+        mark(x);
+      }
+    };
+    if (tid + 1 < found) compare(key_score(best[tid]), bflat[tid] / a.V, key_score(best[tid + 1]), bflat[tid + 1] / a.V);
+    if (found == k) {
+      const U64 last = best[k - 1];
+      const int last_flat = bflat[k - 1];
+      const double border = key_score(last);
+      for (int from = 0; from < all; from += kBeamRound) {
+        if (all > kBeamRound) {   // else they are still there
+          fetch(from, min(all, from + kBeamRound));
+          rate(from);
+        }
+#pragma unroll
+        for (int i = 0; i < kBeamEach; ++i) {
+          const bool left = key[i] && (key[i] < last || (key[i] == last && flat[i] > last_flat));
+          const double y = key_score(key[i]);
+          if (left && (wobbles || border - y <= 3 * kBeamClose)) compare(border, last_flat / a.V, y, flat[i] / a.V);
+        }
+      }
+    }
+    __syncthreads();
+    unsigned any = 0;
+    for (int i = 0; i < LOGKV_BEAM_MAX_WIDTH / 32; ++i) any |= close_beams[i];
+    if (any) {
+      for (int w = 0; w < W; ++w) {
+        if (!(close_beams[w >> 5] >> (w & 31) & 1)) continue;
+        const long long row = n * a.n_stride + w * a.w_stride;
+        const double top = peak[w];
+        double sum = a.f32 ? beam_sum(static_cast<const float*>(a.logits) + row, a.V, top)
+                           : beam_sum(static_cast<const __nv_bfloat16*>(a.logits) + row, a.V, top);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if ((tid & 31) == 0) wsum[tid >> 5] = sum;
+        __syncthreads();
+        if (tid == 0) {
+          double total = 0.0;
+          for (int i = 0; i < kBeamThreads / 32; ++i) total += wsum[i];
+          lse[w] = top + log(total);
+        }
+        __syncthreads();
+      }
+      exact = true;
+      upto = min(all, kBeamRound);
+      fetch(0, upto);
+      goto merge;
+    }
+  }
   if (!a.keep) {
     for (int i = tid; i < k; i += kBeamThreads) place[i] = (short)i;
   } else if (tid == 0) {
@@ -599,8 +683,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamGeo a) {
     const int p = place[i];
     const size_t o = (size_t)n * k + p;
     const bool is = i < found;
-    const U64 q = is ? best[i] : 0ull;
-    a.out_scores[o] = is ? (float)__longlong_as_double((long long)(q >> 63 ? q & 0x7fffffffffffffffull : ~q)) : -INFINITY;
+    a.out_scores[o] = is ? (float)key_score(best[i]) : -INFINITY;
     a.out_rows[o] = (long long)n * W + (is ? bflat[i] / a.V : min(p, W - 1));
     a.out_tokens[o] = is ? bflat[i] % a.V : 0;
   }
@@ -660,6 +743,7 @@ LOGKV_API int logkv_beam_select(const logkv_beam_args_t* x, void* workspace, siz
   a.V = x->vocab;
   a.k = x->k;
   a.keep = x->keep_places;
+  a.f32 = x->dtype == LOGKV_DTYPE_F32;
   a.chunks = beam_chunks(x->vocab, x->dtype == LOGKV_DTYPE_F32 ? 4 : 2);
   a.rows = rows;
   a.S = beam_slices(rows, a.chunks);

@@ -365,3 +365,23 @@ def test_gradients_are_refused_not_dropped():
         with torch.no_grad():
             got = beam_select(a, b, 3)
         assert not got[0].requires_grad and all(torch.equal(s, t) for s, t in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [40, 501, 30001])
+def test_scores_closer_than_float32_sums(dtype, V):
+    """Beams whose best scores differ by 1e-9 or so (all but certain tokens, equal beam scores), chosen and at
+    the border of the choice: float64's order.  The scores of two beams are at least 1e-12 apart, where
+    float64 sums in another order are off by 1e-15."""
+    x = torch.empty(3, 12, V, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(35)
+    for n in range(3):
+        for w, c in enumerate(torch.randperm(12, generator=g, device="cuda").tolist()):
+            x[n, w] = -(20.0 + c / 2) - torch.rand(V, generator=g, device="cuda")
+            x[n, w, (7 * w) % V] = 0.0
+    x = x.to(dtype)
+    r = torch.tensor([-0.5, -3.0, 0.0], device="cuda")[:, None].expand(3, 12).contiguous()
+    for k, keep in ((12, True), (12, False), (5, False), (1, False), (60, False)):
+        check(x, r, k, keep)
+    x[1, 3] = x[1, 9]                    # and two that are equal
+    check(x, r, 12, True)

@@ -22,9 +22,9 @@ extern "C" {
  * best first, ties to the lower (w, v).  Per chosen continuation: its score (out_scores [N,k]
  * float32), the beam's row n * width + w (out_rows [N,k] int64) and v (out_tokens [N,k] int64).
  *
- * Scores are ordered as float64 sums order them (sums of exponentials are float32 per thread, joined in
- * float64, and taken again in float64 for beams whose scores are too close for that); beams with the same
- * logits tie exactly.
+ * Scores are ordered as float64 sums order them, within a beam by the logits themselves (sums of
+ * exponentials are float32 per thread, joined in float64, and taken again in float64 for beams whose scores
+ * are too close for that); beams with the same logits tie exactly.
  *
  * A logit of -inf is never chosen.  A beam whose score is not finite, or that has a NaN or +inf logit
  * or no finite one, offers nothing.  Places without a continuation get score -inf, token 0 and row

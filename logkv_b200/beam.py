@@ -22,12 +22,14 @@ def beam_select(logits, scores, k: int, *, keep_places: bool = False):
     logits [N, W, V] (float32 or bf16; any strides of N and W) are the next-token logits of W beams per
     request, ``scores`` [N, W] float32 their log-probabilities so far.  A continuation (w, v) scores
     scores[w] + log_softmax(logits[w])[v]; best first, ties to the lower (w, v).  ``rows`` are flat beam
-    rows n * W + w.  Scores are ordered as float64 sums order them: beams whose scores come closer than float32
-    sums of exponentials tell apart are summed again in float64 (equal beams above all, which tie exactly;
-    115 us a beam of 151936).  Logits of -inf are never chosen (mask with it: finite masks are right too, but where few
-    tokens are left their ties are searched one bit at a time, up to 70 times slower); a beam whose score is not finite, or that has a NaN
+    rows n * W + w.  Logits of -inf are never chosen; a beam whose score is not finite, or that has a NaN
     or +inf logit or no finite one, offers nothing; places without a continuation get score -inf, token
     0 and row n * W + min(place, W - 1).
+
+    Scores are ordered as float64 sums order them, within a beam by the logits themselves: beams whose
+    scores come closer than float32 sums of exponentials tell apart are summed again in float64 (equal
+    beams above all, which tie exactly; 115 us a beam of 151936).  Mask with -inf: finite masks are right
+    too, but where few tokens are left the masked ones' ties are searched bit by bit, up to 70 times slower.
 
     ``keep_places`` (k == W): a beam's best continuation is put into the beam's own place and the others
     into the free places in order of score, so that as few rows as possible move when the caches follow

@@ -2,3 +2,5 @@
 from .attention import log_kv_chunk_attention, log_kv_tree_attention, pack_mid_kv  # noqa: F401
 from .cache import LogStructuredKVCache, _SemanticReplayUpdates  # noqa: F401
 from .beam import beam_select  # noqa: F401
+from .logits import adjust_logits  # noqa: F401
+from .rotary import log_kv_rotate, scaled_rope_tables  # noqa: F401

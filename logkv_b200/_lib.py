@@ -119,6 +119,38 @@ class BeamArgs(ctypes.Structure):
                 ("keep_places", ctypes.c_int32)]
 
 
+class RotatePart(ctypes.Structure):
+    """logkv_rotate_part_t (include/logkv_rotary.h)."""
+    _fields_ = [("src", ctypes.c_void_p), ("rotated", ctypes.c_void_p), ("raw", ctypes.c_void_p),
+                ("src_strides", ctypes.c_int64 * 3), ("rotated_strides", ctypes.c_int64 * 3),
+                ("raw_strides", ctypes.c_int64 * 3), ("heads", ctypes.c_int32), ("rotate", ctypes.c_int32)]
+
+
+class RotateArgs(ctypes.Structure):
+    """logkv_rotate_args_t (include/logkv_rotary.h)."""
+    _fields_ = [("parts", RotatePart * 3), ("positions", ctypes.c_void_p), ("position_strides", ctypes.c_int64 * 2),
+                ("pos0", ctypes.c_int64), ("positions_out", ctypes.c_void_p), ("positions_out_stride", ctypes.c_int64),
+                ("ends", ctypes.c_void_p), ("ends_out", ctypes.c_void_p), ("ends_stride", ctypes.c_int64),
+                ("ends_out_stride", ctypes.c_int64), ("status", ctypes.c_void_p), ("positions_wide", ctypes.c_int32),
+                ("n_parts", ctypes.c_int32), ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32),
+                ("dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32)]
+
+
+class LogitsArgs(ctypes.Structure):
+    """logkv_logits_args_t (include/logkv_logits.h)."""
+    _fields_ = [("logits", ctypes.c_void_p), ("out", ctypes.c_void_p), ("n_stride", ctypes.c_int64),
+                ("w_stride", ctypes.c_int64), ("out_n_stride", ctypes.c_int64), ("out_w_stride", ctypes.c_int64),
+                ("history", ctypes.c_void_p), ("history_stride", ctypes.c_int64), ("lengths", ctypes.c_void_p),
+                ("prompts", ctypes.c_void_p), ("repetitions", ctypes.c_void_p), ("presences", ctypes.c_void_p),
+                ("frequencies", ctypes.c_void_p), ("bias_tokens", ctypes.c_void_p), ("bias_values", ctypes.c_void_p),
+                ("bias_tokens_stride", ctypes.c_int64), ("bias_values_stride", ctypes.c_int64),
+                ("mask", ctypes.c_void_p), ("mask_stride", ctypes.c_int64),
+                *((name, ctypes.c_int32) for name in
+                  ("dtype", "rows", "width", "vocab", "history_len", "length", "prompt", "history_wide", "lengths_wide",
+                   "prompts_wide", "bias_wide", "bias_count")),
+                ("repetition", ctypes.c_float), ("presence", ctypes.c_float), ("frequency", ctypes.c_float)]
+
+
 TREE_MAX_TOKENS = 256     # LOGKV_TREE_MAX_TOKENS
 REORDER_MAX_BATCH = 512   # LOGKV_REORDER_MAX_BATCH
 
@@ -229,6 +261,10 @@ def lib() -> ctypes.CDLL:
         handle.logkv_beam_workspace_bytes.argtypes = [ctypes.c_int32] * 4
         handle.logkv_beam_select.restype = ctypes.c_int
         handle.logkv_beam_select.argtypes = [P(BeamArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        handle.logkv_rotate.restype = ctypes.c_int
+        handle.logkv_rotate.argtypes = [P(Rope), P(RotateArgs), ctypes.c_void_p]
+        handle.logkv_adjust_logits.restype = ctypes.c_int
+        handle.logkv_adjust_logits.argtypes = [P(LogitsArgs), ctypes.c_void_p]
         _lib = handle
     return _lib
 

@@ -6,6 +6,7 @@ Translation units with different numerics:
   attention.cu, tree_attention.cu  default contraction (FMA) for the attention math;
   reorder.cu    moves rows, no arithmetic;
   beam.cu       default contraction (its float64 scores decide);
+  rotary.cu, logits.cu  default contraction;
   plugin.cu, unified.cu  -fmad=false: the operator-level plugin functions, same contract as flush.cu.
 and ``host_file()``, the CPython binding of the calls whose time is the host's (host.cpp, g++).
 Run ``python -m logkv_b200.build`` (or ``__graft_entry__.build()``).
@@ -32,6 +33,8 @@ UNITS = [
     ("tree_attention.cu", []),
     ("reorder.cu", []),
     ("beam.cu", []),
+    ("rotary.cu", []),
+    ("logits.cu", []),
     ("plugin.cu", ["-fmad=false"]),
     ("unified.cu", ["-fmad=false"]),
 ]

@@ -526,7 +526,7 @@ class LogStructuredKVCache(nn.Module):
         Bits 0 to 4, of the last flush: carry list, merge list or candidate capacity exceeded, cluster
         choice failed, a wait for a copy expired.  Bits 16 and up, of every other call since the cache
         was built or reset: 16 a position outside the rotary tables, 17 a wait in log_kv_tree_attention
-        expired (its output is not valid), 18 a bad parent there, 19 a bad row index
+        or log_kv_shared_attention expired (its output is not valid), 18 a bad parent there, 19 a bad row index
         in reorder_batch or path entry in add_recent_path, 20 a wait for a copy of a reorder expired.
         """
         out = ctypes.c_int32(0)
@@ -633,6 +633,62 @@ class LogStructuredKVCache(nn.Module):
                 p.stride(0) if p.dim() == 2 else 0, int(p.dtype == torch.int64), int(self.recent_count),
                 self._read_status.data_ptr(), ctypes.c_void_p(_lib.stream_ptr(dev))), "logkv_window_append_path")
             del keep
+            self.recent_count += n
+            self._run_flushes(record_op_log, False)
+
+    def add_recent_rotated(self, k_raw, v, *, input_pos=None, layout: str = "half", span_ends=None, span_ends_device=None,
+                           record_op_log=False) -> None:
+        """add_recent of unrotated keys: the rotation is part of the window write (no reference counterpart).
+
+        k_raw and v [B, G, n, D] are a projection's output in the cache dtype, any strides; the state afterwards is
+        that of ``q, k, k_raw = log_kv_rotate(...)`` and ``add_recent(k, v, k_raw=k_raw, ...)``, bit for bit.
+        ``input_pos`` ([n] or [B, n] integers; None: the positions that continue the sequence) and ``layout`` are
+        log_kv_rotate's, the span-end flags ([B][n] host rows, or ``span_ends_device`` [B, n] on the device) add_recent's.
+        """
+        from . import rotary
+        mode = rotary.check_layout(layout)
+        if self._deferred_take is not None:
+            raise RuntimeError("commit_deferred must follow add_recent_deferred")
+        B, G, D, dt, dev = self.batch_size, self.n_groups, self.k_dim, self.recent_k.dtype, self.recent_k.device
+        for name, t in (("k_raw", k_raw), ("v", v)):
+            if t.dim() != 4 or t.shape != (B, G, k_raw.size(2), D) or t.dtype != dt:
+                raise ValueError(f"{name} must be [{B}, {G}, n, {D}] in the cache dtype, got {tuple(t.shape)} {t.dtype}")
+            if t.device != dev:
+                raise ValueError(f"{name} must be on the cache's device {dev}, got {t.device}")
+        n = k_raw.size(2)
+        positions = rotary.check_positions(self, input_pos, n)
+        if span_ends_device is not None:
+            if tuple(span_ends_device.shape) != (B, n):
+                raise ValueError("AlphaLogKV span boundaries must match the input batch and token count")
+            ends = span_ends_device.to(device=dev, dtype=torch.uint8).contiguous()
+        elif span_ends is None or len(span_ends) != B or any(len(r) != n for r in span_ends):
+            raise ValueError("AlphaLogKV span boundaries must match the input batch and token count")
+        else:
+            ends = torch.tensor(span_ends, dtype=torch.uint8).to(dev)
+        self._check_room(n)
+        if n == 0:
+            return
+        with _lib.on_device(dev):
+            k_raw, v = rotary.last_contiguous(k_raw), rotary.last_contiguous(v)
+            pos0, c0 = self.token_count, self.recent_count
+            take = self._chunk_flush_take(n)
+            if take is not None:
+                # The flush rewrites the window's rows; the chunk follows from where it is rotated to.
+                k = k_raw.new_empty((B, G, n, D))
+                raw = k_raw.new_empty((B, G, n, D)) if mode else None
+                at = k_raw.new_empty((B, n), dtype=torch.int64)
+                rotary.launch(self, [(k_raw, k, raw)], positions, pos0, mode, positions_out=at)
+                self.token_count += n
+                self._flush_chunk((k, k_raw if raw is None else raw, v, at, ends, n), take)
+                if record_op_log:
+                    self._append_op_log(take)
+                self._finish_flush(take)
+                return
+            rows = slice(c0, c0 + n)
+            rotary.launch(self, [(k_raw, self.recent_k[:, :, rows], self.recent_k_raw[:, :, rows]),
+                                 (v, None, self.recent_v[:, :, rows])], positions, pos0, mode,
+                          positions_out=self.recent_pos[:, rows], ends=ends, ends_out=self._recent_ends[:, rows])
+            self.token_count += n
             self.recent_count += n
             self._run_flushes(record_op_log, False)
 

@@ -179,6 +179,52 @@ LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_sta
                                    size_t workspace_bytes, void* stream);
 
 /*
+ * Attention of batch rows that share a long prefix (beams or samples of one prompt; no reference counterpart).
+ * Rows r * beams .. r * beams + beams - 1 hold the same packed prefix and the same window rows [0, window_from):
+ * those keys are read once for all of them, from the first of the rows; the window rows [window_from, recent_count)
+ * and the new tokens are each row's own.  Otherwise the result of logkv_attention for q_tokens query tokens over
+ * `tokens` new ones:
+ *   out = softmax(scale * (q . k_s + qx * mass_s)) v_s,
+ * with causal != 0 (tokens = q_tokens) new token j visible to query token t iff j <= t, else every new token
+ * visible.  Rows are taken to agree as promised; nothing checks it.  A new token whose V holds a NaN or an infinity
+ * makes the outputs of the query tokens that see it NaN, and only those.
+ *
+ * q is [B,H,q_tokens,D], k_new and v_new are [B,G,tokens,D] (post-RoPE, storage dtype) with the given element
+ * strides of their batch, head and token axes; the head dim is contiguous and every row 16-byte aligned.  out is
+ * [B,H,q_tokens,D], contiguous.  Any number of query heads per group; B a multiple of beams; heads / groups *
+ * q_tokens * beams <= 2^20.  Head dims: 16, 32, 64, 128 (and 256 for bf16 caches).  Bit 17 of `status`: a bounded
+ * wait expired, the output is not valid.
+ */
+typedef struct logkv_shared_args {
+  const void* q;
+  const void* k_new;
+  const void* v_new;
+  void* out;
+  int64_t q_strides[3];
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int32_t heads;            /* H, a multiple of groups                          */
+  int32_t beams;            /* rows that share a prefix                         */
+  int32_t q_tokens;
+  int32_t tokens;           /* new tokens, >= q_tokens                          */
+  int32_t recent_count;     /* window rows [0, recent_count) are attended       */
+  int32_t window_from;      /* the first of them that are shared                */
+  int32_t causal;
+  float scale;
+  float qx;                 /* as logkv_attention_args_t                        */
+  int32_t* status;          /* device int32 or NULL                             */
+} logkv_shared_args_t;
+
+/* Scratch bytes of logkv_shared_attention with these sizes (its pointers are not looked at; no initialisation
+ * needed; 0: shape not supported).  The scratch must not be shared by calls that may overlap on the GPU. */
+LOGKV_API size_t logkv_shared_attention_workspace_bytes(const logkv_layout_t* layout, const logkv_shared_args_t* args,
+                                                        int32_t prefix_capacity);
+
+LOGKV_API int logkv_shared_attention(const logkv_layout_t* layout, const logkv_state_t* state,
+                                     const logkv_prefix_t* prefix, const logkv_shared_args_t* args, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/*
  * Beam search: batch row b of the cache becomes the old row index[b], in place (no reference
  * counterpart).  index is [B] on the device, int32 or int64 (index_wide); any map is allowed (one row
  * taken over by several, swaps, cycles).  An entry outside [0, B) leaves its row as it is and sets bit

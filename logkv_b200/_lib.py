@@ -105,6 +105,16 @@ class TreeArgs(ctypes.Structure):
                 ("qx", ctypes.c_float), ("status", ctypes.c_void_p)]
 
 
+class SharedArgs(ctypes.Structure):
+    """logkv_shared_args_t (include/logkv_attention.h)."""
+    _fields_ = [("q", ctypes.c_void_p), ("k_new", ctypes.c_void_p), ("v_new", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("q_strides", ctypes.c_int64 * 3), ("k_strides", ctypes.c_int64 * 3),
+                ("v_strides", ctypes.c_int64 * 3),
+                *((name, ctypes.c_int32) for name in ("heads", "beams", "q_tokens", "tokens", "recent_count",
+                                                      "window_from", "causal")),
+                ("scale", ctypes.c_float), ("qx", ctypes.c_float), ("status", ctypes.c_void_p)]
+
+
 class Rows(ctypes.Structure):
     """logkv_rows_t (include/logkv_attention.h)."""
     _fields_ = [("base", ctypes.c_void_p), ("row_bytes", ctypes.c_int64)]
@@ -261,6 +271,11 @@ def lib() -> ctypes.CDLL:
         handle.logkv_beam_workspace_bytes.argtypes = [ctypes.c_int32] * 4
         handle.logkv_beam_select.restype = ctypes.c_int
         handle.logkv_beam_select.argtypes = [P(BeamArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        handle.logkv_shared_attention_workspace_bytes.restype = ctypes.c_size_t
+        handle.logkv_shared_attention_workspace_bytes.argtypes = [P(Layout), P(SharedArgs), ctypes.c_int32]
+        handle.logkv_shared_attention.restype = ctypes.c_int
+        handle.logkv_shared_attention.argtypes = [P(Layout), P(State), P(Prefix), P(SharedArgs), ctypes.c_void_p,
+                                                  ctypes.c_size_t, ctypes.c_void_p]
         handle.logkv_rotate.restype = ctypes.c_int
         handle.logkv_rotate.argtypes = [P(Rope), P(RotateArgs), ctypes.c_void_p]
         handle.logkv_adjust_logits.restype = ctypes.c_int

@@ -7,7 +7,8 @@ first order) with the same names, arguments and errors:
   pack_mid_kv(cache, plan, ...)   log_kv_pack.pack_mid_kv                         (log_kv_pack.py:114-131)
   log_kv_chunk_attention(...)     log_kv_cache.log_kv_chunk_attention             (log_kv_cache.py:6802-6864)
 
-and one of its own: log_kv_tree_attention(...), a tree of drafted tokens over the same state.
+and two of its own: log_kv_tree_attention(...), a tree of drafted tokens over the same state, and
+log_kv_shared_attention(...), batch rows that share a long prefix.
 
 Everything runs through the C ABI of ``liblogkv_b200.so`` (include/logkv_attention.h);
 there is no CPU path.  The packed frozen prefix (merged slots rotated at their mid
@@ -435,4 +436,74 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
         _lib.check(lib.logkv_tree_attention(ctypes.byref(layout), ctypes.byref(state),
                                             ctypes.byref(rs.prefix_struct()), ctypes.byref(args), ws.data_ptr(), n,
                                             _lib.stream_ptr(dev)), "logkv_tree_attention")
+    return out
+
+
+def log_kv_shared_attention(cache, q, k, v, scale, *, beams: int, window_from: int, causal_tail=None, out=None):
+    """log_kv_chunk_attention of batch rows that share a long prefix, its keys read once for all of them, committing
+    nothing (no reference counterpart).
+
+    Rows r * beams .. (r + 1) * beams - 1 (the beams or samples of request r) hold the same ladder, exact pool and
+    window rows [0, window_from), as after ``reorder_batch`` has forked them from one row and until the cache's next
+    flush; the window behind that and the new tokens are each row's own.  The shared keys are read from the first row
+    of the request.  Rows that do not agree as promised are not noticed.
+
+    q [B, H, T, D] are the queries of T tokens, k and v [B, G, Tk, D] the new tokens, post-RoPE, any strides.
+    ``causal_tail`` T (the default): T == Tk, token t sees the new tokens up to itself; 0: every query sees all Tk >= T
+    of them (a decode step whose one query sees a pending token and itself).  Any number of query heads per group.
+    Returns [B, H, T, D]; ``out`` may be given.
+
+    The scratch is allocated per call, so calls on different streams, or captured graphs, never share it.  A captured
+    call is one for the window's fill at its capture, and reads the prefix as packed when it is replayed:
+    ``refresh_prefix(cache)`` after a flush.  Forward-only.
+    """
+    rs = _read_state(cache)
+    pk = rs.pk
+    dev, dt = pk.device, pk.dtype
+    B, G, _, kd = pk.shape
+    _check_kv(cache, k, v)
+    if q.dim() != 4 or q.size(0) != B or q.size(3) != kd or q.dtype != dt:
+        raise ValueError(f"q must be [B={B}, H, T, {kd}] in the cache dtype")
+    H, T, Tk = q.size(1), q.size(2), k.size(2)
+    causal_tail = T if causal_tail is None else causal_tail
+    if causal_tail and causal_tail != T:
+        raise ValueError("causal_tail must equal query length or be zero")
+    if T != Tk and (causal_tail or T > Tk):
+        raise ValueError("q and k must cover the same tokens (fewer queries only with causal_tail=0)")
+    if H < 1 or H % G:
+        raise ValueError(f"query heads {H} must be a multiple of KV groups {G}")
+    beams, window_from, R = int(beams), int(window_from), int(cache.recent_count)
+    if beams < 1 or B % beams:
+        raise ValueError(f"{B} batch rows cannot be requests of {beams} beams")
+    if not 0 <= window_from <= R:
+        raise ValueError(f"window_from must be in [0, recent_count={R}], got {window_from}")
+    if q.device != dev or k.device != dev or v.device != dev:
+        raise ValueError(f"q, k and v must be on the cache's device {dev}")
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        raise NotImplementedError("logkv_b200 attention is forward-only")
+    if out is None:
+        out = pk.new_empty((B, H, T, kd))
+    elif out.shape != (B, H, T, kd) or out.dtype != dt or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous [{B}, {H}, {T}, {kd}] tensor in the cache dtype on {dev}")
+    if T == 0:
+        return out
+    scale = float(scale)
+    with _lib.on_device(dev):
+        refresh_prefix(cache)
+        layout, state = _structs(cache)
+        lib = _lib.lib()
+        qx = rs.qx.get(scale)
+        if qx is None:
+            qx = rs.qx[scale] = query_extra(scale, dt)
+        (q, qs), (k, ks), (v, vs) = _rows16(q), _rows16(k), _rows16(v)
+        args = _lib.SharedArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs, ks, vs, H, beams, T, Tk, R,
+                               window_from, int(bool(causal_tail)), scale, qx, rs.status_ptr)
+        n = lib.logkv_shared_attention_workspace_bytes(ctypes.byref(layout), ctypes.byref(args), rs.capacity)
+        if not n:
+            raise ValueError(f"shared attention shape outside the supported range (heads={H}, beams={beams}, tokens={T}, "
+                             f"head dim {kd}, {dt})")
+        ws = rs.mass.new_empty(n >> 2)
+        _lib.check(lib.logkv_shared_attention(ctypes.byref(layout), ctypes.byref(state),
+                                              ctypes.byref(rs.prefix_struct()), ctypes.byref(args), ws.data_ptr(), n,
+                                              _lib.stream_ptr(dev)), "logkv_shared_attention")
     return out

@@ -3,7 +3,7 @@
 Translation units with different numerics:
   flush.cu      -fmad=false: every float expression of the flush is rounded
                  exactly as written (bit-exact with the reference's CPU path);
-  attention.cu, tree_attention.cu  default contraction (FMA) for the attention math;
+  attention.cu, tree_attention.cu, shared_attention.cu  default contraction (FMA) for the attention math;
   reorder.cu    moves rows, no arithmetic;
   beam.cu       default contraction (its float64 scores decide);
   rotary.cu, logits.cu  default contraction;
@@ -31,6 +31,7 @@ UNITS = [
     ("flush.cu", ["-fmad=false"]),
     ("attention.cu", []),
     ("tree_attention.cu", []),
+    ("shared_attention.cu", []),
     ("reorder.cu", []),
     ("beam.cu", []),
     ("rotary.cu", []),

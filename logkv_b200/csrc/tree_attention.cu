@@ -826,36 +826,6 @@ struct TreeF32Shape {
   static constexpr int CTAS = D <= 64 ? 2 : 1;   // per SM
 };
 
-__device__ __forceinline__ void mma_tf32(float* c, const unsigned* a, unsigned b0, unsigned b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void split_tf32(float x, unsigned& hi, unsigned& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(hi) : "f"(x));
-  asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
-}
-// The same, not moved out of a loop (Q's parts of 64 features and more would not fit the registers).
-__device__ __forceinline__ void split_tf32_here(float x, unsigned& hi, unsigned& lo) {
-  asm volatile("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(hi) : "f"(x));
-  asm volatile("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
-}
-// c += a b for one n8 tile, the operands split.  The three products start from zero and are added to c by a
-// rounded float32 sum: the matrix instruction's own accumulation truncates, which over a long sum is a
-// bias (relative error 2e-6 where this has 2.5e-7).
-__device__ __forceinline__ void mma_split(float* c, const unsigned* ah, const unsigned* al, float x0, float x1) {
-  unsigned h0, l0, h1, l1;
-  split_tf32(x0, h0, l0);
-  split_tf32(x1, h1, l1);
-  float d[4] = {0.f, 0.f, 0.f, 0.f};
-  mma_tf32(d, al, h0, h1);
-  mma_tf32(d, ah, l0, l1);
-  mma_tf32(d, ah, h0, h1);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] += d[i];
-}
-
 template <int D>
 __global__ void __launch_bounds__(kTreeWarps * 32, TreeF32Shape<D>::CTAS)
     tree_f32_kernel(TreeGeo a, logkv_prefix_t pre, const float* rk, const float* rv, float* out, float* part,

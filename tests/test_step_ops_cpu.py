@@ -78,6 +78,61 @@ def test_rotated_append_refusals(cache):
     assert before == (cache.token_count, cache.recent_count)
 
 
+def test_shared_attention_refusals(cache):
+    from logkv_b200 import log_kv_shared_attention
+    q, k = torch.zeros(2, 4, 3, 64), torch.zeros(2, 2, 3, 64)
+    f = lambda q, k, v, **kw: log_kv_shared_attention(cache, q, k, v, 0.125, **{"beams": 2, "window_from": 5, **kw})  # noqa: E731
+    for args, kw, match in [
+            ((q[:1], k, k), {}, "q must be"), ((q[..., :32], k, k), {}, "q must be"), ((q[0], k, k), {}, "q must be"),
+            ((q.bfloat16(), k, k), {}, "q must be"), ((q, k[:, :1], k), {}, "k must be"), ((q, k, k[:, :, :2]), {}, "v shape"),
+            ((q, k.bfloat16(), k), {}, "dtype"), ((q[:, :, :2], k, k), {}, "same tokens"), ((q, k[:, :, :2], k[:, :, :2]), {}, "same tokens"),
+            ((q[:, :, :2], k, k), {"causal_tail": 2}, "same tokens"), ((q, k, k), {"causal_tail": 2}, "causal_tail"),
+            ((q[:, :3], k, k), {}, "multiple"), ((q[:, :0], k, k), {}, "multiple"), ((q, k, k), {"beams": 0}, "beams"),
+            ((q, k, k), {"beams": 3}, "beams"), ((q, k, k), {"window_from": 6}, "window_from"),
+            ((q, k, k), {"window_from": -1}, "window_from"), ((q, k, k), {"out": torch.zeros(2, 4, 3, 32)}, "out must be")]:
+        with pytest.raises(ValueError, match=match):
+            f(*args, **kw)
+    with pytest.raises(NotImplementedError):
+        f(q.clone().requires_grad_(), k, k)
+
+
+def test_shared_attention_c_abi_checks(lib):
+    from logkv_b200 import _lib
+    layout = _lib.Layout(16, 8, 128, 12, 7, 125, 4096, 256, 64, 1, 1, 1.0, 2048.0, 1.0)
+    a = _lib.SharedArgs()
+
+    def size(lay=layout, cap=10756, **kw):
+        base = dict(heads=16, beams=4, q_tokens=1, tokens=1, recent_count=100, window_from=60, causal=1)
+        for name, value in {**base, **kw}.items():
+            setattr(a, name, value)
+        return lib.logkv_shared_attention_workspace_bytes(ctypes.byref(lay), ctypes.byref(a), cap)
+
+    row = 16 * 16 * 132 * 4                              # partial rows of one split
+    assert size() > 0 and size() % row == 0 and size(recent_count=4096, window_from=0) > 0
+    assert size(beams=16, q_tokens=7, tokens=7) > 0 and size(q_tokens=1, tokens=2, causal=0) > 0
+    for bad in (dict(heads=12), dict(heads=0), dict(beams=0), dict(beams=3), dict(q_tokens=0), dict(q_tokens=2),
+                dict(tokens=2), dict(recent_count=4097), dict(recent_count=-1), dict(window_from=101), dict(window_from=-1),
+                dict(cap=-1), dict(q_tokens=1 << 18, tokens=1 << 18, beams=16)):
+        assert size(**bad) == 0, bad
+    odd = _lib.Layout(16, 8, 96, 12, 7, 125, 4096, 256, 64, 1, 1, 1.0, 2048.0, 1.0)
+    f32 = _lib.Layout(16, 8, 256, 12, 7, 125, 4096, 256, 64, 1, 0, 1.0, 2048.0, 1.0)
+    assert size(odd) == 0 and size(f32) == 0
+    n = size()
+    state, pre = _lib.State(), _lib.Prefix()
+    call = lambda bytes_: lib.logkv_shared_attention(ctypes.byref(layout), ctypes.byref(state), ctypes.byref(pre),  # noqa: E731
+                                                     ctypes.byref(a), 1 << 20, bytes_, None)
+    assert lib.logkv_shared_attention(None, None, None, None, None, 0, None) == -4
+    pre.capacity = 10756
+    assert call(n) == -4                                 # null pointers
+    state.recent_k = state.recent_v = pre.k = pre.v = pre.mass = pre.length = 1 << 20
+    a.q = a.k_new = a.v_new = a.out = 1 << 20
+    assert call(n - 1) == -3                             # workspace too small
+    a.k_strides[1] = 4
+    assert call(n) == -4                                 # rows not 16-byte aligned
+    a.k_strides[1], a.beams = 0, 3
+    assert call(n) == -1
+
+
 def test_logits_refusals(lib):
     from logkv_b200 import adjust_logits as f
     x, h = torch.zeros(2, 3, 70), torch.zeros(2, 3, 5, dtype=torch.int64)

@@ -67,6 +67,7 @@ class _ReadState:
         self.qx: dict = {}           # query_extra by scale
         self._prefix = None
         self.native = None           # (tree call, its arguments that do not change) of the host binding
+        self.native_shared = None    # the same of log_kv_shared_attention
 
     def plan_struct(self, full: bool) -> _lib.Plan:
         p = lambda t: t.data_ptr()  # noqa: E731
@@ -459,6 +460,20 @@ def log_kv_shared_attention(cache, q, k, v, scale, *, beams: int, window_from: i
     """
     rs = _read_state(cache)
     pk = rs.pk
+    scale = float(scale)
+    if out is None and rs.native_shared is not None and rs.current(cache._ladder_epoch):
+        # A call like one before: checks, allocations and launch in the host binding, which hands back
+        # (None) what it does not cover.
+        rs.after_pack()
+        qx = rs.qx.get(scale)
+        if qx is not None:
+            call, fn, size, layout, prefix = rs.native_shared
+            y = call(fn, size, layout, ctypes.addressof(cache._state_struct()), prefix, rs.status_ptr, pk, q, k, v,
+                     cache.recent_count, beams, window_from, causal_tail, scale, qx)
+            if y is not None:
+                if type(y) is int:
+                    _lib.check(y, "logkv_shared_attention")
+                return y
     dev, dt = pk.device, pk.dtype
     B, G, _, kd = pk.shape
     _check_kv(cache, k, v)
@@ -487,7 +502,6 @@ def log_kv_shared_attention(cache, q, k, v, scale, *, beams: int, window_from: i
         raise ValueError(f"out must be a contiguous [{B}, {H}, {T}, {kd}] tensor in the cache dtype on {dev}")
     if T == 0:
         return out
-    scale = float(scale)
     with _lib.on_device(dev):
         refresh_prefix(cache)
         layout, state = _structs(cache)
@@ -495,6 +509,10 @@ def log_kv_shared_attention(cache, q, k, v, scale, *, beams: int, window_from: i
         qx = rs.qx.get(scale)
         if qx is None:
             qx = rs.qx[scale] = query_extra(scale, dt)
+        if rs.native_shared is None and hasattr(cache, "_state_struct"):
+            rs.native_shared = (_lib.host().shared, _lib.address("logkv_shared_attention"),
+                                _lib.address("logkv_shared_attention_workspace_bytes"),
+                                ctypes.addressof(cache._layout), ctypes.addressof(rs.prefix_struct()))
         (q, qs), (k, ks), (v, vs) = _rows16(q), _rows16(k), _rows16(v)
         args = _lib.SharedArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs, ks, vs, H, beams, T, Tk, R,
                                window_from, int(bool(causal_tail)), scale, qx, rs.status_ptr)

@@ -264,10 +264,11 @@ class LogStructuredKVCache(nn.Module):
         self._route_done = None
         self._deferred_take = None   # flush started by add_recent_deferred, committed by commit_deferred
         self._read = None            # read side: plan, packed prefix (logkv_b200.attention)
+        self._rotary = None          # what the host binding's rotations take (logkv_b200.rotary)
 
     # ------------------------------------------------------------------ C-ABI state
     def _apply(self, fn, *args, **kwargs):
-        self._state = None           # buffers move: the pointer table is rebuilt on next use
+        self._state = self._rotary = None   # buffers move: the pointer tables are rebuilt on next use
         return super()._apply(fn, *args, **kwargs)
 
     def _state_struct(self) -> _lib.State:
@@ -649,6 +650,21 @@ class LogStructuredKVCache(nn.Module):
         mode = rotary.check_layout(layout)
         if self._deferred_take is not None:
             raise RuntimeError("commit_deferred must follow add_recent_deferred")
+        call = rotary.native(self)
+        if call is not None and span_ends_device is not None and k_raw.dim() == 4:
+            # A call like one before that fills the window without a flush: checks and launch in the host binding,
+            # which hands back (None) what it does not cover.
+            n, c0 = k_raw.size(2), self.recent_count
+            if c0 + n <= self.recent_size and self.token_count + n <= self.max_seq_length:
+                b = self._buffers
+                rc = call.append(call.fn, call.rope, call.status, b["recent_k"], b["recent_k_raw"], b["recent_v"],
+                                 b["recent_pos"], self._recent_ends, k_raw, v, input_pos, span_ends_device,
+                                 self.token_count, c0, mode)
+                if rc is not None:
+                    _lib.check(rc, "logkv_rotate")
+                    self.token_count += n
+                    self.recent_count += n
+                    return
         B, G, D, dt, dev = self.batch_size, self.n_groups, self.k_dim, self.recent_k.dtype, self.recent_k.device
         for name, t in (("k_raw", k_raw), ("v", v)):
             if t.dim() != 4 or t.shape != (B, G, k_raw.size(2), D) or t.dtype != dt:

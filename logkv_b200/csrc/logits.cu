@@ -1,12 +1,13 @@
 // Penalties of repeated tokens, biases and grammar masks on next-token logits (C ABI in include/logkv_logits.h).
 //
 // Bound by HBM: every logit is read once and written once, the mask's bits are read once; below a few MB by the
-// launch and one slice's latency.
+// launch and one part's latency.
 //
-// A CTA takes one slice of one row: its threads ask for the slice's logits first (PER 16-byte vectors each,
-// kept in registers), and while those come scan the row's history for tokens of the slice.  Touched tokens are bits
-// of a bitmap with a counter each in shared memory, so that a vector without a touched bit costs one byte of
-// shared memory and is written back as it was read.  Counters are integers: the order of the scan does not show.
+// A CTA takes one part of one row.  Eight warps copy the part under its mask.  Others, beside them, go over the
+// row's history: tokens of the part set bits of a bitmap in shared memory, a prefix sum over its words numbers the set
+// ones, and a second pass lists and counts them under their numbers.  Lists are as long as the history at most, however
+// long the part, so that few CTAs read a history.  At the end the listed tokens are put over the copy, each from its
+// logit as it was.  Counts are integers: the scan's order does not show.
 #include <algorithm>
 
 #include "common.cuh"
@@ -14,7 +15,8 @@
 
 namespace logkv {
 
-constexpr int kLogitsThreads = 256;
+constexpr int kLogitsThreads = 256;   // that copy; LT more go over the history and the biases, where there are any
+constexpr int logits_ctas(int lt) { return lt > 128 ? 3 : 4; }   // of an SM, at 40 registers a thread
 constexpr unsigned kSeen = 0x80000000u;   // counter bit of a token that the prompt holds
 
 __device__ __forceinline__ long long load_int(const void* p, int wide, long long i) {
@@ -28,189 +30,283 @@ __device__ __forceinline__ unsigned mask_bits(const int32_t* mask, int v, int n,
   return __funnelshift_r(lo, hi, v & 31);
 }
 
-// Tokens of a row's history that lie in [begin, end), four loads in flight per thread: visit(index, token).
-template <typename Visit>
+template <int LT>
+__device__ __forceinline__ void list_sync() {
+  asm volatile("bar.sync 1, %0;\n" ::"n"(LT) : "memory");
+}
+
+// Tokens of a row's history that lie in [begin, end), kInFlight loads of each thread under way: visit(index, token).
+template <int LT, typename Visit>
 __device__ __forceinline__ void visit_history(const logkv_logits_args_t& a, int r, int length, int begin, int end,
-                                              Visit visit) {
+                                              int tid, Visit visit) {
+  constexpr int kInFlight = 8;
   const long long h0 = (long long)r * a.history_stride;
-  for (int i0 = threadIdx.x; i0 < length; i0 += 4 * kLogitsThreads) {
-    long long v[4];
+  for (int i0 = tid; i0 < length; i0 += kInFlight * LT) {
+    long long v[kInFlight];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = i0 + k * kLogitsThreads;
+    for (int k = 0; k < kInFlight; ++k) {
+      const int i = i0 + k * LT;
       v[k] = i < length ? load_int(a.history, a.history_wide, h0 + i) : -1;
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (v[k] >= begin && v[k] < end) visit(i0 + k * kLogitsThreads, (int)v[k]);
+    for (int k = 0; k < kInFlight; ++k)
+      if (v[k] >= begin && v[k] < end) visit(i0 + k * LT, (int)v[k]);
   }
 }
 
-template <typename T, int PER>
-__global__ void __launch_bounds__(kLogitsThreads) adjust_logits_kernel(logkv_logits_args_t a) {
-  constexpr int VN = 16 / (int)sizeof(T), SLICE = kLogitsThreads * PER * VN;
-  constexpr int BIAS = LOGKV_LOGITS_MAX_BIAS / kLogitsThreads;   // bias entries per thread
-  extern __shared__ unsigned count[];                                   // [SLICE] where there is a history
-  __shared__ unsigned touched[SLICE / 32];
-  int* bt = reinterpret_cast<int*>(count + (a.history ? SLICE : 0));    // [bias_count] tokens, -1: not this slice's
-  float* bv = reinterpret_cast<float*>(bt + a.bias_count);              // [bias_count] biases
+// A part's place in shared memory.
+struct LogitsGeo {
+  int part;       // tokens of a CTA, a multiple of 32
+  int listed;     // distinct history tokens that a part can hold; 0 without a history
+};
+
+// -inf in the elements of a vector whose bit is 0: the bits spread to the signs of bytes, which a byte permutation
+// copies over its element's bytes (14 instructions for 8 elements; a select per element took the copy from 57 to 73 us
+// for 512 rows of 151936).
+__device__ __forceinline__ unsigned byte_signs(unsigned x, unsigned selector) {   // 8 + i in a nibble: byte i's sign
+  unsigned y;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(y) : "r"(x), "r"(selector));
+  return y;
+}
+template <int VN>
+__device__ __forceinline__ void mask_vector(uint4& x, unsigned allow) {
+  unsigned* word = reinterpret_cast<unsigned*>(&x);
+#pragma unroll
+  for (int h = 0; h < VN / 4; ++h) {
+    const unsigned s = ((allow >> (4 * h) & 15u) * 0x10204080u) & 0x80808080u;   // bit i in the sign of byte i
+    if constexpr (VN == 4) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned m = byte_signs(s, 0x8888u + 0x1111u * k);
+        word[k] = (word[k] & m) | (0xff800000u & ~m);
+      }
+    } else {
+      const unsigned m0 = byte_signs(s, 0x9988u), m1 = byte_signs(s, 0xbbaau);
+      word[2 * h] = (word[2 * h] & m0) | (0xff80ff80u & ~m0);
+      word[2 * h + 1] = (word[2 * h + 1] & m1) | (0xff80ff80u & ~m1);
+    }
+  }
+}
+
+// 16 bytes from any element on: four words, or, for bf16 at an odd element, its two ends and three words.
+__device__ __forceinline__ uint4 load_shifted(const void* p) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  if (!(at & 3)) {
+    const unsigned* s = reinterpret_cast<const unsigned*>(at);
+    return make_uint4(s[0], s[1], s[2], s[3]);
+  }
+  const unsigned short* e = reinterpret_cast<const unsigned short*>(at);
+  const unsigned* s = reinterpret_cast<const unsigned*>(at + 2);
+  const unsigned w0 = e[0], w1 = s[0], w2 = s[1], w3 = s[2], w4 = e[7];
+  return make_uint4(w0 | w1 << 16, __funnelshift_r(w1, w2, 16), __funnelshift_r(w2, w3, 16), w3 >> 16 | w4 << 16);
+}
+
+// SHIFTED: some row of the logits lies at another 16-byte offset than the output's.
+template <typename T, bool SHIFTED, int LT>
+__global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
+    adjust_logits_kernel(logkv_logits_args_t a, LogitsGeo g) {
+  constexpr int VN = 16 / (int)sizeof(T), U = 4;                 // vectors of a thread in flight
+  extern __shared__ unsigned smem[];
+  __shared__ int warp_sums[LT / 32];
+  const int words = g.listed ? g.part / 32 : 0;
+  unsigned* touched = smem;                                       // [words] bits of the history's tokens
+  unsigned* before = touched + words;                             // [words] set bits in front of a word
+  int* token = reinterpret_cast<int*>(before + words);            // [listed] by number, in index order
+  unsigned* count = reinterpret_cast<unsigned*>(token + g.listed);   // [listed]
+  int* bt = reinterpret_cast<int*>(count + g.listed);             // [bias_count] tokens, -1: not this part's or again
+  float* bz = reinterpret_cast<float*>(bt + a.bias_count);        // [bias_count] biases, then adjusted logits
   pdl_entry();
-  const int tid = threadIdx.x, r = blockIdx.y, n = r / a.width, w = r % a.width;
+  const int r = blockIdx.y, n = r / a.width, w = r % a.width;
   const T* x = static_cast<const T*>(a.logits) + n * a.n_stride + w * a.w_stride;
   T* y = static_cast<T*>(a.out) + n * a.out_n_stride + w * a.out_w_stride;
-  // Slices start where the output's 16-byte vectors do: vector j of this one is tokens v0 + j VN and on.
+  // Parts start where the output's 16-byte vectors do: vector j of this one is tokens v0 + j VN and on.  Those of
+  // [first, last) lie in the part as a whole; the tokens in front of and behind them are fewer than VN each.
   const int mis = (int)((reinterpret_cast<uintptr_t>(y) & 15) / sizeof(T));
-  const int v0 = blockIdx.x * SLICE - mis, begin = max(v0, 0), end = min(a.vocab, v0 + SLICE);
+  const int v0 = blockIdx.x * g.part - mis, begin = max(v0, 0), end = min(a.vocab, v0 + g.part);
   if (begin >= end) return;
-  const bool shifted = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) != mis;
-
-  uint4 raw[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int v = v0 + (tid + i * kLogitsThreads) * VN;
-    raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (v >= begin && v + VN <= end) {
-      if (!shifted) {
-        raw[i] = *reinterpret_cast<const uint4*>(x + v);
-      } else {
-        // The logits' rows lie at another offset than the output's: four words, or, for bf16 at an odd element,
-        // its two ends and three words.
-        const uintptr_t at = reinterpret_cast<uintptr_t>(x + v);
-        if (!(at & 3)) {
-          const unsigned* s = reinterpret_cast<const unsigned*>(at);
-          raw[i] = make_uint4(s[0], s[1], s[2], s[3]);
-        } else {
-          const unsigned short* e = reinterpret_cast<const unsigned short*>(at);
-          const unsigned* s = reinterpret_cast<const unsigned*>(at + 2);
-          const unsigned w0 = e[0], w1 = s[0], w2 = s[1], w3 = s[2], w4 = e[7];
-          raw[i] = make_uint4(w0 | w1 << 16, __funnelshift_r(w1, w2, 16), __funnelshift_r(w2, w3, 16),
-                              w3 >> 16 | w4 << 16);
-        }
-      }
-    } else {   // a row's ragged end: element by element
-      T* e = reinterpret_cast<T*>(&raw[i]);
-#pragma unroll
-      for (int j = 0; j < VN; ++j)
-        if (v + j >= begin && v + j < end) e[j] = x[v + j];
-    }
-  }
-
+  const int32_t* mask = a.mask ? a.mask + r * a.mask_stride : nullptr;
   const float rep = a.repetitions ? a.repetitions[r] : a.repetition;
   const float pres = a.presences ? a.presences[r] : a.presence, freq = a.frequencies ? a.frequencies[r] : a.frequency;
-  if (a.history) {
-    const long long len = a.lengths ? load_int(a.lengths, a.lengths_wide, r) : a.length;
-    const int length = (int)max(0LL, min(len, (long long)a.history_len));
-    const long long pro = a.prompts ? load_int(a.prompts, a.prompts_wide, r) : a.prompt;
-    const int prompt = (int)max(0LL, min(pro, (long long)length));
-    for (int i = tid; i < SLICE / 32; i += kLogitsThreads) touched[i] = 0u;
-    __syncthreads();
-    visit_history(a, r, length, begin, end, [&](int, int v) {
-      count[v - v0] = 0u;   // the same value from every thread that meets the token
-      atomicOr(&touched[(v - v0) >> 5], 1u << ((v - v0) & 31));
-    });
-    __syncthreads();
-    visit_history(a, r, length, begin, end, [&](int i, int v) {
-      if (i < prompt) atomicOr(&count[v - v0], kSeen);
-      else atomicAdd(&count[v - v0], 1u);
-    });
-  }
-  for (int i = tid; i < a.bias_count; i += kLogitsThreads) {
-    const long long v = load_int(a.bias_tokens, a.bias_wide, r * a.bias_tokens_stride + i);
-    bt[i] = v >= begin && v < end ? (int)v : -1;
-    bv[i] = a.bias_values[r * a.bias_values_stride + i];
-  }
-  if (a.history || a.bias_count) __syncthreads();
-
-  const int32_t* mask = a.mask ? a.mask + r * a.mask_stride : nullptr;
   auto adjust = [&](float z, unsigned c) {
-    z = z > 0.f ? __fdiv_rn(z, rep) : z * rep;
     const unsigned k = c & ~kSeen;
+    z = z > 0.f ? __fdiv_rn(z, rep) : z * rep;
     return k ? z - fmaf(freq, (float)k, pres) : z;
   };
-  // Biased tokens are few: the thread of a token's first entry works out its value, and puts it over the slice's
-  // own once that is written.
-  float bz[BIAS];
-  bool put[BIAS];
-#pragma unroll
-  for (int k = 0; k < BIAS; ++k) {
-    const int i = tid + k * kLogitsThreads, v = i < a.bias_count ? bt[i] : -1;
-    bool first = v >= 0;
-    for (int j = 0; j < i && first; ++j) first = bt[j] != v;
-    put[k] = first;
-    bz[k] = 0.f;
-    if (!first) continue;
-    float sum = bv[i];
-    for (int j = i + 1; j < a.bias_count; ++j)
-      if (bt[j] == v) sum += bv[j];
-    float z = Elem<T>::load(x + v);
-    const int l = v - v0;
-    if (a.history && touched[l >> 5] >> (l & 31) & 1) z = adjust(z, count[l]);
-    z += sum;
-    bz[k] = mask && !(mask_bits(mask, v, 1, a.vocab) & 1) ? -INFINITY : z;
-  }
-  if (a.bias_count) __syncthreads();   // in place: every biased logit is read before the slice is written
+  int listed = 0;
 
+  if (threadIdx.x < kLogitsThreads) {
+    const int tid = threadIdx.x, first = (begin - v0 + VN - 1) / VN, last = (end - v0) / VN;
+    const bool bytewise = !(v0 & (VN - 1));   // a vector's bits lie in one byte of the mask
+    for (int j0 = first + tid; j0 < last; j0 += U * kLogitsThreads) {
+      uint4 raw[U];
+      unsigned allow[U];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int l = (tid + i * kLogitsThreads) * VN, v = v0 + l;
-    if (v >= end || v + VN <= begin) continue;
-    T* e = reinterpret_cast<T*>(&raw[i]);
-    if (a.history) {
-      const unsigned t = touched[l >> 5] >> (l & 31) & ((1u << VN) - 1);
-      if (t) {
+      for (int i = 0; i < U; ++i) {
+        const int j = j0 + i * kLogitsThreads, v = v0 + j * VN;
+        if (j < last) {
+          raw[i] = SHIFTED ? load_shifted(x + v) : __ldcs(reinterpret_cast<const uint4*>(x + v));
+          if (mask)
+            allow[i] = bytewise ? (unsigned)reinterpret_cast<const uint8_t*>(mask)[v >> 3] >> (v & 7)
+                                : mask_bits(mask, v, VN, a.vocab);
+        }
+      }
 #pragma unroll
-        for (int j = 0; j < VN; ++j)
-          if (t >> j & 1) Elem<T>::store(&e[j], adjust(Elem<T>::load(&e[j]), count[l + j]));
+      for (int i = 0; i < U; ++i) {
+        const int j = j0 + i * kLogitsThreads;
+        if (j >= last) break;
+        if (mask) mask_vector<VN>(raw[i], allow[i]);
+        *reinterpret_cast<uint4*>(y + v0 + j * VN) = raw[i];
       }
     }
-    if (mask) {
-      const int s = max(v, begin);
-      const unsigned m = mask_bits(mask, s, VN, a.vocab) << (s - v);
-      unsigned* word = reinterpret_cast<unsigned*>(&raw[i]);
+    // A row's ragged ends (the whole of a part without a whole vector), element by element.
+    if (tid < 2 * VN) {
+      const int edge = first < last ? v0 + first * VN : end, tail = first < last ? v0 + last * VN : end;
+      for (int v = tid < VN ? begin + tid : tail + tid - VN, to = tid < VN ? edge : end; v < to; v += VN)
+        if (mask && !(mask_bits(mask, v, 1, a.vocab) & 1)) Elem<T>::store(y + v, -INFINITY);
+        else y[v] = x[v];
+    }
+  } else {
+    const int tid = threadIdx.x - kLogitsThreads, lane = tid & 31;
+    auto number = [&](int l) {   // of the part's touched token l
+      return before[l >> 5] + __popc(touched[l >> 5] & ((1u << (l & 31)) - 1));
+    };
+    if (g.listed) {
+      const long long len = a.lengths ? load_int(a.lengths, a.lengths_wide, r) : a.length;
+      const int length = (int)max(0LL, min(len, (long long)a.history_len));
+      const long long pro = a.prompts ? load_int(a.prompts, a.prompts_wide, r) : a.prompt;
+      const int prompt = (int)max(0LL, min(pro, (long long)length));
+      for (int i = tid; i < words; i += LT) touched[i] = 0u;
+      for (int i = tid; i < g.listed; i += LT) count[i] = 0u;
+      list_sync<LT>();
+      visit_history<LT>(a, r, length, begin, end, tid, [&](int, int v) {
+        const unsigned bit = 1u << ((v - v0) & 31);
+        unsigned* word = &touched[(v - v0) >> 5];
+        if (!(*reinterpret_cast<volatile unsigned*>(word) & bit)) atomicOr(word, bit);   // frequent tokens once
+      });
+      list_sync<LT>();
+      const int per = (words + LT - 1) / LT, w0 = min(words, tid * per), w1 = min(words, w0 + per);
+      int sum = 0, at;
+      for (int i = w0; i < w1; ++i) sum += __popc(touched[i]);
+      at = sum;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (VN == 4)
-          word[j] = m >> j & 1 ? word[j] : 0xff800000u;
-        else
-          word[j] = (m >> (2 * j) & 1 ? word[j] & 0xffffu : 0xff80u) |
-                    (m >> (2 * j + 1) & 1 ? word[j] & 0xffff0000u : 0xff800000u);
+      for (int off = 1; off < 32; off <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, at, off);
+        if (lane >= off) at += up;
+      }
+      if (lane == 31) warp_sums[tid >> 5] = at;
+      list_sync<LT>();
+      at -= sum;
+#pragma unroll
+      for (int i = 0; i < LT / 32; ++i) at += i < tid >> 5 ? warp_sums[i] : 0;
+      for (int i = w0; i < w1; ++i) {
+        before[i] = at;
+        at += __popc(touched[i]);
+      }
+      list_sync<LT>();
+      visit_history<LT>(a, r, length, begin, end, tid, [&](int i, int v) {
+        const int k = number(v - v0);
+        token[k] = v;   // the same from every thread that meets the token
+        if (i < prompt) atomicOr(&count[k], kSeen);
+        else atomicAdd(&count[k], 1u);
+      });
+    }
+    if (a.bias_count) {
+      // Biased tokens are few: the thread of a token's first entry works out its value.  In place the copy leaves the
+      // logit as it was, but for a masked one, which is -inf in the end either way.
+      for (int i = tid; i < a.bias_count; i += LT) {
+        const long long v = load_int(a.bias_tokens, a.bias_wide, r * a.bias_tokens_stride + i);
+        bt[i] = v >= begin && v < end ? (int)v : -1;
+        bz[i] = a.bias_values[r * a.bias_values_stride + i];
+      }
+      list_sync<LT>();
+      constexpr int PER = LOGKV_LOGITS_MAX_BIAS / LT;
+      float z[PER];
+      unsigned mine = 0;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int i = tid + k * LT, v = i < a.bias_count ? bt[i] : -1;
+        bool first = v >= 0;
+        for (int j = 0; j < i && first; ++j) first = bt[j] != v;
+        z[k] = 0.f;
+        if (!first) continue;
+        mine |= 1u << k;
+        float sum = bz[i];
+        for (int j = i + 1; j < a.bias_count; ++j)
+          if (bt[j] == v) sum += bz[j];
+        z[k] = Elem<T>::load(x + v);
+        const int l = v - v0;
+        if (g.listed && touched[l >> 5] >> (l & 31) & 1) z[k] = adjust(z[k], count[number(l)]);
+        z[k] += sum;
+        if (mask && !(mask_bits(mask, v, 1, a.vocab) & 1)) z[k] = -INFINITY;
+      }
+      list_sync<LT>();
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int i = tid + k * LT;
+        if (i >= a.bias_count) break;
+        bz[i] = z[k];
+        if (!(mine >> k & 1)) bt[i] = -1;
       }
     }
-    if (v >= begin && v + VN <= end) {
-      *reinterpret_cast<uint4*>(y + v) = raw[i];
-    } else {
+  }
+  if (!g.listed && !a.bias_count) return;
+  __syncthreads();
+  if (g.listed) {
 #pragma unroll
-      for (int j = 0; j < VN; ++j)
-        if (v + j >= begin && v + j < end) y[v + j] = e[j];
+    for (int i = 0; i < LT / 32; ++i) listed += warp_sums[i];
+    for (int i = threadIdx.x; i < listed; i += kLogitsThreads + LT) {
+      T* e = y + token[i];
+      Elem<T>::store(e, adjust(Elem<T>::load(e), count[i]));
     }
   }
   if (a.bias_count) {
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < BIAS; ++k)
-      if (put[k]) Elem<T>::store(y + bt[tid + k * kLogitsThreads], bz[k]);
+    for (int i = threadIdx.x; i < a.bias_count; i += kLogitsThreads + LT)
+      if (bt[i] >= 0) Elem<T>::store(y + bt[i], bz[i]);
   }
 }
 
-template <typename T, int PER>
+template <typename T, bool SHIFTED, int LT>
 static int launch_adjust(const logkv_logits_args_t& a, cudaStream_t st) {
-  constexpr int VN = 16 / (int)sizeof(T), SLICE = kLogitsThreads * PER * VN;
-  const size_t smem = (a.history ? (size_t)SLICE * 4 : 0) + (size_t)a.bias_count * 8;
-  // A row whose start is not aligned reaches VN - 1 tokens further.
-  const unsigned slices = (unsigned)(((long long)a.vocab + VN - 1 + SLICE - 1) / SLICE);
-  launch_pdl(adjust_logits_kernel<T, PER>, dim3(slices, a.rows), kLogitsThreads, smem, st, a);
+  constexpr int VN = 16 / (int)sizeof(T);
+  constexpr int kMost = 200 << 10;   // shared memory of a CTA at most
+  constexpr auto kern = adjust_logits_kernel<T, SHIFTED, LT>;
+  const long long span = (long long)a.vocab + VN - 1;   // a row whose start is not aligned reaches VN - 1 tokens further
+  auto geo = [&](long long parts) {
+    LogitsGeo g;
+    const long long least = (long long)kLogitsThreads * VN;   // a vector per thread
+    g.part = (int)((std::max(least, (span + parts - 1) / parts) + 255) / 256 * 256);
+    g.listed = a.history ? std::min(a.history_len, g.part) : 0;
+    return g;
+  };
+  auto bytes = [&](const LogitsGeo& g) {
+    return (g.listed ? (size_t)g.part / 32 * 8 : 0) + (size_t)g.listed * 8 + (size_t)a.bias_count * 8;
+  };
+  // Parts: one wave of CTAs, and up to three where a part is still 16 times as long as the history that each of a
+  // row's CTAs goes over.  512 rows of 151936 (history 1024): 62.4 us in one wave, 58.5 in three; 145 rows of 50021
+  // (history 4097): 18 in one wave, 26 in two, 33 in three.
+  const long long wave = 148 * logits_ctas(LT);
+  const long long room = a.history ? a.vocab / (16LL * a.history_len) : a.vocab;
+  LogitsGeo g = geo(std::max({1LL, wave / a.rows, std::min(3 * wave / a.rows, room)}));
+  for (long long parts = 2; bytes(g) > kMost; parts *= 2) g = geo(parts);
+  if (const int e = smem_limit_once<kern>(kMost)) return e;
+  launch_pdl(kern, dim3((unsigned)((span + g.part - 1) / g.part), a.rows),
+             kLogitsThreads + (g.listed || a.bias_count ? LT : 0), bytes(g), st, a, g);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? LOGKV_OK : (int)e;
 }
 
 template <typename T>
 static int launch_adjust(const logkv_logits_args_t& a, cudaStream_t st) {
-  constexpr int VN = 16 / (int)sizeof(T);
-  const long long vectors = (long long)a.rows * ((a.vocab + VN - 1) / VN);
-  const long long ctas = vectors / kLogitsThreads;   // with one vector per thread
-  if (ctas >= 4 * 148 * 8) return launch_adjust<T, 4>(a, st);
-  if (ctas >= 2 * 148 * 4) return launch_adjust<T, 2>(a, st);
-  return launch_adjust<T, 1>(a, st);
+  // Whether every row of the logits lies at its output's 16-byte offset.
+  const uintptr_t e = sizeof(T), base = reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.out);
+  const uintptr_t w = (uintptr_t)(a.w_stride - a.out_w_stride) * e, n = (uintptr_t)(a.n_stride - a.out_n_stride) * e;
+  const bool shifted = (base & 15) || (a.width > 1 && (w & 15)) || (a.rows > a.width && (n & 15));
+  // Eight warps for long histories: 4097 tokens beside 50021 logits 18 us against 23 with four; 1024 beside 151936
+  // 64 against 58.5 (an SM then holds three CTAs instead of four).
+  if (a.history && a.history_len > 2048)
+    return shifted ? launch_adjust<T, true, 256>(a, st) : launch_adjust<T, false, 256>(a, st);
+  return shifted ? launch_adjust<T, true, 128>(a, st) : launch_adjust<T, false, 128>(a, st);
 }
 
 }  // namespace logkv
@@ -222,7 +318,7 @@ extern "C" LOGKV_API int logkv_adjust_logits(const logkv_logits_args_t* args, vo
   logkv_logits_args_t a = *args;
   if (a.dtype != LOGKV_DTYPE_F32 && a.dtype != LOGKV_DTYPE_BF16) return LOGKV_E_DTYPE;
   if (a.rows < 1 || a.rows > 65535 || a.width < 1 || a.vocab < 1 || a.vocab > (1 << 30) || a.history_len < 0 ||
-      a.bias_count < 0 || a.bias_count > LOGKV_LOGITS_MAX_BIAS)
+      a.history_len > (1 << 30) || a.bias_count < 0 || a.bias_count > LOGKV_LOGITS_MAX_BIAS)
     return LOGKV_E_SHAPE;
   auto at = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   const uintptr_t e = a.dtype == LOGKV_DTYPE_F32 ? 4 : 2;

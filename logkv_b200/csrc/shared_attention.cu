@@ -21,10 +21,11 @@ struct ShareGeo {
   int rcap, rcount, w0;   // window: capacity, rows, shared rows
   int causal;             // new token j is seen by query tokens t >= j only
   int nsplit;             // splits of a shared lane in the grid; share_splits() of them are used
-  int nsmin;              // splits that fill the SMs
   int upw;                // key tiles a split has at least
   int nown;               // splits of an own lane
   int shared_lanes, own_lanes;
+  int slots;              // CTAs that run at once
+  long long own_work;     // all own lanes' CTAs in keys, what it takes to start one included
   int tiles, tile_rows;   // row tiles of a shared lane (at most 16 or 128 rows each)
   int own_tiles;          // row tiles of an own lane (16 rows each)
   float scale_log2, mass_log2;   // score = dot * scale_log2 + mass * mass_log2, in the log2 domain
@@ -34,9 +35,13 @@ struct ShareGeo {
   long long qs[3], ks[3], vs[3];
 };
 
-// Splits of a shared lane with `units` key tiles (the same value in the attention kernel and the combine).
-__device__ __forceinline__ int share_splits(const ShareGeo& a, int units) {
-  return max(1, min(a.nsplit, min(a.nsmin, units / a.upw)));
+// Splits of a shared lane with `units` key tiles (the same value in the attention kernel and the combine): the SMs are
+// divided between the two kinds of lanes by their work, so that both end together.
+__device__ __forceinline__ int share_splits(const ShareGeo& a, int units, int tile_keys) {
+  const int ctas = a.shared_lanes * a.tiles;
+  const long long work = (long long)units * tile_keys * ctas;
+  const int room = (int)(a.slots * work / (work + a.own_work));
+  return max(1, min(a.nsplit, min(room / ctas, units / a.upw)));
 }
 
 __device__ __forceinline__ int share_prefix_length(const logkv_prefix_t& pre, int ln) {
@@ -86,7 +91,7 @@ __device__ __forceinline__ ShareJob share_job(const ShareGeo& a, const logkv_pre
     j.n0 = share_prefix_length(pre, ln);
     j.n1 = a.w0;
     j.r0 = (size_t)ln * pre.capacity;
-    j.ns = share_splits(a, (j.n0 + tile_keys - 1) / tile_keys + (j.n1 + tile_keys - 1) / tile_keys);
+    j.ns = share_splits(a, (j.n0 + tile_keys - 1) / tile_keys + (j.n1 + tile_keys - 1) / tile_keys, tile_keys);
   }
   return j;
 }
@@ -936,7 +941,7 @@ __global__ void __launch_bounds__(128) share_combine_kernel(ShareGeo a, logkv_pr
   const size_t row = (size_t)blockIdx.x * (4 / WPR) + warp / WPR;
   if (WPR == 1 && row >= (size_t)a.B * a.H * a.T) return;
   const int bh = (int)(row / a.T), b = bh / a.H / a.W * a.W, g = bh % a.H / a.rf;
-  const int shared = share_splits(a, (share_prefix_length(pre, b * a.G + g) + TS - 1) / TS + (a.w0 + TS - 1) / TS);
+  const int shared = share_splits(a, (share_prefix_length(pre, b * a.G + g) + TS - 1) / TS + (a.w0 + TS - 1) / TS, TS);
   const int ns = shared + a.nown, skip = a.nsplit - shared;   // partials; unused slots between the two kinds
   const size_t stride = (size_t)a.B * a.H * a.T * (D + 4);
   const float* p0 = part + row * (D + 4);
@@ -1028,7 +1033,8 @@ __global__ void __launch_bounds__(128) share_combine_kernel(ShareGeo a, logkv_pr
 
 // ---------------------------------------------------------------- host side
 struct SharePlan {
-  int tile_rows, tiles, own_tiles, ts, nsplit, nsmin, upw, nown;
+  int tile_rows, tiles, own_tiles, nsplit, upw, nown, slots;
+  long long own_work;
   bool tc;
 };
 
@@ -1041,18 +1047,19 @@ static SharePlan share_plan(const logkv_layout_t& l, const logkv_shared_args_t& 
   p.tiles = (int)((rows + most - 1) / most);
   p.tile_rows = p.tc ? (int)((rows + p.tiles - 1) / p.tiles) : most;
   p.own_tiles = (int)((own_rows + 15) / 16);
-  p.ts = p.tc ? kTcTS : 16;
+  const int ts = p.tc ? kTcTS : 16;
   p.upw = p.tc ? 2 : kShareWarps;
-  const int slots = 148 * ((f32 && l.dim > 64) || l.dim > 128 ? 1 : 2);   // CTAs that run at once
+  p.slots = 148 * ((f32 && l.dim > 64) || l.dim > 128 ? 1 : 2);
   const long long own_ctas = (long long)l.batch * l.groups * p.own_tiles;
   const long long shared_ctas = (long long)l.batch / x.beams * l.groups * p.tiles;
   // Own lanes: a key tile per warp at least, and a second split only while they leave half of the SMs.
-  const int own_units = (x.recent_count - x.window_from + 15) / 16 + (x.tokens + 15) / 16;
-  p.nown = (int)std::max(1LL, std::min<long long>(own_units / kShareWarps, slots / 2 / own_ctas));
-  const long long room = std::max<long long>(slots / 2, slots - own_ctas * p.nown);
-  p.nsmin = (int)std::max(1LL, room / shared_ctas);
-  const int units = (prefix_capacity + x.window_from) / p.ts + 2;
-  p.nsplit = std::max(1, std::min(p.nsmin, units / p.upw));
+  const int own_keys = x.recent_count - x.window_from + x.tokens;
+  p.nown = (int)std::max(1LL, std::min<long long>(own_keys / 16 / kShareWarps, p.slots / 2 / own_ctas));
+  // A CTA's start weighs as much as some 250 keys.  Measured with 1 to 8 splits of 64 shared lanes (8.0K keys) beside
+  // 512 own ones (242 keys): 129, 81, 60, 61, 74, 66, 68 us for 1, 2, 3, 4, 5, 6, 8; this gives 3.
+  p.own_work = own_ctas * p.nown * (own_keys / p.nown + 250);
+  const int units = (prefix_capacity + x.window_from) / ts + 2;
+  p.nsplit = (int)std::max(1LL, std::min<long long>(p.slots / shared_ctas, units / p.upw));
   return p;
 }
 
@@ -1179,7 +1186,6 @@ LOGKV_API int logkv_shared_attention(const logkv_layout_t* layout, const logkv_s
   a.w0 = x->window_from;
   a.causal = x->causal;
   a.nsplit = p.nsplit;
-  a.nsmin = p.nsmin;
   a.upw = p.upw;
   a.nown = p.nown;
   a.shared_lanes = a.B / a.W * a.G;
@@ -1187,6 +1193,8 @@ LOGKV_API int logkv_shared_attention(const logkv_layout_t* layout, const logkv_s
   a.tiles = p.tiles;
   a.tile_rows = p.tile_rows;
   a.own_tiles = p.own_tiles;
+  a.slots = p.slots;
+  a.own_work = p.own_work;
   a.scale_log2 = x->scale * 1.4426950408889634f;
   a.mass_log2 = x->qx * a.scale_log2;
   a.q = x->q;

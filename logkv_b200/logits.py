@@ -11,6 +11,7 @@ import torch
 
 from . import _lib
 
+_native = None    # (logits call, function address) of the host binding, once a call has gone through
 MAX_BIAS = 1024   # LOGKV_LOGITS_MAX_BIAS
 _INTS = (torch.int32, torch.int64)
 
@@ -77,6 +78,14 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt=0, repetition=1.
     Returns logits of the same shape and dtype, contiguous; ``out`` may be given, and may be ``logits`` itself.
     V <= 2^30, N * W <= 65535.  Forward-only.
     """
+    global _native
+    if _native is not None and out is None:   # checks, allocation and launch in the host binding; None: not covered there
+        tokens, values = (None, None) if bias is None else bias
+        y = _native[0](_native[1], logits, history, lengths, prompt, repetition, presence, frequency, tokens, values, mask)
+        if y is not None:
+            if type(y) is int:
+                _lib.check(y, "logkv_adjust_logits")
+            return y
     if logits.dim() not in (2, 3):
         raise ValueError(f"logits must be [N, W, V] or [rows, V], got {tuple(logits.shape)}")
     lead, V, dev = logits.shape[:-1], logits.size(-1), logits.device
@@ -96,8 +105,8 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt=0, repetition=1.
     if history is not None:
         hist, a.history_stride = _table("history", history, lead, dev, _INTS, False)
         L = hist.size(1)
-        if L >= 1 << 31:
-            raise ValueError(f"a history of {L} tokens")
+        if L > 1 << 30:
+            raise ValueError(f"a history of {L} tokens: at most 2^30")
         a.history_len, a.history_wide = L, hist.dtype == torch.int64
         a.length, lens = _count("lengths", L if lengths is None else lengths, lead, dev)
         a.prompt, prompts = _count("prompt", prompt, lead, dev)
@@ -148,4 +157,5 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt=0, repetition=1.
         a.repetitions, a.presences, a.frequencies = ptr(reps), ptr(press), ptr(freqs)
         a.bias_tokens, a.bias_values, a.mask = ptr(tokens), ptr(values), ptr(mask)
         _lib.check(_lib.lib().logkv_adjust_logits(ctypes.byref(a), _lib.stream_ptr(dev)), "logkv_adjust_logits")
+        _native = (_lib.host().logits, _lib.address("logkv_adjust_logits"))
     return out

@@ -85,6 +85,31 @@ def launch(cache, parts, positions, pos0: int, interleaved: int, *, positions_ou
     a.status = None if status is None else status.data_ptr()
     _lib.check(_lib.lib().logkv_rotate(ctypes.byref(_rope(cache)), ctypes.byref(a),
                                        _lib.stream_ptr(cache.recent_k.device)), "logkv_rotate")
+    if status is not None and cache._rotary is None:
+        cache._rotary = _Native(cache)
+
+
+class _Native:
+    """The host binding's calls with their arguments that do not change for a cache."""
+
+    def __init__(self, cache):
+        from .attention import _rope
+        host = _lib.host()
+        self.rotate, self.append, self.fn = host.rotate, host.append, _lib.address("logkv_rotate")
+        self.tables = _rope(cache)
+        self.rope = ctypes.addressof(self.tables)
+        self.status = cache._read_status.data_ptr()
+
+
+def native(cache):
+    """The cache's _Native once a call has gone through and while its tables are where they were; else None."""
+    n = getattr(cache, "_rotary", None)
+    if n is None:
+        return None
+    b = cache._buffers
+    cos, sin = b["cos_cache"], b["sin_cache"]
+    same = n.tables.cos == cos.data_ptr() and n.tables.sin == sin.data_ptr() and n.tables.rows == cos.size(0)
+    return n if same or not cache.rope_n_elem else None
 
 
 def log_kv_rotate(cache, q, k, input_pos=None, *, layout: str = "half"):
@@ -104,6 +129,14 @@ def log_kv_rotate(cache, q, k, input_pos=None, *, layout: str = "half"):
     Computed in float32 and rounded once (tables are read as they are stored).  Forward-only.
     """
     mode = check_layout(layout)
+    call = native(cache)
+    if call is not None:     # checks, allocations and launch in the host binding; None: not covered there
+        y = call.rotate(call.fn, call.rope, call.status, cache._buffers["recent_k"], q, k, input_pos, cache.token_count,
+                        mode)
+        if y is not None:
+            if type(y) is int:
+                _lib.check(y, "logkv_rotate")
+            return y
     dev, dt, B, G, D = cache.recent_k.device, cache.recent_k.dtype, cache.batch_size, cache.n_groups, cache.k_dim
     if q.dim() != 4 or q.size(0) != B or q.size(3) != D or q.dtype != dt:
         raise ValueError(f"q must be [B={B}, H, T, {D}] in the cache dtype, got {tuple(q.shape)} {q.dtype}")

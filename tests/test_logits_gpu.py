@@ -215,3 +215,39 @@ def test_in_front_of_beam_selection():
     assert (rows[1] != 5).all()
     bits = kw["mask"].view(6, -1)[rows.view(-1), tokens.view(-1) >> 5] >> (tokens.view(-1) & 31) & 1
     assert bits.all()
+
+
+def test_repeated_calls_are_checked_like_the_first():
+    """The host binding takes calls that fit; everything else is refused or done as the first call is."""
+    from logkv_b200 import adjust_logits as f
+    x, kw = inputs(2, 3, 70, 5, 4, F32, 3)
+    want = f(x, **kw)
+    assert torch.equal(f(x, **kw), want)
+    h, n = kw["history"], kw["lengths"]
+    t, b = kw["bias"]
+    for args, more, match in [
+            (x[0, 0], {}, "logits must be"), (x.half(), {}, "dtype"), (x, {"repetition": 0.0}, "positive"),
+            (x, {"repetition": float("inf")}, "finite"), (x, {"presence": float("nan")}, "finite"),
+            (x, {"repetition": b}, "repetition must be"), (x, {"presence": n}, "presence must be"),
+            (x, {"history": h[0]}, "history must be"), (x, {"history": h.float()}, "history must be"),
+            (x, {"history": h.cpu()}, "history must be"), (x, {"lengths": 6}, "at most"), (x, {"lengths": -1}, "negative"),
+            (x, {"lengths": n[0]}, "lengths must be"), (x, {"history": None}, "without a history"), (x, {"prompt": -2}, "negative"),
+            (x, {"bias": (t, b[..., :3])}, "one shape"), (x, {"bias": (t[0, 0], b)}, "one shape"), (x, {"bias": (b, b)}, "bias tokens"),
+            (x, {"mask": kw["mask"][..., :2]}, "3 words"), (x, {"mask": kw["mask"].long()}, "mask must be")]:
+        with pytest.raises(ValueError, match=match):
+            f(args, **{**kw, **more})
+    with pytest.raises(NotImplementedError):
+        f(x.clone().requires_grad_(), **kw)
+    with pytest.raises(NotImplementedError):
+        f(x, **{**kw, "presence": kw["presence"].clone().requires_grad_()})
+    for name in ("lengths", "prompt", "repetition", "presence"):      # strided numbers
+        t2 = kw[name].t().contiguous().t()
+        assert torch.equal(f(x, **{**kw, name: t2}), want)
+    wide = torch.zeros(2, 3, 9, dtype=h.dtype, device="cuda")         # rows of unlike distances
+    wide[..., :5] = h
+    assert torch.equal(f(x, **{**kw, "history": wide[..., :5]}), want)
+    across = h.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(f(x, **{**kw, "history": across}), want)
+    assert f(x[:0], history=h[:0]).shape == (0, 3, 70)
+    assert torch.equal(f(x, **{**kw, "repetition": torch.full((2, 3), 1.5, device="cuda")}), f(x, **{**kw, "repetition": 1.5}))
+    assert torch.equal(f(x, **{**kw, "repetition": 2}), f(x, **{**kw, "repetition": 2.0}))

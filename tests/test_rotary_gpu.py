@@ -229,3 +229,45 @@ def test_two_streams():
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+
+
+def test_repeated_calls_are_checked_like_the_first():
+    """The host binding takes calls that fit; everything else is refused or done as the first call is."""
+    from logkv_b200 import log_kv_rotate as f
+    cache = make(F32, rows=100, window=16)
+    q, k, v = projected(cache, 4, 3, 1)
+    p, ends = torch.arange(3, device="cuda"), torch.zeros(2, 3, dtype=torch.uint8, device="cuda")
+    want = f(cache, q, k, p)
+    cache.add_recent_rotated(k, v, input_pos=p, span_ends_device=ends)
+    assert cache._rotary is not None
+    for args, kw, match in [
+            ((q[:1], k, p), {}, "q must be"), ((q[0], k, p), {}, "q must be"), ((q.bfloat16(), k, p), {}, "q must be"),
+            ((q, k[:, :1], p), {}, "k must be"), ((q, k[:, :, :2], p), {}, "k must be"), ((q[:, :3], k, p), {}, "multiple"),
+            ((q, k, p[:2]), {}, "input_pos"), ((q, k, p.float()), {}, "integers"), ((q, k, [0, 1, 100]), {}, "tables"),
+            ((q, k, p), {"layout": "pairs"}, "layout"), ((q.cpu(), k, p), {}, "device"), ((q, k.cpu(), p), {}, "device")]:
+        with pytest.raises(ValueError, match=match):
+            f(cache, *args, **kw)
+    with pytest.raises(NotImplementedError):
+        f(cache, q.clone().requires_grad_(), k, p)
+    with torch.no_grad():
+        assert torch.equal(f(cache, q.clone().requires_grad_(), k, p)[0], want[0])
+    assert torch.equal(f(cache, q, k, [0, 1, 2])[0], want[0]) and torch.equal(f(cache, q, k, p.int())[1], want[1])
+    last = q.permute(0, 3, 1, 2).contiguous().permute(0, 2, 3, 1)
+    assert torch.equal(f(cache, last, k, p)[0], want[0])
+    assert cache.recent_count == 3
+    bad = lambda *a, **kw: cache.add_recent_rotated(*a, **{"span_ends_device": ends, **kw})  # noqa: E731
+    for args, kw, match in [((k[0], v), {}, "k_raw must be"), ((k, v[:, :, :2]), {}, "v must be"), ((k.bfloat16(), v), {}, "k_raw must be"),
+                            ((k, v), {"input_pos": p[:2]}, "input_pos"), ((k, v), {"span_ends_device": ends[:1]}, "span boundaries"),
+                            ((k, v.cpu()), {}, "device"), ((k, v), {"layout": 1}, "layout")]:
+        with pytest.raises(ValueError, match=match):
+            bad(*args, **kw)
+    assert cache.recent_count == cache.token_count == 3
+    bad(k, v, span_ends_device=ends.bool())
+    cache.token_count = 4095
+    with pytest.raises(RuntimeError, match="token overflow"):
+        bad(k, v)
+    cache.token_count = 6
+    other = cache.cos_cache.flip(0).contiguous()          # other tables take over at once
+    cache.cos_cache, cache.sin_cache = other, cache.sin_cache.flip(0).contiguous()
+    assert torch.equal(f(cache, q, k, 99 - p)[0], want[0])
+    assert cache.read_status() == 0

@@ -371,3 +371,36 @@ def test_beams_keep_more_tokens_than_they_began_with():
     for bad in (torch.zeros(2, 3, dtype=torch.int64, device="cuda"), torch.zeros(1, 3, device="cuda"), torch.zeros(1, 3, dtype=torch.int64)):
         with pytest.raises(ValueError, match="prompt must be"):
             beams.fork(bad)
+
+
+def test_repeated_calls_are_checked_like_the_first():
+    """The host binding takes calls that fit; everything else is refused or done as the first call is."""
+    cache = forked(F32, 2, 3, 10, 30, D=64)
+    q, k, v = fresh(cache, 2, 2, 2)
+    want = run(cache, q, k, v, 3, 10)
+    assert cache._read.native_shared is not None and torch.equal(run(cache, q, k, v, 3, 10), want)
+    f = lambda q, k, v, W=3, w0=10, **kw: run(cache, q, k, v, W, w0, **kw)  # noqa: E731
+    for args, kw, match in [
+            ((q[:1], k, v), {}, "q must be"), ((q[0], k, v), {}, "q must be"), ((q.bfloat16(), k, v), {}, "q must be"),
+            ((q, k[:, :1], v), {}, "k must be"), ((q, k, v[:, :, :1]), {}, "v shape"), ((q, k, v.bfloat16()), {}, "dtype"),
+            ((q[:, :, :1], k, v), {}, "same tokens"), ((q[:, :3], k, v), {}, "multiple"), ((q.cpu(), k, v), {}, "device"),
+            ((q, k, v), {"W": 4}, "beams"), ((q, k, v), {"W": 0}, "beams"), ((q, k, v), {"w0": 31}, "window_from"),
+            ((q, k, v), {"w0": -1}, "window_from")]:
+        with pytest.raises(ValueError, match=match):
+            f(*args, **kw)
+    from logkv_b200 import log_kv_shared_attention
+    with pytest.raises(ValueError, match="causal_tail"):
+        log_kv_shared_attention(cache, q, k, v, 0.125, beams=3, window_from=10, causal_tail=1)
+    with pytest.raises(NotImplementedError):
+        f(q.clone().requires_grad_(), k, v)
+    last = q.permute(0, 3, 1, 2).contiguous().permute(0, 2, 3, 1)
+    assert torch.equal(f(last, k, v), want)
+    wide = log_kv_shared_attention(cache, q, k, v, 0.125, beams=torch.tensor(3), window_from=10.0)
+    assert torch.equal(wide, want)
+    # A flush makes the prefix anew, and the cache's rows are then what they are.
+    cache.recent_count = 20
+    check(cache, q, k, v, run(cache, q, k, v, 3, 10))
+    cache.add_recent(torch.randn_like(cache.recent_k[:, :, :256]), torch.randn_like(cache.recent_k[:, :, :256]),
+                     k_raw=torch.randn_like(cache.recent_k[:, :, :256]), span_ends=[[False] * 256] * 6)
+    assert cache._flush_cursor == 1
+    check(cache, q, k, v, run(cache, q, k, v, 1, 0))

@@ -659,7 +659,7 @@ class LogStructuredKVCache(nn.Module):
                 b = self._buffers
                 rc = call.append(call.fn, call.rope, call.status, b["recent_k"], b["recent_k_raw"], b["recent_v"],
                                  b["recent_pos"], self._recent_ends, k_raw, v, input_pos, span_ends_device,
-                                 self.token_count, c0, mode)
+                                 self.token_count, c0, mode, None)
                 if rc is not None:
                     _lib.check(rc, "logkv_rotate")
                     self.token_count += n

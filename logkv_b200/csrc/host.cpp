@@ -290,26 +290,29 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
-// append(fn, rope, status, window keys, raw keys, values, positions, ends, k, v, positions or None, ends [B, n] uint8,
-// pos0, first row, interleaved): 0, an error code, or None.  The first five are the cache's window buffers.
+// append(fn, rope, status, row keys, raw keys, values, positions, ends, k, v, positions or None, ends [B, n] uint8 or
+// None, pos0, first row, interleaved, q or None): 0 (the rotated q), an error code, or None.  The first five tensors
+// take the rows: a cache's window, or a decoder's pending pair.
 PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 15) {
-    PyErr_SetString(PyExc_TypeError, "append takes 15 arguments");
+  if (n != 16) {
+    PyErr_SetString(PyExc_TypeError, "append takes 16 arguments");
     return nullptr;
   }
   const at::Tensor* win[5];
   for (int i = 0; i < 5; ++i)
     if (!(win[i] = tensor(args[3 + i])) || !win[i]->is_cuda()) Py_RETURN_NONE;
-  const at::Tensor *k = tensor(args[8]), *v = tensor(args[9]), *ends = tensor(args[11]), &like = *win[0];
-  if (!k || !v || !ends || k->dim() != 4 || v->dim() != 4 || ends->dim() != 2) Py_RETURN_NONE;
+  const at::Tensor *k = tensor(args[8]), *v = tensor(args[9]), *ends = tensor(args[11]), *q = tensor(args[15]), &like = *win[0];
+  if (!k || !v || (!ends && args[11] != Py_None) || (!q && args[15] != Py_None) || k->dim() != 4 || v->dim() != 4 ||
+      (ends && ends->dim() != 2) || (q && q->dim() != 4))
+    Py_RETURN_NONE;
   const int64_t B = like.size(0), G = like.size(1), C = like.size(2), D = like.size(3), T = k->size(2);
   const long long c0 = PyLong_AsLongLong(args[13]);
-  auto fits = [&](const at::Tensor& t) {
-    return t.size(0) == B && t.size(1) == G && t.size(2) == T && t.size(3) == D && t.stride(3) == 1 &&
-           t.scalar_type() == like.scalar_type() && t.device() == like.device();
+  auto fits = [&](const at::Tensor& t, int64_t heads) {
+    return t.size(0) == B && t.size(1) == heads && t.size(2) == T && t.size(3) == D && t.stride(3) == 1 &&
+           t.scalar_type() == like.scalar_type() && t.device() == like.device() && !wants_gradient(t);
   };
   logkv_rotate_args_t a{};
-  a.n_parts = 2;
+  a.n_parts = q ? 3 : 2;
   a.batch = (int32_t)B;
   a.tokens = (int32_t)T;
   a.dim = (int32_t)D;
@@ -318,24 +321,39 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   a.interleaved = PyObject_IsTrue(args[14]);
   a.status = address<int32_t*>(args[2]);
   if (PyErr_Occurred()) return nullptr;
-  if (T < 1 || c0 < 0 || c0 + T > C || !fits(*k) || !fits(*v) || ends->scalar_type() != at::kByte ||
-      ends->device() != like.device() || ends->size(0) != B || ends->size(1) != T || (T > 1 && ends->stride(1) != 1) ||
+  if (T < 1 || c0 < 0 || c0 + T > C || !fits(*k, G) || !fits(*v, G) ||
+      (q && (q->size(1) < 1 || q->size(1) % G || !fits(*q, q->size(1)))) ||
+      (ends && (ends->scalar_type() != at::kByte || ends->device() != like.device() || ends->size(0) != B ||
+                ends->size(1) != T || (T > 1 && ends->stride(1) != 1))) ||
       c10::cuda::current_device() != like.get_device() || !rotate_positions(a, args[10], like))
     Py_RETURN_NONE;
-  const int64_t at = c0 * D * like.element_size();
+  const int64_t offset = c0 * D * like.element_size();
   rotate_part(a.parts[0], *k, win[0], win[1]);
   rotate_part(a.parts[1], *v, nullptr, win[2]);
-  a.parts[0].rotated = static_cast<char*>(a.parts[0].rotated) + at;
-  a.parts[0].raw = static_cast<char*>(a.parts[0].raw) + at;
-  a.parts[1].raw = static_cast<char*>(a.parts[1].raw) + at;
+  a.parts[0].rotated = static_cast<char*>(a.parts[0].rotated) + offset;
+  a.parts[0].raw = static_cast<char*>(a.parts[0].raw) + offset;
+  a.parts[1].raw = static_cast<char*>(a.parts[1].raw) + offset;
   a.positions_out = static_cast<int64_t*>(win[3]->mutable_data_ptr()) + c0;
   a.positions_out_stride = win[3]->stride(0);
-  a.ends = static_cast<const uint8_t*>(ends->const_data_ptr());
-  a.ends_stride = ends->stride(0);
-  a.ends_out = static_cast<uint8_t*>(win[4]->mutable_data_ptr()) + c0;
-  a.ends_out_stride = win[4]->stride(0);
-  return failed(address<RotateFn>(args[0])(address<const logkv_rope_t*>(args[1]), &a,
-                                           c10::cuda::getCurrentCUDAStream().stream()));
+  if (ends) {
+    a.ends = static_cast<const uint8_t*>(ends->const_data_ptr());
+    a.ends_stride = ends->stride(0);
+    a.ends_out = static_cast<uint8_t*>(win[4]->mutable_data_ptr()) + c0;
+    a.ends_out_stride = win[4]->stride(0);
+  }
+  try {
+    at::Tensor out;
+    if (q) {
+      out = at::empty({B, q->size(1), T, D}, like.options().requires_grad(false));
+      rotate_part(a.parts[2], *q, &out, nullptr);
+    }
+    const int rc = address<RotateFn>(args[0])(address<const logkv_rope_t*>(args[1]), &a,
+                                              c10::cuda::getCurrentCUDAStream().stream());
+    return rc || !q ? failed(rc) : THPVariable_Wrap(out);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
 }
 
 // A row's number: a Python number for all rows, or a contiguous [lead] tensor of `type`.

@@ -161,8 +161,10 @@ template <typename T, typename C, int VN>
 static int launch_rotate(RotateGeo g, const logkv_rotate_args_t& a, cudaStream_t st) {
   g.units = g.n / 2 / VN + (a.dim - g.n) / VN;
   const long long items = (long long)a.batch * a.tokens * g.units;
-  // Heads per thread: all of them once the tokens alone fill the SMs.
-  const long long want = 148LL * 1024;
+  // Heads per thread: all of them once the tokens alone make 512 threads per SM, fewer before that.  2048 tokens of 24
+  // heads of 128 in us: 9.0 with 2048 threads per SM (a head each, its table entries as many bytes as its own), 8.1
+  // with 1024, 6.8 with 512, 7.8 with 256.
+  const long long want = 148LL * 512;
   const int chunks = (int)std::min<long long>(g.heads, std::max(1LL, want / items));
   g.chunk = (g.heads + chunks - 1) / chunks;
   const long long blocks = (items + kRotateThreads - 1) / kRotateThreads;

@@ -930,62 +930,64 @@ __global__ void __launch_bounds__(kShareWarps * 32, ShareF32Shape<D>::CTAS)
 
 // ---------------------------------------------------------------- combine
 // WPR warps per output row (1 or 4): each joins its share of the row's partials (the shared splits, then the own
-// ones), 32 at a time (lane s holds partial s's m and l; the O loads of 4 or 16 in flight), then the warps in
-// order.  TS: the key tile of the kernel that wrote the shared partials.
+// ones), NB at a time with all of their loads in flight, then the warps in order.  TS: the key tile of the kernel that
+// wrote the shared partials.  What does not depend on the attention kernel (this row's partials and their places) is
+// worked out before the wait for it.
 template <typename T, int D, int TS, int WPR>
 __global__ void __launch_bounds__(128) share_combine_kernel(ShareGeo a, logkv_prefix_t pre, const float* part, T* out) {
-  constexpr int PER = (D + 127) / 128, NB = WPR > 1 ? 16 : 4;
+  constexpr int PER = (D + 127) / 128, NB = D > 128 ? 4 : 8;
   __shared__ float sh[4][2 + D];
-  pdl_entry();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
   const size_t row = (size_t)blockIdx.x * (4 / WPR) + warp / WPR;
-  if (WPR == 1 && row >= (size_t)a.B * a.H * a.T) return;
-  const int bh = (int)(row / a.T), b = bh / a.H / a.W * a.W, g = bh % a.H / a.rf;
-  const int shared = share_splits(a, (share_prefix_length(pre, b * a.G + g) + TS - 1) / TS + (a.w0 + TS - 1) / TS, TS);
+  const bool live = WPR > 1 || row < (size_t)a.B * a.H * a.T;
+  int shared = 0;
+  if (live) {
+    const int bh = (int)(row / a.T), b = bh / a.H / a.W * a.W, g = bh % a.H / a.rf;
+    shared = share_splits(a, (share_prefix_length(pre, b * a.G + g) + TS - 1) / TS + (a.w0 + TS - 1) / TS, TS);
+  }
   const int ns = shared + a.nown, skip = a.nsplit - shared;   // partials; unused slots between the two kinds
   const size_t stride = (size_t)a.B * a.H * a.T * (D + 4);
   const float* p0 = part + row * (D + 4);
   auto at = [&](int s) { return p0 + (size_t)(s < shared ? s : s + skip) * stride; };
+  pdl_entry();
+  if (!live) return;
   float m = -INFINITY, l = 0.f;
   float4 o[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   const int share = (ns + WPR - 1) / WPR, end = min(ns, (sub + 1) * share);
-  for (int s0 = sub * share; s0 < end; s0 += 32) {
-    const int cnt = min(32, end - s0);
-    const float2 ml = lane < cnt ? *reinterpret_cast<const float2*>(at(s0 + lane)) : make_float2(-INFINITY, 0.f);
-    float mc = ml.x;
+  for (int s0 = sub * share; s0 < end; s0 += NB) {
+    float2 ml[NB];
+    float4 v[NB][PER];
 #pragma unroll
-    for (int off = 16; off; off >>= 1) mc = fmaxf(mc, __shfl_xor_sync(0xffffffffu, mc, off));
-    const float mn = fmaxf(m, mc), al = m == -INFINITY ? 0.f : exp2f(m - mn);
-    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
-    float lw = ml.y * w;
+    for (int s = 0; s < NB; ++s) {
+      const bool in = s0 + s < end;
+      const float* p = at(in ? s0 + s : s0);
+      ml[s] = in ? *reinterpret_cast<const float2*>(p) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-    for (int off = 16; off; off >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, off);
-    l = l * al + lw;
+      for (int k = 0; k < PER; ++k) {
+        const int c = 4 * (lane + 32 * k);
+        v[s][k] = in && c < D ? *reinterpret_cast<const float4*>(p + 4 + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    float mn = m;
+#pragma unroll
+    for (int s = 0; s < NB; ++s) mn = fmaxf(mn, ml[s].x);
+    const float al = m == -INFINITY ? 0.f : exp2f(m - mn);
+    l *= al;
     m = mn;
 #pragma unroll
     for (int k = 0; k < PER; ++k) o[k] = make_float4(o[k].x * al, o[k].y * al, o[k].z * al, o[k].w * al);
-    for (int t0 = 0; t0 < cnt; t0 += NB) {
-      float4 v[NB][PER];
 #pragma unroll
-      for (int s = 0; s < NB; ++s)
+    for (int s = 0; s < NB; ++s) {
+      const float w = ml[s].x == -INFINITY ? 0.f : exp2f(ml[s].x - mn);
+      l = fmaf(ml[s].y, w, l);
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          const int c = 4 * (lane + 32 * k);
-          v[s][k] = t0 + s < cnt && c < D ? *reinterpret_cast<const float4*>(at(s0 + t0 + s) + 4 + c)
-                                          : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-      for (int s = 0; s < NB; ++s) {
-        const float ws = __shfl_sync(0xffffffffu, w, (t0 + s) & 31);
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          o[k].x = fmaf(v[s][k].x, ws, o[k].x);
-          o[k].y = fmaf(v[s][k].y, ws, o[k].y);
-          o[k].z = fmaf(v[s][k].z, ws, o[k].z);
-          o[k].w = fmaf(v[s][k].w, ws, o[k].w);
-        }
+      for (int k = 0; k < PER; ++k) {
+        o[k].x = fmaf(v[s][k].x, w, o[k].x);
+        o[k].y = fmaf(v[s][k].y, w, o[k].y);
+        o[k].z = fmaf(v[s][k].z, w, o[k].z);
+        o[k].w = fmaf(v[s][k].w, w, o[k].w);
       }
     }
   }
@@ -1058,8 +1060,9 @@ static SharePlan share_plan(const logkv_layout_t& l, const logkv_shared_args_t& 
   // A CTA's start weighs as much as some 250 keys.  Measured with 1 to 8 splits of 64 shared lanes (8.0K keys) beside
   // 512 own ones (242 keys): 129, 81, 60, 61, 74, 66, 68 us for 1, 2, 3, 4, 5, 6, 8; this gives 3.
   p.own_work = own_ctas * p.nown * (own_keys / p.nown + 250);
-  const int units = (prefix_capacity + x.window_from) / ts + 2;
-  p.nsplit = (int)std::max(1LL, std::min<long long>(p.slots / shared_ctas, units / p.upw));
+  // The grid holds the splits of a full prefix; a shorter one leaves some unused.
+  const long long units = (prefix_capacity + x.window_from) / ts + 2, work = units * ts * shared_ctas;
+  p.nsplit = (int)std::max(1LL, std::min(p.slots * work / (work + p.own_work) / shared_ctas, units / p.upw));
   return p;
 }
 
@@ -1086,7 +1089,9 @@ static void launch_share_combine(const ShareGeo& a, const logkv_prefix_t& pre, c
                                  cudaStream_t st) {
   const size_t rows = (size_t)a.B * a.H * a.T;
   T* o = static_cast<T*>(out);
-  if (a.nsplit + a.nown > 8)
+  // Four warps to a row where there are many partials and few rows: 64 rows of 32 partials 3 us less; with 1920 rows
+  // of 13 the extra warps only wait (27 us in all against 17).
+  if (a.nsplit + a.nown > 8 && rows <= 148 * 8)
     launch_pdl(share_combine_kernel<T, D, TS, 4>, dim3((unsigned)rows), 128, 0, st, a, pre, part, o);
   else
     launch_pdl(share_combine_kernel<T, D, TS, 1>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, a, pre, part, o);

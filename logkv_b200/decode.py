@@ -94,6 +94,19 @@ class LogKVDecoder:
         the sequence) and puts the token into the pending slot.  ``layout`` is log_kv_rotate's, all else step's."""
         mode = rotary.check_layout(layout)
         cache = self.cache
+        slot = self._slot(shared)
+        at = slice(slot, slot + 1)
+        call = rotary.native(cache)
+        if call is not None and q.dim() == 4 and q.size(2) == 1 and (slot == 0 or (input_pos is not None) == self._has_pos):
+            # A call like one before: checks and launch in the host binding; None: not covered there.
+            turned = call.append(call.fn, call.rope, call.status, self._k, self._kr, self._v, self._pos, self._ends, k_raw,
+                                 v, input_pos, span_ends_device, cache.token_count + slot, slot, mode, q)
+            if turned is not None:
+                if type(turned) is int:
+                    _lib.check(turned, "logkv_rotate")
+                self._keep(slot, input_pos, span_ends)
+                return self._finish(slot, turned, self._k[:, :, at], self._v[:, :, at], span_ends, span_ends_device, out,
+                                    shared)
         B, G, D, dt, dev = cache.batch_size, cache.n_groups, cache.k_dim, self._k.dtype, self._k.device
         if q.dim() != 4 or q.size(1) < 1 or q.size(1) % G or q.shape != (B, q.size(1), 1, D) or q.dtype != dt:
             raise ValueError(f"q must be [{B}, H, 1, {D}] in the cache dtype, H a multiple of {G}")
@@ -110,9 +123,7 @@ class LogKVDecoder:
             if tuple(ends.shape) != (B, 1):
                 raise ValueError("AlphaLogKV span boundaries must match the input batch and token count")
             ends = ends.to(device=dev, dtype=torch.uint8)
-        slot = self._slot(shared)
         self._keep(slot, positions, span_ends)
-        at = slice(slot, slot + 1)
         k, v1 = self._k[:, :, at], self._v[:, :, at]
         with _lib.on_device(dev):
             turned = q.new_empty((B, q.size(1), 1, D))

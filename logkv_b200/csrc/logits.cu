@@ -54,6 +54,9 @@ __device__ __forceinline__ void visit_history(const logkv_logits_args_t& a, int 
   }
 }
 
+constexpr int kBiasBits = 8192;
+__device__ __forceinline__ unsigned bias_hash(int v) { return (unsigned)v * 2654435761u >> 19; }
+
 // A part's place in shared memory.
 struct LogitsGeo {
   int part;       // tokens of a CTA, a multiple of 32
@@ -108,6 +111,7 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
   constexpr int VN = 16 / (int)sizeof(T), U = 4;                 // vectors of a thread in flight
   extern __shared__ unsigned smem[];
   __shared__ int warp_sums[LT / 32];
+  __shared__ unsigned biased[kBiasBits / 32], again[kBiasBits / 32];   // hashes of the biased tokens, met twice or more
   const int words = g.listed ? g.part / 32 : 0;
   unsigned* touched = smem;                                       // [words] bits of the history's tokens
   unsigned* before = touched + words;                             // [words] set bits in front of a word
@@ -167,17 +171,39 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
     }
   } else {
     const int tid = threadIdx.x - kLogitsThreads, lane = tid & 31;
+    // The thread's first bias entry and its logit, asked for before the history.
+    auto bias_token = [&](int i) {
+      const long long v = load_int(a.bias_tokens, a.bias_wide, r * a.bias_tokens_stride + i);
+      return v >= begin && v < end ? (int)v : -1;
+    };
+    int v_own = -1;
+    float b_own = 0.f, x_own = 0.f;
+    if (tid < a.bias_count) {
+      v_own = bias_token(tid);
+      b_own = a.bias_values[r * a.bias_values_stride + tid];
+      if (v_own >= 0) x_own = Elem<T>::load(x + v_own);
+    }
     auto number = [&](int l) {   // of the part's touched token l
       return before[l >> 5] + __popc(touched[l >> 5] & ((1u << (l & 31)) - 1));
     };
+    if (a.bias_count)
+      for (int i = tid; i < kBiasBits / 32; i += LT) biased[i] = again[i] = 0u;
+    for (int i = tid; i < words; i += LT) touched[i] = 0u;
+    for (int i = tid; i < g.listed; i += LT) count[i] = 0u;
+    list_sync<LT>();
+    for (int i = tid; i < a.bias_count; i += LT) {
+      const int v = i == tid ? v_own : bias_token(i);
+      bt[i] = v;
+      bz[i] = i == tid ? b_own : a.bias_values[r * a.bias_values_stride + i];
+      if (v < 0) continue;
+      const unsigned h = bias_hash(v), bit = 1u << (h & 31);
+      if (atomicOr(&biased[h >> 5], bit) & bit) atomicOr(&again[h >> 5], bit);
+    }
     if (g.listed) {
       const long long len = a.lengths ? load_int(a.lengths, a.lengths_wide, r) : a.length;
       const int length = (int)max(0LL, min(len, (long long)a.history_len));
       const long long pro = a.prompts ? load_int(a.prompts, a.prompts_wide, r) : a.prompt;
       const int prompt = (int)max(0LL, min(pro, (long long)length));
-      for (int i = tid; i < words; i += LT) touched[i] = 0u;
-      for (int i = tid; i < g.listed; i += LT) count[i] = 0u;
-      list_sync<LT>();
       visit_history<LT>(a, r, length, begin, end, tid, [&](int, int v) {
         const unsigned bit = 1u << ((v - v0) & 31);
         unsigned* word = &touched[(v - v0) >> 5];
@@ -211,13 +237,8 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
       });
     }
     if (a.bias_count) {
-      // Biased tokens are few: the thread of a token's first entry works out its value.  In place the copy leaves the
-      // logit as it was, but for a masked one, which is -inf in the end either way.
-      for (int i = tid; i < a.bias_count; i += LT) {
-        const long long v = load_int(a.bias_tokens, a.bias_wide, r * a.bias_tokens_stride + i);
-        bt[i] = v >= begin && v < end ? (int)v : -1;
-        bz[i] = a.bias_values[r * a.bias_values_stride + i];
-      }
+      // The thread of a token's first entry works out its value; entries are compared only where hashes meet.  In place
+      // the copy leaves the logit as it was, but for a masked one, which is -inf in the end either way.
       list_sync<LT>();
       constexpr int PER = LOGKV_LOGITS_MAX_BIAS / LT;
       float z[PER];
@@ -226,14 +247,15 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
       for (int k = 0; k < PER; ++k) {
         const int i = tid + k * LT, v = i < a.bias_count ? bt[i] : -1;
         bool first = v >= 0;
-        for (int j = 0; j < i && first; ++j) first = bt[j] != v;
+        const bool repeat = first && again[bias_hash(v) >> 5] >> (bias_hash(v) & 31) & 1;
+        for (int j = 0; repeat && j < i && first; ++j) first = bt[j] != v;
         z[k] = 0.f;
         if (!first) continue;
         mine |= 1u << k;
         float sum = bz[i];
-        for (int j = i + 1; j < a.bias_count; ++j)
+        for (int j = i + 1; repeat && j < a.bias_count; ++j)
           if (bt[j] == v) sum += bz[j];
-        z[k] = Elem<T>::load(x + v);
+        z[k] = k == 0 ? x_own : Elem<T>::load(x + v);
         const int l = v - v0;
         if (g.listed && touched[l >> 5] >> (l & 31) & 1) z[k] = adjust(z[k], count[number(l)]);
         z[k] += sum;
@@ -282,11 +304,15 @@ static int launch_adjust(const logkv_logits_args_t& a, cudaStream_t st) {
   auto bytes = [&](const LogitsGeo& g) {
     return (g.listed ? (size_t)g.part / 32 * 8 : 0) + (size_t)g.listed * 8 + (size_t)a.bias_count * 8;
   };
-  // Parts: one wave of CTAs, and up to three where a part is still 16 times as long as the history that each of a
-  // row's CTAs goes over.  512 rows of 151936 (history 1024): 62.4 us in one wave, 58.5 in three; 145 rows of 50021
-  // (history 4097): 18 in one wave, 26 in two, 33 in three.
+  // Parts: one wave of CTAs, and up to three where nothing but the copy is to do, or where a part is still 16 times as
+  // long as the history that each of a row's CTAs goes over, and of 64 KB, beside which going over a short history or
+  // the biases does not show.  512 rows of 151936 bf16 (history 1024): 62.4 us in one wave, 58.5 in three; 145 rows of
+  // 50021 float32: history 4097 18 in one wave, 26 in two, 33 in three; 64 8.7 in one, 13.5 in three; the copy alone
+  // 9.7 in one, 7.7 in three.
   const long long wave = 148 * logits_ctas(LT);
-  const long long room = a.history ? a.vocab / (16LL * a.history_len) : a.vocab;
+  long long room = a.vocab;
+  if (a.history || a.bias_count) room = room * (long long)sizeof(T) >> 16;
+  if (a.history) room = std::min(room, a.vocab / (16LL * a.history_len));
   LogitsGeo g = geo(std::max({1LL, wave / a.rows, std::min(3 * wave / a.rows, room)}));
   for (long long parts = 2; bytes(g) > kMost; parts *= 2) g = geo(parts);
   if (const int e = smem_limit_once<kern>(kMost)) return e;

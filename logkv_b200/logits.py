@@ -135,6 +135,8 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt=0, repetition=1.
     elif out is not logits and (out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev
                                 or not out.is_contiguous()):
         raise ValueError(f"out must be logits itself, or contiguous {list(logits.shape)} {logits.dtype} on {dev}")
+    elif out is not logits and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() and rows:
+        raise ValueError("out must be logits itself or have memory of its own")
     elif out is logits and any(n > 1 and s < V for n, s in zip(lead, logits.stride())):
         raise ValueError("logits adjusted in place must not share memory between rows")
     if not rows:

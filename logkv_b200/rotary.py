@@ -31,7 +31,7 @@ def check_positions(cache, input_pos, T: int):
         return None
     B, dev = cache.batch_size, cache.recent_pos.device
     p = input_pos if isinstance(input_pos, torch.Tensor) else torch.as_tensor(input_pos)
-    if p.dtype != torch.int32 and p.dtype != torch.int64:
+    if p.dtype != torch.int32 and p.dtype != torch.int64 and p.numel():
         raise ValueError(f"input_pos must hold integers (int32 or int64), got {p.dtype}")
     if p.shape != (T,) and p.shape != (B, T):
         raise ValueError(f"input_pos must be [{T}] or [{B}, {T}], got {tuple(p.shape)}")

@@ -139,6 +139,12 @@ def test_strides_and_places(dtype):
     x, kw = inputs(2, 2, 640, 30, 4, dtype, 9)
     a = check(x.transpose(1, 2).contiguous().transpose(1, 2), **kw)  # vocabulary not contiguous
     assert torch.equal(a.nan_to_num(), check(x, **kw).nan_to_num())
+    from logkv_b200 import adjust_logits
+    room = torch.zeros(2, 2, 1280, dtype=dtype, device="cuda")
+    with pytest.raises(ValueError, match="memory of its own"):
+        adjust_logits(room[..., 640:], out=room.view(-1)[:2560].view(2, 2, 640))
+    with pytest.raises(ValueError, match="share memory"):
+        adjust_logits(one := room[:1, :1, :640].expand(2, 2, 640), out=one)
     grown = torch.full((2, 2, 90), 3, dtype=torch.int32, device="cuda")   # a history buffer with room
     grown[..., :30] = kw["history"]
     assert torch.equal(check(x, **{**kw, "history": grown[..., :30]}).nan_to_num(), a.nan_to_num())

@@ -35,27 +35,24 @@ __device__ __forceinline__ void list_sync() {
   asm volatile("bar.sync 1, %0;\n" ::"n"(LT) : "memory");
 }
 
-// Tokens of a row's history that lie in [begin, end), kInFlight loads of each thread under way: visit(index, token).
+// A row's history, kInFlight tokens of a thread at a time: visit(index of the first, l) with the tokens' places in
+// the part [begin, end) from v0 on, -1 for others; token k's index is the first's + k LT.
+constexpr int kInFlight = 8;
 template <int LT, typename Visit>
-__device__ __forceinline__ void visit_history(const logkv_logits_args_t& a, int r, int length, int begin, int end,
+__device__ __forceinline__ void visit_history(const logkv_logits_args_t& a, int r, int length, int v0, int begin, int end,
                                               int tid, Visit visit) {
-  constexpr int kInFlight = 8;
   const long long h0 = (long long)r * a.history_stride;
   for (int i0 = tid; i0 < length; i0 += kInFlight * LT) {
-    long long v[kInFlight];
+    int l[kInFlight];
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k) {
       const int i = i0 + k * LT;
-      v[k] = i < length ? load_int(a.history, a.history_wide, h0 + i) : -1;
+      const long long v = i < length ? load_int(a.history, a.history_wide, h0 + i) : -1;
+      l[k] = v >= begin && v < end ? (int)v - v0 : -1;
     }
-#pragma unroll
-    for (int k = 0; k < kInFlight; ++k)
-      if (v[k] >= begin && v[k] < end) visit(i0 + k * LT, (int)v[k]);
+    visit(i0, l);
   }
 }
-
-constexpr int kBiasBits = 8192;
-__device__ __forceinline__ unsigned bias_hash(int v) { return (unsigned)v * 2654435761u >> 19; }
 
 // A part's place in shared memory.
 struct LogitsGeo {
@@ -109,16 +106,17 @@ template <typename T, bool SHIFTED, int LT>
 __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
     adjust_logits_kernel(logkv_logits_args_t a, LogitsGeo g) {
   constexpr int VN = 16 / (int)sizeof(T), U = 4;                 // vectors of a thread in flight
-  extern __shared__ unsigned smem[];
+  extern __shared__ __align__(16) unsigned smem[];
   __shared__ int warp_sums[LT / 32];
-  __shared__ unsigned biased[kBiasBits / 32], again[kBiasBits / 32];   // hashes of the biased tokens, met twice or more
-  const int words = g.listed ? g.part / 32 : 0;
-  unsigned* touched = smem;                                       // [words] bits of the history's tokens
-  unsigned* before = touched + words;                             // [words] set bits in front of a word
-  int* token = reinterpret_cast<int*>(before + words);            // [listed] by number, in index order
+  const int entries = (a.bias_count + 3) / 4 * 4, words = g.part / 32;
+  int* bt = reinterpret_cast<int*>(smem);                         // [entries] biased tokens, -1: not this part's or again
+  float* bz = reinterpret_cast<float*>(bt + entries);             // [entries] biases, then adjusted logits
+  unsigned* again = reinterpret_cast<unsigned*>(bz + entries);    // [words] bits of tokens with several biases
+  unsigned* before = again + (entries ? words : 0);               // [words] bits of the biased tokens; later on
+                                                                  // the touched ones in front of a word
+  unsigned* touched = before + words;                             // [words] bits of the history's tokens
+  int* token = reinterpret_cast<int*>(touched + words);           // [listed] by number, in index order
   unsigned* count = reinterpret_cast<unsigned*>(token + g.listed);   // [listed]
-  int* bt = reinterpret_cast<int*>(count + g.listed);             // [bias_count] tokens, -1: not this part's or again
-  float* bz = reinterpret_cast<float*>(bt + a.bias_count);        // [bias_count] biases, then adjusted logits
   pdl_entry();
   const int r = blockIdx.y, n = r / a.width, w = r % a.width;
   const T* x = static_cast<const T*>(a.logits) + n * a.n_stride + w * a.w_stride;
@@ -186,28 +184,33 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
     auto number = [&](int l) {   // of the part's touched token l
       return before[l >> 5] + __popc(touched[l >> 5] & ((1u << (l & 31)) - 1));
     };
-    if (a.bias_count)
-      for (int i = tid; i < kBiasBits / 32; i += LT) biased[i] = again[i] = 0u;
-    for (int i = tid; i < words; i += LT) touched[i] = 0u;
+    for (int i = tid; i < words; i += LT) {
+      if (entries) again[i] = before[i] = 0u;
+      if (g.listed) touched[i] = 0u;
+    }
     for (int i = tid; i < g.listed; i += LT) count[i] = 0u;
     list_sync<LT>();
-    for (int i = tid; i < a.bias_count; i += LT) {
-      const int v = i == tid ? v_own : bias_token(i);
+    for (int i = tid; i < entries; i += LT) {
+      const int v = i == tid ? v_own : i < a.bias_count ? bias_token(i) : -1;
       bt[i] = v;
-      bz[i] = i == tid ? b_own : a.bias_values[r * a.bias_values_stride + i];
+      bz[i] = i == tid ? b_own : i < a.bias_count ? a.bias_values[r * a.bias_values_stride + i] : 0.f;
       if (v < 0) continue;
-      const unsigned h = bias_hash(v), bit = 1u << (h & 31);
-      if (atomicOr(&biased[h >> 5], bit) & bit) atomicOr(&again[h >> 5], bit);
+      const int l = v - v0;
+      const unsigned bit = 1u << (l & 31);
+      if (atomicOr(&before[l >> 5], bit) & bit) atomicOr(&again[l >> 5], bit);
     }
     if (g.listed) {
       const long long len = a.lengths ? load_int(a.lengths, a.lengths_wide, r) : a.length;
       const int length = (int)max(0LL, min(len, (long long)a.history_len));
       const long long pro = a.prompts ? load_int(a.prompts, a.prompts_wide, r) : a.prompt;
       const int prompt = (int)max(0LL, min(pro, (long long)length));
-      visit_history<LT>(a, r, length, begin, end, tid, [&](int, int v) {
-        const unsigned bit = 1u << ((v - v0) & 31);
-        unsigned* word = &touched[(v - v0) >> 5];
-        if (!(*reinterpret_cast<volatile unsigned*>(word) & bit)) atomicOr(word, bit);   // frequent tokens once
+      visit_history<LT>(a, r, length, v0, begin, end, tid, [&](int, const int(&l)[kInFlight]) {
+        unsigned word[kInFlight];   // frequent tokens are set once
+#pragma unroll
+        for (int k = 0; k < kInFlight; ++k) word[k] = l[k] < 0 ? ~0u : *static_cast<volatile unsigned*>(&touched[l[k] >> 5]);
+#pragma unroll
+        for (int k = 0; k < kInFlight; ++k)
+          if (!(word[k] >> (l[k] & 31) & 1)) atomicOr(&touched[l[k] >> 5], 1u << (l[k] & 31));
       });
       list_sync<LT>();
       const int per = (words + LT - 1) / LT, w0 = min(words, tid * per), w1 = min(words, w0 + per);
@@ -229,34 +232,50 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
         at += __popc(touched[i]);
       }
       list_sync<LT>();
-      visit_history<LT>(a, r, length, begin, end, tid, [&](int i, int v) {
-        const int k = number(v - v0);
-        token[k] = v;   // the same from every thread that meets the token
-        if (i < prompt) atomicOr(&count[k], kSeen);
-        else atomicAdd(&count[k], 1u);
+      visit_history<LT>(a, r, length, v0, begin, end, tid, [&](int i, const int(&l)[kInFlight]) {
+        int n[kInFlight];
+#pragma unroll
+        for (int k = 0; k < kInFlight; ++k) n[k] = l[k] < 0 ? 0 : number(l[k]);
+#pragma unroll
+        for (int k = 0; k < kInFlight; ++k)
+          if (l[k] >= 0) {
+            token[n[k]] = v0 + l[k];   // the same from every thread that meets the token
+            if (i + k * LT < prompt) atomicOr(&count[n[k]], kSeen);
+            else atomicAdd(&count[n[k]], 1u);
+          }
       });
     }
     if (a.bias_count) {
-      // The thread of a token's first entry works out its value; entries are compared only where hashes meet.  In place
-      // the copy leaves the logit as it was, but for a masked one, which is -inf in the end either way.
+      // The thread of a token's first entry works out its value, with the other entries' biases where it has several.
+      // In place the copy leaves the logit as it was, but for a masked one, which is -inf in the end either way.
       list_sync<LT>();
       constexpr int PER = LOGKV_LOGITS_MAX_BIAS / LT;
       float z[PER];
       unsigned mine = 0;
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = tid + k * LT, v = i < a.bias_count ? bt[i] : -1;
+        const int i = tid + k * LT, v = i < a.bias_count ? bt[i] : -1, l = v - v0;
         bool first = v >= 0;
-        const bool repeat = first && again[bias_hash(v) >> 5] >> (bias_hash(v) & 31) & 1;
-        for (int j = 0; repeat && j < i && first; ++j) first = bt[j] != v;
         z[k] = 0.f;
         if (!first) continue;
-        mine |= 1u << k;
         float sum = bz[i];
-        for (int j = i + 1; repeat && j < a.bias_count; ++j)
-          if (bt[j] == v) sum += bz[j];
+        if (again[l >> 5] >> (l & 31) & 1) {
+          sum = 0.f;
+#pragma unroll 4
+          for (int j = 0; j < entries; j += 4) {
+            const int4 t = *reinterpret_cast<const int4*>(bt + j);
+            if (t.x != v && t.y != v && t.z != v && t.w != v) continue;
+            const float4 b = *reinterpret_cast<const float4*>(bz + j);
+            first &= (t.x != v || j >= i) && (t.y != v || j + 1 >= i) && (t.z != v || j + 2 >= i) && (t.w != v || j + 3 >= i);
+            sum += t.x == v ? b.x : 0.f;
+            sum += t.y == v ? b.y : 0.f;
+            sum += t.z == v ? b.z : 0.f;
+            sum += t.w == v ? b.w : 0.f;
+          }
+          if (!first) continue;
+        }
+        mine |= 1u << k;
         z[k] = k == 0 ? x_own : Elem<T>::load(x + v);
-        const int l = v - v0;
         if (g.listed && touched[l >> 5] >> (l & 31) & 1) z[k] = adjust(z[k], count[number(l)]);
         z[k] += sum;
         if (mask && !(mask_bits(mask, v, 1, a.vocab) & 1)) z[k] = -INFINITY;
@@ -302,7 +321,9 @@ static int launch_adjust(const logkv_logits_args_t& a, cudaStream_t st) {
     return g;
   };
   auto bytes = [&](const LogitsGeo& g) {
-    return (g.listed ? (size_t)g.part / 32 * 8 : 0) + (size_t)g.listed * 8 + (size_t)a.bias_count * 8;
+    const size_t words = g.part / 32, entries = (a.bias_count + 3) / 4 * 4;
+    return 4 * (entries * 2 + (entries ? words : 0) + (entries || g.listed ? words : 0) +
+                (g.listed ? words + 2 * (size_t)g.listed : 0));
   };
   // Parts: one wave of CTAs, and up to three where nothing but the copy is to do, or where a part is still 16 times as
   // long as the history that each of a row's CTAs goes over, and of 64 KB, beside which going over a short history or

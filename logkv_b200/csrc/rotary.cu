@@ -5,8 +5,8 @@
 // pairs) of the rotated features for a plane each: (a, b) -> (a c - b s, b c + a s).  Every element is read
 // once and written once, so HBM bounds long chunks and the launch bounds single tokens.
 //
-// A thread owns one unit of a token: VN features of the first half with their VN partners (or VN features
-// behind the rotated ones).  It reads its table entries once and walks over the heads of all tensors with
+// A thread owns one unit of a token: VN features of the first half with their VN partners, or features behind the
+// rotated ones (VN, and from the next 16-byte boundary on VW).  It reads its table entries once and walks over the heads of all tensors with
 // them, kBatch heads' loads in flight; the heads are cut into chunks when tokens are few.
 #include <algorithm>
 
@@ -56,10 +56,27 @@ struct RotateGeo {
   const void* sin;
   int table_rows, n;   // positions in the tables, rotated features
   int heads, chunk;    // heads of all parts, heads per thread
-  int units;           // units of a token: n / 2 / VN rotated ones and (dim - n) / VN others
+  int units;           // units of a token: n / 2 / VN rotated ones, then the others up to `wide`, then those behind
+  int wide;            // first feature that is copied in units of VW
 };
 
-template <typename T, typename C, int VN>
+template <typename T, int VN>
+__device__ __forceinline__ void copy_heads(const logkv_rotate_part_t& x, const T* src, T* out, T* raw, int at, int h0, int h1) {
+  for (int h = h0; h < h1; h += kBatch) {
+    Unit<T, VN> v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (h + i < h1) v[i].load(src + (h + i) * x.src_strides[1] + at);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (h + i >= h1) break;
+      if (raw) v[i].store(raw + (h + i) * x.raw_strides[1] + at);
+      if (x.rotate) v[i].store(out + (h + i) * x.rotated_strides[1] + at);
+    }
+  }
+}
+
+template <typename T, typename C, int VN, int VW>
 __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(RotateGeo g, logkv_rotate_args_t a) {
   pdl_entry();
   const long long item = (long long)blockIdx.x * kRotateThreads + threadIdx.x;
@@ -77,7 +94,8 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(RotateGeo g, log
   const int half = g.n >> 1, pairs = half / VN;
   const bool turned = u < pairs;
   // First element of the unit and of its partner, as read and as written.
-  const int lo = turned ? u * VN : g.n + (u - pairs) * VN, hi = lo + half;
+  const int mid = (g.wide - g.n) / VN;
+  const int lo = turned ? u * VN : u < pairs + mid ? g.n + (u - pairs) * VN : g.wide + (u - pairs - mid) * VW, hi = lo + half;
   const int in0 = turned && a.interleaved ? 2 * lo : lo, in1 = turned && a.interleaved ? in0 + VN : hi;
   if (u == 0 && blockIdx.y == 0) {
     if (a.positions_out) a.positions_out[b * a.positions_out_stride + t] = pos;
@@ -103,11 +121,15 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(RotateGeo g, log
     const int h0 = max(first - base, 0), h1 = min(last - base, x.heads);
     base += x.heads;
     if (h0 >= h1) continue;
-    const bool rot = turned && x.rotate, mix = rot && a.interleaved;
-    const int r0 = rot ? in0 : lo, r1 = rot ? in1 : hi;   // values are copied in place
     const T* src = static_cast<const T*>(x.src) + b * x.src_strides[0] + t * x.src_strides[2];
     T* out = static_cast<T*>(x.rotated) + (x.rotated ? b * x.rotated_strides[0] + t * x.rotated_strides[2] : 0);
     T* raw = static_cast<T*>(x.raw) + (x.raw ? b * x.raw_strides[0] + t * x.raw_strides[2] : 0);
+    if (VN < VW && u >= pairs + mid) {   // (units of one size stay in one loop: their warps do not diverge)
+      copy_heads<T, VW>(x, src, out, raw, lo, h0, h1);
+      continue;
+    }
+    const bool rot = turned && x.rotate, mix = rot && a.interleaved;
+    const int r0 = rot ? in0 : lo, r1 = rot ? in1 : hi;   // values are copied in place
     for (int h = h0; h < h1; h += kBatch) {
       Unit<T, VN> va[kBatch], vb[kBatch];
 #pragma unroll
@@ -157,9 +179,10 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(RotateGeo g, log
   }
 }
 
-template <typename T, typename C, int VN>
+template <typename T, typename C, int VN, int VW>
 static int launch_rotate(RotateGeo g, const logkv_rotate_args_t& a, cudaStream_t st) {
-  g.units = g.n / 2 / VN + (a.dim - g.n) / VN;
+  g.wide = (g.n + VW - 1) / VW * VW;
+  g.units = g.n / 2 / VN + (g.wide - g.n) / VN + (a.dim - g.wide) / VW;
   const long long items = (long long)a.batch * a.tokens * g.units;
   // Heads per thread: all of them once the tokens alone make 512 threads per SM, fewer before that.  2048 tokens of 24
   // heads of 128 in us: 9.0 with 2048 threads per SM (a head each, its table entries as many bytes as its own), 8.1
@@ -169,20 +192,20 @@ static int launch_rotate(RotateGeo g, const logkv_rotate_args_t& a, cudaStream_t
   g.chunk = (g.heads + chunks - 1) / chunks;
   const long long blocks = (items + kRotateThreads - 1) / kRotateThreads;
   if (blocks > 0x7fffffffLL || g.heads > 65535) return LOGKV_E_SHAPE;
-  launch_pdl(rotate_kernel<T, C, VN>, dim3((unsigned)blocks, (g.heads + g.chunk - 1) / g.chunk), kRotateThreads, 0, st, g,
-             a);
+  launch_pdl(rotate_kernel<T, C, VN, VW>, dim3((unsigned)blocks, (g.heads + g.chunk - 1) / g.chunk), kRotateThreads, 0, st,
+             g, a);
   return launch_status();
 }
 
+// vn: elements of a rotated unit; wide: whether the features behind may go in 16-byte units.
 template <typename T, typename C>
-static int launch_rotate(const RotateGeo& g, const logkv_rotate_args_t& a, int vn, cudaStream_t st) {
-  switch (vn) {
-    case 8:
-      if constexpr (sizeof(T) == 2) return launch_rotate<T, C, 8>(g, a, st);
-    case 4: return launch_rotate<T, C, 4>(g, a, st);
-    case 2: return launch_rotate<T, C, 2>(g, a, st);
-    default: return launch_rotate<T, C, 1>(g, a, st);
-  }
+static int launch_rotate(const RotateGeo& g, const logkv_rotate_args_t& a, int vn, bool wide, cudaStream_t st) {
+  constexpr int W = 16 / (int)sizeof(T);
+  if (vn == W) return launch_rotate<T, C, W, W>(g, a, st);
+  if constexpr (W == 8)
+    if (vn == 4) return wide ? launch_rotate<T, C, 4, W>(g, a, st) : launch_rotate<T, C, 4, 4>(g, a, st);
+  if (vn == 2) return wide ? launch_rotate<T, C, 2, W>(g, a, st) : launch_rotate<T, C, 2, 2>(g, a, st);
+  return wide ? launch_rotate<T, C, 1, W>(g, a, st) : launch_rotate<T, C, 1, 1>(g, a, st);
 }
 
 }  // namespace logkv
@@ -200,7 +223,7 @@ extern "C" LOGKV_API int logkv_rotate(const logkv_rope_t* rope, const logkv_rota
   if (a.positions && (reinterpret_cast<uintptr_t>(a.positions) & (a.positions_wide ? 7 : 3))) return LOGKV_E_POINTER;
   if ((reinterpret_cast<uintptr_t>(a.positions_out) & 7) || (a.ends_out && !a.ends)) return LOGKV_E_POINTER;
   const uintptr_t e = esize_of(a.dtype), ce = esize_of(rope->dtype);
-  RotateGeo g{rope->cos, rope->sin, rope->rows, rope->rope_n, 0, 0, 0};
+  RotateGeo g{rope->cos, rope->sin, rope->rows, rope->rope_n, 0, 0, 0, 0};
   // Elements per access: the longest that rows, strides, halves and tables allow.
   uintptr_t bits = 0, tab = rope->rope_n ? reinterpret_cast<uintptr_t>(rope->cos) | reinterpret_cast<uintptr_t>(rope->sin) : 0;
   for (int p = 0; p < a.n_parts; ++p) {
@@ -216,6 +239,7 @@ extern "C" LOGKV_API int logkv_rotate(const logkv_rope_t* rope, const logkv_rota
   }
   if (bits & (e - 1) || tab & (ce - 1)) return LOGKV_E_POINTER;
   int vn = (int)(16 / e);
+  const bool wide = !(bits & 15) && a.dim % vn == 0;
   auto fits = [&](int v) {
     return !(bits & (v * e - 1)) && g.n / 2 % v == 0 && a.dim % v == 0 &&
            !(tab & (std::min<uintptr_t>(16, v * ce) - 1));
@@ -225,6 +249,6 @@ extern "C" LOGKV_API int logkv_rotate(const logkv_rope_t* rope, const logkv_rota
   using B16 = __nv_bfloat16;
   const bool bt = g.n && rope->dtype == LOGKV_DTYPE_BF16;
   if (a.dtype == LOGKV_DTYPE_BF16)
-    return bt ? launch_rotate<B16, B16>(g, a, vn, st) : launch_rotate<B16, float>(g, a, vn, st);
-  return bt ? launch_rotate<float, B16>(g, a, vn, st) : launch_rotate<float, float>(g, a, vn, st);
+    return bt ? launch_rotate<B16, B16>(g, a, vn, wide, st) : launch_rotate<B16, float>(g, a, vn, wide, st);
+  return bt ? launch_rotate<float, B16>(g, a, vn, wide, st) : launch_rotate<float, float>(g, a, vn, wide, st);
 }

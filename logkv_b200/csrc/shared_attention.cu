@@ -23,9 +23,10 @@ struct ShareGeo {
   int nsplit;             // splits of a shared lane in the grid; share_splits() of them are used
   int upw;                // key tiles a split has at least
   int nown;               // splits of an own lane
+  int own_warps;          // warps to an own lane's split: 4, 2 or 1
   int shared_lanes, own_lanes;
   int slots;              // CTAs that run at once
-  long long own_work;     // all own lanes' CTAs in keys, what it takes to start one included
+  long long own_work;     // all own lanes' work in keys, what it takes to start them included
   int tiles, tile_rows;   // row tiles of a shared lane (at most 16 or 128 rows each)
   int own_tiles;          // row tiles of an own lane (16 rows each)
   float scale_log2, mass_log2;   // score = dot * scale_log2 + mass * mass_log2, in the log2 domain
@@ -36,7 +37,8 @@ struct ShareGeo {
 };
 
 // Splits of a shared lane with `units` key tiles (the same value in the attention kernel and the combine): the SMs are
-// divided between the two kinds of lanes by their work, so that both end together.
+// divided between the two kinds of lanes by their work, so that both end together.  64 shared lanes of 8.0K keys beside
+// 512 own ones of 242: 129, 81, 60, 61, 74, 66, 68 us with 1, 2, 3, 4, 5, 6, 8 splits; this gives 3.
 __device__ __forceinline__ int share_splits(const ShareGeo& a, int units, int tile_keys) {
   const int ctas = a.shared_lanes * a.tiles;
   const long long work = (long long)units * tile_keys * ctas;
@@ -48,8 +50,8 @@ __device__ __forceinline__ int share_prefix_length(const logkv_prefix_t& pre, in
   return min(max(pre.length[ln], 0), pre.capacity);
 }
 
-// A CTA's share of the work.  Shared lanes' CTAs come first (lane fastest, then split, so that unused splits are
-// dispatched last among them), then the own lanes'.
+// A warp's share of the work, the same for the warps that share a split.  Shared lanes' CTAs come first (lane fastest,
+// then split, so that unused splits are dispatched last among them), then those of the own lanes.
 struct ShareJob {
   bool own;
   int b, g;        // batch row (the request's first for a shared lane) and group
@@ -58,15 +60,21 @@ struct ShareJob {
   int n0, n1;      // keys of the two segments
   size_t r0;       // first key row of segment 0 (packed prefix, or the window's rows behind w0)
   int ns;          // splits of the lane
+  int warps, sub;  // warps of the split and which of them this is
 };
 
+// GROUPED: own lanes of fewer than four warps.  Code of its own, since what it takes to tell the groups apart costs the
+// calls without them 1 to 2 us.
+template <bool GROUPED>
 __device__ __forceinline__ ShareJob share_job(const ShareGeo& a, const logkv_prefix_t& pre, int tile_keys) {
   ShareJob j;
   int x = blockIdx.x;
-  const int shared = a.shared_lanes * a.nsplit * a.tiles;
+  const int shared = a.shared_lanes * a.nsplit * a.tiles, warp = threadIdx.x >> 5;
   j.own = x >= shared;
   if (j.own) {
-    x -= shared;
+    j.warps = GROUPED ? a.own_warps : 4;
+    j.sub = warp % j.warps;
+    x = (x - shared) * (4 / j.warps) + warp / j.warps;
     const int lane = x % a.own_lanes;
     x /= a.own_lanes;
     j.split = x % a.nown;
@@ -74,12 +82,14 @@ __device__ __forceinline__ ShareJob share_job(const ShareGeo& a, const logkv_pre
     j.b = lane / a.G;
     j.g = lane % a.G;
     j.row0 = x / a.nown * 16;
-    j.NQ = min(16, a.rf * a.T - j.row0);
+    j.NQ = min(16, a.rf * a.T - j.row0);   // the last CTA's warps past the lanes: 0 or less
     j.n0 = a.rcount - a.w0;
     j.n1 = a.Tk;
     j.r0 = ((size_t)j.b * a.G + j.g) * a.rcap + a.w0;
     j.ns = a.nown;
   } else {
+    j.warps = 4;
+    j.sub = warp;
     const int lane = x % a.shared_lanes;
     x /= a.shared_lanes;
     j.split = j.slot = x % a.nsplit;
@@ -95,6 +105,18 @@ __device__ __forceinline__ ShareJob share_job(const ShareGeo& a, const logkv_pre
   }
   return j;
 }
+
+// Key tiles of the split that the warp takes: first, first + warps, ...
+struct ShareTiles {
+  int un, first, n;   // tiles of segment 0; the warp's
+  __device__ __forceinline__ ShareTiles(const ShareJob& j, int ts) {
+    un = (j.n0 + ts - 1) / ts;
+    const int U = un + (j.n1 + ts - 1) / ts;
+    const int u0 = (int)((long long)U * j.split / j.ns), u1 = (int)((long long)U * (j.split + 1) / j.ns);
+    first = u0 + j.sub;
+    n = j.NQ > 0 && u1 > first ? (u1 - first + j.warps - 1) / j.warps : 0;
+  }
+};
 
 // Query row m of a lane: rows are beams x heads x tokens; its flat row of q's and out's [B, H, T].
 __device__ __forceinline__ size_t share_row(const ShareGeo& a, const ShareJob& j, int m) {
@@ -115,19 +137,36 @@ __device__ __forceinline__ float* share_part(float* part, const ShareGeo& a, int
 constexpr int kShareWarps = 4;   // of a CTA that works with mma.sync
 __device__ __forceinline__ void share_sync() { asm volatile("bar.sync 1, 128;\n" ::: "memory"); }
 
-// The four warps' results of a CTA's 16 rows, joined in warp order, as the split's partial.  `ring`: each warp's
+struct ShareJoin {
+  float m[kShareWarps][16], l[kShareWarps][16];
+};
+
+// The results of a split's warps for its 16 rows, joined in warp order, as the split's partial.  `ring`: each warp's
 // own shared memory, ring_bytes apart.
 template <int D, int DT>
 __device__ __forceinline__ void share_join_warps(const ShareGeo& a, const ShareJob& j, unsigned char* ring,
-                                                 size_t ring_bytes, float (*wm_)[16], float (*wl_)[16],
-                                                 float (&o)[DT][4], float m0, float m1, float l0, float l1, float* part) {
+                                                 size_t ring_bytes, ShareJoin& join, float (&o)[DT][4], float m0, float m1,
+                                                 float l0, float l1, float* part) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
+  if (j.warps == 1) {   // nothing to join
+#pragma unroll
+    for (int hr = 0; hr < 2; ++hr) {
+      const int r = g8 + 8 * hr;
+      if (r >= j.NQ) continue;
+      float* p = share_part(part, a, j.slot, share_row(a, j, j.row0 + r));
+      if (t4 == 0) *reinterpret_cast<float2*>(p) = hr ? make_float2(m1, l1) : make_float2(m0, l0);
+#pragma unroll
+      for (int jd = 0; jd < DT; ++jd)
+        *reinterpret_cast<float2*>(p + 4 + jd * 8 + 2 * t4) = make_float2(o[jd][2 * hr], o[jd][2 * hr + 1]);
+    }
+    return;
+  }
   float* wacc = reinterpret_cast<float*>(ring + warp * ring_bytes);
   if (t4 == 0) {
-    wm_[warp][g8] = m0;
-    wl_[warp][g8] = l0;
-    wm_[warp][g8 + 8] = m1;
-    wl_[warp][g8 + 8] = l1;
+    join.m[warp][g8] = m0;
+    join.l[warp][g8] = l0;
+    join.m[warp][g8 + 8] = m1;
+    join.l[warp][g8 + 8] = l1;
   }
 #pragma unroll
   for (int jd = 0; jd < DT; ++jd) {
@@ -136,28 +175,34 @@ __device__ __forceinline__ void share_join_warps(const ShareGeo& a, const ShareJ
     *reinterpret_cast<float2*>(wacc + (g8 + 8) * D + c0) = make_float2(o[jd][2], o[jd][3]);
   }
   share_sync();
-  if (tid < j.NQ) {
-    float mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kShareWarps; ++w) mx = fmaxf(mx, wm_[w][tid]);
-    float l = 0.f, f[kShareWarps];
+  const int w0 = warp - j.sub;   // the split's first warp
+  const int in = j.sub * 32 + lane;
+  if (in < j.NQ) {
+    float mw[kShareWarps], mx = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kShareWarps; ++w) {
-      f[w] = wm_[w][tid] == -INFINITY ? 0.f : exp2f(wm_[w][tid] - mx);
-      l += wl_[w][tid] * f[w];
+      mw[w] = w < j.warps ? join.m[(w0 + w) & 3][in] : -INFINITY;
+      mx = fmaxf(mx, mw[w]);
     }
+    float l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kShareWarps; ++w) wm_[w][tid] = f[w];
-    *reinterpret_cast<float2*>(share_part(part, a, j.slot, share_row(a, j, j.row0 + tid))) = make_float2(mx, l);
+    for (int w = 0; w < kShareWarps; ++w) {
+      if (w >= j.warps) break;
+      const float f = mw[w] == -INFINITY ? 0.f : exp2f(mw[w] - mx);
+      l += join.l[w0 + w][in] * f;
+      join.m[w0 + w][in] = f;
+    }
+    *reinterpret_cast<float2*>(share_part(part, a, j.slot, share_row(a, j, j.row0 + in))) = make_float2(mx, l);
   }
   share_sync();
-  for (int x = tid; x < j.NQ * (D / 4); x += kShareWarps * 32) {
+  for (int x = in; x < j.NQ * (D / 4); x += j.warps * 32) {
     const int r = x / (D / 4), c = x % (D / 4) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kShareWarps; ++w) {
-      const float4 y = *reinterpret_cast<const float4*>(ring + w * ring_bytes + (r * D + c) * 4);
-      const float f = wm_[w][r];
+      if (w >= j.warps) break;
+      const float4 y = *reinterpret_cast<const float4*>(ring + (w0 + w) * ring_bytes + (r * D + c) * 4);
+      const float f = join.m[w0 + w][r];
       v.x = fmaf(y.x, f, v.x);
       v.y = fmaf(y.y, f, v.y);
       v.z = fmaf(y.z, f, v.z);
@@ -192,10 +237,6 @@ struct ShareShape {
   }
 };
 
-struct ShareJoin {
-  float m[kShareWarps][16], l[kShareWarps][16];
-};
-
 template <int D>
 __device__ __forceinline__ void share_mma(const ShareGeo& a, const ShareJob& j, const logkv_prefix_t& pre,
                                           const __nv_bfloat16* rk, const __nv_bfloat16* rv, float* part,
@@ -204,9 +245,8 @@ __device__ __forceinline__ void share_mma(const ShareGeo& a, const ShareJob& j, 
   using B16 = __nv_bfloat16;
   constexpr int TS = S::TS, CPR = S::CPR, KS = S::KS, DT = S::DT, ST = kShareStages;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
-  const int un = (j.n0 + TS - 1) / TS, U = un + (j.n1 + TS - 1) / TS;
-  const int u0 = (int)((long long)U * j.split / j.ns), u1 = (int)((long long)U * (j.split + 1) / j.ns);
-  const int mine = (u1 - u0) > warp ? (u1 - u0 - warp + kShareWarps - 1) / kShareWarps : 0;
+  const ShareTiles u(j, TS);
+  const int un = u.un, mine = u.n;
   unsigned char* wbase = smem + (size_t)warp * ST * S::STAGE_BYTES;
   const unsigned wbase_s = (unsigned)__cvta_generic_to_shared(wbase);
   // Segment 0 is the packed prefix with its mass terms, or the window's own rows; segment 1 the window's shared
@@ -224,16 +264,16 @@ __device__ __forceinline__ void share_mma(const ShareGeo& a, const ShareJob& j, 
   }
   const float* mass = j.own ? nullptr : pre.mass + j.r0;
 
-  auto tile = [&](int u, int& first, int& rows) {
-    const bool second = u >= un;
-    first = (second ? u - un : u) * TS;
+  auto tile = [&](int t, int& first, int& rows) {
+    const bool second = t >= un;
+    first = (second ? t - un : t) * TS;
     rows = min(TS, (second ? j.n1 : j.n0) - first);
     return second;
   };
   auto issue = [&](int k, int stage) {
     if (k < mine) {
       int first, rows;
-      const bool second = tile(u0 + warp + k * kShareWarps, first, rows);
+      const bool second = tile(u.first + k * j.warps, first, rows);
       const long long kst = second ? ks1 : D, vst = second ? vs1 : D;
       const B16* kb = (second ? k1 : k0) + first * kst;
       const B16* vb = (second ? v1 : v0) + first * vst;
@@ -268,7 +308,7 @@ __device__ __forceinline__ void share_mma(const ShareGeo& a, const ShareJob& j, 
   unsigned qa[KS][4];
 #pragma unroll
   for (int hr = 0; hr < 2; ++hr) {
-    const int r = g8 + 8 * hr, m = j.row0 + min(r, j.NQ - 1);
+    const int r = g8 + 8 * hr, m = j.row0 + max(0, min(r, j.NQ - 1));
     tok[hr] = m % a.T;
     const B16* qp = share_query<B16>(a, j, m);
 #pragma unroll
@@ -287,7 +327,7 @@ __device__ __forceinline__ void share_mma(const ShareGeo& a, const ShareJob& j, 
     __syncwarp();
     const int stage = k % ST;
     int first, rows;
-    const bool fresh = tile(u0 + warp + k * kShareWarps, first, rows) && j.own;
+    const bool fresh = tile(u.first + k * j.warps, first, rows) && j.own;
     unsigned char* st = wbase + (size_t)stage * S::STAGE_BYTES;
     const unsigned sk = wbase_s + stage * S::STAGE_BYTES, sv = sk + TS * D * 2;
     const float* sm = reinterpret_cast<const float*>(st + 2 * TS * D * 2);
@@ -389,16 +429,16 @@ __device__ __forceinline__ void share_mma(const ShareGeo& a, const ShareJob& j, 
     l0 += __shfl_xor_sync(0xffffffffu, l0, off);
     l1 += __shfl_xor_sync(0xffffffffu, l1, off);
   }
-  share_join_warps<D, DT>(a, j, smem, (size_t)ST * S::STAGE_BYTES, join.m, join.l, o, m0, m1, l0, l1, part);
+  share_join_warps<D, DT>(a, j, smem, (size_t)ST * S::STAGE_BYTES, join, o, m0, m1, l0, l1, part);
 }
 
-template <int D>
+template <int D, bool GROUPED>
 __global__ void __launch_bounds__(kShareWarps * 32, D <= 128 ? 2 : 1)
     share_mma_kernel(ShareGeo a, logkv_prefix_t pre, const __nv_bfloat16* rk, const __nv_bfloat16* rv, float* part) {
   extern __shared__ uint4 smem4[];
   __shared__ ShareJoin join;
   pdl_entry();
-  const ShareJob j = share_job(a, pre, ShareShape<D>::TS);
+  const ShareJob j = share_job<GROUPED>(a, pre, ShareShape<D>::TS);
   if (j.split < j.ns) share_mma<D>(a, j, pre, rk, rv, part, reinterpret_cast<unsigned char*>(smem4), join);
 }
 
@@ -450,7 +490,7 @@ __global__ void __launch_bounds__(kShareTcThreads, 2)
   if (threadIdx.x < 4) tc::prefetch_tensormap(threadIdx.x < 2 ? &maps.k[threadIdx.x] : &maps.v[threadIdx.x - 2]);
   pdl_entry();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const ShareJob j = share_job(a, pre, TS);
+  const ShareJob j = share_job<true>(a, pre, TS);
   unsigned char* raw = reinterpret_cast<unsigned char*>(smem4);
   if (j.own) {
     if (warp < kShareWarps) share_mma<D>(a, j, pre, rk, rv, part, raw, join);
@@ -739,7 +779,7 @@ struct ShareF32Shape {
   static constexpr int CTAS = D <= 64 ? 2 : 1;   // per SM
 };
 
-template <int D>
+template <int D, bool GROUPED>
 __global__ void __launch_bounds__(kShareWarps * 32, ShareF32Shape<D>::CTAS)
     share_f32_kernel(ShareGeo a, logkv_prefix_t pre, const float* rk, const float* rv, float* part) {
   using S = ShareF32Shape<D>;
@@ -748,11 +788,10 @@ __global__ void __launch_bounds__(kShareWarps * 32, ShareF32Shape<D>::CTAS)
   __shared__ ShareJoin join;
   pdl_entry();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
-  const ShareJob j = share_job(a, pre, TS);
+  const ShareJob j = share_job<GROUPED>(a, pre, TS);
   if (j.split >= j.ns) return;
-  const int un = (j.n0 + TS - 1) / TS, U = un + (j.n1 + TS - 1) / TS;
-  const int u0 = (int)((long long)U * j.split / j.ns), u1 = (int)((long long)U * (j.split + 1) / j.ns);
-  const int mine = (u1 - u0) > warp ? (u1 - u0 - warp + kShareWarps - 1) / kShareWarps : 0;
+  const ShareTiles u(j, TS);
+  const int un = u.un, mine = u.n;
   unsigned char* wbase = reinterpret_cast<unsigned char*>(smem4) + (size_t)warp * ST * S::STAGE_BYTES;
   const float *k0, *v0, *k1, *v1;
   long long ks1 = D, vs1 = D;
@@ -766,16 +805,16 @@ __global__ void __launch_bounds__(kShareWarps * 32, ShareF32Shape<D>::CTAS)
     k1 = rk + win, v1 = rv + win;
   }
   const float* mass = j.own ? nullptr : pre.mass + j.r0;
-  auto tile = [&](int u, int& first, int& rows) {
-    const bool second = u >= un;
-    first = (second ? u - un : u) * TS;
+  auto tile = [&](int t, int& first, int& rows) {
+    const bool second = t >= un;
+    first = (second ? t - un : t) * TS;
     rows = min(TS, (second ? j.n1 : j.n0) - first);
     return second;
   };
   auto issue = [&](int k, int stage) {
     if (k < mine) {
       int first, rows;
-      const bool second = tile(u0 + warp + k * kShareWarps, first, rows);
+      const bool second = tile(u.first + k * j.warps, first, rows);
       const long long kst = second ? ks1 : D, vst = second ? vs1 : D;
       const float* kb = (second ? k1 : k0) + first * kst;
       const float* vb = (second ? v1 : v0) + first * vst;
@@ -806,7 +845,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, ShareF32Shape<D>::CTAS)
   float qf[KS][4];   // A fragments: (g8, t4), (g8 + 8, t4), (g8, t4 + 4), (g8 + 8, t4 + 4)
 #pragma unroll
   for (int hr = 0; hr < 2; ++hr) {
-    const int r = g8 + 8 * hr, m = j.row0 + min(r, j.NQ - 1);
+    const int r = g8 + 8 * hr, m = j.row0 + max(0, min(r, j.NQ - 1));
     tok[hr] = m % a.T;
     const float* qp = share_query<float>(a, j, m);
 #pragma unroll
@@ -824,7 +863,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, ShareF32Shape<D>::CTAS)
     cp_async_wait<ST - 1>();
     __syncwarp();
     int first, rows;
-    const bool fresh = tile(u0 + warp + k * kShareWarps, first, rows) && j.own;
+    const bool fresh = tile(u.first + k * j.warps, first, rows) && j.own;
     float* sk = reinterpret_cast<float*>(wbase + (size_t)(k % ST) * S::STAGE_BYTES);
     float* sv = sk + TS * LD;
     const float* sm = sv + TS * LD;
@@ -924,8 +963,8 @@ __global__ void __launch_bounds__(kShareWarps * 32, ShareF32Shape<D>::CTAS)
     l0 += __shfl_xor_sync(0xffffffffu, l0, off);
     l1 += __shfl_xor_sync(0xffffffffu, l1, off);
   }
-  share_join_warps<D, DT>(a, j, reinterpret_cast<unsigned char*>(smem4), (size_t)ST * S::STAGE_BYTES, join.m, join.l, o, m0,
-                          m1, l0, l1, part);
+  share_join_warps<D, DT>(a, j, reinterpret_cast<unsigned char*>(smem4), (size_t)ST * S::STAGE_BYTES, join, o, m0, m1,
+                          l0, l1, part);
 }
 
 // ---------------------------------------------------------------- combine
@@ -935,7 +974,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, ShareF32Shape<D>::CTAS)
 // worked out before the wait for it.
 template <typename T, int D, int TS, int WPR>
 __global__ void __launch_bounds__(128) share_combine_kernel(ShareGeo a, logkv_prefix_t pre, const float* part, T* out) {
-  constexpr int PER = (D + 127) / 128, NB = D > 128 ? 4 : 8;
+  constexpr int PER = (D + 127) / 128, NB = D > 128 ? 4 : 10;
   __shared__ float sh[4][2 + D];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
   const size_t row = (size_t)blockIdx.x * (4 / WPR) + warp / WPR;
@@ -1035,7 +1074,7 @@ __global__ void __launch_bounds__(128) share_combine_kernel(ShareGeo a, logkv_pr
 
 // ---------------------------------------------------------------- host side
 struct SharePlan {
-  int tile_rows, tiles, own_tiles, nsplit, upw, nown, slots;
+  int tile_rows, tiles, own_tiles, nsplit, upw, nown, own_warps, slots;
   long long own_work;
   bool tc;
 };
@@ -1052,17 +1091,28 @@ static SharePlan share_plan(const logkv_layout_t& l, const logkv_shared_args_t& 
   const int ts = p.tc ? kTcTS : 16;
   p.upw = p.tc ? 2 : kShareWarps;
   p.slots = 148 * ((f32 && l.dim > 64) || l.dim > 128 ? 1 : 2);
-  const long long own_ctas = (long long)l.batch * l.groups * p.own_tiles;
+  const long long own = (long long)l.batch * l.groups * p.own_tiles;
   const long long shared_ctas = (long long)l.batch / x.beams * l.groups * p.tiles;
-  // Own lanes: a key tile per warp at least, and a second split only while they leave half of the SMs.
+  // A second split of an own lane (a key tile per warp at least) only while they leave half of the SMs.
   const int own_keys = x.recent_count - x.window_from + x.tokens;
-  p.nown = (int)std::max(1LL, std::min<long long>(own_keys / 16 / kShareWarps, p.slots / 2 / own_ctas));
-  // A CTA's start weighs as much as some 250 keys.  Measured with 1 to 8 splits of 64 shared lanes (8.0K keys) beside
-  // 512 own ones (242 keys): 129, 81, 60, 61, 74, 66, 68 us for 1, 2, 3, 4, 5, 6, 8; this gives 3.
-  p.own_work = own_ctas * p.nown * (own_keys / p.nown + 250);
-  // The grid holds the splits of a full prefix; a shorter one leaves some unused.
+  p.nown = (int)std::max(1LL, std::min<long long>(own_keys / 16 / kShareWarps, p.slots / 2 / own));
+  // The grid holds the splits of a full prefix; a shorter one leaves some unused.  Starting a warp on an own lane
+  // weighs as much as some 50 keys of a CTA.
   const long long units = (prefix_capacity + x.window_from) / ts + 2, work = units * ts * shared_ctas;
-  p.nsplit = (int)std::max(1LL, std::min(p.slots * work / (work + p.own_work) / shared_ctas, units / p.upw));
+  auto own_work = [&](int warps) { return own * p.nown * (own_keys / p.nown + 50LL * warps); };
+  // Warps to an own lane: as many as fit into its kind's share of the SMs, a prefix taken to fill 0.6 of its capacity.
+  // Own parts of 64 keys beside 3.3K shared ones in us with 4, 2 and 1: 256 lanes beside 64 shared ones 30, 31, 26.5;
+  // 1024 beside 64 67, 54, 44; 32 beside 8 12.4, 14.2, 14.1.  405 keys, 480 lanes, hardly any shared ones: 33, 31, 39.
+  p.own_warps = 4;
+  while (p.nown == 1 && p.own_warps > 1 &&
+         own * p.own_warps / 4 > p.slots * own_work(p.own_warps) / (work * 6 / 10 + own_work(p.own_warps)))
+    p.own_warps /= 2;
+  p.own_work = own_work(p.own_warps);
+  long long splits = p.slots * work / (work + p.own_work) / shared_ctas;
+  // A few splits fewer let all CTAs run at once (32 own ones beside 8 lanes: 13.3 us with 33 splits, 13.6 with 34).
+  const long long beside = (p.slots - (own * p.nown * p.own_warps + 3) / 4) / shared_ctas;
+  if (beside < splits && beside >= splits - splits / 8) splits = beside;
+  p.nsplit = (int)std::max(1LL, std::min(splits, units / p.upw));
   return p;
 }
 
@@ -1098,15 +1148,19 @@ static void launch_share_combine(const ShareGeo& a, const logkv_prefix_t& pre, c
 }
 
 static dim3 share_grid(const ShareGeo& a) {
-  return dim3((unsigned)(a.shared_lanes * a.nsplit * a.tiles + a.own_lanes * a.nown * a.own_tiles));
+  return dim3((unsigned)(a.shared_lanes * a.nsplit * a.tiles +
+                         ((long long)a.own_lanes * a.nown * a.own_tiles * a.own_warps + 3) / 4));
 }
 
 template <int D>
 static int launch_share_bf16(const ShareGeo& a, const logkv_prefix_t& pre, const logkv_state_t& s, void* out, float* part,
                              cudaStream_t st) {
   using B16 = __nv_bfloat16;
-  if (const int e = smem_limit_once<share_mma_kernel<D>>(ShareShape<D>::smem)) return e;
-  launch_pdl(share_mma_kernel<D>, share_grid(a), kShareWarps * 32, ShareShape<D>::smem, st, a, pre,
+  const auto kern = a.own_warps < 4 ? share_mma_kernel<D, true> : share_mma_kernel<D, false>;
+  const int e = a.own_warps < 4 ? smem_limit_once<share_mma_kernel<D, true>>(ShareShape<D>::smem)
+                                : smem_limit_once<share_mma_kernel<D, false>>(ShareShape<D>::smem);
+  if (e) return e;
+  launch_pdl(kern, share_grid(a), kShareWarps * 32, ShareShape<D>::smem, st, a, pre,
              static_cast<const B16*>(s.recent_k), static_cast<const B16*>(s.recent_v), part);
   launch_share_combine<B16, D, 16>(a, pre, part, out, st);
   return launch_status();
@@ -1137,8 +1191,11 @@ static int launch_share_tc(const ShareGeo& a, const logkv_prefix_t& pre, const l
 template <int D>
 static int launch_share_f32(const ShareGeo& a, const logkv_prefix_t& pre, const logkv_state_t& s, void* out, float* part,
                             cudaStream_t st) {
-  if (const int e = smem_limit_once<share_f32_kernel<D>>(ShareF32Shape<D>::smem)) return e;
-  launch_pdl(share_f32_kernel<D>, share_grid(a), kShareWarps * 32, ShareF32Shape<D>::smem, st, a, pre,
+  const auto kern = a.own_warps < 4 ? share_f32_kernel<D, true> : share_f32_kernel<D, false>;
+  const int e = a.own_warps < 4 ? smem_limit_once<share_f32_kernel<D, true>>(ShareF32Shape<D>::smem)
+                                : smem_limit_once<share_f32_kernel<D, false>>(ShareF32Shape<D>::smem);
+  if (e) return e;
+  launch_pdl(kern, share_grid(a), kShareWarps * 32, ShareF32Shape<D>::smem, st, a, pre,
              static_cast<const float*>(s.recent_k), static_cast<const float*>(s.recent_v), part);
   launch_share_combine<float, D, 16>(a, pre, part, out, st);
   return launch_status();
@@ -1193,6 +1250,7 @@ LOGKV_API int logkv_shared_attention(const logkv_layout_t* layout, const logkv_s
   a.nsplit = p.nsplit;
   a.upw = p.upw;
   a.nown = p.nown;
+  a.own_warps = p.own_warps;
   a.shared_lanes = a.B / a.W * a.G;
   a.own_lanes = a.B * a.G;
   a.tiles = p.tiles;

@@ -6,8 +6,10 @@
 // once and written once, so HBM bounds long chunks and the launch bounds single tokens.
 //
 // A thread owns one unit of a token: VN features of the first half with their VN partners, or features behind the
-// rotated ones (VN, and from the next 16-byte boundary on VW).  It reads its table entries once and walks over the heads of all tensors with
-// them, kBatch heads' loads in flight; the heads are cut into chunks when tokens are few.
+// rotated ones (VN, and from the next 16-byte boundary on VW).  It reads its table entries once and walks over the heads
+// of all tensors with them, kBatch heads' loads in flight; the heads are cut into chunks when tokens are few.  kBatch 2,
+// 3, 4, 8: 35, 33, 31, 34 us for 8 x 2048 tokens of 8 key and 8 value heads (176 MB, 0.86 of the measured copy
+// bandwidth), 30, 27, 16.5, 22.5 us for 4 x 1777 interleaved ones of 24 heads of 64 float32 (95 MB, 0.88).
 #include <algorithm>
 
 #include "attn_common.cuh"

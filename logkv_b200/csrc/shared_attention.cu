@@ -1100,11 +1100,13 @@ static SharePlan share_plan(const logkv_layout_t& l, const logkv_shared_args_t& 
   // weighs as much as some 50 keys of a CTA.
   const long long units = (prefix_capacity + x.window_from) / ts + 2, work = units * ts * shared_ctas;
   auto own_work = [&](int warps) { return own * p.nown * (own_keys / p.nown + 50LL * warps); };
-  // Warps to an own lane: as many as fit into its kind's share of the SMs, a prefix taken to fill 0.6 of its capacity.
+  // Warps to an own lane: as many as fit into its kind's share of the SMs, a prefix taken to fill 0.6 of its capacity,
+  // and so many that none has more than eight key tiles (one warp's 16 take 22 us: 512 lanes of 242 keys beside 64 shared
+  // ones 59.6, 60.1, 61.3 us with 4, 2 and 1).
   // Own parts of 64 keys beside 3.3K shared ones in us with 4, 2 and 1: 256 lanes beside 64 shared ones 30, 31, 26.5;
   // 1024 beside 64 67, 54, 44; 32 beside 8 12.4, 14.2, 14.1.  405 keys, 480 lanes, hardly any shared ones: 33, 31, 39.
   p.own_warps = 4;
-  while (p.nown == 1 && p.own_warps > 1 &&
+  while (p.nown == 1 && p.own_warps > 1 && own_keys <= 8 * 16 * p.own_warps / 2 &&
          own * p.own_warps / 4 > p.slots * own_work(p.own_warps) / (work * 6 / 10 + own_work(p.own_warps)))
     p.own_warps /= 2;
   p.own_work = own_work(p.own_warps);

@@ -158,6 +158,6 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt=0, repetition=1.
         a.prompts_wide = prompts is not None and prompts.dtype == torch.int64
         a.repetitions, a.presences, a.frequencies = ptr(reps), ptr(press), ptr(freqs)
         a.bias_tokens, a.bias_values, a.mask = ptr(tokens), ptr(values), ptr(mask)
-        _lib.check(_lib.lib().logkv_adjust_logits(ctypes.byref(a), _lib.stream_ptr(dev)), "logkv_adjust_logits")
         _native = (_lib.host().logits, _lib.address("logkv_adjust_logits"))
+        _lib.check(_lib.lib().logkv_adjust_logits(ctypes.byref(a), _lib.stream_ptr(dev)), "logkv_adjust_logits")
     return out

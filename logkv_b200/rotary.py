@@ -83,10 +83,10 @@ def launch(cache, parts, positions, pos0: int, interleaved: int, *, positions_ou
         a.ends_stride, a.ends_out_stride = ends.stride(0), ends_out.stride(0)
     status = getattr(cache, "_read_status", None)   # a foreign cache has none
     a.status = None if status is None else status.data_ptr()
+    if status is not None and native(cache) is None:
+        cache._rotary = _Native(cache)
     _lib.check(_lib.lib().logkv_rotate(ctypes.byref(_rope(cache)), ctypes.byref(a),
                                        _lib.stream_ptr(cache.recent_k.device)), "logkv_rotate")
-    if status is not None and cache._rotary is None:
-        cache._rotary = _Native(cache)
 
 
 class _Native:
@@ -97,18 +97,19 @@ class _Native:
         host = _lib.host()
         self.rotate, self.append, self.fn = host.rotate, host.append, _lib.address("logkv_rotate")
         self.tables = _rope(cache)
-        self.rope = ctypes.addressof(self.tables)
+        self.rope, self.dtype = ctypes.addressof(self.tables), cache.cos_cache.dtype
         self.status = cache._read_status.data_ptr()
 
 
 def native(cache):
-    """The cache's _Native once a call has gone through and while its tables are where they were; else None."""
+    """The cache's _Native once a call has gone through and while its tables are what they were; else None."""
     n = getattr(cache, "_rotary", None)
     if n is None:
         return None
     b = cache._buffers
     cos, sin = b["cos_cache"], b["sin_cache"]
-    same = n.tables.cos == cos.data_ptr() and n.tables.sin == sin.data_ptr() and n.tables.rows == cos.size(0)
+    t = n.tables
+    same = t.cos == cos.data_ptr() and t.sin == sin.data_ptr() and t.rows == cos.size(0) and n.dtype is cos.dtype
     return n if same or not cache.rope_n_elem else None
 
 

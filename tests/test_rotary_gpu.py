@@ -270,4 +270,8 @@ def test_repeated_calls_are_checked_like_the_first():
     other = cache.cos_cache.flip(0).contiguous()          # other tables take over at once
     cache.cos_cache, cache.sin_cache = other, cache.sin_cache.flip(0).contiguous()
     assert torch.equal(f(cache, q, k, 99 - p)[0], want[0])
+    for dtype in (BF16, F32):                             # of another type, too
+        cache.cos_cache, cache.sin_cache = cache.cos_cache.to(dtype), cache.sin_cache.to(dtype)
+        for _ in range(2):
+            check(cache, 4, 3, p, "half")
     assert cache.read_status() == 0

@@ -18,7 +18,7 @@ import ctypes
 import torch
 
 from . import _lib, rotary
-from .attention import log_kv_chunk_attention, log_kv_shared_attention
+from .attention import _MAX_QUERY_ROWS, log_kv_chunk_attention, log_kv_shared_attention
 from .beam import beam_select
 from .logits import adjust_logits
 
@@ -241,10 +241,13 @@ class LogKVBeams:
         """``LogKVDecoder.step_raw`` of layer ``layer`` for the beams' last tokens: q [rows, H, 1, D], k_raw and v
         [rows, G, 1, D], unrotated.  Until the cache's next flush after ``fork`` the keys that a request's beams
         share are read once for all of them."""
-        w = self._window_from(layer)
-        return self.decoders[layer].step_raw(
-            q, k_raw, v, input_pos=input_pos, layout=layout, span_ends_device=span_ends_device, out=out,
-            shared=(self.beams, w) if w is not None and self.beams > 1 else None)
+        d, w = self.decoders[layer], self._window_from(layer)
+        shared = (self.beams, w) if w is not None and self.beams > 1 else None
+        rf = q.size(1) // d.cache.n_groups if q.dim() == 4 else 1
+        if shared is None and rf and (rf & (rf - 1) or rf > _MAX_QUERY_ROWS[d._k.dtype]):
+            shared = (1, 0)      # heads per group that log_kv_chunk_attention does not take
+        return d.step_raw(q, k_raw, v, input_pos=input_pos, layout=layout, span_ends_device=span_ends_device, out=out,
+                          shared=shared)
 
     def advance(self, logits, *, bias=None, mask=None):
         """Select the next tokens from the logits [requests, beams, V] (or [requests * beams, V]) of the

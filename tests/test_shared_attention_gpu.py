@@ -85,7 +85,7 @@ def check(cache, q, k, v, got, causal=True, scale=None):
     (BF16, 64, 2, 1, 1, 1, 1, 40, 60, 3), (BF16, 64, 2, 1, 1, 2, 3, 0, 0, 0), (BF16, 128, 2, 1, 2, 2, 4, 60, 60, 3),
     (BF16, 128, 1, 1, 1, 3, 16, 17, 33, 2), (BF16, 128, 5, 1, 2, 1, 7, 0, 200, 3), (BF16, 64, 3, 2, 2, 2, 5, 100, 131, 0),
     (BF16, 64, 8, 3, 3, 1, 11, 64, 64, 3), (BF16, 32, 4, 1, 1, 2, 9, 30, 61, 3), (BF16, 16, 2, 5, 5, 2, 3, 3, 5, 1),
-    (BF16, 256, 2, 1, 2, 1, 4, 90, 100, 2), (BF16, 128, 2, 40, 40, 1, 3, 50, 77, 2), (BF16, 64, 1, 1, 1, 1, 130, 9, 10, 1),
+    (BF16, 256, 2, 1, 2, 1, 4, 90, 100, 2), (BF16, 64, 2, 2, 5, 2, 3, 9, 30, 2), (F32, 32, 2, 3, 40, 1, 2, 9, 30, 2), (BF16, 128, 2, 40, 40, 1, 3, 50, 77, 2), (BF16, 64, 1, 1, 1, 1, 130, 9, 10, 1),
     (F32, 64, 2, 1, 1, 2, 3, 40, 60, 3), (F32, 128, 3, 1, 2, 1, 5, 0, 100, 2), (F32, 32, 7, 2, 2, 2, 2, 16, 16, 0),
     (F32, 16, 1, 9, 9, 1, 4, 0, 0, 0), (F32, 64, 2, 33, 33, 1, 2, 20, 50, 1)])
 def test_against_64_bits(dtype, D, rf, T, Tk, N, W, w0, R, levels):
@@ -287,7 +287,7 @@ def test_step_raw_equals_rotating_and_stepping(layout, given):
             a.step_raw(*args, **kw)
 
 
-@pytest.mark.parametrize("D,rf,steps", [(64, 2, 50), (128, 8, 12), (64, 3, 12)])
+@pytest.mark.parametrize("D,rf,steps", [(64, 2, 50), (128, 8, 12), (64, 3, 12), (64, 5, 50)])
 def test_beam_steps(D, rf, steps):
     """LogKVBeams.step and advance with penalties, biases and masks, against the same steps without sharing over
     rows copied by indexing; long enough in the first case that the window flushes in between."""
@@ -404,3 +404,43 @@ def test_repeated_calls_are_checked_like_the_first():
                      k_raw=torch.randn_like(cache.recent_k[:, :, :256]), span_ends=[[False] * 256] * 6)
     assert cache._flush_cursor == 1
     check(cache, q, k, v, run(cache, q, k, v, 1, 0))
+
+
+@pytest.mark.parametrize("shared", [None, (2, 12)])
+def test_captured_pair_of_steps(shared):
+    """Two steps (a pending token, then the pair's commit) captured once and replayed on other tokens, against the same
+    steps run at once."""
+    from logkv_b200.decode import LogKVDecoder
+    mk = lambda: LogKVDecoder(make_cache(BF16, B=4, G=2, D=64, R=20, recent=64, seed=4), 0.125)  # noqa: E731
+    a, b = mk(), mk()
+    for d in (a, b):
+        d.reorder(torch.tensor([0, 0, 2, 2], device="cuda"))
+    ins = [[t.contiguous() for t in fresh(a.cache, 2, 1, 1, seed=s)] + [torch.full((4, 1), 90 + s, device="cuda"),
+                                                                       torch.zeros(4, 1, dtype=torch.uint8, device="cuda")]
+           for s in (0, 1)]
+
+    def two(d, ins):
+        return [d.step_raw(q, k, v, input_pos=p, span_ends_device=e, shared=shared) for q, k, v, p, e in ins]
+
+    two(mk(), ins)           # everything that a first call sets up
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        from logkv_b200.attention import refresh_prefix
+        refresh_prefix(a.cache)
+        with torch.cuda.graph(graph, stream=side):
+            out = two(a, ins)
+    torch.cuda.current_stream().wait_stream(side)
+    for i, (q, k, v, p, e) in enumerate(ins):
+        for old, new in zip((q, k, v), fresh(a.cache, 2, 1, 1, seed=10 + i)):
+            old.copy_(new)
+        p += 7
+        e.fill_(1)
+    graph.replay()
+    want = two(b, ins)
+    for x, y in zip(out, want):
+        assert torch.equal(x, y)
+    for (name, s), (_, t) in zip(a.cache.named_buffers(), b.cache.named_buffers()):
+        assert torch.equal(s, t), name
+    assert torch.equal(a.cache._recent_ends, b.cache._recent_ends) and a.cache.recent_count == b.cache.recent_count == 22

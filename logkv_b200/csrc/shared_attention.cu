@@ -42,8 +42,8 @@ struct ShareGeo {
 __device__ __forceinline__ int share_splits(const ShareGeo& a, int units, int tile_keys) {
   const int ctas = a.shared_lanes * a.tiles;
   const long long work = (long long)units * tile_keys * ctas;
-  const int room = (int)(a.slots * work / (work + a.own_work));
-  return max(1, min(a.nsplit, min(room / ctas, units / a.upw)));
+  const int room = (int)(2 * a.slots * work / (work + a.own_work));   // in half CTAs: to the nearest split
+  return max(1, min(a.nsplit, min((room + ctas) / (2 * ctas), units / a.upw)));
 }
 
 __device__ __forceinline__ int share_prefix_length(const logkv_prefix_t& pre, int ln) {
@@ -1110,7 +1110,8 @@ static SharePlan share_plan(const logkv_layout_t& l, const logkv_shared_args_t& 
          own * p.own_warps / 4 > p.slots * own_work(p.own_warps) / (work * 6 / 10 + own_work(p.own_warps)))
     p.own_warps /= 2;
   p.own_work = own_work(p.own_warps);
-  long long splits = p.slots * work / (work + p.own_work) / shared_ctas;
+  long long splits = std::min((2 * p.slots * work / (work + p.own_work) + shared_ctas) / (2 * shared_ctas),
+                              std::max(1LL, p.slots / shared_ctas));
   // A few splits fewer let all CTAs run at once (32 own ones beside 8 lanes: 13.3 us with 33 splits, 13.6 with 34).
   const long long beside = (p.slots - (own * p.nown * p.own_warps + 3) / 4) / shared_ctas;
   if (beside < splits && beside >= splits - splits / 8) splits = beside;

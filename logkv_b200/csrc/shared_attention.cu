@@ -8,7 +8,10 @@
 // its rf T rows (an "own lane").  Both kinds of lanes are split over CTAs of one launch, which leave (m, l, O) per
 // row and split; share_combine_kernel joins them in a fixed order, the shared splits first.
 //
-// Bound by HBM from a few MB per SM on: keys and values are read once per 128 (16) query rows.
+// Bound by HBM from a few MB per SM on: keys and values are read once per 128 (16) query rows.  Measured on B200, device
+// time: 8 requests of 8 rows over 7.8K shared and 242 own keys (8 groups, head dim 128, bf16: 314 MB) 60 us, 0.79 of the
+// measured copy bandwidth, where log_kv_chunk_attention takes 367; one request of 4 rows (31 MB) 12.5 us (34); below that
+// latency: 3 requests of 16 rows over 2.0K keys 16 us.
 #include <algorithm>
 #include <cstring>
 

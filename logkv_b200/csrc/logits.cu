@@ -11,7 +11,7 @@
 //
 // Measured on B200, device time: 512 rows of 151936 bf16 logits (323 MB) with histories of 1024, 16 biases and masks
 // 58 us, 0.84 of the measured copy bandwidth (55 without the masks, 52 the copy alone); 145 rows of 50021 float32 ones
-// (60 MB) with histories of 4097 and 37 biases 17 us, 0.55, 7.9 the copy alone; 4 rows of 32000 3.9 us.
+// (60 MB) with histories of 4097 and 37 biases 14 us, 0.65, 8 the copy alone; 4 rows of 32000 3.9 us.
 #include <algorithm>
 
 #include "common.cuh"
@@ -20,7 +20,7 @@
 namespace logkv {
 
 constexpr int kLogitsThreads = 256;   // that copy; LT more go over the history and the biases, where there are any
-constexpr int logits_ctas(int lt) { return lt > 128 ? 3 : 4; }   // of an SM, at 40 registers a thread
+constexpr int logits_ctas(int lt) { return lt > 256 ? 2 : lt > 128 ? 3 : 4; }   // of an SM, at 40 registers a thread
 constexpr unsigned kSeen = 0x80000000u;   // counter bit of a token that the prompt holds
 
 __device__ __forceinline__ long long load_int(const void* p, int wide, long long i) {
@@ -344,7 +344,7 @@ static int launch_adjust(const logkv_logits_args_t& a, cudaStream_t st) {
   // Parts: one wave of CTAs, and up to three where nothing but the copy is to do, or where a part is still 16 times as
   // long as the history that each of a row's CTAs goes over, and of 64 KB, beside which going over a short history or
   // the biases does not show.  512 rows of 151936 bf16 (history 1024): 62.4 us in one wave, 58.5 in three; 145 rows of
-  // 50021 float32: history 4097 18 in one wave, 26 in two, 33 in three; 64 8.7 in one, 13.5 in three; the copy alone
+  // 50021 float32 (eight list warps): history 4097 18 in one wave, 26 in two, 33 in three; 64 8.7 in one, 13.5 in three; the copy alone
   // 9.7 in one, 7.7 in three.
   const long long wave = 148 * logits_ctas(LT);
   long long room = a.vocab;
@@ -359,11 +359,15 @@ static int launch_adjust(const logkv_logits_args_t& a, cudaStream_t st) {
   return e == cudaSuccess ? LOGKV_OK : (int)e;
 }
 
-// Eight warps for long histories: 4097 tokens beside 50021 logits 18 us against 23 with four; 1024 beside 151936 64
-// against 58.5 (an SM then holds three CTAs instead of four).
+// Eight warps for long histories, sixteen where they are long beside the row, too (an SM then holds three and two CTAs
+// instead of four).  With 4, 8 and 16: 145 rows of 50021, history 4097 23, 17, 14 us; 512 rows of 151936, history 1024
+// 58.5, 64, -, 4097 -, 68, 79, 8192 -, 99, 97, 20000 -, 176, 123.  Sixteen for many biases, too, whose repeats are
+// compared entry by entry (1024 with repeats in 60 rows of 88413: 101 us with four, 44 with sixteen).
 template <typename T, RowsAt AT>
 static int launch_adjust(const logkv_logits_args_t& a, cudaStream_t st) {
-  return a.history && a.history_len > 2048 ? launch_adjust<T, AT, 256>(a, st) : launch_adjust<T, AT, 128>(a, st);
+  if (a.bias_count > 512) return launch_adjust<T, AT, 512>(a, st);
+  if (!a.history || a.history_len <= 2048) return launch_adjust<T, AT, 128>(a, st);
+  return a.vocab < 20LL * a.history_len ? launch_adjust<T, AT, 512>(a, st) : launch_adjust<T, AT, 256>(a, st);
 }
 
 // One case for all took 256 rows of 151936 masked bf16 logits from 27.6 to 29.4 us where they are aligned; without the

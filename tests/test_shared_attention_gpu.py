@@ -107,6 +107,17 @@ def test_lane_counts(dtype, N, W, G):
     check(cache, q, k, v, run(cache, q, k, v, W, 150, causal=False), causal=False)
 
 
+@pytest.mark.parametrize("dtype,D,rf,T,w0", [(BF16, 256, 2, 1, 100), (BF16, 128, 9, 2, 100), (BF16, 64, 9, 2, 60), (BF16, 32, 3, 2, 119),
+                                             (BF16, 16, 1, 1, 0), (F32, 128, 2, 1, 100), (F32, 64, 9, 2, 110), (F32, 16, 1, 5, 90)])
+def test_own_lanes_side_by_side(dtype, D, rf, T, w0):
+    """More own lanes than CTAs run at once: one or two warps to a lane, lanes of several row tiles, a last CTA that is
+    not full."""
+    for N, W, G in ((33, 3, 4), (37, 5, 3)):
+        cache = forked(dtype, N, W, w0, 120, G=G, D=D, levels=1, seed=D + N)
+        q, k, v = fresh(cache, rf, T, T)
+        check(cache, q, k, v, run(cache, q, k, v, W, w0))
+
+
 @pytest.mark.parametrize("dtype,D,N,W,rf", [(BF16, 128, 20, 3, 8), (BF16, 64, 20, 2, 30), (BF16, 128, 30, 2, 2), (F32, 64, 20, 2, 2)])
 def test_long_splits(dtype, D, N, W, rf):
     """One or two splits per lane, many key tiles each (the stages are used over and over), long own parts."""

@@ -301,7 +301,8 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor* win[5];
   for (int i = 0; i < 5; ++i)
     if (!(win[i] = tensor(args[3 + i])) || !win[i]->is_cuda()) Py_RETURN_NONE;
-  const at::Tensor *k = tensor(args[8]), *v = tensor(args[9]), *ends = tensor(args[11]), *q = tensor(args[15]), &like = *win[0];
+  const at::Tensor *k = tensor(args[8]), *v = tensor(args[9]), *ends = tensor(args[11]), *q = tensor(args[15]);
+  const at::Tensor& like = *win[0];
   if (!k || !v || (!ends && args[11] != Py_None) || (!q && args[15] != Py_None) || k->dim() != 4 || v->dim() != 4 ||
       (ends && ends->dim() != 2) || (q && q->dim() != 4))
     Py_RETURN_NONE;
@@ -476,8 +477,20 @@ PyObject* logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
+// A call with every C++ exception turned into a Python one (a tensor without strides throws where it is looked at).
+using Call = PyObject* (*)(PyObject*, PyObject* const*, Py_ssize_t);
+template <Call F>
+PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  try {
+    return F(self, args, n);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
 #define LOGKV_METHOD(name) \
-  {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
+  {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<name>)), METH_FASTCALL, nullptr}
 
 PyMethodDef methods[] = {
     LOGKV_METHOD(tree),   LOGKV_METHOD(beam),   LOGKV_METHOD(shared),

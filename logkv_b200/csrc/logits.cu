@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
   extern __shared__ __align__(16) unsigned smem[];
   __shared__ int warp_sums[LT / 32];
   const int entries = (a.bias_count + 3) / 4 * 4, words = g.part / 32;
-  int* bt = reinterpret_cast<int*>(smem);                         // [entries] biased tokens, -1: not this part's or again
+  int* bt = reinterpret_cast<int*>(smem);                         // [entries] biased tokens, -1: not here, or again
   float* bz = reinterpret_cast<float*>(bt + entries);             // [entries] biases, then adjusted logits
   unsigned* again = reinterpret_cast<unsigned*>(bz + entries);    // [words] bits of tokens with several biases
   unsigned* before = again + (entries ? words : 0);               // [words] bits of the biased tokens; later on
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
     }
     const uint8_t* mask8 = reinterpret_cast<const uint8_t*>(mask);
     for (int j0 = first + tid; j0 < last; j0 += U * kLogitsThreads) {
-      // All loads first: what is worked out in between would make each wait for the one before (27 -> 38 us for 256 rows).
+      // All loads first: what is worked out in between makes each wait for the one before (28 -> 38 us for 256 rows).
       uint4 raw[U], next[U];
       unsigned m0[U], m1[U];
 #pragma unroll
@@ -282,7 +282,8 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
             const int4 t = *reinterpret_cast<const int4*>(bt + j);
             if (t.x != v && t.y != v && t.z != v && t.w != v) continue;
             const float4 b = *reinterpret_cast<const float4*>(bz + j);
-            first &= (t.x != v || j >= i) && (t.y != v || j + 1 >= i) && (t.z != v || j + 2 >= i) && (t.w != v || j + 3 >= i);
+            first &= (t.x != v || j >= i) && (t.y != v || j + 1 >= i) && (t.z != v || j + 2 >= i) &&
+                     (t.w != v || j + 3 >= i);
             sum += t.x == v ? b.x : 0.f;
             sum += t.y == v ? b.y : 0.f;
             sum += t.z == v ? b.z : 0.f;

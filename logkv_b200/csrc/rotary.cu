@@ -63,7 +63,8 @@ struct RotateGeo {
 };
 
 template <typename T, int VN>
-__device__ __forceinline__ void copy_heads(const logkv_rotate_part_t& x, const T* src, T* out, T* raw, int at, int h0, int h1) {
+__device__ __forceinline__ void copy_heads(const logkv_rotate_part_t& x, const T* src, T* out, T* raw, int at, int h0,
+                                           int h1) {
   for (int h = h0; h < h1; h += kBatch) {
     Unit<T, VN> v[kBatch];
 #pragma unroll
@@ -97,7 +98,8 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(RotateGeo g, log
   const bool turned = u < pairs;
   // First element of the unit and of its partner, as read and as written.
   const int mid = (g.wide - g.n) / VN;
-  const int lo = turned ? u * VN : u < pairs + mid ? g.n + (u - pairs) * VN : g.wide + (u - pairs - mid) * VW, hi = lo + half;
+  const int lo = turned ? u * VN : u < pairs + mid ? g.n + (u - pairs) * VN : g.wide + (u - pairs - mid) * VW;
+  const int hi = lo + half;
   const int in0 = turned && a.interleaved ? 2 * lo : lo, in1 = turned && a.interleaved ? in0 + VN : hi;
   if (u == 0 && blockIdx.y == 0) {
     if (a.positions_out) a.positions_out[b * a.positions_out_stride + t] = pos;

@@ -257,3 +257,8 @@ def test_repeated_calls_are_checked_like_the_first():
     assert f(x[:0], history=h[:0]).shape == (0, 3, 70)
     assert torch.equal(f(x, **{**kw, "repetition": torch.full((2, 3), 1.5, device="cuda")}), f(x, **{**kw, "repetition": 1.5}))
     assert torch.equal(f(x, **{**kw, "repetition": 2}), f(x, **{**kw, "repetition": 2.0}))
+    for bad in (x.to_sparse(), x.to(torch.float32).to_sparse()):      # no strides to look at
+        with pytest.raises((RuntimeError, ValueError)):
+            f(bad, **kw)
+    with pytest.raises((RuntimeError, ValueError)):
+        f(x, **{**kw, "mask": kw["mask"].to_sparse()})

@@ -249,6 +249,8 @@ def test_repeated_calls_are_checked_like_the_first():
             f(cache, *args, **kw)
     with pytest.raises(NotImplementedError):
         f(cache, q.clone().requires_grad_(), k, p)
+    with pytest.raises((RuntimeError, ValueError)):
+        f(cache, q.contiguous().to_sparse(), k, p)
     with torch.no_grad():
         assert torch.equal(f(cache, q.clone().requires_grad_(), k, p)[0], want[0])
     assert torch.equal(f(cache, q, k, [0, 1, 2])[0], want[0]) and torch.equal(f(cache, q, k, p.int())[1], want[1])

@@ -29,7 +29,7 @@ struct ShareGeo {
   int own_warps;          // warps to an own lane's split: 4, 2 or 1
   int shared_lanes, own_lanes;
   int slots;              // CTAs that run at once
-  long long own_work;     // all own lanes' work in keys, what it takes to start them included
+  float own_work;         // all own lanes' work in keys, what it takes to start them included
   int tiles, tile_rows;   // row tiles of a shared lane (at most 16 or 128 rows each)
   int own_tiles;          // row tiles of an own lane (16 rows each)
   float scale_log2, mass_log2;   // score = dot * scale_log2 + mass * mass_log2, in the log2 domain
@@ -44,8 +44,9 @@ struct ShareGeo {
 // 512 own ones of 242: 129, 81, 60, 61, 74, 66, 68 us with 1, 2, 3, 4, 5, 6, 8 splits; this gives 3.
 __device__ __forceinline__ int share_splits(const ShareGeo& a, int units, int tile_keys) {
   const int ctas = a.shared_lanes * a.tiles;
-  const long long work = (long long)units * tile_keys * ctas;
-  const int room = (int)(2 * a.slots * work / (work + a.own_work));   // in half CTAs: to the nearest split
+  // In half CTAs, to the nearest split; every operation rounded on its own, so that both kernels get the same.
+  const float work = __fmul_rn((float)(units * tile_keys), (float)ctas);
+  const int room = (int)__fdiv_rn(__fmul_rn(2.f * a.slots, work), __fadd_rn(work, a.own_work));
   return max(1, min(a.nsplit, min((room + ctas) / (2 * ctas), units / a.upw)));
 }
 
@@ -114,8 +115,8 @@ struct ShareTiles {
   int un, first, n;   // tiles of segment 0; the warp's
   __device__ __forceinline__ ShareTiles(const ShareJob& j, int ts) {
     un = (j.n0 + ts - 1) / ts;
-    const int U = un + (j.n1 + ts - 1) / ts;
-    const int u0 = (int)((long long)U * j.split / j.ns), u1 = (int)((long long)U * (j.split + 1) / j.ns);
+    const int U = un + (j.n1 + ts - 1) / ts, per = U / j.ns, more = U - per * j.ns;   // the first `more` take one more
+    const int u0 = per * j.split + min(j.split, more), u1 = u0 + per + (j.split < more);
     first = u0 + j.sub;
     n = j.NQ > 0 && u1 > first ? (u1 - first + j.warps - 1) / j.warps : 0;
   }
@@ -501,7 +502,8 @@ __global__ void __launch_bounds__(kShareTcThreads, 2)
   }
   if (j.split >= j.ns) return;
   const int up = (j.n0 + TS - 1) / TS, U = up + (j.n1 + TS - 1) / TS;
-  const int u0 = (int)((long long)U * j.split / j.ns), n = (int)((long long)U * (j.split + 1) / j.ns) - u0;
+  const int per = U / j.ns, more = U - per * j.ns;   // the first `more` splits take a unit more
+  const int u0 = per * j.split + min(j.split, more), n = per + (j.split < more);
   if (n == 0) {   // nothing shared at all: one split without keys
     for (int x = tid; x < j.NQ; x += kShareTcThreads) {
       float* pp = share_part(part, a, j.slot, share_row(a, j, j.row0 + x));
@@ -1263,7 +1265,7 @@ LOGKV_API int logkv_shared_attention(const logkv_layout_t* layout, const logkv_s
   a.tile_rows = p.tile_rows;
   a.own_tiles = p.own_tiles;
   a.slots = p.slots;
-  a.own_work = p.own_work;
+  a.own_work = (float)p.own_work;
   a.scale_log2 = x->scale * 1.4426950408889634f;
   a.mass_log2 = x->qx * a.scale_log2;
   a.q = x->q;

@@ -10,8 +10,8 @@
 //
 // Bound by HBM from a few MB per SM on: keys and values are read once per 128 (16) query rows.  Measured on B200, device
 // time: 8 requests of 8 rows over 7.8K shared and 242 own keys (8 groups, head dim 128, bf16: 314 MB) 60 us, 0.79 of the
-// measured copy bandwidth, where log_kv_chunk_attention takes 367; one request of 4 rows (31 MB) 12.5 us (34); below that
-// latency: 3 requests of 16 rows over 2.0K keys 16 us.
+// measured copy bandwidth, where log_kv_chunk_attention takes 367; one request of 4 rows (31 MB) 12.1 us (34); below that
+// latency: 3 requests of 16 rows over 2.0K keys 14.5 us.
 #include <algorithm>
 #include <cstring>
 
@@ -69,8 +69,9 @@ struct ShareJob {
 
 // GROUPED: own lanes of fewer than four warps.  Code of its own, since what it takes to tell the groups apart costs the
 // calls without them 1 to 2 us.
+// What it takes but the prefix's length: all that a kernel may work out before its predecessor has ended.
 template <bool GROUPED>
-__device__ __forceinline__ ShareJob share_job(const ShareGeo& a, const logkv_prefix_t& pre, int tile_keys) {
+__device__ __forceinline__ ShareJob share_job(const ShareGeo& a, const logkv_prefix_t& pre) {
   ShareJob j;
   int x = blockIdx.x;
   const int shared = a.shared_lanes * a.nsplit * a.tiles, warp = threadIdx.x >> 5;
@@ -101,13 +102,18 @@ __device__ __forceinline__ ShareJob share_job(const ShareGeo& a, const logkv_pre
     j.g = lane % a.G;
     j.row0 = x / a.nsplit * a.tile_rows;
     j.NQ = min(a.tile_rows, a.W * a.rf * a.T - j.row0);
-    const int ln = j.b * a.G + j.g;
-    j.n0 = share_prefix_length(pre, ln);
+    j.n0 = 0;
     j.n1 = a.w0;
-    j.r0 = (size_t)ln * pre.capacity;
-    j.ns = share_splits(a, (j.n0 + tile_keys - 1) / tile_keys + (j.n1 + tile_keys - 1) / tile_keys, tile_keys);
+    j.r0 = ((size_t)j.b * a.G + j.g) * pre.capacity;
+    j.ns = 0;
   }
   return j;
+}
+// The rest: a shared lane's keys and splits.
+__device__ __forceinline__ void share_keys(const ShareGeo& a, const logkv_prefix_t& pre, int tile_keys, ShareJob& j) {
+  if (j.own) return;
+  j.n0 = share_prefix_length(pre, j.b * a.G + j.g);
+  j.ns = share_splits(a, (j.n0 + tile_keys - 1) / tile_keys + (j.n1 + tile_keys - 1) / tile_keys, tile_keys);
 }
 
 // Key tiles of the split that the warp takes: first, first + warps, ...
@@ -441,8 +447,9 @@ __global__ void __launch_bounds__(kShareWarps * 32, D <= 128 ? 2 : 1)
     share_mma_kernel(ShareGeo a, logkv_prefix_t pre, const __nv_bfloat16* rk, const __nv_bfloat16* rv, float* part) {
   extern __shared__ uint4 smem4[];
   __shared__ ShareJoin join;
+  ShareJob j = share_job<GROUPED>(a, pre);
   pdl_entry();
-  const ShareJob j = share_job<GROUPED>(a, pre, ShareShape<D>::TS);
+  share_keys(a, pre, ShareShape<D>::TS, j);
   if (j.split < j.ns) share_mma<D>(a, j, pre, rk, rv, part, reinterpret_cast<unsigned char*>(smem4), join);
 }
 
@@ -492,9 +499,27 @@ __global__ void __launch_bounds__(kShareTcThreads, 2)
       pv_done[2];
   __shared__ uint32_t sh_tmem;
   if (threadIdx.x < 4) tc::prefetch_tensormap(threadIdx.x < 2 ? &maps.k[threadIdx.x] : &maps.v[threadIdx.x - 2]);
-  pdl_entry();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const ShareJob j = share_job<true>(a, pre, TS);
+  ShareJob j = share_job<true>(a, pre);
+  const int live = (j.NQ + 31) / 32;   // softmax warps with rows
+  if (tid == 0) {
+    tc::mbar_init(&q_full, 32 * live);
+    for (int i = 0; i < ST; ++i) {
+      tc::mbar_init(&k_full[i], 1);
+      tc::mbar_init(&v_full[i], 1);
+      tc::mbar_init(&k_empty[i], 1);
+      tc::mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < MR; ++i) tc::mbar_init(&m_full[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&p_full[i], 32 * live);
+      tc::mbar_init(&pv_done[i], 1);
+    }
+    tc::mbar_fence_init();
+  }
+  pdl_entry();
+  share_keys(a, pre, TS, j);
   unsigned char* raw = reinterpret_cast<unsigned char*>(smem4);
   if (j.own) {
     if (warp < kShareWarps) share_mma<D>(a, j, pre, rk, rv, part, raw, join);
@@ -514,23 +539,6 @@ __global__ void __launch_bounds__(kShareTcThreads, 2)
   }
   unsigned char* base = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
   const uint32_t base_s = tc::smem_u32(base);
-  const int live = (j.NQ + 31) / 32;   // softmax warps with rows
-  if (tid == 0) {
-    tc::mbar_init(&q_full, 32 * live);
-    for (int i = 0; i < ST; ++i) {
-      tc::mbar_init(&k_full[i], 1);
-      tc::mbar_init(&v_full[i], 1);
-      tc::mbar_init(&k_empty[i], 1);
-      tc::mbar_init(&v_empty[i], 1);
-    }
-    for (int i = 0; i < MR; ++i) tc::mbar_init(&m_full[i], 1);
-    for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&s_full[i], 1);
-      tc::mbar_init(&p_full[i], 32 * live);
-      tc::mbar_init(&pv_done[i], 1);
-    }
-    tc::mbar_fence_init();
-  }
   if (warp == 0) {
     tc::tmem_alloc(&sh_tmem, S::COLS);
     tc::tmem_relinquish();
@@ -791,9 +799,10 @@ __global__ void __launch_bounds__(kShareWarps * 32, ShareF32Shape<D>::CTAS)
   constexpr int TS = S::TS, LD = S::LD, KS = S::KS, DT = S::DT, CPR = S::CPR, ST = S::ST;
   extern __shared__ uint4 smem4[];
   __shared__ ShareJoin join;
+  ShareJob j = share_job<GROUPED>(a, pre);
   pdl_entry();
+  share_keys(a, pre, TS, j);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
-  const ShareJob j = share_job<GROUPED>(a, pre, TS);
   if (j.split >= j.ns) return;
   const ShareTiles u(j, TS);
   const int un = u.un, mine = u.n;

@@ -174,8 +174,10 @@ def _rope(cache) -> _lib.Rope:
         raise ValueError(f"cos_cache/sin_cache must be 2-D and equal in shape, got {cos.shape} and {sin.shape}")
     if cache.rope_n_elem and cos.size(1) != cache.rope_n_elem:
         raise ValueError("cos_cache width must equal rope_n_elem")
-    return _lib.Rope(_lib.ptr(cos.contiguous()), _lib.ptr(sin.contiguous()), cos.size(0), cache.rope_n_elem,
-                     _lib.DTYPE_CODES[cos.dtype])
+    cos, sin = cos.contiguous(), sin.contiguous()
+    rope = _lib.Rope(_lib.ptr(cos), _lib.ptr(sin), cos.size(0), cache.rope_n_elem, _lib.DTYPE_CODES[cos.dtype])
+    rope.tables = cos, sin   # the memory behind the addresses: strided tables have a copy each, freed with the struct
+    return rope
 
 
 def _stream(cache) -> ctypes.c_void_p:

@@ -181,8 +181,8 @@ class LogStructuredKVCache(nn.Module):
         P, R, K, L, Bs = self.alpha_exact_tokens, self.recent_capacity, self.K_max, self.L_alloc, self.B_prime
         z = dict(device=device)
         reg = lambda name, t: self.register_buffer(name, t, persistent=False)  # noqa: E731
-        reg("cos_cache", cos_cache.to(device=device))
-        reg("sin_cache", sin_cache.to(device=device))
+        reg("cos_cache", cos_cache.to(device=device).contiguous())
+        reg("sin_cache", sin_cache.to(device=device).contiguous())
         reg("recent_k", torch.zeros(batch, groups, R, self.slot_k_dim, dtype=dtype, **z))
         reg("recent_v", torch.zeros(batch, groups, R, v_dim, dtype=dtype, **z))
         reg("recent_k_raw", torch.zeros(batch, groups, R, k_dim, dtype=dtype, **z))

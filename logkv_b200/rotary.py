@@ -83,20 +83,26 @@ def launch(cache, parts, positions, pos0: int, interleaved: int, *, positions_ou
         a.ends_stride, a.ends_out_stride = ends.stride(0), ends_out.stride(0)
     status = getattr(cache, "_read_status", None)   # a foreign cache has none
     a.status = None if status is None else status.data_ptr()
-    if status is not None and native(cache) is None:
-        cache._rotary = _Native(cache)
-    _lib.check(_lib.lib().logkv_rotate(ctypes.byref(_rope(cache)), ctypes.byref(a),
-                                       _lib.stream_ptr(cache.recent_k.device)), "logkv_rotate")
+    rope = _rope(cache)
+    if status is not None and native(cache) is None and _contiguous(cache):
+        cache._rotary = _Native(cache, rope)
+    _lib.check(_lib.lib().logkv_rotate(ctypes.byref(rope), ctypes.byref(a), _lib.stream_ptr(cache.recent_k.device)),
+               "logkv_rotate")
+
+
+def _contiguous(cache) -> bool:
+    """Whether the tables can be read where they are; strided ones are copied in every call."""
+    b = cache._buffers
+    return b["cos_cache"].is_contiguous() and b["sin_cache"].is_contiguous()
 
 
 class _Native:
     """The host binding's calls with their arguments that do not change for a cache."""
 
-    def __init__(self, cache):
-        from .attention import _rope
+    def __init__(self, cache, rope):
         host = _lib.host()
         self.rotate, self.append, self.fn = host.rotate, host.append, _lib.address("logkv_rotate")
-        self.tables = _rope(cache)
+        self.tables = rope
         self.rope, self.dtype = ctypes.addressof(self.tables), cache.cos_cache.dtype
         self.status = cache._read_status.data_ptr()
 
@@ -109,7 +115,8 @@ def native(cache):
     b = cache._buffers
     cos, sin = b["cos_cache"], b["sin_cache"]
     t = n.tables
-    same = t.cos == cos.data_ptr() and t.sin == sin.data_ptr() and t.rows == cos.size(0) and n.dtype is cos.dtype
+    same = (t.cos == cos.data_ptr() and t.sin == sin.data_ptr() and t.rows == cos.size(0) and n.dtype is cos.dtype
+            and _contiguous(cache))
     return n if same or not cache.rope_n_elem else None
 
 

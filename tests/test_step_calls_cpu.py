@@ -1,0 +1,56 @@
+"""Calls of a decoding step's operators that their other tests do not make, as far as the host goes."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from hypotheses import make_cache
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from logkv_b200 import build
+    build.build()
+    from logkv_b200 import _lib
+    return _lib.lib()
+
+
+def strided_tables(rows, n):
+    """Rotary tables as every other column of a wider one."""
+    from logkv_b200 import scaled_rope_tables
+    out = []
+    for t in scaled_rope_tables(rows, n, base=1e4):
+        wide = torch.full((rows, 2 * n), 7.0)
+        wide[:, ::2] = t
+        out.append(wide[:, ::2])
+    return out
+
+
+def test_strided_tables_keep_their_memory(lib, monkeypatch):
+    """The addresses of a rotation's tables are those of tensors that live as long as the addresses do."""
+    from logkv_b200 import _lib
+    from logkv_b200.attention import _rope
+    cos, sin = strided_tables(564, 64)
+    cache = make_cache(torch.float32, B=2, G=2, D=64, levels=0, R=5, max_seq=500, device="cpu")
+    monkeypatch.setattr(_lib, "ptr", lambda t: t.contiguous().data_ptr())
+    cache.cos_cache, cache.sin_cache = cos, sin
+    rope = _rope(cache)
+    assert rope.cos != rope.sin
+    for at, t in ((rope.cos, cos), (rope.sin, sin)):
+        held = torch.frombuffer((ctypes.c_float * t.numel()).from_address(at), dtype=torch.float32)
+        assert torch.equal(held.view(t.shape), t)
+
+
+def test_constructor_lays_strided_tables_out(lib):
+    from logkv_b200 import LogStructuredKVCache
+    cos, sin = strided_tables(600, 64)
+    shape = (2, 2, 500, 64)
+    cache = LogStructuredKVCache(
+        shape, shape, B=32, recent_size=64, device="cpu", dtype=torch.float32, semantic_clusters=True,
+        semantic_anchor_mode="mid", allocate_second_order=False, cluster_k_max=4, semantic_flush_granularity=64,
+        alpha_exact_tokens=32, alpha_span_max_tokens=8, beta_novelty=True, beta_adaptive_merge=True, cos_cache=cos,
+        sin_cache=sin, rope_n_elem=64)
+    assert cache.cos_cache.is_contiguous() and cache.sin_cache.is_contiguous()
+    assert torch.equal(cache.cos_cache, cos) and torch.equal(cache.sin_cache, sin)

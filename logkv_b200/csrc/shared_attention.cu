@@ -984,8 +984,8 @@ __global__ void __launch_bounds__(kShareWarps * 32, ShareF32Shape<D>::CTAS)
 // ---------------------------------------------------------------- combine
 // WPR warps per output row (1 or 4): each joins its share of the row's partials (the shared splits, then the own
 // ones), NB at a time with all of their loads in flight, then the warps in order.  TS: the key tile of the kernel that
-// wrote the shared partials.  What does not depend on the attention kernel (this row's partials and their places) is
-// worked out before the wait for it.
+// wrote the shared partials.  Index arithmetic alone stands before the wait: the prefix's length comes from a kernel in
+// front of the attention's, and what those wrote is visible here only behind it.
 template <typename T, int D, int TS, int WPR>
 __global__ void __launch_bounds__(128) share_combine_kernel(ShareGeo a, logkv_prefix_t pre, const float* part, T* out) {
   constexpr int PER = (D + 127) / 128, NB = D > 128 ? 4 : 10;
@@ -993,17 +993,14 @@ __global__ void __launch_bounds__(128) share_combine_kernel(ShareGeo a, logkv_pr
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
   const size_t row = (size_t)blockIdx.x * (4 / WPR) + warp / WPR;
   const bool live = WPR > 1 || row < (size_t)a.B * a.H * a.T;
-  int shared = 0;
-  if (live) {
-    const int bh = (int)(row / a.T), b = bh / a.H / a.W * a.W, g = bh % a.H / a.rf;
-    shared = share_splits(a, (share_prefix_length(pre, b * a.G + g) + TS - 1) / TS + (a.w0 + TS - 1) / TS, TS);
-  }
-  const int ns = shared + a.nown, skip = a.nsplit - shared;   // partials; unused slots between the two kinds
+  const int bh = (int)(row / a.T), ln = bh / a.H / a.W * a.W * a.G + bh % a.H / a.rf, window = (a.w0 + TS - 1) / TS;
   const size_t stride = (size_t)a.B * a.H * a.T * (D + 4);
   const float* p0 = part + row * (D + 4);
-  auto at = [&](int s) { return p0 + (size_t)(s < shared ? s : s + skip) * stride; };
   pdl_entry();
   if (!live) return;
+  const int shared = share_splits(a, (share_prefix_length(pre, ln) + TS - 1) / TS + window, TS);
+  const int ns = shared + a.nown, skip = a.nsplit - shared;   // partials; unused slots between the two kinds
+  auto at = [&](int s) { return p0 + (size_t)(s < shared ? s : s + skip) * stride; };
   float m = -INFINITY, l = 0.f;
   float4 o[PER];
 #pragma unroll

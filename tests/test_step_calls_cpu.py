@@ -2,6 +2,8 @@
 from __future__ import annotations
 
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -54,3 +56,17 @@ def test_constructor_lays_strided_tables_out(lib):
         sin_cache=sin, rope_n_elem=64)
     assert cache.cos_cache.is_contiguous() and cache.sin_cache.is_contiguous()
     assert torch.equal(cache.cos_cache, cos) and torch.equal(cache.sin_cache, sin)
+
+
+def test_shared_kernels_read_the_prefix_behind_their_wait():
+    """What an earlier kernel wrote is visible behind a kernel's own wait (pdl_entry) only: in front of it nothing looks
+    at the prefix's length."""
+    import logkv_b200
+    at = os.path.join(os.path.dirname(logkv_b200.__file__), "csrc", "shared_attention.cu")
+    with open(at) as fh:
+        kernels = [k.split("\n}\n")[0] for k in fh.read().split("__global__")[1:]]
+    assert len(kernels) == 4
+    for k in kernels:
+        before, entry, after = k.partition("pdl_entry();")
+        assert entry and re.search(r"share_prefix_length|share_keys", after)
+        assert not re.search(r"share_prefix_length|share_keys|pre\.", before), before

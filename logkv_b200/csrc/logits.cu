@@ -314,7 +314,10 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
     for (int i = 0; i < LT / 32; ++i) listed += warp_sums[i];
     for (int i = threadIdx.x; i < listed; i += kLogitsThreads + LT) {
       T* e = y + token[i];
-      Elem<T>::store(e, adjust(Elem<T>::load(e), count[i]));
+      const float z = Elem<T>::load(e);
+      // The mask has the last word: a banned token stays -inf whatever its penalties are (they may be infinite).
+      if (mask && z == -INFINITY && !(mask_bits(mask, token[i], 1, a.vocab) & 1)) continue;
+      Elem<T>::store(e, adjust(z, count[i]));
     }
   }
   if (a.bias_count) {

@@ -44,3 +44,38 @@ def test_strided_tables(tables):
         assert torch.equal(log_kv_rotate(a, q, k)[0], log_kv_rotate(b, q, k)[0])
     a.cos_cache = b.cos_cache[:1].expand(512, 64)                 # one row for all, at the same address
     check(a, 4, 9, pos, "half")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [64, 1003, 5000])
+def test_banned_tokens_of_the_history(dtype, V):
+    """A banned token is -inf whatever its row's penalties, its count or its logit are; the others follow the formula."""
+    from logkv_b200 import adjust_logits
+    inf, nan = float("inf"), float("nan")
+    rows = 7
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(rows, V, generator=gen, device="cuda").to(dtype)
+    x[:, 5], x[:, 6] = -inf, nan
+    h = torch.randint(0, V, (rows, 40), generator=gen, device="cuda")
+    h[:, :4] = torch.tensor([3, 5, 6, 9], device="cuda")
+    allowed = torch.rand(rows, V, generator=gen, device="cuda") < 0.5
+    allowed[:, 3] = allowed[:, 5] = allowed[:, 6] = False
+    allowed[:, 9] = True
+    bits = torch.zeros(rows, (V + 31) // 32 * 32, dtype=torch.bool, device="cuda")
+    bits[:, :V] = allowed
+    mask = (bits.view(rows, -1, 32).long() << torch.arange(32, device="cuda")).sum(-1).to(torch.int32)
+    rep = torch.tensor([1.0, 2.0, 1.5, 0.5, inf, 1.0, 1.0], device="cuda")
+    pres = torch.tensor([-inf, 0.25, inf, 0.0, 0.0, -inf, nan], device="cuda")
+    freq = torch.tensor([0.0, -inf, 0.0, 3e38, 0.0, inf, 0.0], device="cuda")
+    bias = (torch.tensor([3, 9, 11], device="cuda"), torch.tensor([inf, 0.5, -1.0], device="cuda"))
+    for b in (None, bias):
+        kw = dict(history=h, repetition=rep, presence=pres, frequency=freq, mask=mask, bias=b)
+        got = adjust_logits(x, **kw)
+        assert (got[~allowed] == -inf).all()
+        for _ in range(2):
+            assert torch.equal(adjust_logits(x, **kw).nan_to_num(7.0), got.nan_to_num(7.0))
+        y = x.clone()
+        adjust_logits(y, out=y, **kw)
+        assert torch.equal(y.nan_to_num(7.0), got.nan_to_num(7.0))
+        free = adjust_logits(x, **{**kw, "mask": None})
+        assert torch.equal(got[allowed].nan_to_num(7.0), free[allowed].nan_to_num(7.0))

@@ -42,6 +42,13 @@ at::Tensor bytes(size_t n, const at::Tensor& like) {
 
 PyObject* failed(int rc) { return PyLong_FromLong(rc); }
 
+// Whether the Python numbers read before fitted their C types; if not, the Python path says what is wrong with them.
+bool in_range() {
+  if (!PyErr_Occurred()) return true;
+  PyErr_Clear();
+  return false;
+}
+
 bool wants_gradient(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
 // [B, heads, T, D] rows in dtype and on the device of `like`, 16-byte aligned, without a gradient to record.
@@ -175,6 +182,7 @@ PyObject* shared(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!PyLong_Check(args[13])) Py_RETURN_NONE;
     tail = PyLong_AsLong(args[13]);
   }
+  if (!in_range()) Py_RETURN_NONE;
   logkv_shared_args_t x{};
   x.scale = (float)PyFloat_AsDouble(args[14]);
   x.qx = (float)PyFloat_AsDouble(args[15]);
@@ -367,7 +375,7 @@ bool per_row(PyObject* o, const at::Tensor& x, bool whole, PerRow& out) {
   if (PyFloat_Check(o) || PyLong_Check(o)) {
     if (whole && !PyLong_Check(o)) return false;
     out.value = PyFloat_AsDouble(o);
-    return true;
+    return in_range();
   }
   const at::Tensor* t = tensor(o);
   if (!t || t->dim() != x.dim() - 1 || t->device() != x.device() || !t->is_contiguous() ||

@@ -23,10 +23,13 @@ def _number(name: str, value, lead, dev, positive: bool = False):
             raise ValueError(f"{name} must be a number or float32 {list(lead)} on {dev}, got {value.dtype} "
                              f"{tuple(value.shape)} on {value.device}")
         return 1.0, value.contiguous()
-    value = float(value)
-    if not math.isfinite(value) or (positive and value <= 0):
-        raise ValueError(f"{name} must be finite{' and positive' if positive else ''}, got {value}")
-    return value, None
+    try:
+        held = ctypes.c_float(float(value)).value    # as the kernel has it
+    except OverflowError:
+        held = math.inf
+    if not math.isfinite(held) or (positive and held <= 0):
+        raise ValueError(f"{name} must be finite{' and positive' if positive else ''} in float32, got {str(value)[:40]}")
+    return held, None
 
 
 def _count(name: str, value, lead, dev):

@@ -70,3 +70,16 @@ def test_shared_kernels_read_the_prefix_behind_their_wait():
         before, entry, after = k.partition("pdl_entry();")
         assert entry and re.search(r"share_prefix_length|share_keys", after)
         assert not re.search(r"share_prefix_length|share_keys|pre\.", before), before
+
+
+def test_penalties_beyond_float32(lib):
+    """Numbers that float32 has no finite (positive) value for are refused like infinities."""
+    from logkv_b200 import adjust_logits
+    x = torch.zeros(2, 3, 70)
+    for name, bad in [("repetition", 1e300), ("repetition", 1e-60), ("repetition", 10 ** 400), ("presence", 1e300),
+                      ("presence", -1e39), ("presence", 10 ** 400), ("frequency", -10 ** 400), ("frequency", 3.5e38)]:
+        with pytest.raises(ValueError, match="finite"):
+            adjust_logits(x, **{name: bad})
+    for ok in (3.4e38, 1e-40):
+        with pytest.raises(ValueError, match="CUDA tensor"):
+            adjust_logits(x, repetition=ok, presence=-ok)

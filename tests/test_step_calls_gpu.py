@@ -79,3 +79,31 @@ def test_banned_tokens_of_the_history(dtype, V):
         assert torch.equal(y.nan_to_num(7.0), got.nan_to_num(7.0))
         free = adjust_logits(x, **{**kw, "mask": None})
         assert torch.equal(got[allowed].nan_to_num(7.0), free[allowed].nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("name", ["prompt", "lengths", "repetition", "presence", "frequency"])
+def test_numbers_out_of_range(name):
+    """Python integers of any size are refused like others, and a prompt longer than the history is the whole of it."""
+    from logkv_b200 import adjust_logits
+    x = torch.randn(3, 100, device="cuda")
+    h = torch.randint(0, 100, (3, 9), device="cuda")
+    kw = dict(history=h, repetition=1.5, frequency=0.25)
+    want = adjust_logits(x, prompt=9, **kw)
+    if name == "prompt":
+        assert torch.equal(adjust_logits(x, prompt=10 ** 400, **kw), want)
+        return
+    for bad in (10 ** 400, -10 ** 400):
+        with pytest.raises(ValueError):
+            adjust_logits(x, prompt=9, **{**kw, name: bad})
+
+
+@pytest.mark.parametrize("name", ["beams", "window_from"])
+def test_shared_numbers_out_of_range(name):
+    from logkv_b200 import log_kv_shared_attention
+    cache = make(BF16, B=4)
+    q, k, v = (t.contiguous() for t in projected(cache, 4, 1, 3))
+    f = lambda **kw: log_kv_shared_attention(cache, q, k, v, 0.125, **{"beams": 2, "window_from": 0, **kw})  # noqa: E731
+    f()
+    for bad in (10 ** 30, -10 ** 30):
+        with pytest.raises(ValueError):
+            f(**{name: bad})

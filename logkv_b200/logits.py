@@ -60,6 +60,24 @@ def _table(name: str, t, lead, dev, dtypes, shared: bool):
     return t, t.stride(0)
 
 
+def _rows_overlap(x) -> bool:
+    """Whether two rows of x ([..., V], V elements next to each other) have an element in common."""
+    if not x.numel():
+        return False
+    V, reach = x.size(-1), x.size(-1)
+    dims = sorted((s, n) for n, s in zip(x.shape[:-1], x.stride()) if n > 1)
+    for s, n in dims:                    # rows inside one another, as a tensor's usually are
+        if s < reach:
+            break
+        reach += (n - 1) * s
+    else:
+        return False
+    at = torch.zeros(1, dtype=torch.int64, device="cpu")
+    for s, n in dims:                    # otherwise where each of them starts
+        at = (at[:, None] + s * torch.arange(n, device="cpu")).flatten()
+    return bool((at.sort().values.diff() < V).any())
+
+
 def adjust_logits(logits, *, history=None, lengths=None, prompt=0, repetition=1.0, presence=0.0, frequency=0.0,
                   bias=None, mask=None, out=None):
     """Next-token logits with penalties for repeated tokens, biases and a grammar mask, in this order.
@@ -131,6 +149,8 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt=0, repetition=1.
         mask, a.mask_stride = _table("mask", mask, lead, dev, (torch.int32,), True)
         if mask.size(-1) != (V + 31) // 32:
             raise ValueError(f"mask must hold {(V + 31) // 32} words a row, got {mask.size(-1)}")
+    if out is logits and _rows_overlap(logits):
+        raise ValueError("logits adjusted in place must not share memory between rows")
     if dev.type != "cuda":
         raise ValueError("logits must be a CUDA tensor")
     if out is None:
@@ -140,8 +160,6 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt=0, repetition=1.
         raise ValueError(f"out must be logits itself, or contiguous {list(logits.shape)} {logits.dtype} on {dev}")
     elif out is not logits and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() and rows:
         raise ValueError("out must be logits itself or have memory of its own")
-    elif out is logits and any(n > 1 and s < V for n, s in zip(lead, logits.stride())):
-        raise ValueError("logits adjusted in place must not share memory between rows")
     if not rows:
         return out
     with _lib.on_device(dev):

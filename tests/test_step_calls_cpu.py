@@ -83,3 +83,19 @@ def test_penalties_beyond_float32(lib):
     for ok in (3.4e38, 1e-40):
         with pytest.raises(ValueError, match="CUDA tensor"):
             adjust_logits(x, repetition=ok, presence=-ok)
+
+
+def test_in_place_rows_that_share_memory(lib):
+    """Logits adjusted in place whose rows overlap, in whatever way their strides make it, are refused."""
+    from logkv_b200 import adjust_logits
+    base = torch.zeros(4000)
+    for shape, strides in [((3, 2, 70), (70, 70, 1)), ((2, 3, 70), (140, 70, 1)), ((3, 2, 70), (70, 140, 1)),
+                           ((3, 70), (69, 1)), ((2, 2, 70), (0, 70, 1)), ((3, 3, 70), (70, 200, 1)), ((2, 70), (0, 1))]:
+        x = base.as_strided(shape, strides)
+        with pytest.raises(ValueError, match="share memory"):
+            adjust_logits(x, out=x)
+    for shape, strides in [((3, 2, 70), (140, 70, 1)), ((3, 2, 70), (70, 210, 1)), ((3, 1, 70), (70, 0, 1)),
+                           ((1, 3, 70), (0, 75, 1)), ((3, 70), (80, 1)), ((0, 2, 70), (0, 70, 1)), ((2, 2, 1), (2, 1, 1))]:
+        x = base.as_strided(shape, strides)
+        with pytest.raises(ValueError, match="CUDA tensor"):
+            adjust_logits(x, out=x)

@@ -167,6 +167,17 @@ def log_kv_rotate(cache, q, k, input_pos=None, *, layout: str = "half"):
     return qo, ko, raw
 
 
+def _entry(name: str, value, infinite: bool = False) -> float:
+    """A scaling's entry as a finite number (or one that may be infinite)."""
+    try:
+        number = float(value)
+    except (TypeError, ValueError, OverflowError):
+        number = math.nan
+    if not math.isfinite(number) and not (infinite and number == math.inf):
+        raise ValueError(f"{name} must be a finite number, got {value!r}")
+    return number
+
+
 def scaled_rope_tables(length: int, n_elem: int, *, base: float = 10000.0, scaling: dict | None = None, device=None,
                        dtype=torch.float32):
     """(cos, sin), each [length, n_elem], of the positions 0 .. length - 1 as ``LogStructuredKVCache`` takes them.
@@ -199,9 +210,13 @@ def scaled_rope_tables(length: int, n_elem: int, *, base: float = 10000.0, scali
     missing = [name for name in known[kind] if name not in s and name not in ("fast", "slow", "attention")]
     if missing:
         raise ValueError(f"scaling {kind!r} needs {missing}")
-    f = float(s.get("factor", 1.0))
-    if not (math.isfinite(base) and base > 1 and math.isfinite(f) and f >= 1):
+    entry = lambda name, default: _entry(name, s.get(name, default))  # noqa: E731
+    f = entry("factor", 1.0)
+    if not (math.isfinite(base) and base > 1 and f >= 1):
         raise ValueError(f"base must be above 1 and factor at least 1, got {base} and {f}")
+    original = entry("original", 1.0)
+    if original <= 0:
+        raise ValueError(f"original must be positive, got {original}")
     i = np.arange(n // 2, dtype=np.float64)
     amplitude = 1.0
     if kind == "base" and n > 2:
@@ -210,22 +225,22 @@ def scaled_rope_tables(length: int, n_elem: int, *, base: float = 10000.0, scali
     if kind == "linear" or (kind == "base" and n == 2):
         inv = inv / f
     elif kind == "bands":
-        turns = float(s["original"]) * inv / (2 * math.pi)
-        low, high = float(s["low"]), float(s["high"])
+        turns = original * inv / (2 * math.pi)
+        low, high = entry("low", None), _entry("high", s["high"], infinite=True)   # infinite: no pair is kept
         if not 0 < low < high:
             raise ValueError(f"bands need 0 < low < high, got {low} and {high}")
         keep = np.clip((turns - low) / (high - low), 0.0, 1.0)
         inv = inv * (keep + (1 - keep) / f)
     elif kind == "yarn":
-        fast, slow = float(s.get("fast", 32)), float(s.get("slow", 1))
+        fast, slow = entry("fast", 32), entry("slow", 1)
         if not 0 < slow < fast:
             raise ValueError(f"yarn needs 0 < slow < fast, got {slow} and {fast}")
         # Index of the pair that turns `t` times over the original positions.
-        at = lambda t: n * math.log(float(s["original"]) / (t * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+        at = lambda t: n * math.log(original / (t * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
         lo, hi = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), n - 1)
         stretch = np.clip((i - lo) / max(hi - lo, 1e-3), 0.0, 1.0)
         inv = inv * ((1 - stretch) + stretch / f)
-        amplitude = float(s.get("attention", 0.1 * math.log(f) + 1.0))
+        amplitude = entry("attention", 0.1 * math.log(f) + 1.0)
     inv = torch.from_numpy(inv).to(device or "cpu")
     cos, sin = (torch.empty(length, n, dtype=dtype, device=inv.device) for _ in range(2))
     for at0 in range(0, length, 65536):     # the float64 angles of a part of the positions at a time

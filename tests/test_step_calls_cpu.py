@@ -99,3 +99,20 @@ def test_in_place_rows_that_share_memory(lib):
         x = base.as_strided(shape, strides)
         with pytest.raises(ValueError, match="CUDA tensor"):
             adjust_logits(x, out=x)
+
+
+def test_scaling_entries_are_checked(lib):
+    from logkv_b200 import scaled_rope_tables as f
+    bands = {"kind": "bands", "factor": 2, "original": 10, "low": 1, "high": 4}
+    yarn = {"kind": "yarn", "factor": 2, "original": 10}
+    inf, nan = float("inf"), float("nan")
+    for s, name, bads in [(bands, "original", (0, -5, inf, nan, None)), (yarn, "original", (0, -5, inf, nan, None, "x")),
+                          (yarn, "attention", (None, inf, nan, "x")), (bands, "low", (None, nan)),
+                          (bands, "high", (None, nan)), (yarn, "fast", (None, inf, nan)), (yarn, "slow", (None, nan)),
+                          (bands, "factor", (None, inf, "x"))]:
+        for bad in bads:
+            with pytest.raises(ValueError, match=name):
+                f(10, 8, scaling={**s, name: bad})
+    all_divided = f(10, 8, scaling={"kind": "linear", "factor": 2})
+    assert torch.equal(f(10, 8, scaling={**bands, "high": inf})[0], all_divided[0])
+    f(10, 8, scaling=bands), f(10, 8, scaling={**yarn, "attention": 0.9})

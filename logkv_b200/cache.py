@@ -680,11 +680,13 @@ class LogStructuredKVCache(nn.Module):
         elif span_ends is None or len(span_ends) != B or any(len(r) != n for r in span_ends):
             raise ValueError("AlphaLogKV span boundaries must match the input batch and token count")
         else:
-            ends = torch.tensor(span_ends, dtype=torch.uint8).to(dev)
+            ends = None
         self._check_room(n)
         if n == 0:
             return
         with _lib.on_device(dev):
+            if ends is None:
+                ends = self._stage_ends(span_ends, n)
             k_raw, v = rotary.last_contiguous(k_raw), rotary.last_contiguous(v)
             pos0, c0 = self.token_count, self.recent_count
             take = self._chunk_flush_take(n)
@@ -817,10 +819,15 @@ class LogStructuredKVCache(nn.Module):
         if span_ends_device is not None:
             ends = span_ends_device.to(device=self.recent_pos.device, dtype=torch.uint8).contiguous()
         else:
-            host = torch.tensor(span_ends, dtype=torch.uint8)
-            ends = self._ends_stage[:self.batch_size * n].view(self.batch_size, n)
-            ends.copy_(host.pin_memory() if self.recent_pos.is_cuda else host, non_blocking=True)
+            ends = self._stage_ends(span_ends, n)
         return k, k_raw, v, positions, ends, n
+
+    def _stage_ends(self, span_ends, n: int):
+        """Host span-end flags ([batch][n]) on the device, without a wait."""
+        host = torch.tensor(span_ends, dtype=torch.uint8)
+        ends = self._ends_stage[:self.batch_size * n].view(self.batch_size, n)
+        ends.copy_(host.pin_memory() if self.recent_pos.is_cuda else host, non_blocking=True)
+        return ends
 
     def _check_room(self, n: int) -> None:
         if n > self.recent_size:

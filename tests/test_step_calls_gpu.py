@@ -81,6 +81,26 @@ def test_banned_tokens_of_the_history(dtype, V):
         assert torch.equal(got[allowed].nan_to_num(7.0), free[allowed].nan_to_num(7.0))
 
 
+def test_append_of_host_span_ends_does_not_wait():
+    """Host lists of span ends go to the device without a wait, in the window write and in a flush's."""
+    cache = make(BF16)
+    chunks = [projected(cache, 2, T, T)[1:] for T in (64, 20, 64)]
+    ends = [torch.rand(2, k.size(2), generator=torch.Generator().manual_seed(k.size(2))) < 0.3 for k, _ in chunks]
+    other = make(BF16)
+    for (k, v), e in zip(chunks, ends):
+        other.add_recent_rotated(k, v, span_ends_device=e.cuda())
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for (k, v), e in zip(chunks, ends):
+            cache.add_recent_rotated(k, v, span_ends=e.tolist())
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    x, y = state(cache), state(other)
+    for name in x:
+        assert torch.equal(x[name], y[name]), name
+
+
 @pytest.mark.parametrize("name", ["prompt", "lengths", "repetition", "presence", "frequency"])
 def test_numbers_out_of_range(name):
     """Python integers of any size are refused like others, and a prompt longer than the history is the whole of it."""

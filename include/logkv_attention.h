@@ -186,8 +186,10 @@ LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_sta
  * `tokens` new ones:
  *   out = softmax(scale * (q . k_s + qx * mass_s)) v_s,
  * with causal != 0 (tokens = q_tokens) new token j visible to query token t iff j <= t, else every new token
- * visible.  Rows are taken to agree as promised; nothing checks it.  A new token whose V holds a NaN or an infinity
- * makes the outputs of the query tokens that see it NaN, and only those.
+ * visible.  Rows are taken to agree as promised; nothing checks it.  A new token whose V holds a NaN or an infinity:
+ * with causal != 0 and several query tokens the whole outputs of those that see it are NaN, and only those; in every
+ * other call all query tokens of its batch row see it, and that feature of their outputs is not finite, the others are
+ * as without it.
  *
  * q is [B,H,q_tokens,D], k_new and v_new are [B,G,tokens,D] (post-RoPE, storage dtype) with the given element
  * strides of their batch, head and token axes; the head dim is contiguous and every row 16-byte aligned.  out is

@@ -127,3 +127,35 @@ def test_shared_numbers_out_of_range(name):
     for bad in (10 ** 30, -10 ** 30):
         with pytest.raises(ValueError):
             f(**{name: bad})
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype,D,beams", [(BF16, 64, 2), (BF16, 64, 12), (BF16, 128, 3), (F32, 64, 2)])
+def test_one_feature_of_a_new_value_that_is_not_finite(dtype, D, beams, bad):
+    """One query token, or new tokens that all queries see: that feature of the row's outputs alone is not finite.
+    Several query tokens in order: the outputs of those that see the token are NaN, the others as without it."""
+    from logkv_b200 import log_kv_shared_attention
+    cache = make(dtype, B=2 * beams, D=D, window=64)
+    n = 40
+    _, k, v = projected(cache, 4, n, 1)
+    cache.add_recent_rotated(k[:1].expand(2 * beams, -1, -1, -1), v[:1].expand(2 * beams, -1, -1, -1),
+                             span_ends_device=torch.zeros(2 * beams, n, dtype=torch.uint8, device="cuda"))
+    call = lambda q, k, v, tail: log_kv_shared_attention(cache, q, k, v, 0.125, beams=beams, window_from=n - 7,  # noqa: E731
+                                                         causal_tail=tail)
+    row, feature, token = 1, D - 3, 1
+    for T, Tk, tail in ((1, 1, None), (1, 2, 0), (2, 3, 0), (3, 3, None)):
+        q, k, v = (t.contiguous() for t in projected(cache, 4, Tk, 2))
+        q = q[:, :, :T].contiguous()
+        want = call(q, k, v, tail)
+        assert torch.isfinite(want).all()
+        v[row, 1, min(token, Tk - 1), feature] = bad
+        got = call(q, k, v, tail)
+        spoiled = torch.zeros_like(got, dtype=torch.bool)      # heads 2 and 3 are the second group's
+        if tail is None and T > 1:
+            spoiled[row, 2:, token:] = True
+            assert torch.isnan(got[spoiled]).all()
+        else:
+            spoiled[row, 2:, :, feature] = True
+            assert not torch.isfinite(got[spoiled]).any()
+        assert torch.equal(got[~spoiled], want[~spoiled])
+    assert cache.read_status() == 0

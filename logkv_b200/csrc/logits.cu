@@ -34,6 +34,14 @@ __device__ __forceinline__ unsigned mask_bits(const int32_t* mask, int v, int n,
   return __funnelshift_r(lo, hi, v & 31);
 }
 
+// Whether token v, whose logit is z after the copy under the mask, is a banned one.  The look at the mask is code of
+// its own, which hardly any token of a history comes to: inline it took 145 rows of 50021 (history 4097, no mask) from
+// 14.6 to 15.3 us, this way to 14.8.
+__device__ __noinline__ bool mask_bans(const int32_t* mask, int v) { return !(mask[v >> 5] >> (v & 31) & 1); }
+__device__ __forceinline__ bool banned(const int32_t* mask, float z, int v) {
+  return z == -INFINITY && mask && mask_bans(mask, v);
+}
+
 template <int LT>
 __device__ __forceinline__ void list_sync() {
   asm volatile("bar.sync 1, %0;\n" ::"n"(LT) : "memory");
@@ -316,7 +324,7 @@ __global__ void __launch_bounds__(kLogitsThreads + LT, logits_ctas(LT))
       T* e = y + token[i];
       const float z = Elem<T>::load(e);
       // The mask has the last word: a banned token stays -inf whatever its penalties are (they may be infinite).
-      if (mask && z == -INFINITY && !(mask_bits(mask, token[i], 1, a.vocab) & 1)) continue;
+      if (banned(mask, z, token[i])) continue;
       Elem<T>::store(e, adjust(z, count[i]));
     }
   }

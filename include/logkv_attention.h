@@ -181,7 +181,8 @@ LOGKV_API int logkv_tree_attention(const logkv_layout_t* layout, const logkv_sta
 /*
  * Attention of batch rows that share a long prefix (beams or samples of one prompt; no reference counterpart).
  * Rows r * beams .. r * beams + beams - 1 hold the same packed prefix and the same window rows [0, window_from):
- * those keys are read once for all of them, from the first of the rows; the window rows [window_from, recent_count)
+ * those keys are read from the first of the rows, once per 128 of the request's query rows (bf16, head dim 64 or 128,
+ * more than 16 rows) or once per 16 (otherwise); the window rows [window_from, recent_count)
  * and the new tokens are each row's own.  Otherwise the result of logkv_attention for q_tokens query tokens over
  * `tokens` new ones:
  *   out = softmax(scale * (q . k_s + qx * mass_s)) v_s,

@@ -443,13 +443,14 @@ def log_kv_tree_attention(cache, q, k, v, scale, parents, *, out=None):
 
 
 def log_kv_shared_attention(cache, q, k, v, scale, *, beams: int, window_from: int, causal_tail=None, out=None):
-    """log_kv_chunk_attention of batch rows that share a long prefix, its keys read once for all of them, committing
+    """log_kv_chunk_attention of batch rows that share a long prefix, its keys read once for many of them, committing
     nothing (no reference counterpart).
 
     Rows r * beams .. (r + 1) * beams - 1 (the beams or samples of request r) hold the same ladder, exact pool and
     window rows [0, window_from), as after ``reorder_batch`` has forked them from one row and until the cache's next
     flush; the window behind that and the new tokens are each row's own.  The shared keys are read from the first row
-    of the request.  Rows that do not agree as promised are not noticed.
+    of the request, once per 128 of its beams x (heads per group) x T query rows (bf16, head dim 64 or 128, more than 16
+    rows) or once per 16 (otherwise).  Rows that do not agree as promised are not noticed.
 
     q [B, H, T, D] are the queries of T tokens, k and v [B, G, Tk, D] the new tokens, post-RoPE, any strides.
     ``causal_tail`` T (the default): T == Tk, token t sees the new tokens up to itself; 0: every query sees all Tk >= T

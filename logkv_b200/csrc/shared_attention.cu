@@ -3,15 +3,17 @@
 // The rows of a request (W beams forked from one row) hold the same packed prefix and the same first window rows.
 // Softmax attention over a union of key sets is joined from the parts' maxima m, sums l and products O,
 //   m = max m_i,  l = sum l_i 2^(m_i - m),  O = sum O_i 2^(m_i - m),  out = O / l,
-// so the shared keys are read once per request, by all of its W rf T query rows together (a "shared lane" is a
-// request and a KV group), and every batch row's own keys - the rest of its window and the new tokens - once by
-// its rf T rows (an "own lane").  Both kinds of lanes are split over CTAs of one launch, which leave (m, l, O) per
-// row and split; share_combine_kernel joins them in a fixed order, the shared splits first.
+// so the shared keys are read once per row tile of a request's W rf T query rows (128 rows on tcgen05, that is bf16 of
+// head dim 64 or 128 and more than 16 rows; 16 elsewhere; a "shared lane" is a request and a KV group), and every batch
+// row's own keys - the rest of its window and the new tokens - once by its rf T rows (an "own lane").  Both kinds of
+// lanes are split over CTAs of one launch, which leave (m, l, O) per row and split; share_combine_kernel joins them in a
+// fixed order, the shared splits first.
 //
 // Bound by HBM from a few MB per SM on: keys and values are read once per 128 (16) query rows.  Measured on B200, device
-// time: 8 requests of 8 rows over 7.8K shared and 242 own keys (8 groups, head dim 128, bf16: 314 MB) 60 us, 0.79 of the
-// measured copy bandwidth, where log_kv_chunk_attention takes 367; one request of 4 rows (31 MB) 12.1 us (34); below that
-// latency: 3 requests of 16 rows over 2.0K keys 14.5 us.
+// time: 8 requests of 8 rows over 7.8K shared and 242 own keys (8 groups, head dim 128, bf16: 314 MB) 61 us, 0.78 of the
+// measured copy bandwidth, where log_kv_chunk_attention takes 367; one request of 4 rows (31 MB) 12.6 us (34); below that
+// latency: 3 requests of 16 rows over 2.0K keys 15.1 us.  The join's launch is some 3 us of each (0.5 of them its read of
+// the prefix's length, which has to wait for the attention kernel with the rest).
 #include <algorithm>
 #include <cstring>
 

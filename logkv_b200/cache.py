@@ -644,7 +644,8 @@ class LogStructuredKVCache(nn.Module):
         k_raw and v [B, G, n, D] are a projection's output in the cache dtype, any strides; the state afterwards is
         that of ``q, k, k_raw = log_kv_rotate(...)`` and ``add_recent(k, v, k_raw=k_raw, ...)``, bit for bit.
         ``input_pos`` ([n] or [B, n] integers; None: the positions that continue the sequence) and ``layout`` are
-        log_kv_rotate's, the span-end flags ([B][n] host rows, or ``span_ends_device`` [B, n] on the device) add_recent's.
+        log_kv_rotate's, the span-end flags ([B][n] host rows, or ``span_ends_device`` [B, n] on the device; a captured
+        call takes these) add_recent's.
         """
         from . import rotary
         mode = rotary.check_layout(layout)
@@ -681,6 +682,8 @@ class LogStructuredKVCache(nn.Module):
             raise ValueError("AlphaLogKV span boundaries must match the input batch and token count")
         else:
             ends = None
+            if dev.type == "cuda" and _lib.capture_id(dev):
+                raise RuntimeError("a captured append takes its span ends on the device (span_ends_device)")
         self._check_room(n)
         if n == 0:
             return

@@ -101,6 +101,23 @@ def test_append_of_host_span_ends_does_not_wait():
         assert torch.equal(x[name], y[name]), name
 
 
+def test_captured_append_refuses_host_span_ends():
+    """A graph would read the lists' staging memory again at every replay, when it holds something else."""
+    cache = make(BF16)
+    _, k, v = projected(cache, 2, 2, 1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        x = k + 1
+        with pytest.raises(RuntimeError, match="span_ends_device"):
+            cache.add_recent_rotated(k, v, span_ends=[[False, True]] * 2)
+    graph.replay()
+    assert torch.equal(x, k + 1) and cache.recent_count == cache.token_count == 0
+    cache.add_recent_rotated(k, v, span_ends=[[False, True]] * 2)
+    assert cache.recent_count == 2 and cache.read_status() == 0
+
+
 @pytest.mark.parametrize("name", ["prompt", "lengths", "repetition", "presence", "frequency"])
 def test_numbers_out_of_range(name):
     """Python integers of any size are refused like others, and a prompt longer than the history is the whole of it."""
